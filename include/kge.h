@@ -187,6 +187,61 @@ int kge_paged_attn_decode_noalloc(void* out, const void* q, int q_stride, const 
                                   int hd, int block_size, float scale, void* stream);
 int64_t kge_paged_attn_decode_noalloc_max_bytes(void);
 
+/* Key-value cache in 4 bits (no counterpart in the engine this one replaces; its caches hold 16 or 8 bits): what 8 kv heads of 128
+ * numbers take of a token falls from 4096 bytes to 1088, and decode attention reads as much less.
+ *
+ * One buffer holds keys AND values of a layer, kge_kv4_cache_bytes() of it: [num_blocks, KV, block_size / 16] groups of 16 tokens of one
+ * kv head, 16 * (hd + 8) bytes each: key codes, value codes, (scale, low) of the 16 keys, (scale, low) of the 16 values.  A row (token, kv
+ * head) stands for low + scale * code: low is its smallest number, scale its range / 15 rounded up to the 16-bit type, code 0..15 to the
+ * nearest (ties to even), so no number is off by more than scale / 2.  A row with an infinity or NaN, or whose range is not finite in
+ * fp32, reads back as NaN, in every number.  Where a group's codes lie inside it is csrc/kv4.cuh's matter; a block's bytes may be moved or
+ * copied as a whole, and those of one kv head likewise.  hd 64 or 128, block_size a power of two from 16 (attention: up to 4096).
+ * num_blocks * KV * block_size * (hd + 8); negative for sizes that there are not. */
+int64_t kge_kv4_cache_bytes(int64_t num_blocks, int KV, int hd, int block_size);
+
+/* RoPE (neox pairing) on q and k rows of a packed qkv buffer [T, (H + 2 KV) * hd], q to q_out (rows q_out_stride elements apart; the
+ * qkv buffer itself with its stride (H + 2 KV) * hd is allowed: in place), k and v quantised into the cache at their slots.  The
+ * rotation is done in fp32 and rounded once (kge_rope_kvwrite rounds after every operation); what is quantised is the rounded row.  k and
+ * v rows of qkv stay as they are.  cos_sin, positions, slot_mapping as for kge_rope_kvwrite (NULL cos_sin: no rotation; slot < 0: the
+ * row goes to no cache); two rows of one call must not have the same slot. */
+int kge_rope_kv4write(void* q_out, int q_out_stride, void* kv_cache, const void* qkv, const void* cos_sin, const int32_t* positions,
+                      const int64_t* slot_mapping, int T, int H, int KV, int hd, int block_size, void* stream);
+
+/* The rows at T slots in 16 bits: k_out, v_out [T, KV, hd] = low + scale * code, rounded once; zeros where slot < 0.  For parts of a
+ * context that leave the 4-bit cache (another cache's format, another process, inspection). */
+int kge_kv4_read(void* k_out, void* v_out, const void* kv_cache, const int64_t* slot_mapping, int T, int KV, int hd, int block_size,
+                 void* stream);
+
+/* kge_paged_attn over the 4-bit cache, with an optional sliding window: arguments and semantics of kge_paged_attn but
+ *  - kv_cache is the one buffer of keys and values
+ *  - window > 0: a query at position i sees the keys j <= i with i - j < window or j < first (first tokens that stay visible, "sinks");
+ *    window 0: all j <= i.  Pages that no query sees are not read.
+ *  - H / KV up to 128; scale > 0; q_stride >= H * hd; out, q, kv_cache and workspace 16-byte aligned
+ *  - T may be larger than the rows of all requests (a captured step with room to spare): rows behind query_start_loc[B] are left alone,
+ *    as are requests without rows; max_q_len and max_seq_len are upper bounds.  A row without a key (seq_lens 0) is zeros.
+ *  - a NaN row of the cache makes NaN of the queries that see it, and of no others
+ * `workspace`: device scratch of kge_attn_kv4_workspace_bytes(H, KV, hd), whatever the batch is, for H / KV <= 16 (otherwise 0 and NULL
+ * will do); nothing in it needs clearing, and calls that share one must not overlap on the GPU. */
+int kge_paged_attn_kv4(void* out, const void* q, int q_stride, const void* kv_cache, const int32_t* block_table,
+                       int max_blocks_per_seq, const int32_t* seq_lens, const int32_t* query_start_loc, int B, int T, int max_q_len,
+                       int max_seq_len, int H, int KV, int hd, int block_size, float scale, int window, int first, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int64_t kge_attn_kv4_workspace_bytes(int H, int KV, int hd);
+
+/* Block tables, slots, positions and row offsets of a step, built on the GPU from its requests' lengths - what a host scheduler
+ * otherwise prepares and copies in (vllm:v1/worker/block_table.py, compute_slot_mapping) - so that a loop of decode steps, or a captured
+ * step, needs nothing from the host.  For either cache.
+ * In: cached_lens [B] tokens in the cache, new_lens [B] tokens to add (negative counts as 0), free_blocks [num_free] block ids to hand
+ * out, from position *free_first on; block_table [B, max_blocks_per_seq] with the ceil(cached / block_size) blocks that each request holds.
+ * Out: the table with each request's further blocks, taken from the list in the order of the requests; seq_lens [B] = cached + new;
+ * query_start_loc [B + 1]; positions [T] and slot_mapping [T] of the rows, request after request (rows behind the last: position 0, slot
+ * -1); counts [4] = {rows, tokens asked for, position in the free list behind the last block taken, blocks that were lacking}.
+ * Where T, a table row or the free list does not reach, a request gets as many of its new tokens as fit, and all outputs say so.
+ * seq_lens may be cached_lens and free_first may be counts + 2 (the next step goes on from there).  Block size: a power of two; B <= 8192. */
+int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32_t* seq_lens, int32_t* query_start_loc, int32_t* positions,
+                  int64_t* slot_mapping, int32_t* counts, const int32_t* cached_lens, const int32_t* new_lens, const int32_t* free_blocks,
+                  int num_free, const int32_t* free_first, int B, int T, int block_size, void* stream);
+
 /* Greedy sampling, vllm:v1/sample/sampler.py:91,235-236: argmax over fp32(bf16 logits),
  * lowest index wins ties.  logits [B, ld] bf16 (ld >= V: padded vocab columns ignored). */
 int kge_argmax(int32_t* out_ids, const void* logits, int B, int V, int ld, void* stream);
@@ -237,6 +292,14 @@ int kge_paged_attn_f16(void* out, const void* q, int q_stride, const void* k_cac
                        const int32_t* block_table, int max_blocks_per_seq, const int32_t* seq_lens,
                        const int32_t* query_start_loc, int B, int T, int max_q_len, int max_seq_len, int H, int KV, int hd,
                        int block_size, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int kge_rope_kv4write_f16(void* q_out, int q_out_stride, void* kv_cache, const void* qkv, const void* cos_sin, const int32_t* positions,
+                          const int64_t* slot_mapping, int T, int H, int KV, int hd, int block_size, void* stream);
+int kge_kv4_read_f16(void* k_out, void* v_out, const void* kv_cache, const int64_t* slot_mapping, int T, int KV, int hd, int block_size,
+                     void* stream);
+int kge_paged_attn_kv4_f16(void* out, const void* q, int q_stride, const void* kv_cache, const int32_t* block_table,
+                           int max_blocks_per_seq, const int32_t* seq_lens, const int32_t* query_start_loc, int B, int T, int max_q_len,
+                           int max_seq_len, int H, int KV, int hd, int block_size, float scale, int window, int first, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 int kge_argmax_f16(int32_t* out_ids, const void* logits, int B, int V, int ld, void* stream);
 int kge_sample_f16(int32_t* out_ids, const void* logits, int B, int V, int ld, const float* temperature,
                    const int32_t* top_k, const float* top_p, const float* exp_noise, const uint64_t* seeds, uint64_t step,

@@ -91,6 +91,12 @@ SIGNATURES = {
     "kge_attn_workspace_bytes": (_L, [_I, _I, _I, _I]),
     "kge_paged_attn_decode_noalloc": (_I, [_P, _P, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
     "kge_paged_attn_decode_noalloc_max_bytes": (_L, []),
+    "kge_kv4_cache_bytes": (_L, [_L, _I, _I, _I]),
+    "kge_rope_kv4write": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "kge_kv4_read": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "kge_paged_attn_kv4": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _L, _P]),
+    "kge_attn_kv4_workspace_bytes": (_L, [_I, _I, _I]),
+    "kge_step_maps": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
     "kge_argmax": (_I, [_P, _P, _I, _I, _I, _P]),
     "kge_sample": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, C.c_uint64, _P, _L, _P]),
     "kge_sample_workspace_bytes": (_L, [_I, _I]),
@@ -174,7 +180,8 @@ for _n, _t in {"kge_embed": "kge_embed_f16", "kge_rmsnorm": "kge_rmsnorm_f16", "
                "kge_gemm_bf16": "kge_gemm_f16", "kge_gemm_silu_gate_bf16": "kge_gemm_silu_gate_f16",
                "kge_gemm_silu_gate_ws_bf16": "kge_gemm_silu_gate_ws_f16", "kge_gemm_clamped_glu_bf16": "kge_gemm_clamped_glu_f16",
                "kge_rope_kvwrite": "kge_rope_kvwrite_f16", "kge_rope_cache_host": "kge_rope_cache_host_f16",
-               "kge_paged_attn": "kge_paged_attn_f16", "kge_argmax": "kge_argmax_f16", "kge_sample": "kge_sample_f16",
+               "kge_paged_attn": "kge_paged_attn_f16", "kge_rope_kv4write": "kge_rope_kv4write_f16", "kge_kv4_read": "kge_kv4_read_f16",
+               "kge_paged_attn_kv4": "kge_paged_attn_kv4_f16", "kge_argmax": "kge_argmax_f16", "kge_sample": "kge_sample_f16",
                "kge_logprobs": "kge_logprobs_f16", "kge_tp_reduce_add_norm": "kge_tp_reduce_add_norm_f16"}.items():
     SIGNATURES[_t] = SIGNATURES[_n]
 

@@ -25,6 +25,7 @@
 #include "common.cuh"
 #include "f32x2.cuh"
 #include "kge.h"
+#include "kv4.cuh"
 
 namespace kge {
 inline namespace KGE_ELT_NS {
@@ -535,6 +536,7 @@ static dim3 tc_grid(int B, int T, int max_q_len, int TT, int KV, int& by_request
 }
 
 #include "attn_pair.cuh"
+#include "attn_kv4_tc.cuh"
 
 template <int HD>
 static int launch_tc(bf16* out, const bf16* q, int q_stride, const bf16* kc, const bf16* vc, const int32_t* bt,
