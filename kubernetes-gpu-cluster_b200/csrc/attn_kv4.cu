@@ -1,18 +1,21 @@
 // Attention over the 4-bit key-value cache (layout: kv4.cuh), single-token requests; prompts: attn_kv4_tc.cuh.
 //
-// With key k = low_k + s_k c_k and value v = low_v + s_v c_v (c: codes 0..15), centred codes c' = c - 8 and z = low + 8 s,
-//   score = scale (s_k (q . c'_k) + z_k sum(q))            out = (sum_j (p_j s_v,j) c'_v,j + sum_j p_j z_v,j) / sum_j p_j
+// With key k = low_k + s_k n_k and value v = low_v + s_v n_v (n: codes 0..15), z = low + 8 s,
+//   score = scale (s_k (q . n_k) + low_k sum(q))           out = (sum_j (p_j s_v,j) (n_v,j - 8) + sum_j p_j z_v,j) / sum_j p_j
 // so the products run on codes, which 16 bits hold exactly, and the two numbers of a row are applied to scores and weights in fp32.
 //
 // A warp takes 32 keys at a time from a ring of its own (bulk copies that its lane 0 asks for), and multiplies with mma.m16n8k16 whose M side
 // is the keys (scores) or the dimensions (outputs) and whose N side is the query heads of one kv head: 8 columns of which a group of 4 or 8
-// heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build: codes are exact, q is
-// exact but for what lies 2^-24 below its largest number (a power of two moves the largest of the group's heads to 2^14), and weights round at
-// 2^-11.  Weights: w = e s_v with e = 2^(x - R), R a reference per head such that the largest w of a warp lies between 1 and 2^14; R moves
-// only when a weight would pass that, or e 2^100 (values so small that nothing of them is left in 16 bits), so most tiles rescale nothing and
-// need no shuffles.
+// heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
+//   Codes: the bits n in the low half-byte of a float16 are the number n 2^-24 (its denormals), in the next one n 2^-20, so a code costs half an
+//   AND and no arithmetic; powers of two are put right in q (scores) and in the outputs.  (As 1024 + n less 1032: 2.6 instructions a pair.)
+//   q: a power of two moves the largest number of the group's heads to 2^14; exact but for what lies 2^-24 below that.
+//   Weights: w = e s_v with e = 2^(x - R), rounded to float16; R is a reference per head, such that the largest w of a warp lies between 1 and
+//   2^14.  It moves only when a weight would pass that, so most tiles rescale nothing and need no shuffles.  What is taken off for centring, 8
+//   times the sum of the weights, is the sum of the ROUNDED ones (a product with ones), so a rounding's error meets |n - 8| and not n.
 //   scores come out as (key, head) fragments; movmatrix turns a packed 8 x 8 of weights into the B operand of the second product
-// Codes to float16: 0x6400 | n is 1024 + n, exactly; the other nibble of a byte comes as 1024 + 16 n and goes through one fma with 1/16.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kge.h"
 #include "kv4.cuh"
@@ -26,7 +29,8 @@ constexpr int NW = 4, TK = 32, ST = 3;         // warps of a CTA, keys of a tile
 constexpr int CTAS = 3;                        // CTAs of an SM
 constexpr int kMaxCtas = 148 * CTAS;
 constexpr float kLog2e = 1.4426950408889634f, kNoRef = -1e30f;
-constexpr float kWeightMost = 16384.f, kExpMost = 2.8147498e14f /* 2^48 */, kExpRoom = 40.f;
+constexpr float kExpRoom = 40.f;
+constexpr uint32_t kWeightMost = 0x7400;       // 2^14 in float16
 
 struct Args {
   bf16* out;
@@ -60,17 +64,12 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// nibbles 0 and 4 (P even) or 1 and 5 (P odd) of w as two float16 numbers c - 8
-__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-  const uint32_t v = (w & 0x000f000fu) | 0x64006400u;
+// nibbles 0 and 4, or 1 and 5, of w as two float16 numbers: n 2^-24 and n 2^-20
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return w & 0x00f000f0u; }
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x64086408u));              // - 1032
-  return r;
-}
-__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-  const uint32_t v = (w & 0x00f000f0u) | 0x64006400u;
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0x2c002c00u), "r"(0xd480d480u));      // / 16 - 72
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -89,16 +88,16 @@ struct Span {
 
 // A share of the launch's tiles, piece by piece: request-major, then kv head, then tile.
 struct Walk {
-  int64_t u, u1;
+  uint32_t u, u1;
   int b, kvh, t0, t1, n;                       // the current piece: tiles t0 .. t1 of a group of n
-  __device__ __forceinline__ bool next(const int* pre, int KV) {
+  __device__ __forceinline__ bool next(const uint32_t* pre, uint32_t KV) {
     if (u >= u1) return false;
-    while ((int64_t)pre[b + 1] * KV <= u) ++b;
-    n = pre[b + 1] - pre[b];
-    const int64_t rel = u - (int64_t)pre[b] * KV;
-    kvh = (int)(rel / n);
-    t0 = (int)(rel - (int64_t)kvh * n);
-    t1 = (int)min((int64_t)n, t0 + (u1 - u));
+    while (pre[b + 1] * KV <= u) ++b;
+    const uint32_t groups = pre[b + 1] - pre[b], rel = u - pre[b] * KV;
+    n = (int)groups;
+    kvh = (int)(rel / groups);
+    t0 = (int)(rel - kvh * groups);
+    t1 = (int)min(groups, t0 + (u1 - u));
     u += t1 - t0;
     return true;
   }
@@ -115,7 +114,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
   extern __shared__ __align__(128) uint8_t smem[];
   float* red = reinterpret_cast<float*>(smem + ring_bytes<HD>());
   uint64_t* bars = reinterpret_cast<uint64_t*>(red + red_floats<HD>());
-  int* pre = reinterpret_cast<int*>(bars + NW * ST);
+  uint32_t* pre = reinterpret_cast<uint32_t*>(bars + NW * ST);
   const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.H / a.KV;
   const uint32_t ring = s_addr(smem) + warp * ST * 2 * GB, bar0 = s_addr(bars) + warp * ST * 8;
@@ -127,42 +126,39 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
   pdl_wait();
 
   Walk cons, prod;                             // what is computed, what is asked for: the second runs ahead
-  int64_t u0 = 0;
+  uint32_t u0 = 0;
   if (SPLIT) {
     for (int b = tid; b < a.B; b += NW * 32) pre[b + 1] = a.qsl[b + 1] - a.qsl[b] == 1 ? Span(a.len(b), a.window, a.first).n : 0;
     if (tid == 0) pre[0] = 0;
     __syncthreads();
     if (warp == 0) {
       const int per = (a.B + 31) / 32, lo = 1 + lane * per, hi = min(a.B + 1, lo + per);
-      int sum = 0;
+      uint32_t sum = 0;
       for (int i = lo; i < hi; ++i) sum += pre[i];
-      int incl = sum;
+      uint32_t incl = sum;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, d); if (lane >= d) incl += v; }
-      int run = incl - sum;
+      for (int d = 1; d < 32; d <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d); if (lane >= d) incl += v; }
+      uint32_t run = incl - sum;
       for (int i = lo; i < hi; ++i) { run += pre[i]; pre[i] = run; }
     }
     __syncthreads();
-    const int64_t U = (int64_t)pre[a.B] * a.KV;
-    const int chunk = max((int)((U + gridDim.x - 1) / gridDim.x), min_chunk);
-    u0 = (int64_t)blockIdx.x * chunk;
-    cons.u = u0; cons.u1 = min(U, u0 + chunk); cons.b = 0;
+    const uint32_t KV = a.KV, U = pre[a.B] * KV, chunk = max((U + gridDim.x - 1) / gridDim.x, (uint32_t)min_chunk);
+    auto request_of = [&](uint32_t unit) {
+      int lo = 0, hi = a.B - 1;
+      while (lo < hi) { const int mid = (lo + hi) >> 1; if (pre[mid + 1] * KV <= unit) lo = mid + 1; else hi = mid; }
+      return lo;
+    };
+    u0 = min(U, blockIdx.x * chunk);
+    cons.u = u0; cons.u1 = min(U, u0 + chunk); cons.b = u0 < cons.u1 ? request_of(u0) : 0;
     if (tid == 0) {
       // the group that begins in this share and ends beyond it
       int4 d = make_int4(-1, 0, 0, 0);
       if (u0 < cons.u1 && cons.u1 < U) {
-        int lo = 0, hi = a.B - 1;
-        while (lo < hi) { const int mid = (lo + hi) >> 1; if ((int64_t)pre[mid + 1] * a.KV <= cons.u1 - 1) lo = mid + 1; else hi = mid; }
-        const int n = pre[lo + 1] - pre[lo];
-        const int64_t base = (int64_t)pre[lo] * a.KV, kvh = (cons.u1 - 1 - base) / n, g0 = base + kvh * n, g1 = g0 + n;
-        if (g0 >= u0 && g1 > cons.u1) d = make_int4(a.qsl[lo], (int)kvh, (int)((g1 - 1) / chunk), g0 > u0);
+        const int b = request_of(cons.u1 - 1);
+        const uint32_t n = pre[b + 1] - pre[b], base = pre[b] * KV, kvh = (cons.u1 - 1 - base) / n, g0 = base + kvh * n, g1 = g0 + n;
+        if (g0 >= u0 && g1 > cons.u1) d = make_int4(a.qsl[b], (int)kvh, (int)((g1 - 1) / chunk), g0 > u0);
       }
       a.desc[blockIdx.x] = d;
-    }
-    if (u0 < cons.u1) {
-      int lo = 0, hi = a.B - 1;
-      while (lo < hi) { const int mid = (lo + hi) >> 1; if ((int64_t)pre[mid + 1] * a.KV <= u0) lo = mid + 1; else hi = mid; }
-      cons.b = lo;
     }
   } else {
     cons.b = blockIdx.y;
@@ -176,28 +172,34 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
   };
   prod = cons;
 
-  // ---- the ring: lane 0 (and lane 1, where a tile lies in two blocks) asks for this warp's next tile
+  // ---- the ring: lane 0 (and lane 1, where a tile lies in two blocks) asks for this warp's next tile, whose block id it read a tile before
+  const bool two = a.bs_shift == 4;
   bool p_more = piece(prod, false);
-  int p_tile = p_more ? prod.t0 + warp : 0, p_stage = 0;
+  int p_tile = p_more ? prod.t0 + warp : 0, p_stage = 0, p_key0 = 0, p_blk = 0;
   Span p_span(p_more ? a.len(prod.b) : 0, a.window, a.first);
-  auto ask = [&]() {
+  auto settle = [&]() {                        // p_tile is this warp's next tile, in this piece or a later one
     while (p_more && p_tile >= prod.t1) {
       p_more = piece(prod, true);
       if (p_more) { p_tile = prod.t0 + warp; p_span = Span(a.len(prod.b), a.window, a.first); }
     }
+    p_key0 = p_span.key0(p_tile);
+    const int key = p_key0 + lane * 16;
+    if (p_more && lane < 2 && key < p_span.len) p_blk = a.table[(int64_t)prod.b * a.max_blocks + (key >> a.bs_shift)];
+  };
+  settle();
+  auto ask = [&]() {
     if (!p_more) return;
-    const int key0 = p_span.key0(p_tile), groups = min(2, max(0, (p_span.len - key0 + 15) >> 4));
-    const bool two = a.bs_shift == 4;          // blocks of 16: a tile is two copies
+    const int groups = min(2, max(0, (p_span.len - p_key0 + 15) >> 4));
     const uint32_t bar = bar0 + 8 * p_stage;
     if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(groups * GB)) : "memory");
     __syncwarp();
-    if (lane < (two ? groups : min(groups, 1))) {
-      const int key = key0 + lane * 16, blk = a.table[(int64_t)prod.b * a.max_blocks + (key >> a.bs_shift)];
-      const uint8_t* src = a.cache + ((((int64_t)blk * a.KV + prod.kvh) << (a.bs_shift - 4)) + ((key & ((1 << a.bs_shift) - 1)) >> 4)) * GB;
-      bulk_load(ring + p_stage * 2 * GB + lane * GB, src, two ? GB : groups * GB, bar);
-    }
+    if (lane < (two ? groups : min(groups, 1)))
+      bulk_load(ring + (p_stage * 2 + lane) * GB,
+                a.cache + ((((int64_t)p_blk * a.KV + prod.kvh) << (a.bs_shift - 4)) + (((p_key0 + lane * 16) & ((1 << a.bs_shift) - 1)) >> 4)) * GB,
+                two ? GB : groups * GB, bar);
     p_stage = p_stage + 1 == ST ? 0 : p_stage + 1;
     p_tile += NW;
+    settle();
   };
 #pragma unroll 1
   for (int s = 0; s < ST; ++s) ask();
@@ -212,9 +214,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
     float qs[NT][2], fs;                       // scale log2(e) sum(q) of this thread's two columns; what scores are multiplied with
     {
       uint4 raw[NT][W];
-#ifndef KGE_HALF
       float mx = 0.f;
-#endif
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int head = nt * 8 + g;
@@ -228,10 +228,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
           for (int k = 0; k < 4; ++k) {
             const float x = bf_lo(u[k]), y = bf_hi(u[k]);
             sum += x + y;
-#ifndef KGE_HALF
-            const float m = fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f);
-            mx = fmaxf(mx, m);
-#endif
+            mx = fmaxf(mx, fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f));
           }
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -239,30 +236,21 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
         qs[nt][0] = a.scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t);
         qs[nt][1] = a.scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       }
-      fs = a.scale_log2;
-#ifndef KGE_HALF
-      // 2^(14 - exponent of the largest finite number); down to 2^-100, up to 2^100
+      // 2^e brings the largest finite number to 2^14 (e from -100 to 100); high nibbles count 16 times, so what they meet is q 2^(e - 4)
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
       const int e = top ? min(max(141 - (int)(top >> 23), -100), 100) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-      fs *= __uint_as_float((uint32_t)(127 - e) << 23);
-#endif
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23), up4 = __uint_as_float((uint32_t)(123 + e) << 23);
+      fs = a.scale_log2 * __uint_as_float((uint32_t)(151 - e) << 23);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const uint32_t* u = &raw[nt][i].x;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-#ifdef KGE_HALF
-            qb[nt][2 * i + (k >> 1)][k & 1] = u[k];
-#else
-            qb[nt][2 * i + (k >> 1)][k & 1] = pack_h2(bf_lo(u[k]) * up, bf_hi(u[k]) * up);
-#endif
-          }
+          for (int k = 0; k < 4; ++k) qb[nt][2 * i + (k >> 1)][k & 1] = pack_h2(bf_lo(u[k]) * (k & 1 ? up4 : up), bf_hi(u[k]) * (k & 1 ? up4 : up));
         }
     }
-    float o[NM][NT][4], ref[NT][2], l[NT][2], zs[NT][2];
+    float o[NM][NT][4], ws[NT][4], ref[NT][2], l[NT][2], zs[NT][2];      // ws: sums of the rounded weights, from a product with ones
 #pragma unroll
     for (int i = 0; i < NM; ++i)
 #pragma unroll
@@ -270,19 +258,18 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) { ref[nt][h] = kNoRef; l[nt][h] = zs[nt][h] = 0.f; }
+      for (int h = 0; h < 2; ++h) { ref[nt][h] = l[nt][h] = zs[nt][h] = ws[nt][h] = ws[nt][2 + h] = 0.f; }
 
+    bool fresh = true;                         // the first tile sets the references
     for (int tile = cons.t0 + warp; tile < cons.t1; tile += NW) {
       const int key0 = sp.key0(tile);
       mbar_wait(bar0 + 8 * stage, parity);
       const uint8_t* base = smem + (warp * ST + stage) * 2 * GB;
-      // ---- scores in units of log 2: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
+      // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
       float x[2][NT][4], zv[2][2], sv[2][2];
-      const int mine = key0 + kv4::key_token(g);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint8_t* grp = base + i * GB;
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(grp + 16 * HD) + kv4::key_token(g);
         uint32_t ka[W], kb[W];
         if (HD == 128) {
           const uint4 u = *reinterpret_cast<const uint4*>(grp + g * 64 + t * 16), v = *reinterpret_cast<const uint4*>(grp + 512 + g * 64 + t * 16);
@@ -293,32 +280,34 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
           ka[0] = u.x; ka[1] = u.y;
           kb[0] = v.x; kb[1] = v.y;
         }
+        float c[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) x[i][nt][0] = x[i][nt][1] = x[i][nt][2] = x[i][nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < W; ++j) {
           const uint32_t a0 = ka[j], b0 = kb[j], a1 = a0 >> 8, b1 = b0 >> 8;
           const uint32_t f0[4] = {codes_lo(a0), codes_lo(b0), codes_hi(a0), codes_hi(b0)}, f1[4] = {codes_lo(a1), codes_lo(b1), codes_hi(a1), codes_hi(b1)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(x[i][nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
-            mma_f16(x[i][nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+            mma_f16(c[nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+            mma_f16(c[nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
           }
         }
+        const uint32_t* par = reinterpret_cast<const uint32_t*>(grp + 16 * HD) + kv4::key_token(g);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const uint32_t pk = par[8 * r], pv = par[16 + 8 * r];
-          const float sk = bf_lo(pk), zk = fmaf(8.f, sk, bf_hi(pk)), f = fs * sk;
+          const float lk = bf_hi(pk), f = fs * bf_lo(pk);
           sv[i][r] = bf_lo(pv);
           zv[i][r] = fmaf(8.f, sv[i][r], bf_hi(pv));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            x[i][nt][2 * r] = fmaf(x[i][nt][2 * r], f, qs[nt][0] * zk);
-            x[i][nt][2 * r + 1] = fmaf(x[i][nt][2 * r + 1], f, qs[nt][1] * zk);
-          }
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
         }
       }
       if (key0 + TK > sp.len || (key0 < sp.lo && key0 + TK > a.first)) {      // the same for the warp
+        const int mine = key0 + kv4::key_token(g);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -333,58 +322,65 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
       }
       // ---- weights
       uint32_t w[2][NT][2];
-      float e_sum[NT][2], z_sum[NT][2];
-      auto weigh = [&]() {
-        float most = 0.f, e_most = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) e_sum[nt][h] = z_sum[nt][h] = 0.f;
+      float e[2][NT][4];
+      auto weigh = [&]() {                     // false: a weight has passed its bound (or is NaN)
+        uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const float e0 = ex2(x[i][nt][2 * r] - ref[nt][0]), e1 = ex2(x[i][nt][2 * r + 1] - ref[nt][1]);
-              const float w0 = e0 * sv[i][r], w1 = e1 * sv[i][r];
-              e_sum[nt][0] += e0; e_sum[nt][1] += e1;
-              z_sum[nt][0] = fmaf(e0, zv[i][r], z_sum[nt][0]); z_sum[nt][1] = fmaf(e1, zv[i][r], z_sum[nt][1]);
-              most = fmaxf(most, fmaxf(w0, w1));
-              e_most = fmaxf(e_most, fmaxf(e0, e1));
-              w[i][nt][r] = pack_h2(w0, w1);
+            for (int r = 0; r < 2; ++r) {
+              e[i][nt][2 * r] = ex2(x[i][nt][2 * r]);
+              e[i][nt][2 * r + 1] = ex2(x[i][nt][2 * r + 1]);
+              w[i][nt][r] = pack_h2(e[i][nt][2 * r] * sv[i][r], e[i][nt][2 * r + 1] * sv[i][r]);
+              most = max_u16x2(most, w[i][nt][r]);
             }
-        return most > kWeightMost || e_most > kExpMost;
+        return most < (kWeightMost << 16) && (most & 0xffffu) < kWeightMost;
       };
-      if (__any_sync(0xffffffffu, weigh())) {
+      const bool fits = weigh();
+      if (fresh || !__all_sync(0xffffffffu, fits)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float top = ref[nt][h];
+            float top = fresh ? -INFINITY : 0.f;                              // how far the reference goes up (the first: or down)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int r = 0; r < 2; ++r) top = fmaxf(top, fmaxf(x[i][nt][2 * r + h] + lg2(sv[i][r]), x[i][nt][2 * r + h] - kExpRoom));
 #pragma unroll
             for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-            const float f = ex2(ref[nt][h] - top);
-            ref[nt][h] = top;
+            if (top == -INFINITY) top = 0.f;                                  // (only NaN rows)
+            const float f = ex2(-top);
+            ref[nt][h] += top;
             l[nt][h] *= f;
             zs[nt][h] *= f;
+            ws[nt][h] *= f;
 #pragma unroll
             for (int i = 0; i < NM; ++i) { o[i][nt][h] *= f; o[i][nt][2 + h] *= f; }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] -= top;
           }
         weigh();
+        fresh = false;
       }
       uint32_t pb[2][NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) { l[nt][h] += e_sum[nt][h]; zs[nt][h] += z_sum[nt][h]; }
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) { pb[i][nt][0] = turn8x8(w[i][nt][0]); pb[i][nt][1] = turn8x8(w[i][nt][1]); }
-      }
+          for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { l[nt][h] += e[i][nt][2 * r + h]; zs[nt][h] = fmaf(e[i][nt][2 * r + h], zv[i][r], zs[nt][h]); }
+            pb[i][nt][r] = turn8x8(w[i][nt][r]);
+          }
+          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+          mma_f16(ws[nt], ones, pb[i][nt][0], pb[i][nt][1]);
+        }
       // ---- outputs: rows g and g + 8 of fragment 4 j + p are dimensions d = (HD / 8) g + 8 j + 2 p and d + 1; the keys of thread t are
       // t, t + 4, t + 8, t + 12 of the group
 #pragma unroll
@@ -443,11 +439,12 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float* dst = red + (warp * 4 + 2 * (t & 1) + h) * RS;
+            const float rest = fmaf(-8.f, ws[nt][h], zs[nt][h]);
 #pragma unroll
-            for (int i = 0; i < NM; i += 2)
-              *reinterpret_cast<float4*>(dst + g * (HD / 8) + 2 * i) =
-                  make_float4(o[i][nt][h] + zs[nt][h], o[i][nt][2 + h] + zs[nt][h], o[i + 1][nt][h] + zs[nt][h], o[i + 1][nt][2 + h] + zs[nt][h]);
-            if (g == 0) { dst[HD] = ref[nt][h]; dst[HD + 1] = l[nt][h]; }
+            for (int i = 0; i < NM; i += 2)              // fragments of low nibbles (even) and of high ones
+              *reinterpret_cast<float4*>(dst + g * (HD / 8) + 2 * i) = make_float4(fmaf(o[i][nt][h], 16777216.f, rest), fmaf(o[i][nt][2 + h], 16777216.f, rest),
+                                                                                   fmaf(o[i + 1][nt][h], 1048576.f, rest), fmaf(o[i + 1][nt][2 + h], 1048576.f, rest));
+            if (g == 0) { dst[HD] = fresh ? kNoRef : ref[nt][h]; dst[HD + 1] = l[nt][h]; }      // (a warp without a tile)
           }
         __syncthreads();
         for (int it = tid; it < HD; it += NW * 32) {     // (row, 4 dimensions)
@@ -542,9 +539,12 @@ static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
 
 static int decode(ak4::Args a, int hd, int max_seq_len, cudaStream_t st) {
   const int B = a.B, G = a.H / a.KV;
-  for (int b0 = 0; b0 < B; b0 += ak4::kMaxRequests) {
+  // requests of a launch: what shared memory has room for, and tiles that 32 bits count (a table's row bounds a request's)
+  const int64_t tiles = ((((int64_t)a.max_blocks << a.bs_shift) + ak4::TK - 1) / ak4::TK + 1) * a.KV;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(ak4::kMaxRequests, ((1ll << 31) - 1) / tiles));
+  for (int b0 = 0; b0 < B; b0 += most) {
     ak4::Args p = a;
-    p.B = B - b0 < ak4::kMaxRequests ? B - b0 : ak4::kMaxRequests;
+    p.B = std::min(B - b0, most);
     p.table += (int64_t)b0 * a.max_blocks; p.lens += b0; p.qsl += b0;
     int rc;
     if (hd == 128) rc = G <= 8 ? ak4::launch<128, 1>(p, max_seq_len, st) : ak4::launch<128, 2>(p, max_seq_len, st);
