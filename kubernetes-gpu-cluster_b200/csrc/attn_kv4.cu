@@ -4,9 +4,9 @@
 //   score = scale (s_k (q . n_k) + low_k sum(q))           out = (sum_j (p_j s_v,j) (n_v,j - 8) + sum_j p_j z_v,j) / sum_j p_j
 // so the products run on codes, which 16 bits hold exactly, and the two numbers of a row are applied to scores and weights in fp32.
 //
-// A warp takes 32 keys at a time from a ring of its own (bulk copies that its lane 0 asks for), and multiplies with mma.m16n8k16 whose M side
-// is the keys (scores) or the dimensions (outputs) and whose N side is the query heads of one kv head: 8 columns of which a group of 4 or 8
-// heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
+// Four warps take 32 keys each of tiles of 128, which a fifth brings by bulk copies (one per block of a tile), and multiply with mma.m16n8k16
+// whose M side is the keys (scores) or the dimensions (outputs) and whose N side is the query heads of one kv head: 8 columns of which a group
+// of 4 or 8 heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
 //   Codes: the bits n in the low half-byte of a float16 are the number n 2^-24 (its denormals), in the next one n 2^-20, so a code costs half an
 //   AND and no arithmetic; powers of two are put right in q (scores) and in the outputs.  (As 1024 + n less 1032: 2.6 instructions a pair.)
 //   q: a power of two moves the largest number of the group's heads to 2^14; exact but for what lies 2^-24 below that.
@@ -25,9 +25,11 @@ inline namespace KGE_ELT_NS {
 
 namespace ak4 {
 
-constexpr int NW = 4, TK = 32, ST = 3;         // warps of a CTA, keys of a tile, tiles of a warp's ring
-constexpr int CTAS = 3;                        // CTAs of an SM
-constexpr int kMaxCtas = 148 * CTAS;
+constexpr int NW = 4, TK = 128, WK = TK / NW, GROUPS = TK / 16;      // computing warps, keys of a tile, of a warp; groups of a tile
+constexpr int kThreads = NW * 32 + 32;
+__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 3 : 4; }      // tiles on their way; CTAs of an SM
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kMaxCtas = 148 * 3;
 constexpr float kLog2e = 1.4426950408889634f, kNoRef = -1e30f;
 constexpr float kExpRoom = 40.f;
 constexpr uint32_t kWeightMost = 0x7400;       // 2^14 in float16
@@ -85,6 +87,7 @@ struct Span {
   }
   __device__ __forceinline__ int key0(int tile) const { return (tile < npre ? tile : win0 + tile - npre) * TK; }
 };
+__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // the computing warps
 
 // A share of the launch's tiles, piece by piece: request-major, then kv head, then tile.
 struct Walk {
@@ -104,31 +107,38 @@ struct Walk {
 };
 
 template <int HD> __host__ __device__ constexpr int red_floats() { return NW * 4 * (HD + 4); }
-template <int HD> __host__ __device__ constexpr int ring_bytes() { return NW * ST * 2 * kv4::group_bytes(HD); }
+template <int HD, int NT> __host__ __device__ constexpr int ring_bytes() { return stages(NT) * GROUPS * kv4::group_bytes(HD); }
 
 // SPLIT: the tiles of all (request, kv head) groups are one sequence, every CTA takes an equal share of it, and a group that is cut is merged
 // by the kernel behind.  Otherwise a CTA has a whole group.
 template <int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, int min_chunk) {
-  constexpr int GB = kv4::group_bytes(HD), W = HD / 32, NM = HD / 16, RS = HD + 4;      // W: words of a thread's share of a key row
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_kv4_kernel(const Args a, int min_chunk) {
+  constexpr int GB = kv4::group_bytes(HD), W = HD / 32, NM = HD / 16, RS = HD + 4, ST = stages(NT);      // W: words of a thread's share of a key row
   extern __shared__ __align__(128) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + ring_bytes<HD>());
+  float* red = reinterpret_cast<float*>(smem + ring_bytes<HD, NT>());
   uint64_t* bars = reinterpret_cast<uint64_t*>(red + red_floats<HD>());
-  uint32_t* pre = reinterpret_cast<uint32_t*>(bars + NW * ST);
+  uint32_t* pre = reinterpret_cast<uint32_t*>(bars + 2 * ST);
   const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int G = a.H / a.KV;
-  const uint32_t ring = s_addr(smem) + warp * ST * 2 * GB, bar0 = s_addr(bars) + warp * ST * 8;
-  if (lane == 0)
-    for (int s = 0; s < ST; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar0 + 8 * s));
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  __syncwarp();
+  const uint32_t bar0 = s_addr(bars);
+  // full(s): the producer's arrival and its copies' bytes; empty(s): the computing warps.  A wait for either comes before what the next
+  // phase of it needs: a warp arrives on empty(s) only behind its wait for full(s), and the producer refills s only behind empty(s).
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full(s)));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty(s)), "n"(NW));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pdl_launch_dependents();
   pdl_wait();
 
-  Walk cons, prod;                             // what is computed, what is asked for: the second runs ahead
+  Walk cons;
   uint32_t u0 = 0;
   if (SPLIT) {
-    for (int b = tid; b < a.B; b += NW * 32) pre[b + 1] = a.qsl[b + 1] - a.qsl[b] == 1 ? Span(a.len(b), a.window, a.first).n : 0;
+    for (int b = tid; b < a.B; b += kThreads) pre[b + 1] = a.qsl[b + 1] - a.qsl[b] == 1 ? Span(a.len(b), a.window, a.first).n : 0;
     if (tid == 0) pre[0] = 0;
     __syncthreads();
     if (warp == 0) {
@@ -163,50 +173,54 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
   } else {
     cons.b = blockIdx.y;
     if (a.qsl[cons.b + 1] - a.qsl[cons.b] != 1) return;
+    __syncthreads();                           // the barriers are there
   }
-  auto piece = [&](Walk& w, bool again) {
-    if (SPLIT) return w.next(pre, a.KV);
-    w.b = blockIdx.y; w.kvh = blockIdx.x; w.t0 = 0;
-    w.t1 = w.n = Span(a.len(w.b), a.window, a.first).n;
+  auto piece = [&](bool again) {
+    if (SPLIT) return cons.next(pre, a.KV);
+    cons.kvh = blockIdx.x; cons.t0 = 0;
+    cons.t1 = cons.n = Span(a.len(cons.b), a.window, a.first).n;
     return !again;
   };
-  prod = cons;
-
-  // ---- the ring: lane 0 (and lane 1, where a tile lies in two blocks) asks for this warp's next tile, whose block id it read a tile before
-  const bool two = a.bs_shift == 4;
-  bool p_more = piece(prod, false);
-  int p_tile = p_more ? prod.t0 + warp : 0, p_stage = 0, p_key0 = 0, p_blk = 0;
-  Span p_span(p_more ? a.len(prod.b) : 0, a.window, a.first);
-  auto settle = [&]() {                        // p_tile is this warp's next tile, in this piece or a later one
-    while (p_more && p_tile >= prod.t1) {
-      p_more = piece(prod, true);
-      if (p_more) { p_tile = prod.t0 + warp; p_span = Span(a.len(prod.b), a.window, a.first); }
-    }
-    p_key0 = p_span.key0(p_tile);
-    const int key = p_key0 + lane * 16;
-    if (p_more && lane < 2 && key < p_span.len) p_blk = a.table[(int64_t)prod.b * a.max_blocks + (key >> a.bs_shift)];
-  };
-  settle();
-  auto ask = [&]() {
-    if (!p_more) return;
-    const int groups = min(2, max(0, (p_span.len - p_key0 + 15) >> 4));
-    const uint32_t bar = bar0 + 8 * p_stage;
-    if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(groups * GB)) : "memory");
-    __syncwarp();
-    if (lane < (two ? groups : min(groups, 1)))
-      bulk_load(ring + (p_stage * 2 + lane) * GB,
-                a.cache + ((((int64_t)p_blk * a.KV + prod.kvh) << (a.bs_shift - 4)) + (((p_key0 + lane * 16) & ((1 << a.bs_shift) - 1)) >> 4)) * GB,
-                two ? GB : groups * GB, bar);
-    p_stage = p_stage + 1 == ST ? 0 : p_stage + 1;
-    p_tile += NW;
-    settle();
-  };
-#pragma unroll 1
-  for (int s = 0; s < ST; ++s) ask();
-
   int stage = 0;
   uint32_t parity = 0;
-  for (bool more = piece(cons, false); more; more = piece(cons, true)) {
+  auto advance = [&]() { if (++stage == ST) { stage = 0; parity ^= 1; } };
+
+  if (warp == NW) {
+    // ---- the producer: a lane per block of a tile; the ids of the next tile are read while this one's stage is waited for
+    const int bs = 1 << a.bs_shift, box = min(bs, TK);
+    const uint32_t ring = s_addr(smem);
+    bool refill = false;
+    for (bool more = piece(false); more; more = piece(true)) {
+      const Span sp(a.len(cons.b), a.window, a.first);
+      const int32_t* btab = a.table + (int64_t)cons.b * a.max_blocks;
+      // of this lane's block: the keys from `lo` to `hi` that somebody may see (all in one copy), and the block's id
+      int lo = 0, hi = 0, blk = 0;
+      auto look = [&](int tile) {
+        const int k0 = sp.key0(tile) + lane * box;
+        lo = a.first > k0 ? k0 : max(k0, sp.lo & ~15);
+        hi = min(k0 + box, sp.len);
+        if (sp.lo >= hi) hi = min(hi, a.first);
+        if (tile >= cons.t1 || lane * box >= TK) hi = lo;
+        if (lo < hi) blk = btab[lo >> a.bs_shift];
+      };
+      look(cons.t0);
+      for (int tile = cons.t0; tile < cons.t1; ++tile) {
+        const int first = lo & ~15, groups = lo < hi ? (hi - first + 15) >> 4 : 0, id = blk;
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, (uint32_t)groups) * GB, place = (uint32_t)(first - sp.key0(tile)) >> 4;
+        look(tile + 1);
+        if (refill) mbar_wait(empty(stage), parity ^ 1);
+        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(stage)), "r"(bytes) : "memory");
+        __syncwarp();
+        if (groups > 0)
+          bulk_load(ring + (stage * GROUPS + place) * GB, a.cache + ((((int64_t)id * a.KV + cons.kvh) << (a.bs_shift - 4)) + ((first & (bs - 1)) >> 4)) * GB, groups * GB, full(stage));
+        advance();
+        if (stage == 0) refill = true;
+      }
+    }
+    return;
+  }
+
+  for (bool more = piece(false); more; more = piece(true)) {
     const Span sp(a.len(cons.b), a.window, a.first);
     const int qrow = a.qsl[cons.b];
     // ---- the group's query heads: column n of block nt is head 8 nt + n
@@ -261,10 +275,15 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
       for (int h = 0; h < 2; ++h) { ref[nt][h] = l[nt][h] = zs[nt][h] = ws[nt][h] = ws[nt][2 + h] = 0.f; }
 
     bool fresh = true;                         // the first tile sets the references
-    for (int tile = cons.t0 + warp; tile < cons.t1; tile += NW) {
-      const int key0 = sp.key0(tile);
-      mbar_wait(bar0 + 8 * stage, parity);
-      const uint8_t* base = smem + (warp * ST + stage) * 2 * GB;
+    for (int tile = cons.t0; tile < cons.t1; ++tile) {
+      const int key0 = sp.key0(tile) + warp * WK;
+      mbar_wait(full(stage), parity);
+      if (key0 >= sp.len || (key0 + WK <= sp.lo && key0 >= a.first)) {        // nobody sees these keys
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty(stage)) : "memory");
+        advance();
+        continue;
+      }
+      const uint8_t* base = smem + (stage * GROUPS + warp * 2) * GB;
       // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
       float x[2][NT][4], zv[2][2], sv[2][2];
 #pragma unroll
@@ -306,7 +325,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
             for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
         }
       }
-      if (key0 + TK > sp.len || (key0 < sp.lo && key0 + TK > a.first)) {      // the same for the warp
+      if (key0 + WK > sp.len || (key0 < sp.lo && key0 + WK > a.first)) {      // the same for the warp
         const int mine = key0 + kv4::key_token(g);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -412,8 +431,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
         }
       }
       __syncwarp();                                      // the stage is read
-      ask();
-      if (++stage == ST) { stage = 0; parity ^= 1; }
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty(stage)) : "memory");
+      advance();
     }
 
     // ---- the warps' (ref, l, out) of the piece, four heads at a time
@@ -434,7 +453,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
       for (int half = 0; half < 2; ++half) {             // heads 8 nt + 4 half .. + 3: threads t = 2 half and 2 half + 1 of a quad
         const int r0 = 8 * nt + 4 * half;
         if (r0 >= G) continue;
-        __syncthreads();                                 // the pass before is read
+        bar_compute();                                   // the pass before is read
         if ((t >> 1) == half)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -446,7 +465,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) attn_kv4_kernel(const Args a, i
                                                                                    fmaf(o[i + 1][nt][h], 1048576.f, rest), fmaf(o[i + 1][nt][2 + h], 1048576.f, rest));
             if (g == 0) { dst[HD] = fresh ? kNoRef : ref[nt][h]; dst[HD + 1] = l[nt][h]; }      // (a warp without a tile)
           }
-        __syncthreads();
+        bar_compute();
         for (int it = tid; it < HD; it += NW * 32) {     // (row, 4 dimensions)
           const int r = it / (HD / 4), c = it % (HD / 4);
           if (r0 + r >= G) break;
@@ -520,18 +539,18 @@ constexpr int kMaxRequests = 1024;             // requests of one launch (their 
 template <int HD, int NT>
 static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
   const int max_tiles = (max_seq_len + TK - 1) / TK;
-  const int fixed = ring_bytes<HD>() + red_floats<HD>() * 4 + NW * ST * 8;
-  if (max_tiles <= 16) {
+  const int fixed = ring_bytes<HD, NT>() + red_floats<HD>() * 4 + 2 * stages(NT) * 8, ctas = 148 * ctas_per_sm(NT);
+  if (max_tiles <= 4) {
     auto kern = attn_kv4_kernel<HD, NT, false>;
     KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed));
-    KGE_CUDA_OK(launch_pdl(kern, dim3(a.KV, a.B), dim3(NW * 32), fixed, st, a, 0));
+    KGE_CUDA_OK(launch_pdl(kern, dim3(a.KV, a.B), dim3(kThreads), fixed, st, a, 0));
     return 0;
   }
   auto kern = attn_kv4_kernel<HD, NT, true>;
   const int smem = fixed + (a.B + 1) * 4;
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + (kMaxRequests + 1) * 4));
-  KGE_CUDA_OK(launch_pdl(kern, dim3(kMaxCtas), dim3(NW * 32), smem, st, a, NW));
-  KGE_CUDA_OK(launch_pdl(attn_kv4_merge_kernel<HD>, dim3(kMaxCtas, a.H / a.KV), dim3(HD), 0, st, a.out, (const float*)a.part, (const int4*)a.desc, a.H, a.H / a.KV));
+  KGE_CUDA_OK(launch_pdl(kern, dim3(ctas), dim3(kThreads), smem, st, a, 1));
+  KGE_CUDA_OK(launch_pdl(attn_kv4_merge_kernel<HD>, dim3(ctas, a.H / a.KV), dim3(HD), 0, st, a.out, (const float*)a.part, (const int4*)a.desc, a.H, a.H / a.KV));
   return 0;
 }
 
