@@ -4,9 +4,9 @@
 //   score = scale (s_k (q . n_k) + low_k sum(q))           out = (sum_j (p_j s_v,j) (n_v,j - 8) + sum_j p_j z_v,j) / sum_j p_j
 // so the products run on codes, which 16 bits hold exactly, and the two numbers of a row are applied to scores and weights in fp32.
 //
-// Four warps take 32 keys each of tiles of 128, which a fifth brings by bulk copies (one per block of a tile), and multiply with mma.m16n8k16
-// whose M side is the keys (scores) or the dimensions (outputs) and whose N side is the query heads of one kv head: 8 columns of which a group
-// of 4 or 8 heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
+// A warp takes 32 keys at a time (a unit) from a ring of its own, which its lane 0 fills by bulk copies, and multiplies with mma.m16n8k16 whose M
+// side is the keys (scores) or the dimensions (outputs) and whose N side is the query heads of one kv head: 8 columns of which a group of 4 or
+// 8 heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
 //   Codes: the bits n in the low half-byte of a float16 are the number n 2^-24 (its denormals), in the next one n 2^-20, so a code costs half an
 //   AND and no arithmetic; powers of two are put right in q (scores) and in the outputs.  (As 1024 + n less 1032: 2.6 instructions a pair.)
 //   q: a power of two moves the largest number of the group's heads to 2^14; exact but for what lies 2^-24 below that.
@@ -25,11 +25,11 @@ inline namespace KGE_ELT_NS {
 
 namespace ak4 {
 
-constexpr int NW = 4, TK = 128, WK = TK / NW, GROUPS = TK / 16;      // computing warps, keys of a tile, of a warp; groups of a tile
-constexpr int kThreads = NW * 32 + 32;
-__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 3 : 4; }      // tiles on their way; CTAs of an SM
+constexpr int WK = 32, NW = 4, GROUPS = NW * WK / 16;       // keys of a unit, which a warp takes at a time; computing warps of a CTA; groups of a stage
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-constexpr int kMaxCtas = 148 * 3;
+__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 3 : 4; }
+__host__ __device__ constexpr int shares_of(int nt) { return 148 * ctas_per_sm(nt); }
+constexpr int kMaxShares = 148 * 3;
 constexpr float kLog2e = 1.4426950408889634f, kNoRef = -1e30f;
 constexpr float kExpRoom = 40.f;
 constexpr uint32_t kWeightMost = 0x7400;       // 2^14 in float16
@@ -39,8 +39,8 @@ struct Args {
   const bf16* q;
   const uint8_t* cache;
   const int32_t *table, *lens, *qsl;
-  float* part;                                 // partial outputs of the pieces: [2 per CTA][G][HD], then [2 per CTA][G] (R, l)
-  int4* desc;                                  // per CTA: the group that starts in its share and ends in a later one's (merge kernel)
+  float* part;                                 // outputs of the pieces of cut groups: [2 per share][G][HD], then [2 per share][G] (R, l)
+  int4* desc;                                  // per share: the group that begins in it and ends in a later one's: (row of q, kv head, last share, slot)
   int q_stride, max_blocks, B, H, KV, bs_shift, window, first;
   float scale_log2;
   __device__ __forceinline__ int len(int b) const { return min(max(lens[b], 0), max_blocks << bs_shift); }      // (no page beyond the table is read)
@@ -53,6 +53,18 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the same into fresh accumulators
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) { uint32_t v; asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at)); return v; }
+__device__ __forceinline__ uint2 lds64(uint32_t at) { uint2 v; asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at)); return v; }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
 }
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
   uint32_t r;
@@ -69,373 +81,226 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 // nibbles 0 and 4, or 1 and 5, of w as two float16 numbers: n 2^-24 and n 2^-20
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return w & 0x00f000f0u; }
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// The keys that a single-token request of `len` keys sees, in tiles of TK: the first ones that stay visible, then the window.
+// The keys that a single-token request of `len` keys sees, in units of WK: the first ones that stay visible, then the window.
 struct Span {
   int len, lo, npre, win0, n;
+  Span() = default;
   __device__ __forceinline__ Span(int kv_len, int window, int first) {
     len = kv_len;
     lo = window > 0 ? max(kv_len - window, 0) : 0;
-    win0 = lo / TK;
-    npre = min((min(first, lo) + TK - 1) / TK, win0);
-    n = kv_len > 0 ? npre + (kv_len + TK - 1) / TK - win0 : 1;        // (one empty tile writes the zeros of a request without keys)
+    win0 = lo / WK;
+    npre = min((min(first, lo) + WK - 1) / WK, win0);
+    n = kv_len > 0 ? npre + (kv_len + WK - 1) / WK - win0 : 1;        // (one empty unit writes the zeros of a request without keys)
   }
-  __device__ __forceinline__ int key0(int tile) const { return (tile < npre ? tile : win0 + tile - npre) * TK; }
+  __device__ __forceinline__ int key0(int unit) const { return (unit < npre ? unit : win0 + unit - npre) * WK; }
 };
-__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // the computing warps
+// One warp's work on one (request, kv head): the query heads as B operands, and what has been summed so far.  Column n of block nt is head
+// 8 nt + n; of the accumulators, thread (g, t) = (lane / 4, lane % 4) has columns 2 t and 2 t + 1.
+template <int HD, int NT>
+struct Core {
+  static constexpr int GB = kv4::group_bytes(HD), W = HD / 32, NM = HD / 16;      // W: words of a thread's share of a key row
+  uint32_t qb[NT][NM][2];
+  float qs[NT][2], fs;                         // scale log2(e) sum(q) of the two columns; what scores are multiplied with
+  float o[NM][NT][4], ws[NT][4];               // outputs; sums of the rounded weights, from a product with ones
+  float ref[NT][2], l[NT][2], zs[NT][2];
+  bool fresh;                                  // the first unit sets the references
 
-// A share of the launch's tiles, piece by piece: request-major, then kv head, then tile.
-struct Walk {
-  uint32_t u, u1;
-  int b, kvh, t0, t1, n;                       // the current piece: tiles t0 .. t1 of a group of n
-  __device__ __forceinline__ bool next(const uint32_t* pre, uint32_t KV) {
-    if (u >= u1) return false;
-    while (pre[b + 1] * KV <= u) ++b;
-    const uint32_t groups = pre[b + 1] - pre[b], rel = u - pre[b] * KV;
-    n = (int)groups;
-    kvh = (int)(rel / groups);
-    t0 = (int)(rel - kvh * groups);
-    t1 = (int)min(groups, t0 + (u1 - u));
-    u += t1 - t0;
-    return true;
-  }
-};
-
-template <int HD> __host__ __device__ constexpr int red_floats() { return NW * 4 * (HD + 4); }
-template <int HD, int NT> __host__ __device__ constexpr int ring_bytes() { return stages(NT) * GROUPS * kv4::group_bytes(HD); }
-
-// SPLIT: the tiles of all (request, kv head) groups are one sequence, every CTA takes an equal share of it, and a group that is cut is merged
-// by the kernel behind.  Otherwise a CTA has a whole group.
-template <int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_kv4_kernel(const Args a, int min_chunk) {
-  constexpr int GB = kv4::group_bytes(HD), W = HD / 32, NM = HD / 16, RS = HD + 4, ST = stages(NT);      // W: words of a thread's share of a key row
-  extern __shared__ __align__(128) uint8_t smem[];
-  float* red = reinterpret_cast<float*>(smem + ring_bytes<HD, NT>());
-  uint64_t* bars = reinterpret_cast<uint64_t*>(red + red_floats<HD>());
-  uint32_t* pre = reinterpret_cast<uint32_t*>(bars + 2 * ST);
-  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int G = a.H / a.KV;
-  const uint32_t bar0 = s_addr(bars);
-  // full(s): the producer's arrival and its copies' bytes; empty(s): the computing warps.  A wait for either comes before what the next
-  // phase of it needs: a warp arrives on empty(s) only behind its wait for full(s), and the producer refills s only behind empty(s).
-  auto full = [&](int s) { return bar0 + 8u * s; };
-  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
-  if (tid == 0) {
-    for (int s = 0; s < ST; ++s) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(full(s)));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty(s)), "n"(NW));
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  pdl_launch_dependents();
-  pdl_wait();
-
-  Walk cons;
-  uint32_t u0 = 0;
-  if (SPLIT) {
-    for (int b = tid; b < a.B; b += kThreads) pre[b + 1] = a.qsl[b + 1] - a.qsl[b] == 1 ? Span(a.len(b), a.window, a.first).n : 0;
-    if (tid == 0) pre[0] = 0;
-    __syncthreads();
-    if (warp == 0) {
-      const int per = (a.B + 31) / 32, lo = 1 + lane * per, hi = min(a.B + 1, lo + per);
-      uint32_t sum = 0;
-      for (int i = lo; i < hi; ++i) sum += pre[i];
-      uint32_t incl = sum;
+  __device__ __forceinline__ void start(const bf16* q, int G, float scale_log2, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    uint4 raw[NT][W];
+    float mx = 0.f;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d); if (lane >= d) incl += v; }
-      uint32_t run = incl - sum;
-      for (int i = lo; i < hi; ++i) { run += pre[i]; pre[i] = run; }
-    }
-    __syncthreads();
-    const uint32_t KV = a.KV, U = pre[a.B] * KV, chunk = max((U + gridDim.x - 1) / gridDim.x, (uint32_t)min_chunk);
-    auto request_of = [&](uint32_t unit) {
-      int lo = 0, hi = a.B - 1;
-      while (lo < hi) { const int mid = (lo + hi) >> 1; if (pre[mid + 1] * KV <= unit) lo = mid + 1; else hi = mid; }
-      return lo;
-    };
-    u0 = min(U, blockIdx.x * chunk);
-    cons.u = u0; cons.u1 = min(U, u0 + chunk); cons.b = u0 < cons.u1 ? request_of(u0) : 0;
-    if (tid == 0) {
-      // the group that begins in this share and ends beyond it
-      int4 d = make_int4(-1, 0, 0, 0);
-      if (u0 < cons.u1 && cons.u1 < U) {
-        const int b = request_of(cons.u1 - 1);
-        const uint32_t n = pre[b + 1] - pre[b], base = pre[b] * KV, kvh = (cons.u1 - 1 - base) / n, g0 = base + kvh * n, g1 = g0 + n;
-        if (g0 >= u0 && g1 > cons.u1) d = make_int4(a.qsl[b], (int)kvh, (int)((g1 - 1) / chunk), g0 > u0);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int head = nt * 8 + g;
+      const uint4* src = reinterpret_cast<const uint4*>(q + min(head, G - 1) * HD + t * (HD / 4));
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        raw[nt][i] = head < G ? src[i] : make_uint4(0, 0, 0, 0);
+        const uint32_t* u = &raw[nt][i].x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = bf_lo(u[k]), y = bf_hi(u[k]);
+          sum += x + y;
+          mx = fmaxf(mx, fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f));
+        }
       }
-      a.desc[blockIdx.x] = d;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      qs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t);
+      qs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
     }
-  } else {
-    cons.b = blockIdx.y;
-    if (a.qsl[cons.b + 1] - a.qsl[cons.b] != 1) return;
-    __syncthreads();                           // the barriers are there
-  }
-  auto piece = [&](bool again) {
-    if (SPLIT) return cons.next(pre, a.KV);
-    cons.kvh = blockIdx.x; cons.t0 = 0;
-    cons.t1 = cons.n = Span(a.len(cons.b), a.window, a.first).n;
-    return !again;
-  };
-  int stage = 0;
-  uint32_t parity = 0;
-  auto advance = [&]() { if (++stage == ST) { stage = 0; parity ^= 1; } };
-
-  if (warp == NW) {
-    // ---- the producer: a lane per block of a tile; the ids of the next tile are read while this one's stage is waited for
-    const int bs = 1 << a.bs_shift, box = min(bs, TK);
-    const uint32_t ring = s_addr(smem);
-    bool refill = false;
-    for (bool more = piece(false); more; more = piece(true)) {
-      const Span sp(a.len(cons.b), a.window, a.first);
-      const int32_t* btab = a.table + (int64_t)cons.b * a.max_blocks;
-      // of this lane's block: the keys from `lo` to `hi` that somebody may see (all in one copy), and the block's id
-      int lo = 0, hi = 0, blk = 0;
-      auto look = [&](int tile) {
-        const int k0 = sp.key0(tile) + lane * box;
-        lo = a.first > k0 ? k0 : max(k0, sp.lo & ~15);
-        hi = min(k0 + box, sp.len);
-        if (sp.lo >= hi) hi = min(hi, a.first);
-        if (tile >= cons.t1 || lane * box >= TK) hi = lo;
-        if (lo < hi) blk = btab[lo >> a.bs_shift];
-      };
-      look(cons.t0);
-      for (int tile = cons.t0; tile < cons.t1; ++tile) {
-        const int first = lo & ~15, groups = lo < hi ? (hi - first + 15) >> 4 : 0, id = blk;
-        const uint32_t bytes = __reduce_add_sync(0xffffffffu, (uint32_t)groups) * GB, place = (uint32_t)(first - sp.key0(tile)) >> 4;
-        look(tile + 1);
-        if (refill) mbar_wait(empty(stage), parity ^ 1);
-        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(stage)), "r"(bytes) : "memory");
-        __syncwarp();
-        if (groups > 0)
-          bulk_load(ring + (stage * GROUPS + place) * GB, a.cache + ((((int64_t)id * a.KV + cons.kvh) << (a.bs_shift - 4)) + ((first & (bs - 1)) >> 4)) * GB, groups * GB, full(stage));
-        advance();
-        if (stage == 0) refill = true;
+    // 2^e brings the largest finite number to 2^14 (e from -100 to 100); high nibbles count 16 times, so what they meet is q 2^(e - 4)
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+    const int e = top ? min(max(141 - (int)(top >> 23), -100), 100) : 0;
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23), up4 = __uint_as_float((uint32_t)(123 + e) << 23);
+    fs = scale_log2 * __uint_as_float((uint32_t)(151 - e) << 23);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const uint32_t* u = &raw[nt][i].x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) qb[nt][2 * i + (k >> 1)][k & 1] = pack_h2(bf_lo(u[k]) * (k & 1 ? up4 : up), bf_hi(u[k]) * (k & 1 ? up4 : up));
       }
+#pragma unroll
+      for (int i = 0; i < NM; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) ref[nt][h] = l[nt][h] = zs[nt][h] = ws[nt][h] = ws[nt][2 + h] = 0.f;
     }
-    return;
+    fresh = true;
   }
 
-  for (bool more = piece(false); more; more = piece(true)) {
-    const Span sp(a.len(cons.b), a.window, a.first);
-    const int qrow = a.qsl[cons.b];
-    // ---- the group's query heads: column n of block nt is head 8 nt + n
-    uint32_t qb[NT][NM][2];
-    float qs[NT][2], fs;                       // scale log2(e) sum(q) of this thread's two columns; what scores are multiplied with
-    {
-      uint4 raw[NT][W];
-      float mx = 0.f;
+  // A unit whose two groups lie at shared address `at`.  edge: some of its keys are not visible - those from `len` on, and those below `lo` but
+  // the first `first` ones.
+  __device__ __forceinline__ void unit(uint32_t at, int lane, bool edge, int key0, int len, int lo, int first) {
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t k_at = at + g * (HD / 2) + t * (HD / 8), n_at = at + 16 * HD + kv4::key_token(g) * 4;
+    // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
+    float x[2][NT][4], zv[2][2], sv[2][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int head = nt * 8 + g;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)qrow * a.q_stride + (cons.kvh * G + min(head, G - 1)) * HD + t * (HD / 4));
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          raw[nt][i] = head < G ? src[i] : make_uint4(0, 0, 0, 0);
-          const uint32_t* u = &raw[nt][i].x;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float x = bf_lo(u[k]), y = bf_hi(u[k]);
-            sum += x + y;
-            mx = fmaxf(mx, fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f));
-          }
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        qs[nt][0] = a.scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t);
-        qs[nt][1] = a.scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+    for (int i = 0; i < 2; ++i) {
+      uint32_t ka[W], kb[W];
+      if (HD == 128) {
+        const uint4 u = lds128(k_at + i * GB), v = lds128(k_at + i * GB + 512);
+        ka[0] = u.x; ka[1] = u.y; ka[W - 2] = u.z; ka[W - 1] = u.w;
+        kb[0] = v.x; kb[1] = v.y; kb[W - 2] = v.z; kb[W - 1] = v.w;
+      } else {
+        const uint2 u = lds64(k_at + i * GB), v = lds64(k_at + i * GB + 256);
+        ka[0] = u.x; ka[1] = u.y;
+        kb[0] = v.x; kb[1] = v.y;
       }
-      // 2^e brings the largest finite number to 2^14 (e from -100 to 100); high nibbles count 16 times, so what they meet is q 2^(e - 4)
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-      const int e = top ? min(max(141 - (int)(top >> 23), -100), 100) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23), up4 = __uint_as_float((uint32_t)(123 + e) << 23);
-      fs = a.scale_log2 * __uint_as_float((uint32_t)(151 - e) << 23);
+      float c[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < W; ++j) {
+        const uint32_t a0 = ka[j], b0 = kb[j], a1 = a0 >> 8, b1 = b0 >> 8;
+        const uint32_t f0[4] = {codes_lo(a0), codes_lo(b0), codes_hi(a0), codes_hi(b0)}, f1[4] = {codes_lo(a1), codes_lo(b1), codes_hi(a1), codes_hi(b1)};
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const uint32_t* u = &raw[nt][i].x;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) qb[nt][2 * i + (k >> 1)][k & 1] = pack_h2(bf_lo(u[k]) * (k & 1 ? up4 : up), bf_hi(u[k]) * (k & 1 ? up4 : up));
-        }
-    }
-    float o[NM][NT][4], ws[NT][4], ref[NT][2], l[NT][2], zs[NT][2];      // ws: sums of the rounded weights, from a product with ones
-#pragma unroll
-    for (int i = 0; i < NM; ++i)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) { ref[nt][h] = l[nt][h] = zs[nt][h] = ws[nt][h] = ws[nt][2 + h] = 0.f; }
-
-    bool fresh = true;                         // the first tile sets the references
-    for (int tile = cons.t0; tile < cons.t1; ++tile) {
-      const int key0 = sp.key0(tile) + warp * WK;
-      mbar_wait(full(stage), parity);
-      if (key0 >= sp.len || (key0 + WK <= sp.lo && key0 >= a.first)) {        // nobody sees these keys
-        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty(stage)) : "memory");
-        advance();
-        continue;
-      }
-      const uint8_t* base = smem + (stage * GROUPS + warp * 2) * GB;
-      // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
-      float x[2][NT][4], zv[2][2], sv[2][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint8_t* grp = base + i * GB;
-        uint32_t ka[W], kb[W];
-        if (HD == 128) {
-          const uint4 u = *reinterpret_cast<const uint4*>(grp + g * 64 + t * 16), v = *reinterpret_cast<const uint4*>(grp + 512 + g * 64 + t * 16);
-          ka[0] = u.x; ka[1] = u.y; ka[W - 2] = u.z; ka[W - 1] = u.w;
-          kb[0] = v.x; kb[1] = v.y; kb[W - 2] = v.z; kb[W - 1] = v.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(grp + g * 32 + t * 8), v = *reinterpret_cast<const uint2*>(grp + 256 + g * 32 + t * 8);
-          ka[0] = u.x; ka[1] = u.y;
-          kb[0] = v.x; kb[1] = v.y;
-        }
-        float c[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t a0 = ka[j], b0 = kb[j], a1 = a0 >> 8, b1 = b0 >> 8;
-          const uint32_t f0[4] = {codes_lo(a0), codes_lo(b0), codes_hi(a0), codes_hi(b0)}, f1[4] = {codes_lo(a1), codes_lo(b1), codes_hi(a1), codes_hi(b1)};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(c[nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
-            mma_f16(c[nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
-          }
-        }
-        const uint32_t* par = reinterpret_cast<const uint32_t*>(grp + 16 * HD) + kv4::key_token(g);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint32_t pk = par[8 * r], pv = par[16 + 8 * r];
-          const float lk = bf_hi(pk), f = fs * bf_lo(pk);
-          sv[i][r] = bf_lo(pv);
-          zv[i][r] = fmaf(8.f, sv[i][r], bf_hi(pv));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
+        for (int nt = 0; nt < NT; ++nt) {
+          if (j == 0) mma_f16_first(c[nt], f0, qb[nt][0][0], qb[nt][0][1]);
+          else mma_f16(c[nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+          mma_f16(c[nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
         }
       }
-      if (key0 + WK > sp.len || (key0 < sp.lo && key0 + WK > a.first)) {      // the same for the warp
-        const int mine = key0 + kv4::key_token(g);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int key = mine + 16 * i + 8 * r;
-            if (!(key < sp.len && (key >= sp.lo || key < a.first))) {         // its numbers may be anything
-              sv[i][r] = zv[i][r] = 0.f;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) x[i][nt][2 * r] = x[i][nt][2 * r + 1] = -INFINITY;
-            }
-          }
-      }
-      // ---- weights
-      uint32_t w[2][NT][2];
-      float e[2][NT][4];
-      auto weigh = [&]() {                     // false: a weight has passed its bound (or is NaN)
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              e[i][nt][2 * r] = ex2(x[i][nt][2 * r]);
-              e[i][nt][2 * r + 1] = ex2(x[i][nt][2 * r + 1]);
-              w[i][nt][r] = pack_h2(e[i][nt][2 * r] * sv[i][r], e[i][nt][2 * r + 1] * sv[i][r]);
-              most = max_u16x2(most, w[i][nt][r]);
-            }
-        return most < (kWeightMost << 16) && (most & 0xffffu) < kWeightMost;
-      };
-      const bool fits = weigh();
-      if (fresh || !__all_sync(0xffffffffu, fits)) {
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t pk = lds32(n_at + i * GB + 32 * r), pv = lds32(n_at + i * GB + 64 + 32 * r);
+        const float lk = bf_hi(pk), f = fs * bf_lo(pk);
+        sv[i][r] = bf_lo(pv);
+        zv[i][r] = fmaf(8.f, sv[i][r], bf_hi(pv));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top = fresh ? -INFINITY : 0.f;                              // how far the reference goes up (the first: or down)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) top = fmaxf(top, fmaxf(x[i][nt][2 * r + h] + lg2(sv[i][r]), x[i][nt][2 * r + h] - kExpRoom));
-#pragma unroll
-            for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-            if (top == -INFINITY) top = 0.f;                                  // (only NaN rows)
-            const float f = ex2(-top);
-            ref[nt][h] += top;
-            l[nt][h] *= f;
-            zs[nt][h] *= f;
-            ws[nt][h] *= f;
-#pragma unroll
-            for (int i = 0; i < NM; ++i) { o[i][nt][h] *= f; o[i][nt][2 + h] *= f; }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] -= top;
-          }
-        weigh();
-        fresh = false;
+          for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
       }
-      uint32_t pb[2][NT][2];
+    }
+    if (edge) {                                // the same for the warp
+      const int mine = key0 + kv4::key_token(g);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int key = mine + 16 * i + 8 * r;
+          if (!(key < len && (key >= lo || key < first))) {       // its numbers may be anything
+            sv[i][r] = zv[i][r] = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) x[i][nt][2 * r] = x[i][nt][2 * r + 1] = -INFINITY;
+          }
+        }
+    }
+    // ---- weights
+    uint32_t wt[2][NT][2];
+    float e[2][NT][4];
+    auto weigh = [&]() {                       // false: a weight has passed its bound (or is NaN)
+      uint32_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            e[i][nt][2 * r] = ex2(x[i][nt][2 * r]);
+            e[i][nt][2 * r + 1] = ex2(x[i][nt][2 * r + 1]);
+            wt[i][nt][r] = pack_h2(e[i][nt][2 * r] * sv[i][r], e[i][nt][2 * r + 1] * sv[i][r]);
+            most = max_u16x2(most, wt[i][nt][r]);
+          }
+      return most < (kWeightMost << 16) && (most & 0xffffu) < kWeightMost;
+    };
+    const bool fits = weigh();
+    if (fresh || !__all_sync(0xffffffffu, fits)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int h = 0; h < 2; ++h) {
+          float top = fresh ? -INFINITY : 0.f;                    // how far the reference goes up (the first: or down)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) { l[nt][h] += e[i][nt][2 * r + h]; zs[nt][h] = fmaf(e[i][nt][2 * r + h], zv[i][r], zs[nt][h]); }
-            pb[i][nt][r] = turn8x8(w[i][nt][r]);
-          }
-          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-          mma_f16(ws[nt], ones, pb[i][nt][0], pb[i][nt][1]);
+            for (int r = 0; r < 2; ++r) top = fmaxf(top, fmaxf(x[i][nt][2 * r + h] + lg2(sv[i][r]), x[i][nt][2 * r + h] - kExpRoom));
+#pragma unroll
+          for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+          if (top == -INFINITY) top = 0.f;                        // (only NaN rows)
+          const float f = ex2(-top);
+          ref[nt][h] += top;
+          l[nt][h] *= f;
+          zs[nt][h] *= f;
+          ws[nt][h] *= f;
+#pragma unroll
+          for (int i = 0; i < NM; ++i) { o[i][nt][h] *= f; o[i][nt][2 + h] *= f; }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] -= top;
         }
-      // ---- outputs: rows g and g + 8 of fragment 4 j + p are dimensions d = (HD / 8) g + 8 j + 2 p and d + 1; the keys of thread t are
-      // t, t + 4, t + 8, t + 12 of the group
+      weigh();
+      fresh = false;
+    }
+    uint32_t pb[2][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint8_t* val = base + i * GB + 8 * HD;
-        constexpr int VW = HD / 64;                      // words of a thread's share of a value row
-        uint32_t v[4][VW];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tok = t + 4 * k;
-          if (HD == 128) {
-            const uint2 u = *reinterpret_cast<const uint2*>(val + tok * 64 + ((g ^ ((t & 2) << 1)) << 3));      // value_word(): halves exchanged
-            v[k][0] = u.x; v[k][VW - 1] = u.y;
-          } else {
-            v[k][0] = *reinterpret_cast<const uint32_t*>(val + tok * 32 + g * 4);
-          }
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) { l[nt][h] += e[i][nt][2 * r + h]; zs[nt][h] = fmaf(e[i][nt][2 * r + h], zv[i][r], zs[nt][h]); }
+          pb[i][nt][r] = turn8x8(wt[i][nt][r]);
         }
-#pragma unroll
-        for (int j = 0; j < VW; ++j) {
-          const uint32_t xa = __byte_perm(v[0][j], v[1][j], 0x5410), ya = __byte_perm(v[0][j], v[1][j], 0x7632);
-          const uint32_t xb = __byte_perm(v[2][j], v[3][j], 0x5410), yb = __byte_perm(v[2][j], v[3][j], 0x7632);
-          const uint32_t xa8 = xa >> 8, ya8 = ya >> 8, xb8 = xb >> 8, yb8 = yb >> 8;
-          const uint32_t f[4][4] = {{codes_lo(xa), codes_lo(ya), codes_lo(xb), codes_lo(yb)}, {codes_hi(xa), codes_hi(ya), codes_hi(xb), codes_hi(yb)},
-                                    {codes_lo(xa8), codes_lo(ya8), codes_lo(xb8), codes_lo(yb8)}, {codes_hi(xa8), codes_hi(ya8), codes_hi(xb8), codes_hi(yb8)}};
-#pragma unroll
-          for (int p = 0; p < 4; ++p)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[4 * j + p][nt], f[p], pb[i][nt][0], pb[i][nt][1]);
-        }
+        const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+        mma_f16(ws[nt], ones, pb[i][nt][0], pb[i][nt][1]);
       }
-      __syncwarp();                                      // the stage is read
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(empty(stage)) : "memory");
-      advance();
-    }
+    // ---- outputs: a transposing ldmatrix of 16-bit pieces (four codes each) hands a thread the pieces g of two keys, rows 2 t and 2 t + 1 of
+    // eight; rows are keys in the order of the scores' rows.  Matrices: pieces 8 q .. 8 q + 7 of the first and second eight keys, q = 2 m and
+    // 2 m + 1; kv4::value_word exchanges halves of rows.  Row g of fragment 4 m + p is dimension 64 m + 8 (g / 2) + 2 p + g % 2, row g + 8 is 32
+    // further.
+    const int tok = ((lane >> 4) << 3) | kv4::key_token(lane & 7), q0 = (lane >> 3) & 1;
+    const uint32_t v_at = at + 8 * HD + tok * (HD / 2) + (HD == 128 ? (q0 ^ (tok & 2)) * 16 : q0 * 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < HD / 64; ++m) {
+        uint32_t v[4];
+        ldsm_x4_trans(v, (v_at + i * GB) ^ (m * 32));
+        const uint32_t u[4] = {v[0] >> 8, v[1] >> 8, v[2] >> 8, v[3] >> 8};
+        const uint32_t f[4][4] = {{codes_lo(v[0]), codes_lo(v[1]), codes_lo(v[2]), codes_lo(v[3])}, {codes_hi(v[0]), codes_hi(v[1]), codes_hi(v[2]), codes_hi(v[3])},
+                                  {codes_lo(u[0]), codes_lo(u[1]), codes_lo(u[2]), codes_lo(u[3])}, {codes_hi(u[0]), codes_hi(u[1]), codes_hi(u[2]), codes_hi(u[3])}};
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[4 * m + p][nt], f[p], pb[i][nt][0], pb[i][nt][1]);
+      }
+  }
 
-    // ---- the warps' (ref, l, out) of the piece, four heads at a time
+  __device__ __forceinline__ void sums() {     // over the lanes of a column
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -445,112 +310,401 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) attn_kv4_kernel(con
           l[nt][h] += __shfl_xor_sync(0xffffffffu, l[nt][h], m);
           zs[nt][h] += __shfl_xor_sync(0xffffffffu, zs[nt][h], m);
         }
-    const bool whole = !SPLIT || (cons.t0 == 0 && cons.t1 == cons.n);
-    const int slot = SPLIT ? 2 * (int)blockIdx.x + (cons.u - (cons.t1 - cons.t0) == u0 ? 0 : 1) : 0;
+  }
+  // Eight dimensions from dim(m) on of this thread's column h of block nt; the lanes of g and g ^ 1 exchange what the other's eight have.  Low
+  // nibbles (p even) count 2^24, high ones 2^20.
+  static __device__ __forceinline__ int dim(int m, int lane) { return 64 * m + 32 * ((lane >> 2) & 1) + 8 * (lane >> 3); }
+  __device__ __forceinline__ void rows(int nt, int h, int m, int lane, float (&v)[8]) const {
+    const float rest = fmaf(-8.f, ws[nt][h], zs[nt][h]);
+    const bool odd = lane & 4;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int p = 0; p < 4; ++p) {
+      const float up = p & 1 ? 1048576.f : 16777216.f, near = fmaf(o[4 * m + p][nt][h], up, rest), far = fmaf(o[4 * m + p][nt][2 + h], up, rest);
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? near : far, 4);
+      v[2 * p] = odd ? got : near;
+      v[2 * p + 1] = odd ? far : got;
+    }
+  }
+};
+
+__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // the computing warps
+template <int HD> __host__ __device__ constexpr int red_floats() { return NW * 4 * (HD + 4); }
+
+// The four warps' sums of one (request, kv head) in shared memory, four heads at a time: write(row, first of four dimensions, reference, sum, values)
+template <int HD, int NT, typename F>
+__device__ __forceinline__ void combine(Core<HD, NT>& core, float* red, int warp, int lane, int G, F write) {
+  constexpr int RS = HD + 4, NV = HD / 64;
+  const int t = lane & 3;
+  core.sums();
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {             // heads 8 nt + 4 half .. + 3: threads t = 2 half and 2 half + 1 of a quad
-        const int r0 = 8 * nt + 4 * half;
-        if (r0 >= G) continue;
-        bar_compute();                                   // the pass before is read
-        if ((t >> 1) == half)
+  for (int nt = 0; nt < NT; ++nt) {
+    if (8 * nt >= G) break;
+    float v[2][NV][8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float* dst = red + (warp * 4 + 2 * (t & 1) + h) * RS;
-            const float rest = fmaf(-8.f, ws[nt][h], zs[nt][h]);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < NM; i += 2)              // fragments of low nibbles (even) and of high ones
-              *reinterpret_cast<float4*>(dst + g * (HD / 8) + 2 * i) = make_float4(fmaf(o[i][nt][h], 16777216.f, rest), fmaf(o[i][nt][2 + h], 16777216.f, rest),
-                                                                                   fmaf(o[i + 1][nt][h], 1048576.f, rest), fmaf(o[i + 1][nt][2 + h], 1048576.f, rest));
-            if (g == 0) { dst[HD] = fresh ? kNoRef : ref[nt][h]; dst[HD + 1] = l[nt][h]; }      // (a warp without a tile)
+      for (int m = 0; m < NV; ++m) core.rows(nt, h, m, lane, v[h][m]);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {               // heads 8 nt + 4 half .. + 3: threads t = 2 half and 2 half + 1 of a quad
+      const int r0 = 8 * nt + 4 * half;
+      if (r0 >= G) break;
+      bar_compute();                                     // what was there is read
+      if ((t >> 1) == half)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float* dst = red + (warp * 4 + 2 * (t & 1) + h) * RS;
+#pragma unroll
+          for (int m = 0; m < NV; ++m) {
+            float4* at = reinterpret_cast<float4*>(dst + core.dim(m, lane));
+            at[0] = make_float4(v[h][m][0], v[h][m][1], v[h][m][2], v[h][m][3]);
+            at[1] = make_float4(v[h][m][4], v[h][m][5], v[h][m][6], v[h][m][7]);
           }
-        bar_compute();
-        for (int it = tid; it < HD; it += NW * 32) {     // (row, 4 dimensions)
-          const int r = it / (HD / 4), c = it % (HD / 4);
-          if (r0 + r >= G) break;
-          float mm = kNoRef;
-#pragma unroll
-          for (int w2 = 0; w2 < NW; ++w2) mm = fmaxf(mm, red[(w2 * 4 + r) * RS + HD]);
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float ll = 0.f;
-#pragma unroll
-          for (int w2 = 0; w2 < NW; ++w2) {
-            const float* src = red + (w2 * 4 + r) * RS;
-            const float f = ex2(src[HD] - mm);
-            const float4 v = *reinterpret_cast<const float4*>(src + 4 * c);
-            acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-            ll = fmaf(f, src[HD + 1], ll);
-          }
-          if (whole) {
-            const float inv = ll != 0.f ? 1.f / ll : 0.f;
-            *reinterpret_cast<uint2*>(a.out + ((int64_t)qrow * a.H + cons.kvh * G + r0 + r) * HD + 4 * c) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
-          } else {
-            const int64_t row = (int64_t)slot * G + r0 + r;
-            *reinterpret_cast<float4*>(a.part + row * HD + 4 * c) = acc;
-            if (c == 0) *reinterpret_cast<float2*>(a.part + (int64_t)2 * kMaxCtas * G * HD + row * 2) = make_float2(mm, ll);
-          }
+          if (lane < 4) { dst[HD] = core.fresh ? kNoRef : core.ref[nt][h]; dst[HD + 1] = core.l[nt][h]; }      // (a warp without a unit)
         }
+      bar_compute();
+      for (int it = warp * 32 + lane; it < HD; it += NW * 32) {       // (row, 4 dimensions)
+        const int r = it / (HD / 4), c = it % (HD / 4);
+        if (r0 + r >= G) break;
+        float mm = kNoRef;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, red[(w * 4 + r) * RS + HD]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float* src = red + (w * 4 + r) * RS;
+          const float f = ex2(src[HD] - mm);
+          const float4 u = *reinterpret_cast<const float4*>(src + 4 * c);
+          acc.x = fmaf(f, u.x, acc.x); acc.y = fmaf(f, u.y, acc.y); acc.z = fmaf(f, u.z, acc.z); acc.w = fmaf(f, u.w, acc.w);
+          ll = fmaf(f, src[HD + 1], ll);
+        }
+        write(r0 + r, 4 * c, mm, ll, acc);
       }
+    }
   }
 }
+__device__ __forceinline__ uint2 divided(float4 v, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  return make_uint2(pack_bf2(v.x * inv, v.y * inv), pack_bf2(v.z * inv, v.w * inv));
+}
 
-// The groups that were cut: block (c, head) merges the pieces of the group that begins in the share of CTA c, in the order of the shares.
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// `groups` groups of one block from `key` on
 template <int HD>
-__global__ void __launch_bounds__(HD) attn_kv4_merge_kernel(bf16* __restrict__ out, const float* __restrict__ part, const int4* __restrict__ desc, int H, int G) {
+__device__ __forceinline__ void copy_groups(const Args& a, uint32_t dst, int blk, int kvh, int key, int groups, uint32_t bar) {
+  bulk_load(dst, a.cache + ((((int64_t)blk * a.KV + kvh) << (a.bs_shift - 4)) + ((key & ((1 << a.bs_shift) - 1)) >> 4)) * kv4::group_bytes(HD), groups * kv4::group_bytes(HD), bar);
+}
+
+// ---- short contexts: a CTA per (request, kv head), its warps take every fourth unit.  A warp fills a ring of its own: lane 0 (and lane 1, where a
+// unit lies in two blocks) asks for a unit, and asks again in a stage that the warp itself has read, so there is nothing else to wait for.
+template <int HD, int NT>
+__global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(const Args a) {
+  constexpr int ST = 3, GB = kv4::group_bytes(HD);
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const uint32_t ring = s_addr(smem) + warp * ST * 2 * GB, bars = s_addr(smem) + NW * ST * 2 * GB + warp * ST * 8;
+  if (lane == 0)
+    for (int s = 0; s < ST; ++s) mbar_init(bars + 8 * s, 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float4 sh[4][HD / 4];
-  __shared__ float sl[4];
-  const int4 d = desc[blockIdx.x];
-  if (d.x < 0) return;
-  const int c = blockIdx.x, r = blockIdx.y, n = d.z - c + 1, lane = threadIdx.x % (HD / 4), q = threadIdx.x / (HD / 4);      // four streams of pieces
-  const float* ml = part + (int64_t)2 * kMaxCtas * G * HD;
-  auto row = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0 ? d.w : 0)) * G + r; };
-  float mm = kNoRef;
-  for (int i = 0; i < n; ++i) mm = fmaxf(mm, ml[row(i) * 2]);
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float ll = 0.f;
-#pragma unroll 4
-  for (int i = q; i < n; i += 4) {
-    const float2 p = *reinterpret_cast<const float2*>(ml + row(i) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(part + row(i) * HD + 4 * lane);
-    const float f = ex2(p.x - mm);
-    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-    ll = fmaf(f, p.y, ll);
+  const int b = blockIdx.y, kvh = blockIdx.x, G = a.H / a.KV;
+  const int qrow = a.qsl[b];
+  if (a.qsl[b + 1] - qrow != 1) return;
+  const Span sp(a.len(b), a.window, a.first);
+  const bool two = a.bs_shift == 4;
+  auto block_of = [&](int u) {
+    const int key = sp.key0(u) + lane * 16;
+    return u < sp.n && lane < 2 && key < sp.len ? a.table[(int64_t)b * a.max_blocks + (key >> a.bs_shift)] : 0;
+  };
+  auto ask = [&](int u, int stage, int blk) {
+    if (u >= sp.n) return;
+    const int key0 = sp.key0(u), groups = min(2, (sp.len - key0 + 15) >> 4);
+    if (lane == 0) mbar_expect(bars + 8 * stage, (uint32_t)(groups * GB));
+    __syncwarp();
+    if (lane < (two ? groups : min(groups, 1))) copy_groups<HD>(a, ring + (stage * 2 + lane) * GB, blk, kvh, key0 + lane * 16, two ? 1 : groups, bars + 8 * stage);
+  };
+  int blk[ST];
+#pragma unroll
+  for (int s = 0; s < ST; ++s) blk[s] = block_of(warp + s * NW);
+#pragma unroll
+  for (int s = 0; s < ST; ++s) ask(warp + s * NW, s, blk[s]);
+  Core<HD, NT> core;
+  core.start(a.q + (int64_t)qrow * a.q_stride + kvh * G * HD, G, a.scale_log2, lane);
+  int stage = 0;
+  uint32_t parity = 0;
+  for (int u = warp; u < sp.n; u += NW) {
+    const int key0 = sp.key0(u), next = block_of(u + ST * NW);
+    mbar_wait(bars + 8 * stage, parity);
+    if (sp.len > 0) core.unit(ring + stage * 2 * GB, lane, key0 + WK > sp.len || (key0 < sp.lo && key0 + WK > a.first), key0, sp.len, sp.lo, a.first);
+    __syncwarp();
+    ask(u + ST * NW, stage, next);
+    if (++stage == ST) { stage = 0; parity ^= 1; }
   }
-  sh[q][lane] = acc;
-  if (lane == 0) sl[q] = ll;
+  combine<HD, NT>(core, reinterpret_cast<float*>(smem), warp, lane, G, [&](int r, int d, float, float l, float4 v) {      // over the rings, which are read
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)qrow * a.H + kvh * G + r) * HD + d) = divided(v, l);
+  });
+}
+
+// ---- long contexts: the units of all (request, kv head) groups, request-major, are one sequence, of which every CTA takes an equal share in a
+// row.  A share covers the end of one group, whole groups and the start of another; whole groups go to the output, pieces to the workspace, and
+// the kernel behind merges them.  A producer warp finds the share's pieces and runs ahead of the computing warps, into the next piece while
+// they combine the last one's; what they need to know of a piece lies beside its query heads in shared memory.
+template <int HD, int NT> __host__ __device__ constexpr int q_bytes() { return 2 * NT * 8 * HD * 2; }
+template <int HD, int NT> __host__ __device__ constexpr int share_smem() {
+  return stages(NT) * GROUPS * kv4::group_bytes(HD) + q_bytes<HD, NT>() + red_floats<HD>() * 4 + 2 * 48 + (2 * stages(NT) + 4) * 8;
+}
+struct __align__(16) Piece { int t0, t1, row, kvh; Span span; int slot; int pad[2]; };      // t0 == t1: no more; slot: of the workspace, -1: a whole group
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_kernel(const Args a) {
+  constexpr int GB = kv4::group_bytes(HD), ST = stages(NT), STAGE = GROUPS * GB;
+  static_assert(sizeof(Piece) == 48, "as the launch counts");
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* sq = smem + ST * STAGE;                       // query heads of a piece, two buffers
+  float* red = reinterpret_cast<float*>(sq + q_bytes<HD, NT>());
+  Piece* pieces = reinterpret_cast<Piece*>(red + red_floats<HD>());
+  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, G = a.H / a.KV;
+  const uint32_t ring = s_addr(smem), bar0 = s_addr(pieces + 2);
+  // full(s), p_full(i): the producer's arrival and its copies' bytes; empty(s), p_empty(i): the computing warps.  A wait for one comes before
+  // what its next phase needs: a warp arrives on empty(s) only behind its wait for full(s), and the producer refills s only behind empty(s).
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (ST + s); };
+  auto p_full = [&](int i) { return bar0 + 8u * (2 * ST + i); };
+  auto p_empty = [&](int i) { return bar0 + 8u * (2 * ST + 2 + i); };
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), NW); }
+    for (int i = 0; i < 2; ++i) { mbar_init(p_full(i), 1); mbar_init(p_empty(i), NW); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   __syncthreads();
-  if (q == 0) {
-    for (int k = 1; k < 4; ++k) {
-      const float4 v = sh[k][lane];
-      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-      ll += sl[k];
+  pdl_launch_dependents();
+  pdl_wait();
+  int stage = 0, pi = 0;
+  uint32_t parity = 0, p_parity = 0;
+
+  if (warp == NW) {
+    // ---- the producer: all units, then the request that holds this share's first
+    auto units_of = [&](int b) { return a.qsl[b + 1] - a.qsl[b] == 1 ? (uint32_t)Span(a.len(b), a.window, a.first).n : 0u; };
+    uint32_t sum = 0;
+    for (int b = lane; b < a.B; b += 32) sum += units_of(b);
+    const uint32_t U = __reduce_add_sync(0xffffffffu, sum) * a.KV, chunk = max((U + gridDim.x - 1) / gridDim.x, (uint32_t)NW), u0 = min(U, blockIdx.x * chunk);
+    const uint32_t all = min(U, u0 + chunk) - u0;
+    uint32_t left = all, before = 0;
+    int b = 0, n = 0, kvh = 0, t0 = 0;                   // the current piece begins at unit t0 of the n of (b, kvh)
+    for (int b0 = 0; left; b0 += 32) {
+      const uint32_t mine = b0 + lane < a.B ? units_of(b0 + lane) : 0;
+      uint32_t incl = mine * a.KV;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) { const uint32_t v = __shfl_up_sync(0xffffffffu, incl, d); if (lane >= d) incl += v; }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + incl > u0);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = b0 + l;
+        n = (int)__shfl_sync(0xffffffffu, mine, l);
+        before += __shfl_sync(0xffffffffu, incl, l) - n * a.KV;
+        kvh = (int)((u0 - before) / n);
+        t0 = (int)(u0 - before) - kvh * n;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    *reinterpret_cast<uint2*>(out + ((int64_t)d.x * H + d.y * G + r) * HD + 4 * lane) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+    int4 desc = make_int4(-1, 0, 0, 0);
+    // a lane per unit of a stage (two lanes where blocks have 16 tokens); the block ids of the next stage are read while this one is waited for
+    const int unit = a.bs_shift == 4 ? lane >> 1 : lane, sub = a.bs_shift == 4 ? (lane & 1) * 16 : 0, box = a.bs_shift == 4 ? 16 : WK;
+    bool refill = false, refill_p = false;
+    while (left) {
+      const int t1 = (int)min((uint32_t)n, t0 + left), row = a.qsl[b];
+      const Span sp(a.len(b), a.window, a.first);
+      int key = 0, groups = 0, blk = 0;                  // this lane's copy of the next stage
+      auto look = [&](int u) {
+        key = sp.key0(u + unit) + sub;
+        groups = unit < NW && u + unit < t1 ? max(min(box, sp.len - key + 15), 0) >> 4 : 0;
+        if (groups) blk = a.table[(int64_t)b * a.max_blocks + (key >> a.bs_shift)];
+      };
+      look(t0);
+      if (refill_p) mbar_wait_idle(p_empty(pi), p_parity ^ 1);
+      if (lane == 0) {
+        Piece p;
+        p.t0 = t0; p.t1 = t1; p.row = row; p.kvh = kvh; p.span = sp;
+        p.slot = t0 == 0 && t1 == n ? -1 : 2 * (int)blockIdx.x + (t0 == 0);      // slot 0: the end or the middle of a group, slot 1: its start
+        pieces[pi] = p;
+        mbar_expect(p_full(pi), (uint32_t)(G * HD * 2));
+        bulk_load(s_addr(sq) + pi * (q_bytes<HD, NT>() / 2), a.q + (int64_t)row * a.q_stride + kvh * G * HD, (uint32_t)(G * HD * 2), p_full(pi));
+      }
+      pi ^= 1;
+      if (pi == 0) { p_parity ^= 1; refill_p = true; }
+      if (t0 == 0 && t1 < n) desc = make_int4(row, kvh, (int)((u0 + all - 1 + n - t1) / chunk), 0);      // (the share's last piece)
+      for (int u = t0; u < t1; u += NW) {
+        const int now = groups, id = blk, at = key;
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, (uint32_t)now) * GB;
+        look(u + NW);
+        if (refill) mbar_wait_idle(empty(stage), parity ^ 1);
+        if (lane == 0) mbar_expect(full(stage), bytes);
+        __syncwarp();
+        if (now) copy_groups<HD>(a, ring + stage * STAGE + (unit * 2 + (sub >> 4)) * GB, id, kvh, at, now, full(stage));
+        if (++stage == ST) { stage = 0; parity ^= 1; refill = true; }
+      }
+      left -= t1 - t0;
+      t0 = 0;
+      if (left && ++kvh == a.KV) {
+        kvh = 0;
+        do ++b; while ((n = (int)units_of(b)) == 0);
+      }
+    }
+    if (refill_p) mbar_wait_idle(p_empty(pi), p_parity ^ 1);
+    if (lane == 0) {
+      pieces[pi].t0 = pieces[pi].t1 = 0;
+      mbar_arrive(p_full(pi));
+      a.desc[blockIdx.x] = desc;
+    }
+    return;
+  }
+
+  const uint32_t own = ring + warp * 2 * GB;
+  while (true) {
+    mbar_wait(p_full(pi), p_parity);
+    const Piece p = pieces[pi];
+    if (p.t0 == p.t1) break;
+    Core<HD, NT> core;
+    core.start(reinterpret_cast<const bf16*>(sq + pi * (q_bytes<HD, NT>() / 2)), G, a.scale_log2, lane);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(p_empty(pi));
+    pi ^= 1;
+    if (pi == 0) p_parity ^= 1;
+    for (int u = p.t0; u < p.t1; u += NW) {
+      mbar_wait(full(stage), parity);
+      if (u + warp < p.t1 && p.span.len > 0) {
+        const int key0 = p.span.key0(u + warp);
+        core.unit(own + stage * STAGE, lane, key0 + WK > p.span.len || (key0 < p.span.lo && key0 + WK > a.first), key0, p.span.len, p.span.lo, a.first);
+      }
+      __syncwarp();                                      // the stage is read
+      if (lane == 0) mbar_arrive(empty(stage));
+      if (++stage == ST) { stage = 0; parity ^= 1; }
+    }
+    if (p.slot < 0) {
+      combine<HD, NT>(core, red, warp, lane, G, [&](int r, int d, float, float l, float4 v) {
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)p.row * a.H + p.kvh * G + r) * HD + d) = divided(v, l);
+      });
+    } else {
+      combine<HD, NT>(core, red, warp, lane, G, [&](int r, int d, float m, float l, float4 v) {
+        const int64_t at = (int64_t)p.slot * G + r;
+        *reinterpret_cast<float4*>(a.part + at * HD + d) = v;
+        if (d == 0) *reinterpret_cast<float2*>(a.part + (int64_t)2 * kMaxShares * G * HD + at * 2) = make_float2(m, l);
+      });
+    }
   }
 }
 
-constexpr int64_t workspace_bytes(int G, int hd) { return (int64_t)kMaxCtas * 16 + (int64_t)2 * kMaxCtas * G * (hd + 2) * 4; }
-constexpr int kMaxRequests = 1024;             // requests of one launch (their tile counts lie in shared memory)
+// Groups that were cut: warp (share, row) merges the pieces of the group that begins in the share, in the order of the shares; where there are
+// many, the whole block does, piece i by warp i mod 8.
+constexpr int MW = 8, kFewPieces = 12;
+template <int HD>
+__global__ void __launch_bounds__(MW * 32) attn_kv4_merge_kernel(bf16* __restrict__ out, const float* __restrict__ part, const int4* __restrict__ desc, int H, int G, int shares) {
+  constexpr int C = HD / 4;                    // lanes of a row (the others of a warp idle along)
+  __shared__ float4 sh[MW][C];
+  __shared__ float2 sl[MW];
+  __shared__ int4 sd[MW];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y, c = lane % C;
+  const float2* ml = reinterpret_cast<const float2*>(part + (int64_t)2 * kMaxShares * G * HD);
+  const int4 mine = blockIdx.x * MW + warp < shares ? desc[blockIdx.x * MW + warp] : make_int4(-1, 0, 0, 0);
+  // pieces first .. n - 1 of the group of d that begins in share s, by steps; a running reference and sum
+  auto merge = [&](int s, const int4& d, int first, int step, float& mm, float& ll, float4& acc) {
+    const int n = d.z - s + 1;
+    constexpr int AT_ONCE = 8;
+    for (int i0 = first; i0 < n; i0 += AT_ONCE * step) {
+      float2 p[AT_ONCE];
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int i = min(i0 + k * step, n - 1);
+        const int64_t row = (int64_t)(2 * (s + i) + (i == 0)) * G + r;      // slot 1 of the first share, slot 0 of the others
+        p[k] = ml[row];
+        v[k] = *reinterpret_cast<const float4*>(part + row * HD + 4 * c);
+      }
+      float m = mm;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (i0 + k * step < n) m = fmaxf(m, p[k].x);
+      const float old = ex2(mm - m);
+      mm = m;
+      acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old; ll *= old;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k)
+        if (i0 + k * step < n) {
+          const float f = ex2(p[k].x - m);
+          acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
+          ll = fmaf(f, p[k].y, ll);
+        }
+    }
+  };
+  auto write = [&](const int4& d, float ll, const float4& acc) {
+    const float inv = ll != 0.f ? 1.f / ll : 0.f;
+    *reinterpret_cast<uint2*>(out + ((int64_t)d.x * H + d.y * G + r) * HD + 4 * c) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+  };
+  const bool many = mine.x >= 0 && mine.z - (int)(blockIdx.x * MW + warp) >= kFewPieces;
+  if (mine.x >= 0 && !many) {
+    float mm = kNoRef, ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    merge(blockIdx.x * MW + warp, mine, 0, 1, mm, ll, acc);
+    if (lane < C) write(mine, ll, acc);
+  }
+  if (!__syncthreads_or(many)) return;
+  if (lane == 0) sd[warp] = many ? mine : make_int4(-1, 0, 0, 0);
+  __syncthreads();
+  for (int w = 0; w < MW; ++w) {
+    const int4 d = sd[w];
+    if (d.x < 0) continue;                     // (the same for the block)
+    float mm = kNoRef, ll = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    merge(blockIdx.x * MW + w, d, warp, MW, mm, ll, acc);
+    if (lane < C) sh[warp][c] = acc;
+    if (lane == 0) sl[warp] = make_float2(mm, ll);
+    __syncthreads();
+    if (warp == 0) {
+      float m = kNoRef;
+#pragma unroll
+      for (int k = 0; k < MW; ++k) m = fmaxf(m, sl[k].x);
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      ll = 0.f;
+#pragma unroll
+      for (int k = 0; k < MW; ++k) {
+        const float f = ex2(sl[k].x - m);
+        const float4 v = sh[k][c];
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+        ll = fmaf(f, sl[k].y, ll);
+      }
+      if (lane < C) write(d, ll, acc);
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kDescBytes = kMaxShares * 16;    // the workspace's start
+constexpr int64_t workspace_bytes(int G, int hd) { return kDescBytes + (int64_t)2 * kMaxShares * G * (hd + 2) * 4; }
+constexpr int kMaxRequests = 1024;             // requests of one launch (every warp reads their lengths)
 
 template <int HD, int NT>
 static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
-  const int max_tiles = (max_seq_len + TK - 1) / TK;
-  const int fixed = ring_bytes<HD, NT>() + red_floats<HD>() * 4 + 2 * stages(NT) * 8, ctas = 148 * ctas_per_sm(NT);
-  if (max_tiles <= 4) {
-    auto kern = attn_kv4_kernel<HD, NT, false>;
-    KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed));
-    KGE_CUDA_OK(launch_pdl(kern, dim3(a.KV, a.B), dim3(kThreads), fixed, st, a, 0));
+  if (max_seq_len <= 512) {
+    constexpr int ring = NW * 3 * 2 * kv4::group_bytes(HD) + NW * 3 * 8, smem = ring > red_floats<HD>() * 4 ? ring : red_floats<HD>() * 4;
+    auto kern = attn_kv4_kernel<HD, NT>;
+    KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    KGE_CUDA_OK(launch_pdl(kern, dim3(a.KV, a.B), dim3(NW * 32), smem, st, a));
     return 0;
   }
-  auto kern = attn_kv4_kernel<HD, NT, true>;
-  const int smem = fixed + (a.B + 1) * 4;
-  KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fixed + (kMaxRequests + 1) * 4));
-  KGE_CUDA_OK(launch_pdl(kern, dim3(ctas), dim3(kThreads), smem, st, a, 1));
-  KGE_CUDA_OK(launch_pdl(attn_kv4_merge_kernel<HD>, dim3(ctas, a.H / a.KV), dim3(HD), 0, st, a.out, (const float*)a.part, (const int4*)a.desc, a.H, a.H / a.KV));
+  auto kern = attn_kv4_share_kernel<HD, NT>;
+  const int G = a.H / a.KV, shares = shares_of(NT);
+  KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, share_smem<HD, NT>()));
+  KGE_CUDA_OK(launch_pdl(kern, dim3(shares), dim3(NW * 32 + 32), share_smem<HD, NT>(), st, a));
+  KGE_CUDA_OK(launch_pdl(attn_kv4_merge_kernel<HD>, dim3((shares + MW - 1) / MW, G), dim3(MW * 32), 0, st, a.out, (const float*)a.part, (const int4*)a.desc, a.H, G, shares));
   return 0;
 }
 
@@ -558,8 +712,8 @@ static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
 
 static int decode(ak4::Args a, int hd, int max_seq_len, cudaStream_t st) {
   const int B = a.B, G = a.H / a.KV;
-  // requests of a launch: what shared memory has room for, and tiles that 32 bits count (a table's row bounds a request's)
-  const int64_t tiles = ((((int64_t)a.max_blocks << a.bs_shift) + ak4::TK - 1) / ak4::TK + 1) * a.KV;
+  // requests of a launch: few enough to be read by every warp, and units that 32 bits count (a table's row bounds a request's)
+  const int64_t tiles = ((((int64_t)a.max_blocks << a.bs_shift) + ak4::WK - 1) / ak4::WK + 1) * a.KV;
   const int most = (int)std::max<int64_t>(1, std::min<int64_t>(ak4::kMaxRequests, ((1ll << 31) - 1) / tiles));
   for (int b0 = 0; b0 < B; b0 += most) {
     ak4::Args p = a;
@@ -619,7 +773,7 @@ extern "C" int KGE_API(kge_paged_attn_kv4)(void* out, const void* q, int q_strid
   ak4::Args a;
   a.out = (bf16*)out; a.q = (const bf16*)q; a.cache = (const uint8_t*)kv_cache;
   a.table = block_table; a.lens = seq_lens; a.qsl = query_start_loc;
-  a.desc = (int4*)workspace; a.part = (float*)((uint8_t*)workspace + (int64_t)ak4::kMaxCtas * 16);
+  a.desc = (int4*)workspace; a.part = (float*)((uint8_t*)workspace + ak4::kDescBytes);
   a.q_stride = q_stride; a.max_blocks = max_blocks_per_seq; a.B = B; a.H = H; a.KV = KV;
   a.bs_shift = 4;
   while ((1 << a.bs_shift) < block_size) ++a.bs_shift;

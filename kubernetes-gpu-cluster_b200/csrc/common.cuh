@@ -125,6 +125,16 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity) {
   while (!mbar_try(bar, parity))
     if (clock64() - t0 > kBarrierCycles) __trap();
 }
+// The same for a warp that runs ahead of others and only feeds them: every arrival wakes a waiter, and its tries take issue slots from those
+// that compute (a fifth of a decode attention's instructions), so it sleeps in between.
+__device__ __forceinline__ void mbar_wait_idle(uint32_t bar, uint32_t parity) {
+  if (mbar_try(bar, parity)) return;
+  const long long t0 = clock64();
+  do {
+    __nanosleep(100);
+    if (clock64() - t0 > kBarrierCycles) __trap();
+  } while (!mbar_try(bar, parity));
+}
 
 // Thread-block clusters.  A block's shared memory may be touched by its peers only once it is known to run: a kernel arrives
 // (relaxed: there is nothing to publish) at its start and waits before its first remote access, which its own work hides.
