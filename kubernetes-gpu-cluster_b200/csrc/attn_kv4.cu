@@ -691,9 +691,26 @@ constexpr int kDescBytes = kMaxShares * 16;    // the workspace's start
 constexpr int64_t workspace_bytes(int G, int hd) { return kDescBytes + (int64_t)2 * kMaxShares * G * (hd + 2) * 4; }
 constexpr int kMaxRequests = 1024;             // requests of one launch (every warp reads their lengths)
 
+// Which kernel.  A CTA per (request, kv head) has four CTAs an SM, which cover each other's starts and ends, and the hardware's queue; shares have
+// three, a producer and a merge behind them (4 us), but every SM has work whatever the lengths are.  us with a CTA each / with shares, 32 / 8
+// heads of 128:           1024 keys     1500         2048         2900         4096         6000
+//      8 requests (64 groups)  8.2 / 10.8  11.1 / 11.6  14.0 / 12.0  19.5 / 13.5  27.6 / 16.8  38.9 / 19.2
+//     48 (384)                19.0 / 20.2  24.9 / 24.8  31.1 / 28.8  41.4 / 36.3  55.3 / 45.3  78.4 / 60.5
+//     72 (576)                20.6 / 26.8  26.2 / 35.0  32.6 / 39.0  43.1 / 49.9  57.4 / 63.8  80.9 / 85.1
+//    100 (800)                27.4 / 32.6  36.1 / 40.7  45.7 / 49.1  61.4 / 63.3  82.4 / 82.9   117 / 115
+//    150 (1200)               37.7 / 43.9  50.2 / 55.8  64.2 / 68.2  87.4 / 89.4   118 / 118    170 / 168
+// so: up to 1024 keys, or six groups for every 32 keys; and up to 8192 keys, since one long context among many short ones is a single CTA's
+// work (0.35 us for 128 keys).
+static bool cta_each(int64_t groups, int keys) {
+  const int units = (keys + WK - 1) / WK;
+  return units <= 32 || (units <= 256 && groups >= 6 * units);
+}
+
 template <int HD, int NT>
 static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
-  if (max_seq_len <= 512) {
+  // a window leaves its own keys (from inside a unit on) and the first ones
+  const int keys = a.window > 0 ? (int)std::min<int64_t>(max_seq_len, (int64_t)a.window + a.first + 2 * WK) : max_seq_len;
+  if (cta_each((int64_t)a.B * a.KV, keys)) {
     constexpr int ring = NW * 3 * 2 * kv4::group_bytes(HD) + NW * 3 * 8, smem = ring > red_floats<HD>() * 4 ? ring : red_floats<HD>() * 4;
     auto kern = attn_kv4_kernel<HD, NT>;
     KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
