@@ -3,13 +3,16 @@
 // and probabilities in TMEM, work from the hardware's queue of CTAs not yet launched.
 //
 // What differs is how keys and values become operands.  A producer brings the groups of 64 keys as they lie in the pages (hd + 8 bytes a key, a
-// quarter of 16-bit rows) into a ring, and four warps of their own turn them into the 128-byte-swizzled 16-bit tiles that the MMAs read: a code n
-// becomes fma(n, s, low) in the model's type, the stored number rounded once (half a step; the weights P V multiplies it with are rounded
-// by as much).  64 keys are 16384 codes, 15 instructions for eight of them: 960 of the 5200 issue slots that a tile of two query tiles lasts.
-// The four warps need few registers and the softmax many: 512 threads start with 128 each, and setmaxnreg hands 40 of each of eight warps'
+// quarter of 16-bit rows) into a ring, and four warps of their own turn codes into the 128-byte-swizzled 16-bit tiles that the MMAs read: n - 8,
+// which is exact.  The two numbers of a row are applied in fp32 by the softmax, which has to read every score anyway:
+//   x = (s_k scale) (q . (n - 8)) + (z_k scale) sum(q)       e = 2^(x - R)       P = e s_v, rounded once       out = (P (n - 8) + sum e z_v) / sum e
+// with z = low + 8 s, so besides the result only P is rounded to 16 bits.  (Rows turned to numbers, fma(n, s, low) in 16 bits, round keys and values as
+// well: error against 64 bits 0.0029 for bfloat16 and 0.00041 for float16, where the result's own rounding is 0.0016 and 0.00021.)  R is the largest
+// x + log2 of the tile's largest s_v, so that P is at most 2^8 whatever the values' scale; it moves when it has grown by 2^8.
+// The turning warps need few registers and the softmax many: 512 threads start with 128 each, and setmaxnreg hands 40 of each of eight warps'
 // to the eight softmax warps (168 and 88: 128 (2 x 168 + 2 x 88) = 65536, what the launch holds).
-//   * Rows that read as NaN (kv4.cuh) must not reach queries that do not see them, and infinity or NaN times a weight of zero is none: such
-//     a key's values are zeros here and its key row is NaN, so every query that sees it gets NaN from its score and no other does.
+//   * Rows that read as NaN (kv4.cuh) must not reach queries that do not see them, and infinity or NaN times a weight of zero is none: such a
+//     key has s_v = z_v = 0 here and s_k is NaN, so every query that sees it gets NaN from its score and no other does.
 //   * Rows behind the last key are zeros, whatever the page held.
 //   * A window with first tokens that stay visible: tiles of the first tokens, then those of the windows; only tiles at a border are masked.
 namespace atc4 {
@@ -20,8 +23,9 @@ constexpr int kThreads = 512;                  // warps 0-3 and 4-7: softmax of 
 constexpr int NST = 3, NRAW = 3;               // K tiles and as many V tiles; tiles of codes
 constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "the register shares are what the launch holds");
+constexpr int kNumbers = 1024 + 16;            // of a stage: per pair of keys (s, s, z, z) of the keys and of the values; log2 of the largest s_v
 template <int HD> constexpr int raw_bytes() { return 4 * kv4::group_bytes(HD); }
-template <int HD> constexpr int smem_bytes() { return (2 * 128 + 2 * NST * BNK) * HD * 2 + NRAW * raw_bytes<HD>() + 512 + 8 * 4096 + 128 * 8; }
+template <int HD> constexpr int smem_bytes() { return (2 * 128 + 2 * NST * BNK) * HD * 2 + NRAW * raw_bytes<HD>() + NST * kNumbers + 512 + 8 * 4096 + 128 * 16; }
 
 // n0, n1: key tiles of the two query tiles; n1 < 0: no more work.  split: one query tile, its even key tiles are the first warps', its odd ones
 // the second's.  Tile j holds the keys from 64 j (j < ptiles: first tokens that stay visible) or from 64 (tile_lo + j - ptiles).
@@ -40,19 +44,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 __device__ __forceinline__ void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-// eight codes -> eight numbers low + s n of the model's type, in order (s2, low2: the same number in both halves)
-__device__ __forceinline__ void expand(uint32_t w, uint32_t s2, uint32_t low2, uint32_t (&r)[4]) {
+// eight codes n -> eight numbers n - 8 of the model's type, in order
+__device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) {
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
-    uint32_t n;
 #ifdef KGE_HALF
     const uint32_t u = p < 2 ? w : w >> 8;               // 0x6400 | n = 1024 + n; 0x6400 | n << 4 = 1024 + 16 n
-    if (p & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(n) : "r"((u & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd400d400u));
-    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(n) : "r"((u & 0x000f000fu) | 0x64006400u), "r"(0x64006400u));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[p]) : "r"(n), "r"(s2), "r"(low2));
+    if (p & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[p]) : "r"((u & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));
+    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[p]) : "r"((u & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));
 #else
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(n) : "r"(((w >> (4 * p)) & 0x000f000fu) | 0x43004300u), "r"(0x43004300u));      // 0x4300 | n = 128 + n
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r[p]) : "r"(n), "r"(s2), "r"(low2));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[p]) : "r"(((w >> (4 * p)) & 0x000f000fu) | 0x43004300u), "r"(0x43084308u));      // 0x4300 | n = 128 + n
 #endif
   }
 }
@@ -75,9 +76,10 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   if ((s_addr(smem_raw) & 1023u) != 0) __trap();
   const uint32_t sQ = s_addr(smem_raw), sK = sQ + 2 * Q_TILE, sV = sK + NST * TILE;
   uint8_t* raw = smem_raw + 2 * Q_TILE + 2 * NST * TILE;
-  uint8_t* tail = raw + NRAW * RAW;
+  uint8_t* numbers = raw + NRAW * RAW;
+  uint8_t* tail = numbers + NST * kNumbers;
   uint8_t* stage_out = tail + 512;
-  float2* part = reinterpret_cast<float2*>(stage_out + 8 * 4096);
+  float4* part = reinterpret_cast<float4*>(stage_out + 8 * 4096);
   const uint32_t bar0 = s_addr(tail);
   Item* items = reinterpret_cast<Item*>(tail + 288);                   // 2 slots of 48 bytes
   const uint32_t clc_resp = bar0 + 384;
@@ -89,7 +91,9 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   //   raw_full(r)   the four turning warps, before they arrive on raw_empty(r), without which the producer does not refill it
   //   raw_empty(r)  the producer, before the copy that the next phase of raw_full(r) counts
   //   k_full, v_full: 4 arrivals of the turning warps; k_empty, v_empty: a commit of each issuer, waited for by the turning warps before they
-  //   write the stage again
+  //   write the stage again.  The numbers of a stage are written with its values and read by the softmax, which waits for v_full too: the
+  //   next phase of it needs v_empty, that a P V, and that the P of the waiter
+  //   q_empty       a commit of each issuer, and the softmax warps, which have summed their rows of Q
   auto k_full = [&](int s) { return bar0 + 8u * s; };
   auto k_empty = [&](int s) { return bar0 + 24u + 8u * s; };
   auto v_full = [&](int s) { return bar0 + 48u + 8u * s; };
@@ -115,7 +119,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         for (int t = 0; t < 2; ++t) { mbar_init(p_full(a, t), 4); mbar_init(o_full(a, t), 1); }
         mbar_init(item_full(a), 1); mbar_init(item_empty(a), 14);      // 8 softmax warps, 2 issuers, 4 turning warps
       }
-      mbar_init(q_full, 1); mbar_init(q_empty, 2); mbar_init(clc_full, 1);
+      mbar_init(q_full, 1); mbar_init(q_empty, 10); mbar_init(clc_full, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -338,7 +342,6 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
             for (int pass = 0; pass < 2; ++pass) {
               const int grp = (s >> 4) + 2 * pass, row = grp * 16 + tok;
               const uint8_t* g = raw + rs * RAW + grp * GB;
-              const uint32_t pk = *reinterpret_cast<const uint32_t*>(g + 16 * HD + tok * 4), pv = *reinterpret_cast<const uint32_t*>(g + 16 * HD + 64 + tok * 4);
               const int at = part_v ? 8 * HD + tok * (HD / 2) + 4 * kv4::value_word(HD, tok, W * t) : kv4::key_row(tok) * (HD / 2) + 4 * W * t;
               uint32_t w[4];
               if (HD == 128) {
@@ -348,22 +351,28 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
                 const uint2 u = *reinterpret_cast<const uint2*>(g + at);
                 w[0] = u.x; w[1] = u.y;
               }
-              const bool there = row < left, fine = finite2(pk) && finite2(pv);
-              uint32_t p = part_v ? pv : pk;
-              if (!there || (part_v && !fine)) {
-                p = 0;
+              if (row >= left) {                         // (the other warps multiply these with weights of zero)
 #pragma unroll
-                for (int i = 0; i < W; ++i) w[i] = 0;
-              } else if (!fine) {
-                p = 0x7fff7fffu;                         // NaN in either type
+                for (int i = 0; i < W; ++i) w[i] = 0x88888888u;
               }
-              const uint32_t s2 = __byte_perm(p, p, 0x1010), low2 = __byte_perm(p, p, 0x3232);
 #pragma unroll
               for (int i = 0; i < W; ++i) {
                 uint32_t r[4];
-                expand(swap ? w[i ^ 1] : w[i], s2, low2, r);
+                expand(swap ? w[i ^ 1] : w[i], r);
                 st_shared16(dst + tile_off<BNK>(row, W * t + (swap ? i ^ 1 : i)), r);
               }
+            }
+            if (part_v && d < 64) {                      // warps 12 and 13: the numbers of key d
+              const uint8_t* g = raw + rs * RAW + (d >> 4) * GB + 16 * HD + (d & 15) * 4;
+              const uint32_t pk = *reinterpret_cast<const uint32_t*>(g), pv = *reinterpret_cast<const uint32_t*>(g + 64);
+              const bool there = d < left, fine = finite2(pk) && finite2(pv);
+              const float nan = __uint_as_float(0x7fffffffu);
+              const float sk = there ? (fine ? bf_lo(pk) : nan) * ka.scale_log2 : 0.f, zk = there && fine ? fmaf(8.f, bf_lo(pk), bf_hi(pk)) * ka.scale_log2 : 0.f;
+              const float sv = there && fine ? bf_lo(pv) : 0.f, zv = there && fine ? fmaf(8.f, sv, bf_hi(pv)) : 0.f;
+              float* to = reinterpret_cast<float*>(numbers + st * kNumbers) + (d >> 1) * 8 + (d & 1);
+              to[0] = sk; to[2] = zk; to[4] = sv; to[6] = zv;
+              const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(sv));
+              if (lane == 0) reinterpret_cast<float*>(numbers + st * kNumbers + 1024)[d >> 5] = fmaxf(__log2f(__uint_as_float(most)), -60.f);
             }
             fence_async_smem();
             __syncwarp();
@@ -379,23 +388,35 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
     const int a = warp >> 2, r = threadIdx.x & 127, tk = r / G;
     const uint32_t t_row = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t t_s = t_row + S_COL + a * 128, t_o = t_row + a * 128;
-    const float scale_log2 = ka.scale_log2;
-    const f2 sc2 = pk(scale_log2, scale_log2);
-    uint32_t ns = 0;
+    uint32_t ns = 0, nk = 0;                                           // tiles of this group, key tiles of the items before
     for (uint32_t ni = 0;; ++ni) {
       mbar_wait(item_full(ni & 1), (ni >> 1) & 1);
       const Item it = items[ni & 1];
       __syncwarp();
       if (lane == 0) mbar_arrive(item_empty(ni & 1));
       if (it.n1 < 0) break;
-      const int n = a ? it.n1 : it.n0;
-      if (n <= 0) continue;
+      const int n = a ? it.n1 : it.n0, n_item = it.split ? it.n0 + it.n1 : max(it.n0, it.n1);
       const int qt = it.split ? 0 : a;                                 // the query tile of these warps
+      // sum(q) of this thread's row
+      mbar_wait(q_full, ni & 1);
+      float qsum = 0.f;
+      if (n > 0) {
+        const uint8_t* row = smem_raw + qt * Q_TILE;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(row + tile_off<128>(r, c));
+          qsum += ((bf_lo(u.x) + bf_hi(u.x)) + (bf_lo(u.y) + bf_hi(u.y))) + ((bf_lo(u.z) + bf_hi(u.z)) + (bf_lo(u.w) + bf_hi(u.w)));
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_empty);
+      if (n <= 0) { nk += n_item; continue; }
+      const f2 qs2 = pk(qsum, qsum);
       const bool row_ok = tk < (qt ? it.ntok1 : it.ntok0);
       const int row_tok = it.tok0 + qt * TT + tk;
       const int lim = row_ok ? it.ctx0 + row_tok : -1;                 // last visible key of this row
       const int lo_row = ka.window > 0 ? lim - ka.window + 1 : 0;      // the window's first key; below it only the first tokens
-      float m_ref = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, l = 0.f, zs = 0.f;
       // the second group's exponentials start when the first's of its first tile are done (attn_pair.cuh)
       const bool turns = it.n1 >= 3;
       for (int j = 0; j < n; ++j) {
@@ -411,6 +432,17 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         const int jt = it.split ? 2 * j + a : j, kbase = (jt < it.ptiles ? jt : it.tile_lo + jt - it.ptiles) * BNK;
         const int vis = lim - kbase, from = lo_row - kbase, keep = ka.first - kbase;      // column i is visible: i <= vis and (i >= from or i < keep)
         float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        const int st = (nk + jt) % NST;
+        mbar_wait(v_full(st), ((nk + jt) / NST) & 1);                  // the numbers of the tile's keys and values
+        const ulonglong2* num = reinterpret_cast<const ulonglong2*>(numbers + st * kNumbers);
+#pragma unroll
+        for (int i = 0; i < BNK / 2; ++i) {
+          const ulonglong2 sz = num[2 * i];
+          float x0, x1;
+          upk(fma2(pk(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sz.x, mul2(qs2, sz.y)), x0, x1);
+          sv[2 * i] = __float_as_uint(x0); sv[2 * i + 1] = __float_as_uint(x1);
+        }
+        const float2 lgs = *reinterpret_cast<const float2*>(numbers + st * kNumbers + 1024);
         if (!__all_sync(0xffffffffu, vis >= BNK - 1 && (from <= 0 || keep >= BNK))) {
 #pragma unroll
           for (int i = 0; i < BNK; ++i) sv[i] = i <= vis && (i >= from || i < keep) ? sv[i] : 0xff800000u;
@@ -419,7 +451,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         for (int i = 0; i < BNK; i += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k) mxa[k] = max3(mxa[k], __uint_as_float(sv[i + 2 * k]), __uint_as_float(sv[i + 2 * k + 1]));
-        const float mx = max3(fmaxf(mxa[0], mxa[1]), mxa[2], mxa[3]) * scale_log2;      // -inf stays -inf
+        const float mx = max3(fmaxf(mxa[0], mxa[1]), mxa[2], mxa[3]) + fmaxf(lgs.x, lgs.y);      // -inf stays -inf
         const bool grow = mx > m_ref + kRescaleThreshold;              // includes the first finite maximum
         if (__any_sync(0xffffffffu, grow)) {
           float alpha = 1.f;
@@ -427,6 +459,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
             alpha = (m_ref == -INFINITY) ? 0.f : exp2f(m_ref - mx);
             m_ref = mx;
             l *= alpha;
+            zs *= alpha;
           }
           if (j > 0) {
             mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);         // P V of the tile before
@@ -446,7 +479,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         }
         const float base = (m_ref == -INFINITY) ? 0.f : m_ref;
         const f2 nb2 = pk(-base, -base);
-        f2 rs[2] = {0, 0};
+        f2 rs[2] = {0, 0}, zr[2] = {0, 0};
         if (ns >= 2) { mbar_wait(o_full(a, ns), ((ns - 2) >> 1) & 1); tc_after(); }       // P V of two tiles before has read this buffer
         if (turns && j == 0 && a == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
         const uint32_t t_p = t_s + 64 + (ns & 1) * 32;
@@ -456,9 +489,12 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float p0, p1;
-            upk(fma2(pk(__uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1])), sc2, nb2), p0, p1);
-            p0 = ex2_ftz(p0); p1 = ex2_ftz(p1);                        // masked: -inf -> 0
-            rs[i & 1] = add2(rs[i & 1], pk(p0, p1));
+            upk(add2(pk(__uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1])), nb2), p0, p1);
+            const f2 e = pk(ex2_ftz(p0), ex2_ftz(p1));                 // masked: -inf -> 0
+            const ulonglong2 sz = num[c + 2 * i + 1];
+            rs[i & 1] = add2(rs[i & 1], e);
+            zr[i & 1] = fma2(e, sz.y, zr[i & 1]);
+            upk(mul2(e, sz.x), p0, p1);
             pkd[i] = pack_bf2(p0, p1);
           }
           tmem_st16(t_p + c / 2, pkd);
@@ -470,21 +506,23 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         if (lane == 0) mbar_arrive(p_full(a, ns));
         ++ns;
         l += sum2(add2(rs[0], rs[1]));
+        zs += sum2(add2(zr[0], zr[1]));
       }
       mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);
       tc_after();
       float mine = 1.f, other = 0.f;                                   // weights of the two halves of a split row
       if (it.split) {
-        if (a) part[r] = make_float2(m_ref, l);
+        if (a) part[r] = make_float4(m_ref, l, zs, 0.f);
         tc_before();
         asm volatile("bar.sync 2, 256;" ::: "memory");
         tc_after();
         if (!a) {
-          const float2 p1 = part[r];
+          const float4 p1 = part[r];
           const float m = fmaxf(m_ref, p1.x);
           mine = m_ref == -INFINITY ? (l == l ? 0.f : l) : exp2f(m_ref - m);      // (a half that saw nothing but NaN keeps it)
           other = p1.x == -INFINITY ? (p1.y == p1.y ? 0.f : p1.y) : exp2f(p1.x - m);
           l = l * mine + p1.y * other;
+          zs = zs * mine + p1.z * other;
           m_ref = m;
         }
       }
@@ -512,6 +550,8 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         tc_before();                                                   // the next item's first P V comes behind p_full of these warps
         __syncwarp();
 #pragma unroll
+        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + zs);
+#pragma unroll
         for (int i = 0; i < 64; i += 8) {
           uint4 w;
           w.x = pack_bf2(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv);
@@ -530,6 +570,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         }
       }
       if (it.split) asm volatile("bar.sync 3, 256;" ::: "memory");     // O1 and the sums are read
+      nk += n_item;
     }
   }
   tc_before();
