@@ -18,7 +18,7 @@ def refused(kge, rc, words):
     (dict(q_out=None), "null"), (dict(cache=None), "null"), (dict(qkv=None), "null"), (dict(slots=None), "null"), (dict(pos=None), "without positions"),
     (dict(hd=96), "head_dim"), (dict(bs=8), "power of two from 16"), (dict(bs=48), "power of two from 16"), (dict(H=0), "H=0"), (dict(KV=0), "KV=0"),
     (dict(stride=4 * 64 - 8), "apart"), (dict(stride=4 * 64 + 4), "apart"), (dict(q_out=P + 8), "aligned"), (dict(cache=P + 4), "aligned"), (dict(qkv=P + 2), "aligned"),
-    (dict(cs=P + 8), "aligned"), (dict(T=1 << 27), "in one call")])
+    (dict(cs=P + 8), "aligned"), (dict(H=1 << 20, stride=1 << 26), "heads of")])
 def test_write_refusals(kge, f16, change, words):
     a = dict(q_out=P, stride=256, cache=P, qkv=P, cs=P, pos=P, slots=P, T=3, H=4, KV=2, hd=64, bs=16) | change
     refused(kge, getattr(kge.lib(), "kge_rope_kv4write" + f16)(*a.values(), None), words)
