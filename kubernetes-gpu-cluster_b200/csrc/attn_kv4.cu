@@ -241,6 +241,11 @@ struct Core {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          // only a column that has passed the bound moves: what a head gets does not hang on its neighbours
+          uint32_t most = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) most = max_u16x2(most, max_u16x2(wt[i][nt][0], wt[i][nt][1]));
+          const bool over = __ballot_sync(0xffffffffu, (h ? most >> 16 : most & 0xffffu) >= kWeightMost) & (0x11111111u << t);
           float top = fresh ? -INFINITY : 0.f;                    // how far the reference goes up (the first: or down)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -248,7 +253,7 @@ struct Core {
             for (int r = 0; r < 2; ++r) top = fmaxf(top, fmaxf(x[i][nt][2 * r + h] + lg2(sv[i][r]), x[i][nt][2 * r + h] - kExpRoom));
 #pragma unroll
           for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-          if (top == -INFINITY) top = 0.f;                        // (only NaN rows)
+          if (top == -INFINITY || !(fresh || over)) top = 0.f;    // (the first: only NaN rows)
           const float f = ex2(-top);
           ref[nt][h] += top;
           l[nt][h] *= f;
