@@ -3,9 +3,11 @@ them together as a serving loop uses them.
 
 Tolerances.  u is half a step of the 16-bit type relative to the value, eps / 2 (bf16 2^-8, fp16 2^-11).
   Codes n - 8 are exact in the products, and so is q (but for what lies 2^-24 below its largest number in single-token requests).  Weights p s
-  are rounded once, to float16 (2^-11) in single-token requests and to the 16-bit type (u) in prompts; what they are multiplied with is
+  are rounded once, to float16 (2^-11) in single-token requests and at most to the 16-bit type (u) in prompts; what they are multiplied with is
   |n - 8| <= 8, so that costs 8 max s of it at most.  The result is rounded once, u |out|.  Scores and sums are in fp32: their errors stay below
   2^-13 of the weights here.
+  Prompts in bfloat16 round keys, values and weights to float16, 2^-11 = u / 8 each: with scores of sum |q k| scale < 10 in the numbers of these
+  tests, 2^-11 (2 + 2 x 10) sum p |v| < 0.011 sum p |v|, below the u 8 max s = 0.012 that is allowed for weights rounded to u.
   In the 2-norm the roundings are independent, each of at most u / sqrt(3) in the mean square: result and weights together sqrt(2 / 3) u =
   0.82 u where s (n - 8) is as large as the values (their ends lie about zero), held to 1.2 (u + 2^-11).
 """
@@ -305,6 +307,45 @@ def test_q_beyond_float16(kge, L):
     again = attend(kge, s, scale=scale).reshape(2, 4, 128)
     assert torch.equal(again[0], out.reshape(2, 4, 128)[0]) and torch.equal(again[1, :3], out.reshape(2, 4, 128)[1, :3])
     assert torch.isnan(again[1, 3]).any()
+
+
+@pytest.mark.parametrize("hd,H,KV", [(128, 4, 1), (64, 6, 2)])
+@pytest.mark.parametrize("window,first", [(0, 0), (90, 3)])
+def test_prompts_of_numbers_far_apart(kge, L, hd, H, KV, window, first):
+    """bf16 prompts whose queries, keys and values no float16 holds: 64-key tiles 10^24 apart (within one, 100), rows of q 10^9 apart, rows of
+    zeros, and pages that hold the largest numbers behind the last key and in front of the window."""
+    lens, news = [400, 150, 70], [90, 150, 3]
+    s = setup("bf16", hd, H, KV, 16, lens, news, seed=21)
+    g = torch.Generator().manual_seed(22)
+    for b, n in enumerate(lens):
+        end = -(-n // 16) * 16
+        slots = [int(s["table"][b, j // 16]) * 16 + j % 16 for j in range(end)]
+        within = 10 ** torch.empty(end, 1, 1).uniform_(-1, 1, generator=g)
+        tiles = (10 ** torch.empty(2, end // 64 + 1).uniform_(-12, 12, generator=g)).repeat_interleave(64, 1)[:, :end, None, None]
+        k, v = randn(g, end, KV, hd) * within, randn(g, end, KV, hd) * within * tiles[1]
+        k[torch.arange(end) // 64 % 3 == 0] *= 1e-10
+        k[n:], v[n:] = randn(g, end - n, KV, hd) * 1e37, randn(g, end - n, KV, hd) * 1e37
+        v[5:5 + 64] *= 0 if b == 1 else 1
+        if window and b == 0:
+            k[first:n - news[b] - window + 1], v[first:n - news[b] - window + 1] = 1e37, -1e37
+        s["cache"].put(k.bfloat16(), v.bfloat16(), slots)
+    q = s["q"][:, :H * hd].reshape(-1, H, hd)
+    q *= 10 ** torch.empty(q.shape[0], H, 1).uniform_(-9, 0, generator=g) * 1e12
+    q[3] = 0
+    scale = hd ** -0.5 * 1e-13
+    out = attend(kge, s, window, first, scale=scale)
+    T = s["T"]
+    ref, size, reach = ko.attention(s["cache"], s["q"][:T, :H * hd].reshape(T, H, hd), s["table"], s["lens"], s["qsl"], H, scale, window, first)
+    got, u = out[:T].cpu().double().reshape(T, H, hd), ko.half_step(torch.bfloat16)
+    # 2^-11 each for weights and values, and twice that of the scores' sum |q k| scale for the keys.  Besides, a tile's numbers end at 2^-16 of its
+    # largest scale, here 150 times a row's own at most, which is max |v| / 7.5 at most: 2^-11.6 max |v|, and sum p max |v| < 3 max sum p |v|, so
+    # 2^-10 of that; of a score 2^-16 150 / 7.5 max |k| sum |q| scale, with max |k| < 4 of the mean |k|: 2^-9.6 of its sum, twice that for the weights
+    assert ((got - ref).abs() <= u * ref.abs() * 1.01 + 2 ** -11 * (2 + 8 * reach) * size + 2 ** -10 * size.amax(-1, keepdim=True)).all()
+    q[7, 1, 3] = math.inf                                              # a row that cannot be multiplied, beside others
+    again = attend(kge, s, window, first, scale=scale)[:T].cpu().reshape(T, H, hd)
+    rest = torch.ones(T, H, dtype=torch.bool)
+    rest[7, 1] = False
+    assert torch.equal(again[rest], out[:T].cpu().reshape(T, H, hd)[rest]) and torch.isnan(again[7, 1]).any()
 
 
 def test_offsets_beyond_32_bits(kge, L):
