@@ -785,13 +785,13 @@ extern "C" int KGE_API(kge_paged_attn_kv4)(void* out, const void* q, int q_strid
   cudaStream_t st = (cudaStream_t)stream;
   const int G = H / KV;
   const bool single = G <= 16;                 // a kernel of their own for single-token requests
+  const int64_t need = single ? ak4::workspace_bytes(G, hd) : 0;
+  KGE_REQUIRE(!single || (workspace && workspace_bytes >= need), "kge_paged_attn_kv4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   if (!single || max_q_len > 1)
     if (int rc = paged_attn_kv4_tc((bf16*)out, (const bf16*)q, q_stride, (const uint8_t*)kv_cache, block_table, max_blocks_per_seq, seq_lens, query_start_loc, B, T, max_q_len,
                                    max_seq_len, H, KV, hd, block_size, scale, window, first, single, st))
       return rc;
   if (!single) return 0;
-  const int64_t need = ak4::workspace_bytes(G, hd);
-  KGE_REQUIRE(workspace && workspace_bytes >= need, "kge_paged_attn_kv4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   ak4::Args a;
   a.out = (bf16*)out; a.q = (const bf16*)q; a.cache = (const uint8_t*)kv_cache;
   a.table = block_table; a.lens = seq_lens; a.qsl = query_start_loc;
