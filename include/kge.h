@@ -216,7 +216,7 @@ int kge_kv4_read(void* k_out, void* v_out, const void* kv_cache, const int64_t* 
  *  - kv_cache is the one buffer of keys and values
  *  - window > 0: a query at position i sees the keys j <= i with i - j < window or j < first (first tokens that stay visible, "sinks");
  *    window 0: all j <= i.  Pages that no query sees are not read.
- *  - H / KV up to 128; scale > 0; q_stride >= H * hd; out, q, kv_cache and workspace 16-byte aligned
+ *  - H / KV up to 128; scale > 0; q_stride >= H * hd; out, q, kv_cache and workspace 16-byte aligned; at most 2^30 tokens a request
  *  - T may be larger than the rows of all requests (a captured step with room to spare): rows behind query_start_loc[B] are left alone,
  *    as are requests without rows; max_q_len and max_seq_len are upper bounds.  A row without a key (seq_lens 0) is zeros.
  *  - a NaN row of the cache makes NaN of the queries that see it, and of no others

@@ -777,11 +777,16 @@ extern "C" int KGE_API(kge_paged_attn_kv4)(void* out, const void* q, int q_strid
   KGE_REQUIRE(q_stride % 8 == 0 && q_stride >= H * hd, "kge_paged_attn_kv4: q_stride=%d must be a multiple of 8, at least H * hd", q_stride);
   KGE_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)kv_cache | (uintptr_t)workspace) & 15) == 0, "kge_paged_attn_kv4: pointers must be 16-byte aligned");
   KGE_REQUIRE(window >= 0 && first >= 0, "kge_paged_attn_kv4: window=%d first=%d", window, first);
-  KGE_REQUIRE(scale > 0.f && scale < 3e38f, "kge_paged_attn_kv4: scale=%g must be positive", (double)scale);
+  KGE_REQUIRE(scale > 0.f && scale < 1e38f, "kge_paged_attn_kv4: scale=%g must be positive", (double)scale);
   if (B <= 0 || T <= 0) return 0;
   KGE_REQUIRE(B <= 65535, "kge_paged_attn_kv4: %d requests (at most 65535)", B);
   KGE_REQUIRE(max_q_len >= 1 && max_seq_len >= 1 && max_blocks_per_seq >= 1, "kge_paged_attn_kv4: max_q_len / max_seq_len / max_blocks_per_seq must be >= 1");
-  KGE_REQUIRE((int64_t)max_blocks_per_seq * block_size < (1ll << 31), "kge_paged_attn_kv4: %d blocks of %d tokens a request", max_blocks_per_seq, block_size);
+  KGE_REQUIRE((int64_t)max_blocks_per_seq * block_size <= (1ll << 30), "kge_paged_attn_kv4: %d blocks of %d tokens a request (at most 2^30 tokens)", max_blocks_per_seq,
+              block_size);
+  const int most = max_blocks_per_seq * block_size;      // keys of a request: what is beyond makes no difference, and sums stay in range
+  if (window >= most) window = 0;
+  first = std::min(first, most);
+  max_seq_len = std::min(max_seq_len, most);
   cudaStream_t st = (cudaStream_t)stream;
   const int G = H / KV;
   const bool single = G <= 16;                 // a kernel of their own for single-token requests

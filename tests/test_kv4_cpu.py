@@ -40,7 +40,8 @@ def test_read_refusals(kge, f16, change, words):
     (dict(bs=40), "block_size"), (dict(stride=4 * 64 - 8), "q_stride"), (dict(stride=260), "q_stride"), (dict(out=P + 8), "aligned"), (dict(ws=P + 4), "aligned"),
     (dict(window=-1), "window"), (dict(first=-2), "window"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=-0.5), "scale"),
     (dict(maxq=0), "must be >= 1"), (dict(maxc=0), "must be >= 1"), (dict(mb=0), "must be >= 1"), (dict(mb=1 << 28), "blocks of"), (dict(B=70000), "65535"),
-    (dict(ws=None), "workspace"), (dict(nws=1000), "workspace"), (dict(maxq=3, B=1, nws=1000), "workspace")])      # (before prompts are launched)
+    (dict(ws=None), "workspace"), (dict(nws=1000), "workspace"), (dict(maxq=3, B=1, nws=1000), "workspace"),      # (before prompts are launched)
+    (dict(mb=(1 << 26) + 1), "tokens a request"), (dict(scale=2e38), "scale")])
 def test_attention_refusals(kge, f16, change, words):
     a = dict(out=P, q=P, stride=256, cache=P, table=P, mb=4, lens=P, qsl=P, B=3, T=3, maxq=1, maxc=50, H=4, KV=2, hd=64, bs=16, scale=0.125, window=0, first=0, ws=P,
              nws=1 << 30) | change

@@ -234,6 +234,18 @@ def test_prompts(kge, L, dtype, hd, H, KV, bs, lens, news, window, first):
     check(s, attend(kge, s, window, first), window, first)
 
 
+@pytest.mark.parametrize("dtype,hd,H,KV,bs,lens,news", [
+    ("bf16", 64, 128, 1, 4096, [5000, 1, 70], [1, 1, 3]),                   # 128 heads on one, the largest blocks
+    ("fp16", 128, 128, 128, 16, [37, 9], [1, 9]),                           # as many kv heads
+    ("bf16", 128, 34, 2, 2048, [2049, 300], [2, 1]),                        # one head more than the single-token kernel takes
+    ("fp16", 64, 16, 16, 4096, [4097], [1]), ("bf16", 128, 127, 127, 32, [33, 65], [1, 20])])
+@pytest.mark.parametrize("window,first", [(2 ** 31 - 1, 2 ** 31 - 1), (33, 40)])
+def test_the_largest_sizes(kge, L, dtype, hd, H, KV, bs, lens, news, window, first):
+    """Heads, blocks, windows and bounds at the ends of their ranges, rows of q further apart than they are long."""
+    s = setup(dtype, hd, H, KV, bs, lens, news, seed=31, extra_rows=2, stride_pad=40)
+    check(s, attend(kge, s, window, first, maxq=70000, maxc=2 ** 31 - 1), window, first)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("window,first", [(0, 0), (50, 4)])
 def test_mixed_batches(kge, L, dtype, window, first):
