@@ -419,6 +419,13 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(cons
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.y, kvh = blockIdx.x, G = a.H / a.KV;
+  // the first units' block ids without a window come at the same time as the length that says which of them count
+  int blk[ST];
+#pragma unroll
+  for (int s = 0; s < ST; ++s) {
+    const int64_t at = ((int64_t)(warp + s * NW) * WK + lane * 16) >> a.bs_shift;
+    blk[s] = lane < 2 && at < a.max_blocks && a.window == 0 ? a.table[(int64_t)b * a.max_blocks + at] : 0;
+  }
   const int qrow = a.qsl[b];
   if (a.qsl[b + 1] - qrow != 1) return;
   const Span sp(a.len(b), a.window, a.first);
@@ -434,9 +441,9 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(cons
     __syncwarp();
     if (lane < (two ? groups : min(groups, 1))) copy_groups<HD>(a, ring + (stage * 2 + lane) * GB, blk, kvh, key0 + lane * 16, two ? 1 : groups, bars + 8 * stage);
   };
-  int blk[ST];
+  if (a.window)
 #pragma unroll
-  for (int s = 0; s < ST; ++s) blk[s] = block_of(warp + s * NW);
+    for (int s = 0; s < ST; ++s) blk[s] = block_of(warp + s * NW);
 #pragma unroll
   for (int s = 0; s < ST; ++s) ask(warp + s * NW, s, blk[s]);
   Core<HD, NT> core;
