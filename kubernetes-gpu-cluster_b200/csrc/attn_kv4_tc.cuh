@@ -88,8 +88,9 @@ __device__ __forceinline__ void expand(uint32_t w, const RowNumbers& c, uint32_t
   }
 }
 // The power of two that a tile's rows are multiplied with: the largest s comes to [2^-9, 2^-8), so that s 2^24 is a float16 number, unless a low
-// would pass 2^15.  `most`: over the rows, the largest of the bits of s and those of |low| / 2^23, as fp32 (0: a tile of zeros).
-__device__ __forceinline__ int tile_exponent(int most) { return most < (1 << 23) ? 0 : min(max(118 - (most >> 23), -133), 100); }
+// would pass 2^15.  `most`: over the rows, the largest of the bits of s and those of |low| / 2^23, as fp32 (0: a tile of zeros).  At most 2^90: sums of
+// 2^90 P over 2^20 keys and more stay finite.
+__device__ __forceinline__ int tile_exponent(int most) { return most < (1 << 23) ? 0 : min(max(118 - (most >> 23), -133), 90); }
 __device__ __forceinline__ int row_most(uint32_t p) {
   return max((int)__float_as_uint(bf_lo(p)), (int)(__float_as_uint(bf_hi(p)) & 0x7fffffffu) - (23 << 23));
 }
