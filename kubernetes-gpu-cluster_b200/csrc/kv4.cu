@@ -22,14 +22,17 @@ __device__ __forceinline__ uint32_t bits16(bf16 v) { return __bfloat16_as_ushort
 // Its bytes are the qkv rows in, q rows and HD + 8 a token and kv head out, but instructions and the blocks' lives bound it: 8192 tokens of 32 / 8
 // heads of 128 (179 MB, 27.7 us at the copy's rate) take 60 us with a division for every code, 57 without, 43 with both halves of a pair in one
 // thread (no exchange of lanes, cosines read once for both); two or three tokens a thread 48 and 52, blocks of 64 or 384 threads 55 and 64.
-template <int HD>
+// Few heads: a block of 128 threads takes several tokens (threadIdx.y); 8192 tokens of 8 / 1 heads of 64 10.3 -> 7.5 us, 4 / 2 of 128 11.8 -> 9.0.
+template <int HD, bool TOKENS>
 __global__ void __launch_bounds__(256)
 rope_kv4write_kernel(bf16* q_out, int q_stride, uint8_t* cache, const bf16* qkv, const bf16* __restrict__ cos_sin, const int32_t* __restrict__ positions,
-                     const int64_t* __restrict__ slots, int H, int KV, int bs_shift) {
+                     const int64_t* __restrict__ slots, int T, int H, int KV, int bs_shift) {
   constexpr int L = HD / 16;
   pdl_launch_dependents();
   pdl_wait();
-  const int t = blockIdx.x, rows = H + 2 * KV, lane_at = blockIdx.y * blockDim.x + threadIdx.x;
+  const int t = TOKENS ? blockIdx.x * blockDim.y + threadIdx.y : blockIdx.x;
+  if (TOKENS && t >= T) return;                            // (the same for the warp)
+  const int rows = H + 2 * KV, lane_at = blockIdx.y * blockDim.x + threadIdx.x;
   const int at = min(lane_at, rows * L - 1), head = at / L, c = threadIdx.x % L;      // (a last warp's surplus lanes go along with its last row)
   const bf16* src = qkv + ((int64_t)t * rows + head) * HD + c * 8;
   uint4 v[2] = {*reinterpret_cast<const uint4*>(src), *reinterpret_cast<const uint4*>(src + HD / 2)};
@@ -112,7 +115,8 @@ rope_kv4write_kernel(bf16* q_out, int q_stride, uint8_t* cache, const bf16* qkv,
   if (c == 0) g[64 * L + (key ? 0 : 16) + token] = fine ? s16 | bits16(f2bf(lo)) << 16 : 0x7fff7fffu;
 }
 
-// A thread has 8 dimensions of the key and of the value of one (token, kv head); rows whose slot is negative are zeros.
+// A thread has 8 dimensions of the key and of the value of one (token, kv head); rows whose slot is negative are zeros.  8192 tokens of 8 heads of 128:
+// 10.7 us for 6.6 of bytes, most of them stores; with 16 dimensions a thread 9.8, but 64 tokens 1.9 in place of 1.6.
 template <int HD>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(bf16* __restrict__ k_out, bf16* __restrict__ v_out, const uint8_t* __restrict__ cache, const int64_t* __restrict__ slots, uint32_t lanes, int KV,
@@ -174,9 +178,11 @@ extern "C" int KGE_API(kge_rope_kv4write)(void* q_out, int q_out_stride, void* k
   KGE_REQUIRE((int64_t)(H + 2 * KV) * hd < (1ll << 24), "kge_rope_kv4write: %d heads of %d", H + 2 * KV, hd);
   int shift = 4;
   while ((1 << shift) < block_size) ++shift;
-  const int lanes = (H + 2 * KV) * (hd / 16), th = lanes <= 256 ? (lanes + 31) & ~31 : 128;
-  KGE_CUDA_OK(launch_pdl(hd == 128 ? rope_kv4write_kernel<128> : rope_kv4write_kernel<64>, dim3(T, (lanes + th - 1) / th), dim3(th), 0, (cudaStream_t)stream, (bf16*)q_out,
-                         q_out_stride, (uint8_t*)kv_cache, (const bf16*)qkv, (const bf16*)cos_sin, positions, slot_mapping, H, KV, shift));
+  const int lanes = (H + 2 * KV) * (hd / 16), th = lanes <= 256 ? (lanes + 31) & ~31 : 128, tokens = th <= 64 ? 128 / th : 1;      // (of a block)
+  auto kern = hd == 128 ? (tokens > 1 ? rope_kv4write_kernel<128, true> : rope_kv4write_kernel<128, false>)
+                        : (tokens > 1 ? rope_kv4write_kernel<64, true> : rope_kv4write_kernel<64, false>);
+  KGE_CUDA_OK(launch_pdl(kern, dim3((T + tokens - 1) / tokens, (lanes + th - 1) / th), dim3(th, tokens), 0, (cudaStream_t)stream, (bf16*)q_out,
+                         q_out_stride, (uint8_t*)kv_cache, (const bf16*)qkv, (const bf16*)cos_sin, positions, slot_mapping, T, H, KV, shift));
   return 0;
 }
 

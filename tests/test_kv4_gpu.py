@@ -58,7 +58,8 @@ def turned(x, cs):
 
 WRITES = [  # dtype, hd, H, KV, block, T
     ("bf16", 128, 4, 2, 16, 1), ("bf16", 128, 32, 8, 64, 7), ("fp16", 128, 5, 1, 32, 33), ("bf16", 64, 3, 3, 16, 50), ("fp16", 64, 7, 1, 128, 19),
-    ("fp16", 64, 1, 1, 16, 2), ("bf16", 64, 32, 8, 16, 21), ("bf16", 128, 1, 1, 256, 40), ("fp16", 128, 8, 8, 64, 100)]
+    ("fp16", 64, 1, 1, 16, 2), ("bf16", 64, 32, 8, 16, 21), ("bf16", 128, 1, 1, 256, 40), ("fp16", 128, 8, 8, 64, 100),
+    ("fp16", 64, 4, 1, 16, 4), ("bf16", 64, 8, 1, 32, 129), ("fp16", 128, 4, 2, 16, 131), ("bf16", 128, 6, 1, 64, 2)]
 
 
 @pytest.mark.parametrize("dtype,hd,H,KV,bs,T", WRITES)
