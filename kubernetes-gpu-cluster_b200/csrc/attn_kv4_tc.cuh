@@ -134,8 +134,8 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   //   q_empty       a commit of each issuer, and the softmax warps, which have read or turned their rows of Q
   //   q_ready(a)    the softmax warps of group a; an issuer and, of a shared query tile, the other group wait for it before they let q_empty go
   // (E, F, 2^F) of tile j are written before k_full(j), which an issuer waits for before the products whose commit the softmax waits for.  They
-  // are written again for tile j + NEXP; a turning warp is at most 6 tiles ahead of a softmax warp: it waits for the scores of three tiles
-  // before its own, of those one and, of a split item, two are issued ahead of what the softmax has read, whose every second tile is its own.
+  // are written again for tile j + NEXP: who begins that tile has written the values before it, into a stage from which both issuers had
+  // taken the products of four tiles before, and they had waited for the P of every tile of theirs up to there.
   auto k_full = [&](int s) { return bar0 + 8u * s; };
   auto k_empty = [&](int s) { return bar0 + 24u + 8u * s; };
   auto v_full = [&](int s) { return bar0 + 48u + 8u * s; };
