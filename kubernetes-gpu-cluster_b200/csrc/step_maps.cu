@@ -132,7 +132,8 @@ extern "C" int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32
   a.num_free = num_free; a.max_blocks = max_blocks_per_seq; a.B = B; a.T = T; a.shift = 0;
   while ((1 << a.shift) < block_size) ++a.shift;
   const size_t smem = (size_t)(5 * B + 1) * 4;
-  if (smem > 48 * 1024) KGE_CUDA_OK(cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMapRequests + 1) * 4));
+  // (48 KB would hold the kernel's static shared memory too, so every launch says what the largest needs)
+  KGE_CUDA_OK(cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (5 * kMapRequests + 1) * 4));
   const int ctas = T > 2 * kMapThreads ? kMapCtas : 1;
   prefer_max_shared(step_maps_kernel);
   cudaLaunchConfig_t cfg = {};

@@ -12,6 +12,9 @@ Tolerances.  u is half a step of the 16-bit type relative to the value, eps / 2 
   0.82 u where s (n - 8) is as large as the values (their ends lie about zero), held to 1.2 (u + 2^-11).
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -568,3 +571,25 @@ def test_two_streams_at_once(kge, L):
                  max(s["lens"]), s["H"], s["KV"], 128, s["bs"], 128 ** -0.5, 0, 0, ws, ws.numel(), stream=st)
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_maps_of_any_number_of_requests(kge, L):
+    """What a launch asks of shared memory on the way to its limit: the number of requests goes up in a process of its own, so that no larger
+    launch has come before."""
+    body = """
+import sys
+sys.path[:0] = {path!r}
+import numpy as np, torch
+import kv4_oracle as ko
+from kge_loader import load
+from test_kv4_gpu import run_maps
+for B in (2442, 2443, 2444, 2450, 2457, 2458, 8192):
+    new = [1 + b % 3 for b in range(B)]
+    a = (np.arange(2 * B, dtype=np.int32).reshape(B, 2), [b % 17 for b in range(B)], new, list(range(5 * B, 6 * B)), 3, sum(new) - 5, 16)
+    got, want = run_maps(load(), *a), ko.maps(*a)
+    assert (got[0] == want[0]).all() and got[1:] == tuple(want[1:]), B
+print("all right")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", body.format(path=[os.path.dirname(here), here])], capture_output=True, text=True, timeout=300)
+    assert "all right" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
