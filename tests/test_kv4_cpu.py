@@ -2,7 +2,9 @@
 import re
 import os
 
+import numpy as np
 import pytest
+import torch
 
 import kv4_oracle as ko
 
@@ -82,3 +84,28 @@ def test_the_layouts_arithmetic_is_the_oracles():
         row = eval(body["key_row"], {"token": tok})
         assert ko.KEY_ROWS[row] == tok and eval(body["key_token"], {"row": row}) == tok
     assert "hd == 128 ? j ^ ((token & 2) << 2) : j" in src
+
+
+@pytest.mark.parametrize("dtype,hd", [("bf16", 128), ("fp16", 64)])
+def test_the_oracles_two_ways_agree(dtype, hd):
+    """put() and put_all(), get() and parts(), attention() and attention_terms()."""
+    dt, g = ko.DT[dtype], torch.Generator().manual_seed(3)
+    a, b = (ko.Cache(4, 2, hd, 32, dt, fill=0xA5) for _ in range(2))
+    slots = torch.randperm(128, generator=g)[:90].tolist()
+    k, v = (torch.randn(90, 2, hd, generator=g).to(dt) for _ in range(2))
+    k[5, 1, 3], v[7, 0, 2], v[9] = float("nan"), float("inf"), 2.5
+    a.put(k, v, slots)
+    b.put_all(k, v, slots)
+    assert (a.data == b.data).all()
+    k[5, 1, 3], v[7, 0, 2] = 1, 1
+    a.put(k, v, slots)
+    for whole, (code, s, low) in zip(a.get(slots, 1), a.parts(slots, 1)):
+        assert torch.equal(whole, low + s * code) and code.min() >= 0 and code.max() <= 15
+    c = ko.Cache(4, 2, hd, 32, dt)
+    c.put_all(k, v, list(range(90)))
+    table = np.array([[0, 1], [2, 1]], dtype=np.int32)
+    q = torch.randn(30, 6, hd, generator=g).to(dt)
+    for window, first in ((0, 0), (9, 4)):
+        want = ko.attention(c, q, table, [60, 20], np.array([0, 25, 30]), 6, 0.1, window, first)[0]
+        got = ko.attention_terms(c, q, table, [60, 20], np.array([0, 25, 30]), 6, 0.1, window, first)[0]
+        assert (got - want).abs().max() < 1e-12
