@@ -237,7 +237,7 @@ int64_t kge_attn_kv4_workspace_bytes(int H, int KV, int hd);
  * query_start_loc [B + 1]; positions [T] and slot_mapping [T] of the rows, request after request (rows behind the last: position 0, slot
  * -1); counts [4] = {rows, tokens asked for, position in the free list behind the last block taken, blocks that were lacking}.
  * Where T, a table row or the free list does not reach, a request gets as many of its new tokens as fit, and all outputs say so.
- * seq_lens may be cached_lens and free_first may be counts + 2 (the next step goes on from there).  Block size: a power of two; B <= 8192. */
+ * seq_lens may be cached_lens and free_first may be counts + 2 (the next step goes on from there).  Block size: a power of two; B <= 8192, T <= 2^30. */
 int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32_t* seq_lens, int32_t* query_start_loc, int32_t* positions,
                   int64_t* slot_mapping, int32_t* counts, const int32_t* cached_lens, const int32_t* new_lens, const int32_t* free_blocks,
                   int num_free, const int32_t* free_first, int B, int T, int block_size, void* stream);

@@ -781,7 +781,7 @@ extern "C" int KGE_API(kge_paged_attn_kv4)(void* out, const void* q, int q_strid
   KGE_REQUIRE(H > 0 && KV > 0 && H % KV == 0 && H / KV <= 128, "kge_paged_attn_kv4: H=%d must be a multiple of KV=%d, at most 128 times it", H, KV);
   KGE_REQUIRE(hd == 64 || hd == 128, "kge_paged_attn_kv4: head_dim=%d unsupported (64, 128)", hd);
   KGE_REQUIRE(block_size >= 16 && block_size <= 4096 && (block_size & (block_size - 1)) == 0, "kge_paged_attn_kv4: block_size=%d must be a power of two, 16 to 4096", block_size);
-  KGE_REQUIRE(q_stride % 8 == 0 && q_stride >= H * hd, "kge_paged_attn_kv4: q_stride=%d must be a multiple of 8, at least H * hd", q_stride);
+  KGE_REQUIRE(q_stride % 8 == 0 && q_stride >= (int64_t)H * hd, "kge_paged_attn_kv4: q_stride=%d must be a multiple of 8, at least H * hd", q_stride);
   KGE_REQUIRE((((uintptr_t)out | (uintptr_t)q | (uintptr_t)kv_cache | (uintptr_t)workspace) & 15) == 0, "kge_paged_attn_kv4: pointers must be 16-byte aligned");
   KGE_REQUIRE(window >= 0 && first >= 0, "kge_paged_attn_kv4: window=%d first=%d", window, first);
   KGE_REQUIRE(scale > 0.f && scale < 1e38f, "kge_paged_attn_kv4: scale=%g must be positive", (double)scale);

@@ -161,7 +161,13 @@ extern "C" int64_t kge_kv4_cache_bytes(int64_t num_blocks, int KV, int hd, int b
                    KV, hd);
     return -1;
   }
-  return num_blocks * KV * block_size * (hd + 8);
+  const int64_t block = (int64_t)block_size * (hd + 8);
+  int64_t bytes;
+  if (__builtin_mul_overflow((int64_t)KV, block, &bytes) || __builtin_mul_overflow(num_blocks, bytes, &bytes)) {
+    kge::set_error("kge_kv4_cache_bytes: %lld blocks of %d tokens and %d kv heads are more bytes than 64 bits count", (long long)num_blocks, block_size, KV);
+    return -1;
+  }
+  return bytes;
 }
 #endif
 
@@ -172,10 +178,10 @@ extern "C" int KGE_API(kge_rope_kv4write)(void* q_out, int q_out_stride, void* k
   KGE_REQUIRE(H > 0 && KV > 0, "kge_rope_kv4write: H=%d KV=%d", H, KV);
   KGE_REQUIRE(hd == 64 || hd == 128, "kge_rope_kv4write: head_dim=%d unsupported (64, 128)", hd);
   KGE_REQUIRE(block_size >= 16 && (block_size & (block_size - 1)) == 0, "kge_rope_kv4write: block_size=%d must be a power of two from 16", block_size);
+  KGE_REQUIRE(((int64_t)H + 2ll * KV) * hd < (1ll << 24), "kge_rope_kv4write: %lld heads of %d", (long long)H + 2ll * KV, hd);
   KGE_REQUIRE(q_out_stride >= H * hd && q_out_stride % 8 == 0, "kge_rope_kv4write: rows of q_out %d apart (a multiple of 8, at least H * hd = %d)", q_out_stride, H * hd);
   KGE_REQUIRE(aligned(q_out, 16) && aligned(kv_cache, 16) && aligned(qkv, 16) && aligned(cos_sin, 16), "kge_rope_kv4write: pointers must be 16-byte aligned");
   if (T <= 0) return 0;
-  KGE_REQUIRE((int64_t)(H + 2 * KV) * hd < (1ll << 24), "kge_rope_kv4write: %d heads of %d", H + 2 * KV, hd);
   int shift = 4;
   while ((1 << shift) < block_size) ++shift;
   const int lanes = (H + 2 * KV) * (hd / 16), th = lanes <= 256 ? (lanes + 31) & ~31 : 128, tokens = th <= 64 ? 128 / th : 1;      // (of a block)
@@ -193,8 +199,8 @@ extern "C" int KGE_API(kge_kv4_read)(void* k_out, void* v_out, const void* kv_ca
   KGE_REQUIRE(block_size >= 16 && (block_size & (block_size - 1)) == 0, "kge_kv4_read: block_size=%d must be a power of two from 16", block_size);
   KGE_REQUIRE(aligned(k_out, 16) && aligned(v_out, 16) && aligned(kv_cache, 16), "kge_kv4_read: pointers must be 16-byte aligned");
   if (T <= 0) return 0;
-  const int64_t lanes = (int64_t)T * KV * (hd / 8);
-  KGE_REQUIRE(lanes < (1ll << 32) - 256, "kge_kv4_read: %d tokens of %d heads in one call", T, KV);
+  const int64_t lanes = (int64_t)T * (hd / 8) * (KV < (1 << 24) ? KV : 1 << 24);
+  KGE_REQUIRE(KV < (1 << 24) && lanes < (1ll << 32) - 256, "kge_kv4_read: %d tokens of %d heads in one call", T, KV);
   int shift = 4;
   while ((1 << shift) < block_size) ++shift;
   auto kern = hd == 128 ? kv4_read_kernel<128> : kv4_read_kernel<64>;

@@ -124,7 +124,7 @@ extern "C" int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32
               "kge_step_maps: null pointer");
   KGE_REQUIRE(block_size > 0 && (block_size & (block_size - 1)) == 0, "kge_step_maps: block_size=%d must be a power of two", block_size);
   KGE_REQUIRE(B >= 0 && B <= kMapRequests, "kge_step_maps: %d requests (at most %d)", B, kMapRequests);
-  KGE_REQUIRE(T >= 0 && num_free >= 0 && max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size < (1ll << 31),
+  KGE_REQUIRE(T >= 0 && T <= (1 << 30) && num_free >= 0 && max_blocks_per_seq > 0 && (int64_t)max_blocks_per_seq * block_size < (1ll << 31),
               "kge_step_maps: %d rows, %d free blocks, %d blocks of %d tokens a request", T, num_free, max_blocks_per_seq, block_size);
   MapArgs a;
   a.table = block_table; a.lens = seq_lens; a.qsl = query_start_loc; a.positions = positions; a.counts = counts; a.slots = slot_mapping;

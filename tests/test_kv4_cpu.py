@@ -58,6 +58,19 @@ def test_maps_refusals(kge, change, words):
     refused(kge, kge.lib().kge_step_maps(*a.values(), None), words)
 
 
+def test_sizes_beyond_32_bits_are_refused(kge):
+    """Products and sums of sizes that an int does not hold, the ones that come out small again among them."""
+    L = kge.lib()
+    for H, KV, stride in ((3, 2 ** 31 - 1, 256), (1, 2 ** 30, 256), (2 ** 25 + 1, 1, 128), (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 8)):
+        refused(kge, L.kge_rope_kv4write(P, stride, P, P, P, P, P, 3, H, KV, 128, 16, None), "heads of|apart")
+    for H, KV, stride in ((2 ** 25, 2 ** 25, 8), (2 ** 24, 2 ** 24, 2 ** 31 - 8), (2 ** 25 + 1, 2 ** 25 + 1, 256)):
+        refused(kge, L.kge_paged_attn_kv4(P, P, stride, P, P, 4, P, P, 3, 3, 1, 50, H, KV, 128, 16, 0.125, 0, 0, P, 1 << 30, None), "q_stride")
+    refused(kge, L.kge_step_maps(P, 4, P, P, P, P, P, P, P, P, 9, P, 3, 2 ** 31 - 1, 16, None), "rows")
+    refused(kge, L.kge_kv4_read(P, P, P, P, 2 ** 31 - 1, 2 ** 31 - 1, 128, 16, None), "in one call")
+    for sizes in ((2 ** 40, 2 ** 20, 128, 64), (2 ** 62, 1, 64, 16), (2 ** 33, 2 ** 31 - 1, 128, 2 ** 30)):
+        assert L.kge_kv4_cache_bytes(*sizes) < 0 and b"bytes" in L.kge_last_error()
+
+
 def test_calls_without_rows_do_nothing(kge):
     L = kge.lib()
     assert L.kge_rope_kv4write(P, 256, P, P, P, P, P, 0, 4, 2, 64, 16, None) == 0
