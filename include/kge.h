@@ -219,7 +219,8 @@ int kge_kv4_read(void* k_out, void* v_out, const void* kv_cache, const int64_t* 
  *  - H / KV up to 128; scale > 0; q_stride >= H * hd; out, q, kv_cache and workspace 16-byte aligned; at most 2^30 tokens a request
  *  - T may be larger than the rows of all requests (a captured step with room to spare): rows behind query_start_loc[B] are left alone,
  *    as are requests without rows; max_q_len and max_seq_len are upper bounds.  A row without a key (seq_lens 0) is zeros.
- *  - a NaN row of the cache makes NaN of the queries that see it, and of no others
+ *  - a NaN row of the cache makes NaN of the queries that see it, and of no others; nor do finite rows, however large, change a bit of
+ *    what a query gets that does not see them
  * `workspace`: device scratch of kge_attn_kv4_workspace_bytes(H, KV, hd), whatever the batch is, for H / KV <= 16 (otherwise 0 and NULL
  * will do); nothing in it needs clearing, and calls that share one must not overlap on the GPU. */
 int kge_paged_attn_kv4(void* out, const void* q, int q_stride, const void* kv_cache, const int32_t* block_table,

@@ -3,26 +3,23 @@
 // and probabilities in TMEM, work from the hardware's queue of CTAs not yet launched.
 //
 // What differs is how keys and values become operands.  A producer brings the groups of 64 keys as they lie in the pages (hd + 8 bytes a key, a
-// quarter of 16-bit rows) into a ring, and four warps of their own turn codes into the 128-byte-swizzled tiles that the MMAs read.  Both builds
-// multiply float16, whose 11 bits a rounding costs an eighth of bfloat16's:
-//   bfloat16 model  Rows become numbers 2^E (low + s n), rounded once (a code's bits ARE the float16 number n 2^-24: one AND, one FMA for two).  E
-//                   (keys) and F (values) are the tile's, so that its largest row keeps the range; numbers below 2^-10 of that lose bits, at
-//                   2^-21 of it they end.  Only keys that a query sees count.  Q is turned to float16 in place, with a power of two per row, and
-//                   x = scale 2^-(E + e) S       P = 2^(x - F - R)       out = sum P V / sum 2^F P
-//   float16 model   float16 rows would round twice as much as the result does, so tiles hold n - 8, which is exact, and the softmax applies the
-//                   rows' numbers in fp32 (z = low + 8 s):
-//                   x = scale (s_k S + z_k sum(q))       e = 2^(x - R)       P = e s_v       out = (sum P (n - 8) + sum e z_v) / sum e
-//                   which costs 64 more shared loads of 16 bytes a tile and thread: 130 us against 105 with rows (32 heads, below).
-// R is the largest x - F (x + log2 of the tile's largest s_v) less 6, so that P is 2^6 at its reference, and moves when P would pass 2^14: weights
-// lose bits 2^20 below the largest, whatever the values' scale.
-// Error against 64 bits, largest: bfloat16 0.0017, float16 0.0003, of which the result's own rounding is 0.0016 and 0.00021 (rows and weights
-// in the model's type: 0.0029 and 0.00041).  Times with exact codes / float16 rows / rows and weights in bfloat16, us: prompts of 32 / 8
-// heads of 128 199 / 182 / 163, with a window 138 / 125 / 113; what the last saves is Q's turn (10) and the tile's exponents.
+// quarter of 16-bit rows) into a ring, and four warps of their own turn codes into the 128-byte-swizzled tiles that the MMAs read: n - 8, which is
+// exact, of keys in the model's type, as Q is, of values in float16, as the weights are in either build.  The two numbers of a row are applied in
+// fp32 by the softmax (z = low + 8 s):
+//   x = scale (s_k S + z_k sum(q))       e = 2^(x - R)       P = e s_v       out = (sum P (n - 8) + sum e z_v) / sum e
+// so besides the result only P is rounded to 16 bits, and nothing that a query gets hangs on rows that it does not see, not even in its last bit:
+// scores, numbers and R are its own, and masked weights are zeros that meet finite codes.  (Rows as float16 numbers with a power of two for a tile
+// save the 64 shared loads of 16 bytes a tile and thread that the numbers cost, 182 us against 206 below, but a tile's largest row decides what the
+// others keep: a key 10^5 times as large spoilt queries in front of it.)
+// R is the largest x_j + m_j that its row sees, m_j = log2 of max(2^-6 s_v, 2^-90 |z_v|, 2^-90), of the first tile that it sees something of: P is
+// at most 2^6, and e, e z_v and their sums stay finite whatever the values are.  It moves when a P may pass 2^14 (or they 2^98), so weights lose bits
+// 2^20 below the largest.  It is kept in two parts, a score and an m: scores may be so large that their sum would lose the m (3 % of the time).
+// Error against 64 bits, largest: bfloat16 0.0017, float16 0.0003, of which the result's own rounding is 0.0016 and 0.00021.
 // The turning warps need few registers and the softmax many: 512 threads start with 128 each, and setmaxnreg hands 40 of each of eight warps'
 // to the eight softmax warps (168 and 88: 128 (2 x 168 + 2 x 88) = 65536, what the launch holds).
-//   * Rows that read as NaN (kv4.cuh) must not reach queries that do not see them, and infinity or NaN times a weight of zero is none: such a
-//     key's value is zeros (s_v = z_v = 0) here and its key row (s_k) is NaN, so every query that sees it gets NaN from its score and no other does.
-//   * Rows that no query of the item sees (behind the last key, in front of the windows) are zeros, whatever the page holds.
+//   * Rows that read as NaN (kv4.cuh) must not reach queries that do not see them: such a key has s_v = z_v = 0 here and s_k is NaN, so every query
+//     that sees it gets NaN from its score and no other does.
+//   * Rows behind the last key are zeros, whatever the page holds.
 //   * A window with first tokens that stay visible: tiles of the first tokens, then those of the windows; only tiles at a border are masked.
 namespace atc4 {
 using namespace atc;
@@ -32,18 +29,10 @@ constexpr int kThreads = 512;                  // warps 0-3 and 4-7: softmax of 
 constexpr int NST = 3, NRAW = 3;               // K tiles and as many V tiles; tiles of codes
 constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "the register shares are what the launch holds");
-#ifdef KGE_HALF
-constexpr bool kCodes = true;                  // tiles hold codes n - 8, or the rows' numbers
-constexpr int NEXP = 1;
-constexpr int kNumbers = 1024 + 16;            // of a stage: per pair of keys (s, s, z, z) of the keys and of the values; log2 of the largest s_v
-#else
-constexpr bool kCodes = false;
-constexpr int NEXP = 8;                        // tiles whose (E, F, 2^F) are kept, see the barriers
-constexpr int kNumbers = (NEXP * 16 + NST * 16 - 1) / (NST * 16) * 16;       // (room for them, in NST parts)
-#endif
-constexpr float kLeastTop = 6.f;               // a row's largest P is 2^6 when its reference is set, and 2^(6 + kRescaleThreshold) at most
+constexpr int kNumbers = 1024 + 256 + 16;      // of a stage: per pair of keys (s, s, z, z) of the keys and of the values; m of each key; the largest of 32 each
+constexpr float kLeastTop = 6.f, kRoom = 90.f; // log2 of a row's largest P when R is set; of the largest e, or e z_v
 template <int HD> constexpr int raw_bytes() { return 4 * kv4::group_bytes(HD); }
-template <int HD> constexpr int smem_bytes() { return (2 * 128 + 2 * NST * BNK) * HD * 2 + NRAW * raw_bytes<HD>() + NST * kNumbers + 512 + 8 * 4096 + 128 * 16 + (kCodes ? 0 : 512); }
+template <int HD> constexpr int smem_bytes() { return (2 * 128 + 2 * NST * BNK) * HD * 2 + NRAW * raw_bytes<HD>() + NST * kNumbers + 512 + 8 * 4096 + 128 * 16; }
 
 // n0, n1: key tiles of the two query tiles; n1 < 0: no more work.  split: one query tile, its even key tiles are the first warps', its odd ones
 // the second's.  Tile j holds the keys from 64 j (j < ptiles: first tokens that stay visible) or from 64 (tile_lo + j - ptiles).
@@ -71,28 +60,19 @@ __device__ __forceinline__ void expand(uint32_t w, uint32_t (&r)[4]) {
     else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r[p]) : "r"((u & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));
   }
 }
-// The float16 numbers of a row: s 2^24, s 2^20 and low, each twice in a word.
-struct RowNumbers { uint32_t s24, s20, low; };
+// the same as numbers of the model's type
+__device__ __forceinline__ void expand_key(uint32_t w, uint32_t (&r)[4]) {
+#ifdef KGE_HALF
+  expand(w, r);
+#else
+#pragma unroll
+  for (int p = 0; p < 4; ++p) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[p]) : "r"(((w >> (4 * p)) & 0x000f000fu) | 0x43004300u), "r"(0x43084308u));      // 0x4300 | n = 128 + n
+#endif
+}
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }      // -126 <= e <= 127
-// eight codes n -> eight numbers low + s n, rounded once, in order: a code's bits are the float16 number n 2^-24, or n 2^-20 four bits further up
-__device__ __forceinline__ void expand(uint32_t w, const RowNumbers& c, uint32_t (&r)[4]) {
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const uint32_t u = p < 2 ? w : w >> 8;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[p]) : "r"(u & (p & 1 ? 0x00f000f0u : 0x000f000fu)), "r"(p & 1 ? c.s20 : c.s24), "r"(c.low));
-  }
-}
-// The power of two that a tile's rows are multiplied with: the largest s comes to [2^-9, 2^-8), so that s 2^24 is a float16 number, unless a low
-// would pass 2^15.  `most`: over the rows, the largest of the bits of s and those of |low| / 2^23, as fp32 (0: a tile of zeros).  At most 2^90: sums of
-// 2^90 P over 2^20 keys and more stay finite.
-__device__ __forceinline__ int tile_exponent(int most) { return most < (1 << 23) ? 0 : min(max(118 - (most >> 23), -133), 90); }
-__device__ __forceinline__ int row_most(uint32_t p) {
-  return max((int)__float_as_uint(bf_lo(p)), (int)(__float_as_uint(bf_hi(p)) & 0x7fffffffu) - (23 << 23));
 }
 __device__ __forceinline__ bool finite2(uint32_t p) {    // both 16-bit numbers of a row
 #ifdef KGE_HALF
@@ -107,8 +87,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_constant__ CUtensorMap tm_q1, bf16* __restrict__ out, const KvArgs ka) {
   constexpr uint32_t Q_TILE = 128 * HD * 2, TILE = BNK * HD * 2, RAW = (uint32_t)(4 * kv4::group_bytes(HD)), GB = (uint32_t)kv4::group_bytes(HD);
   constexpr uint32_t S_COL = 256;              // TMEM: O0 and O1, then per query tile the scores (64 columns) and two buffers of probabilities (32 each)
-  constexpr uint32_t IDESC_S = (1u << 4)  | ((uint32_t)(BNK >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-  constexpr uint32_t IDESC_O = (1u << 4)  | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  constexpr uint32_t IDESC_S = (1u << 4) | KGE_IDESC_AB | ((uint32_t)(BNK >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   if ((s_addr(smem_raw) & 1023u) != 0) __trap();
   const uint32_t sQ = s_addr(smem_raw), sK = sQ + 2 * Q_TILE, sV = sK + NST * TILE;
@@ -117,7 +97,6 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   uint8_t* tail = numbers + NST * kNumbers;
   uint8_t* stage_out = tail + 512;
   float4* part = reinterpret_cast<float4*>(stage_out + 8 * 4096);
-  int* q_exps = reinterpret_cast<int*>(part + 128);                    // per row of a shared query tile
   const uint32_t bar0 = s_addr(tail);
   Item* items = reinterpret_cast<Item*>(tail + 288);                   // 2 slots of 48 bytes
   const uint32_t clc_resp = bar0 + 384;
@@ -131,11 +110,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   //   k_full, v_full: 4 arrivals of the turning warps; k_empty, v_empty: a commit of each issuer, waited for by the turning warps before they
   //   write the stage again.  The numbers of a stage are written with its values and read by the softmax, which waits for v_full too: the
   //   next phase of it needs v_empty, that a P V, and that the P of the waiter
-  //   q_empty       a commit of each issuer, and the softmax warps, which have read or turned their rows of Q
-  //   q_ready(a)    the softmax warps of group a; an issuer and, of a shared query tile, the other group wait for it before they let q_empty go
-  // (E, F, 2^F) of tile j are written before k_full(j), which an issuer waits for before the products whose commit the softmax waits for.  They
-  // are written again for tile j + NEXP: who begins that tile has written the values before it, into a stage from which both issuers had
-  // taken the products of four tiles before, and they had waited for the P of every tile of theirs up to there.
+  //   q_empty       a commit of each issuer, and the softmax warps, which have summed their rows of Q
   auto k_full = [&](int s) { return bar0 + 8u * s; };
   auto k_empty = [&](int s) { return bar0 + 24u + 8u * s; };
   auto v_full = [&](int s) { return bar0 + 48u + 8u * s; };
@@ -149,7 +124,6 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
   auto item_full = [&](int s) { return bar0 + 240u + 8u * s; };
   auto item_empty = [&](int s) { return bar0 + 256u + 8u * s; };
   const uint32_t q_full = bar0 + 272u, q_empty = bar0 + 280u, clc_full = bar0 + 408u;
-  auto q_ready = [&](int a) { return kCodes ? q_full : bar0 + 416u + 8u * a; };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int G = ka.H / ka.KV, TT = BM / G, TI = ka.per * TT;           // tokens of a query tile, of an item
 
@@ -163,7 +137,6 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         mbar_init(item_full(a), 1); mbar_init(item_empty(a), 14);      // 8 softmax warps, 2 issuers, 4 turning warps
       }
       mbar_init(q_full, 1); mbar_init(q_empty, 10); mbar_init(clc_full, 1);
-      if (!kCodes) { mbar_init(q_ready(0), 4); mbar_init(q_ready(1), 4); }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
@@ -315,7 +288,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
           if (n1 < 0) break;
           const int n = split ? n0 + n1 : max(n0, n1), na = a ? n1 : n0, ahead = 1 + split;
           const uint64_t qd = desc_kmajor(sQ + (split ? 0 : a) * Q_TILE);
-          mbar_wait(q_ready(split ? 0 : a), ni & 1);
+          mbar_wait(q_full, ni & 1);
           bool first = true;                             // no product P V of this item yet
           for (int j = -ahead; j < n; ++j) {
             const int js = j + ahead;
@@ -376,22 +349,15 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         const int n = it.split ? it.n0 + it.n1 : max(it.n0, it.n1);
         for (int j = 0; j < n; ++j, ++nk) {
           const int st = nk % NST, rs = nk % NRAW;
-          const int key0 = (j < it.ptiles ? j : it.tile_lo + j - it.ptiles) * BNK, left = it.kv_len - key0;      // keys from this tile on
-          const int from = ka.window > 0 ? it.ctx0 + it.tok0 - ka.window + 1 - key0 : 0, keep = ka.first - key0;
-          auto seen = [&](int row) { return row < left && (row >= from || row < keep); };      // by one of the item's queries
+          const int left = it.kv_len - (j < it.ptiles ? j : it.tile_lo + j - it.ptiles) * BNK;      // keys from this tile on
           mbar_wait(raw_full(rs), (nk / NRAW) & 1);
           // everything that this thread needs of the tile's codes is read at once
-          auto pair_at = [&](int row) {                  // the two numbers of a row's key and of its value
-            const uint8_t* g = raw + rs * RAW + (row >> 4) * GB + 16 * HD + (row & 15) * 4;
-            return make_uint2(*reinterpret_cast<const uint32_t*>(g), *reinterpret_cast<const uint32_t*>(g + 64));
-          };
-          const uint2 first_p = pair_at(kCodes ? d & 63 : lane), second_p = kCodes ? first_p : pair_at(lane + 32);
-          uint2 own_p[2];
+          const uint8_t* pairs = raw + rs * RAW + ((d & 63) >> 4) * GB + 16 * HD + (d & 15) * 4;       // the numbers of key d
+          const uint32_t pk = *reinterpret_cast<const uint32_t*>(pairs), pv = *reinterpret_cast<const uint32_t*>(pairs + 64);
           uint32_t w[2][2][4];                           // of keys and values: W words of two rows
 #pragma unroll
           for (int pass = 0; pass < 2; ++pass) {
             const int grp = (s >> 4) + 2 * pass;
-            own_p[pass] = kCodes ? make_uint2(0, 0) : pair_at(grp * 16 + tok);
 #pragma unroll
             for (int part_v = 0; part_v < 2; ++part_v) {
               const int at = part_v ? 8 * HD + tok * (HD / 2) + 4 * kv4::value_word(HD, tok, W * t) : kv4::key_row(tok) * (HD / 2) + 4 * W * t;
@@ -405,38 +371,8 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
               }
             }
           }
-          int ex[2] = {0, 0};                            // E and F
-          if (!kCodes) {
-            int most_k = 0, most_v = 0;
-            if (seen(lane) && finite2(first_p.x) && finite2(first_p.y)) { most_k = max(0, row_most(first_p.x)); most_v = max(0, row_most(first_p.y)); }
-            if (seen(lane + 32) && finite2(second_p.x) && finite2(second_p.y)) { most_k = max(most_k, row_most(second_p.x)); most_v = max(most_v, row_most(second_p.y)); }
-            ex[0] = tile_exponent(__reduce_max_sync(0xffffffffu, most_k));
-            ex[1] = tile_exponent(__reduce_max_sync(0xffffffffu, most_v));
-            if (d == 0) reinterpret_cast<float4*>(numbers)[nk % NEXP] = make_float4(__int_as_float(ex[0]), (float)ex[1], pow2(ex[1] >> 1) * pow2(ex[1] - (ex[1] >> 1)), 0.f);
-          }
 #pragma unroll
           for (int part_v = 0; part_v < 2; ++part_v) {
-            const float up0 = pow2(ex[part_v] >> 1), up1 = pow2(ex[part_v] - (ex[part_v] >> 1));       // (2^-133 is no normal number)
-            RowNumbers c[2];
-#pragma unroll
-            for (int pass = 0; pass < 2; ++pass) {
-              const int row = ((s >> 4) + 2 * pass) * 16 + tok;
-              c[pass] = {0, 0, 0};
-              if (kCodes) {
-                if (row >= left) {                       // (the other warps multiply these with weights of zero)
-#pragma unroll
-                  for (int i = 0; i < W; ++i) w[part_v][pass][i] = 0x88888888u;
-                }
-              } else if (seen(row)) {
-                if (finite2(own_p[pass].x) && finite2(own_p[pass].y)) {
-                  const uint32_t u = part_v ? own_p[pass].y : own_p[pass].x;
-                  const float sc = bf_lo(u) * up0 * up1, low = bf_hi(u) * up0 * up1;
-                  c[pass].s24 = pack_h2(sc * 16777216.f, sc * 16777216.f); c[pass].s20 = pack_h2(sc * 1048576.f, sc * 1048576.f); c[pass].low = pack_h2(low, low);
-                } else if (!part_v) {
-                  c[pass].low = 0x7fff7fffu;
-                }
-              }
-            }
             if (nk >= (uint32_t)NST) mbar_wait(part_v ? v_empty(st) : k_empty(st), (nk / NST - 1) & 1);
             const uint32_t dst = (part_v ? sV : sK) + st * TILE;
 #pragma unroll
@@ -444,23 +380,26 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
               const int row = ((s >> 4) + 2 * pass) * 16 + tok;
 #pragma unroll
               for (int i = 0; i < W; ++i) {
-                const uint32_t x = swap ? w[part_v][pass][i ^ 1] : w[part_v][pass][i];
+                // (a row behind the last key: the other warps multiply it with weights of zero)
+                const uint32_t x = row >= left ? 0x88888888u : swap ? w[part_v][pass][i ^ 1] : w[part_v][pass][i];
                 uint32_t r[4];
-                if (kCodes) expand(x, r);
-                else expand(x, c[pass], r);
+                if (part_v) expand(x, r);
+                else expand_key(x, r);
                 st_shared16(dst + tile_off<BNK>(row, W * t + (swap ? i ^ 1 : i)), r);
               }
             }
-            if (kCodes && part_v && d < 64) {            // warps 12 and 13: the numbers of key d
-              const uint32_t pk = first_p.x, pv = first_p.y;
+            if (part_v && d < 64) {                      // warps 12 and 13: the numbers of key d
               const bool there = d < left, fine = finite2(pk) && finite2(pv);
               const float nan = __uint_as_float(0x7fffffffu);
               const float sk = there ? (fine ? bf_lo(pk) : nan) * ka.scale_log2 : 0.f, zk = there && fine ? fmaf(8.f, bf_lo(pk), bf_hi(pk)) * ka.scale_log2 : 0.f;
               const float sv = there && fine ? bf_lo(pv) : 0.f, zv = there && fine ? fmaf(8.f, sv, bf_hi(pv)) : 0.f;
               float* to = reinterpret_cast<float*>(numbers + st * kNumbers) + (d >> 1) * 8 + (d & 1);
               to[0] = sk; to[2] = zk; to[4] = sv; to[6] = zv;
-              const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(sv));
-              if (lane == 0) reinterpret_cast<float*>(numbers + st * kNumbers + 1024)[d >> 5] = fmaxf(__log2f(__uint_as_float(most)), -60.f);
+              const float m = fmaxf(fmaxf(__log2f(sv) - kLeastTop, __log2f(fabsf(zv)) - kRoom), -kRoom);
+              float* ms = reinterpret_cast<float*>(numbers + st * kNumbers + 1024);
+              ms[d] = m;
+              const int most = __reduce_max_sync(0xffffffffu, __float2int_ru(m));
+              if (lane == 0) ms[64 + (d >> 5)] = (float)most;
             }
             fence_async_smem();
             __syncwarp();
@@ -485,53 +424,18 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
       if (it.n1 < 0) break;
       const int n = a ? it.n1 : it.n0, n_item = it.split ? it.n0 + it.n1 : max(it.n0, it.n1);
       const int qt = it.split ? 0 : a;                                 // the query tile of these warps
-      // this thread's row of Q: its sum, or its float16 numbers, of which the largest comes to [2^13, 2^14), in place of bfloat16 ones
+      // sum(q) of this thread's row
       mbar_wait(q_full, ni & 1);
       float qsum = 0.f;
-      int q_ex = 0;
-      if (kCodes ? n > 0 : n > 0 && qt == a) {
-        if (!kCodes && a) mbar_wait(q_ready(0), ni & 1);               // (one after the other: shared memory's rate bounds this)
-        uint8_t* row = smem_raw + qt * Q_TILE;
-        uint4 u[HD / 8];
-        uint32_t most = 0;
+      if (n > 0) {
+        const uint8_t* row = smem_raw + qt * Q_TILE;
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c) {
-          u[c] = *reinterpret_cast<const uint4*>(row + tile_off<128>(r, c));
-          const uint32_t* v = &u[c].x;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (kCodes) {
-              qsum += bf_lo(v[i]) + bf_hi(v[i]);
-            } else {
-              const uint32_t x = v[i] << 16 & 0x7fffffffu, y = v[i] & 0x7fff0000u;
-              most = max(most, max(x < 0x7f800000u ? x : 0u, y < 0x7f800000u ? y : 0u));
-            }
-          }
-        }
-        if (!kCodes) {
-          q_ex = most ? min(max(140 - (int)(most >> 23), -100), 100) : 0;
-          const float up = pow2(q_ex);
-#pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            const uint32_t* v = &u[c].x;
-            uint4 w;
-            w.x = pack_h2(bf_lo(v[0]) * up, bf_hi(v[0]) * up);
-            w.y = pack_h2(bf_lo(v[1]) * up, bf_hi(v[1]) * up);
-            w.z = pack_h2(bf_lo(v[2]) * up, bf_hi(v[2]) * up);
-            w.w = pack_h2(bf_lo(v[3]) * up, bf_hi(v[3]) * up);
-            *reinterpret_cast<uint4*>(row + tile_off<128>(r, c)) = w;
-          }
-          if (it.split) q_exps[r] = q_ex;
-          fence_async_smem();
+          const uint4 u = *reinterpret_cast<const uint4*>(row + tile_off<128>(r, c));
+          qsum += ((bf_lo(u.x) + bf_hi(u.x)) + (bf_lo(u.y) + bf_hi(u.y))) + ((bf_lo(u.z) + bf_hi(u.z)) + (bf_lo(u.w) + bf_hi(u.w)));
         }
       }
       __syncwarp();
-      if (!kCodes && lane == 0) mbar_arrive(q_ready(a));
-      if (!kCodes && qt != a) {                                        // the other group turns the rows
-        mbar_wait(q_ready(0), ni & 1);
-        q_ex = q_exps[r];
-        __syncwarp();
-      }
       if (lane == 0) mbar_arrive(q_empty);
       if (n <= 0) { nk += n_item; continue; }
       const f2 qs2 = pk(qsum, qsum);
@@ -539,7 +443,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
       const int row_tok = it.tok0 + qt * TT + tk;
       const int lim = row_ok ? it.ctx0 + row_tok : -1;                 // last visible key of this row
       const int lo_row = ka.window > 0 ? lim - ka.window + 1 : 0;      // the window's first key; below it only the first tokens
-      float m_ref = -INFINITY, l = 0.f, zs = 0.f;
+      float x_ref = 0.f, m_ref = -INFINITY, l = 0.f, zs = 0.f;         // R = x_ref + m_ref; none yet: -inf
       // the second group's exponentials start when the first's of its first tile are done (attn_pair.cuh)
       const bool turns = it.n1 >= 3;
       for (int j = 0; j < n; ++j) {
@@ -554,63 +458,77 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         if (lane == 0) mbar_arrive(s_read(a));                         // the next tile's scores may be written
         const int jt = it.split ? 2 * j + a : j, kbase = (jt < it.ptiles ? jt : it.tile_lo + jt - it.ptiles) * BNK;
         const int vis = lim - kbase, from = lo_row - kbase, keep = ka.first - kbase;      // column i is visible: i <= vis and (i >= from or i < keep)
-        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         const int st = (nk + jt) % NST;
-        if (kCodes) mbar_wait(v_full(st), ((nk + jt) / NST) & 1);      // the numbers of the tile's keys and values
+        mbar_wait(v_full(st), ((nk + jt) / NST) & 1);                  // the numbers of the tile's keys and values
         const ulonglong2* num = reinterpret_cast<const ulonglong2*>(numbers + st * kNumbers);
-        float sc = 1.f, shift, unit = 1.f;                             // score = sc S; P = 2^(score - R - shift), e = P unit
-        if (kCodes) {
+        const f2 nx2 = pk(-x_ref, -x_ref);
 #pragma unroll
-          for (int i = 0; i < BNK / 2; ++i) {
-            const ulonglong2 sz = num[2 * i];
-            float x0, x1;
-            upk(fma2(pk(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sz.x, mul2(qs2, sz.y)), x0, x1);
-            sv[2 * i] = __float_as_uint(x0); sv[2 * i + 1] = __float_as_uint(x1);
-          }
-          const float2 lgs = *reinterpret_cast<const float2*>(numbers + st * kNumbers + 1024);
-          shift = -fmaxf(lgs.x, lgs.y);
-        } else {
-          const float4 ef = reinterpret_cast<const float4*>(numbers)[(nk + jt) % NEXP];
-          sc = fmaxf(ka.scale_log2 * pow2(min(max(-(__float_as_int(ef.x) + q_ex), -126), 126)), 1e-37f);      // (above 0: times -inf stays -inf)
-          shift = ef.y;
-          unit = ef.z;
+        for (int i = 0; i < BNK / 2; ++i) {                            // x - x_ref
+          const ulonglong2 sz = num[2 * i];
+          float x0, x1;
+          upk(fma2(pk(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sz.x, fma2(qs2, sz.y, nx2)), x0, x1);
+          sv[2 * i] = __float_as_uint(x0); sv[2 * i + 1] = __float_as_uint(x1);
         }
         if (!__all_sync(0xffffffffu, vis >= BNK - 1 && (from <= 0 || keep >= BNK))) {
 #pragma unroll
           for (int i = 0; i < BNK; ++i) sv[i] = i <= vis && (i >= from || i < keep) ? sv[i] : 0xff800000u;
         }
+        // Whether R has to be set or moved: not where the largest score and the largest m of the tile, be it of keys that this row does not see,
+        // stay below its bound; else the row's own keys say.
+        float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < BNK; i += 8)
 #pragma unroll
           for (int k = 0; k < 4; ++k) mxa[k] = max3(mxa[k], __uint_as_float(sv[i + 2 * k]), __uint_as_float(sv[i + 2 * k + 1]));
-        const float mx = max3(fmaxf(mxa[0], mxa[1]), mxa[2], mxa[3]) * sc - (shift + kLeastTop);      // -inf stays -inf
-        const bool grow = mx > m_ref + kRescaleThreshold;              // includes the first finite maximum
-        if (__any_sync(0xffffffffu, grow)) {
-          float alpha = 1.f;
-          if (grow) {
-            alpha = (m_ref == -INFINITY) ? 0.f : exp2f(m_ref - mx);
-            m_ref = mx;
-            l *= alpha;
-            zs *= alpha;
-          }
-          if (j > 0) {
-            mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);         // P V of the tile before
-            tc_after();
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              uint32_t v[16];
-              asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                           : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
-                             "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(t_o + c));
-              tmem_wait_ld(v);
+        const float2 m_most = *reinterpret_cast<const float2*>(numbers + st * kNumbers + 1024 + 256);
+        const float high = max3(fmaxf(mxa[0], mxa[1]), mxa[2], mxa[3]);          // -inf: no key, or only NaN rows
+        if (__any_sync(0xffffffffu, high + (fmaxf(m_most.x, m_most.y) - m_ref) > kRescaleThreshold)) {
+          const ulonglong2* lg = num + 64;
+          float top[2] = {-INFINITY, -INFINITY};
+          const float less = high > -INFINITY ? -high : 0.f;           // what a new x_ref changes
+          const f2 nh2 = pk(less, less);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-              tmem_st16(t_o + c, v);
+          for (int i = 0; i < BNK; i += 4) {
+            const ulonglong2 m = lg[i / 4];
+            float x0, x1, x2, x3;
+            upk(add2(add2(pk(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), nh2), m.x), x0, x1);
+            upk(add2(add2(pk(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), nh2), m.y), x2, x3);
+            top[i / 4 & 1] = max3(max3(top[i / 4 & 1], x0, x1), x2, x3);
+          }
+          const float m_new = fmaxf(top[0], top[1]), up = high + (m_new - m_ref);
+          const bool grow = up > kRescaleThreshold;
+          if (__any_sync(0xffffffffu, grow)) {
+            float alpha = 1.f, by = 0.f;
+            if (grow) {
+              const float half = exp2f(-0.5f * up);                    // twice the half: the sums may be as large as the change
+              alpha = half * half;
+              l = l * half * half;
+              zs = zs * half * half;
+              x_ref += high;
+              m_ref = m_new;
+              by = less;
+            }
+#pragma unroll
+            for (int i = 0; i < BNK; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) + by);
+            if (j > 0) {
+              mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);       // P V of the tile before
+              tc_after();
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 16) {
+                uint32_t v[16];
+                asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                               "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(t_o + c));
+                tmem_wait_ld(v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                tmem_st16(t_o + c, v);
+              }
             }
           }
         }
         const float base = (m_ref == -INFINITY) ? 0.f : m_ref;
-        const f2 nb2 = kCodes ? pk(-base, -base) : pk(-(base + shift), -(base + shift)), sc2 = pk(sc, sc);
+        const f2 nb2 = pk(-base, -base);
         f2 rs[2] = {0, 0}, zr[2] = {0, 0};
         if (ns >= 2) { mbar_wait(o_full(a, ns), ((ns - 2) >> 1) & 1); tc_after(); }       // P V of two tiles before has read this buffer
         if (turns && j == 0 && a == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -621,15 +539,12 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float p0, p1;
-            const f2 x = pk(__uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1]));
-            upk(kCodes ? add2(x, nb2) : fma2(x, sc2, nb2), p0, p1);
-            p0 = ex2_ftz(p0); p1 = ex2_ftz(p1);                        // masked: -inf -> 0
-            rs[i & 1] = add2(rs[i & 1], pk(p0, p1));
-            if (kCodes) {
-              const ulonglong2 sz = num[c + 2 * i + 1];
-              zr[i & 1] = fma2(pk(p0, p1), sz.y, zr[i & 1]);
-              upk(mul2(pk(p0, p1), sz.x), p0, p1);
-            }
+            upk(add2(pk(__uint_as_float(sv[c + 2 * i]), __uint_as_float(sv[c + 2 * i + 1])), nb2), p0, p1);
+            const f2 e = pk(ex2_ftz(p0), ex2_ftz(p1));                 // masked: -inf -> 0
+            const ulonglong2 sz = num[c + 2 * i + 1];
+            rs[i & 1] = add2(rs[i & 1], e);
+            zr[i & 1] = fma2(e, sz.y, zr[i & 1]);
+            upk(mul2(e, sz.x), p0, p1);
             pkd[i] = pack_h2(p0, p1);
           }
           tmem_st16(t_p + c / 2, pkd);
@@ -640,25 +555,26 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(a, ns));
         ++ns;
-        l = fmaf(unit, sum2(add2(rs[0], rs[1])), l);
-        if (kCodes) zs += sum2(add2(zr[0], zr[1]));
+        l += sum2(add2(rs[0], rs[1]));
+        zs += sum2(add2(zr[0], zr[1]));
       }
       mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);
       tc_after();
       float mine = 1.f, other = 0.f;                                   // weights of the two halves of a split row
       if (it.split) {
-        if (a) part[r] = make_float4(m_ref, l, zs, 0.f);
+        if (a) part[r] = make_float4(x_ref, m_ref, l, zs);
         tc_before();
         asm volatile("bar.sync 2, 256;" ::: "memory");
         tc_after();
         if (!a) {
           const float4 p1 = part[r];
-          const float m = fmaxf(m_ref, p1.x);
-          mine = m_ref == -INFINITY ? (l == l ? 0.f : l) : exp2f(m_ref - m);      // (a half that saw nothing but NaN keeps it)
-          other = p1.x == -INFINITY ? (p1.y == p1.y ? 0.f : p1.y) : exp2f(p1.x - m);
-          l = l * mine + p1.y * other;
-          zs = zs * mine + p1.z * other;
-          m_ref = m;
+          const float up = (p1.x - x_ref) + (p1.y - m_ref);            // R of the other half less this one's
+          const float half0 = m_ref == -INFINITY ? (l == l ? 0.f : l) : exp2f(-0.5f * fmaxf(up, 0.f));      // (a half that saw nothing but NaN keeps it)
+          const float half1 = p1.y == -INFINITY ? (p1.z == p1.z ? 0.f : p1.z) : exp2f(0.5f * fminf(up, 0.f));
+          mine = half0 * half0;
+          other = half1 * half1;
+          l = l * half0 * half0 + p1.z * half1 * half1;
+          zs = zs * half0 * half0 + p1.w * half1 * half1;
         }
       }
       const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
@@ -685,7 +601,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         tc_before();                                                   // the next item's first P V comes behind p_full of these warps
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < (kCodes ? 64 : 0); ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + zs);
+        for (int i = 0; i < 64; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + zs);
 #pragma unroll
         for (int i = 0; i < 64; i += 8) {
           uint4 w;
