@@ -1,5 +1,5 @@
 """Attention over the 4-bit cache, row by row: what a query does not see changes none of its bits, rows of one context may lie as far apart as
-their type allows, and errors are no larger than what is rounded (kv4_oracle.allowed).
+their type allows, and errors are no larger than what is rounded (kv4_oracle.allowed); prompts that fill both query tiles of an item among them.
 
 In the 2-norm a rounding to the nearest of relative step 2 u is 0.392 u of its number where the leading digits are spread evenly over their
 logarithm (the mean of u^2 / 3 over that of x^2, x from 1 to 2); weights are rounded independently, which adds 0.392 2^-11 of their terms' root of
@@ -157,3 +157,39 @@ def test_values_near_the_ends_of_their_type(kge, L, hd, H, KV, lens, news, size)
     for b in range(len(lens)):
         s.v[b] *= size
     s.check(s.fill().run(kge))
+
+
+# -------------------------------------------------------------------------------------------- two query tiles of an item
+
+MANY = [  # dtype, hd, H, KV, block, lengths, rows
+    ("bf16", 128, 32, 8, 64, [700, 333, 150, 900], [700, 201, 150, 650]), ("fp16", 128, 32, 8, 16, [515, 640, 300], [515, 500, 300]),
+    ("bf16", 64, 64, 64, 32, [300, 299, 140], [300, 280, 129]), ("fp16", 64, 48, 16, 16, [411, 200, 390], [411, 200, 160]),
+    ("bf16", 128, 80, 4, 16, [270, 150, 333], [270, 101, 150]), ("fp16", 128, 40, 10, 128, [333, 640, 250], [333, 401, 250])]
+
+
+def tiles_of(H, KV, news):
+    """(query tiles of an item, whether some item has tokens in its second one), as the launch decides for at most 300 x 128 rows."""
+    TT, B, T = 128 // (H // KV), len(news), sum(news)
+    tiles = -(-max(news) // (2 * TT))
+    items = KV * (T // (2 * TT) + B) if tiles > 65535 or 2 * (T // (2 * TT) + B) < tiles * B else KV * B * tiles
+    return (1 if items <= 74 or items <= 148 else 2), any(n % (2 * TT) > TT or n >= 2 * TT for n in news)
+
+
+@pytest.mark.parametrize("dtype,hd,H,KV,bs,lens,news", MANY)
+@pytest.mark.parametrize("window,first", [(0, 0), (100, 4), (64, 0), (7, 130), (400, 70)])
+def test_prompts_of_two_query_tiles_an_item(kge, L, dtype, hd, H, KV, bs, lens, news, window, first):
+    """Enough items that each has two query tiles, walks of unequal length, odd tails and several items a CTA."""
+    assert tiles_of(H, KV, news) == (2, True)
+    s = Batch(dtype, hd, H, KV, bs, lens, news, seed=6).fill()
+    out = s.run(kge, window, first)
+    s.check(out, window, first, norm=True)
+    assert torch.equal(out, s.run(kge, window, first))               # the same bits again
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("news", [[1, 1, 1], [300, 100, 77]])
+def test_errors_are_the_roundings_alone(kge, L, dtype, news):
+    """In the 2-norm: the result's rounding and that of weights to float16, in either type."""
+    s = Batch(dtype, 128, 32, 8, 16, [1500, 200, 900], news, seed=7).fill()
+    s.check(s.run(kge), norm=True)
+    s.check(s.run(kge, 130, 7), 130, 7, norm=True)
