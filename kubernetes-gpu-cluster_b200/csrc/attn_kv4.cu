@@ -254,7 +254,7 @@ struct Core {
 #pragma unroll
           for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
           if (top == -INFINITY || !(fresh || over)) top = 0.f;    // (the first: only NaN rows)
-          const float f = ex2(-top);
+          const float f = fresh ? 1.f : ex2(-top);                // (2^-top may be infinite where the first one goes down, and the sums are zeros)
           ref[nt][h] += top;
           l[nt][h] *= f;
           zs[nt][h] *= f;

@@ -159,6 +159,26 @@ def test_values_near_the_ends_of_their_type(kge, L, hd, H, KV, lens, news, size)
     s.check(s.fill().run(kge))
 
 
+# ---------------------------------------------------------------------------------------------------- scores of any level
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd,H,KV,lens,news", [
+    (128, 4, 1, [1, 20, 64, 200], [1, 1, 1, 1]), (64, 12, 1, [900, 1], [1, 1]), (128, 16, 1, [3, 500], [1, 1]), (128, 32, 8, [1500], [1]), (64, 16, 2, [1300, 1], [1, 1]),
+    (128, 4, 1, [5, 90, 64], [5, 90, 7]), (64, 40, 2, [1, 90], [1, 90]), (128, 32, 8, [300] * 6, [300] * 6)])
+@pytest.mark.parametrize("level", [-1e6, -200, 200, 1e6])
+def test_all_scores_far_from_zero(kge, L, dtype, hd, H, KV, lens, news, level):
+    """Every score of a context lies about one level, far below or above zero: the first reference comes from there."""
+    s = Batch(dtype, hd, H, KV, 16, lens, news, seed=9)
+    for b in range(len(lens)):
+        s.k[b] *= 0.05
+        s.k[b][..., 0] = math.copysign(64, level)
+    s.q[..., 0] = 8
+    scale = abs(level) / 512                                         # the level is q k = 8 x 64 times that
+    out = s.fill().run(kge, scale=scale)
+    assert torch.isfinite(out).all()
+    s.check(out, scale=scale)
+
+
 # -------------------------------------------------------------------------------------------- two query tiles of an item
 
 MANY = [  # dtype, hd, H, KV, block, lengths, rows
