@@ -6,14 +6,15 @@
 // quarter of 16-bit rows) into a ring, and four warps of their own turn codes into the 128-byte-swizzled tiles that the MMAs read: n - 8, which is
 // exact, of keys in the model's type, as Q is, of values in float16, as the weights are in either build.  The two numbers of a row are applied in
 // fp32 by the softmax (z = low + 8 s):
-//   x = scale (s_k S + z_k sum(q))       e = 2^(x - R)       P = e s_v       out = (sum P (n - 8) + sum e z_v) / sum e
+//   x = scale (s_k S + z_k sum(q))       e = 2^(x - X)       P = 2^-M e s_v       out = (sum P (n - 8) + sum 2^-M e z_v) / (2^-M sum e)
 // so besides the result only P is rounded to 16 bits, and nothing that a query gets hangs on rows that it does not see, not even in its last bit:
-// scores, numbers and R are its own, and masked weights are zeros that meet finite codes.  (Rows as float16 numbers with a power of two for a tile
+// scores, numbers, X and M are its own, and masked weights are zeros that meet finite codes.  (Rows as float16 numbers with a power of two for a tile
 // save the 64 shared loads of 16 bytes a tile and thread that the numbers cost, 182 us against 206 below, but a tile's largest row decides what the
 // others keep: a key 10^5 times as large spoilt queries in front of it.)
-// R is the largest x_j + m_j that its row sees, m_j = log2 of max(2^-6 s_v, 2^-90 |z_v|, 2^-90), of the first tile that it sees something of: P is
-// at most 2^6, and e, e z_v and their sums stay finite whatever the values are.  It moves when a P may pass 2^14 (or they 2^98), so weights lose bits
-// 2^20 below the largest.  It is kept in two parts, a score and an m: scores may be so large that their sum would lose the m (3 % of the time).
+// X is the largest score of the first tile in which a row sees keys, M its largest x_j + m_j - X with m_j = log2 of max(2^-6 s_v, 2^-90 |z_v|,
+// 2^-90): P is at most 2^6 then, and 2^-M e z_v and the sums stay finite whatever the values are.  They move when a P may pass 2^14 (or z_v's sums
+// 2^98) or an e 2^60, so weights lose bits 2^20 below the largest.  (One number X + M for both: 3 % less time, but a large score swallows the M, and
+// where values are large their small e end before they count for nothing in sum e.)
 // Error against 64 bits, largest: bfloat16 0.0017, float16 0.0003, of which the result's own rounding is 0.0016 and 0.00021.
 // The turning warps need few registers and the softmax many: 512 threads start with 128 each, and setmaxnreg hands 40 of each of eight warps'
 // to the eight softmax warps (168 and 88: 128 (2 x 168 + 2 x 88) = 65536, what the launch holds).
@@ -30,7 +31,7 @@ constexpr int NST = 3, NRAW = 3;               // K tiles and as many V tiles; t
 constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs == 4 * 128, "the register shares are what the launch holds");
 constexpr int kNumbers = 1024 + 256 + 16;      // of a stage: per pair of keys (s, s, z, z) of the keys and of the values; m of each key; the largest of 32 each
-constexpr float kLeastTop = 6.f, kRoom = 90.f; // log2 of a row's largest P when R is set; of the largest e, or e z_v
+constexpr float kLeastTop = 6.f, kRoom = 90.f, kScoreRoom = 60.f;       // log2 of a row's largest P when M is set; of 2^-M z_v; of e
 template <int HD> constexpr int raw_bytes() { return 4 * kv4::group_bytes(HD); }
 template <int HD> constexpr int smem_bytes() { return (2 * 128 + 2 * NST * BNK) * HD * 2 + NRAW * raw_bytes<HD>() + NST * kNumbers + 512 + 8 * 4096 + 128 * 16; }
 
@@ -443,7 +444,7 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
       const int row_tok = it.tok0 + qt * TT + tk;
       const int lim = row_ok ? it.ctx0 + row_tok : -1;                 // last visible key of this row
       const int lo_row = ka.window > 0 ? lim - ka.window + 1 : 0;      // the window's first key; below it only the first tokens
-      float x_ref = 0.f, m_ref = -INFINITY, l = 0.f, zs = 0.f;         // R = x_ref + m_ref; none yet: -inf
+      float x_ref = -INFINITY, m_ref = 0.f, g = 1.f, l = 0.f, zs = 0.f;      // X (none yet: -inf), M and 2^-M
       // the second group's exponentials start when the first's of its first tile are done (attn_pair.cuh)
       const bool turns = it.n1 >= 3;
       for (int j = 0; j < n; ++j) {
@@ -461,20 +462,19 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         const int st = (nk + jt) % NST;
         mbar_wait(v_full(st), ((nk + jt) / NST) & 1);                  // the numbers of the tile's keys and values
         const ulonglong2* num = reinterpret_cast<const ulonglong2*>(numbers + st * kNumbers);
-        const f2 nx2 = pk(-x_ref, -x_ref);
 #pragma unroll
-        for (int i = 0; i < BNK / 2; ++i) {                            // x - x_ref
+        for (int i = 0; i < BNK / 2; ++i) {
           const ulonglong2 sz = num[2 * i];
           float x0, x1;
-          upk(fma2(pk(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sz.x, fma2(qs2, sz.y, nx2)), x0, x1);
+          upk(fma2(pk(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sz.x, mul2(qs2, sz.y)), x0, x1);
           sv[2 * i] = __float_as_uint(x0); sv[2 * i + 1] = __float_as_uint(x1);
         }
         if (!__all_sync(0xffffffffu, vis >= BNK - 1 && (from <= 0 || keep >= BNK))) {
 #pragma unroll
           for (int i = 0; i < BNK; ++i) sv[i] = i <= vis && (i >= from || i < keep) ? sv[i] : 0xff800000u;
         }
-        // Whether R has to be set or moved: not where the largest score and the largest m of the tile, be it of keys that this row does not see,
-        // stay below its bound; else the row's own keys say.
+        // Whether X and M have to be set or moved: not where the largest score and the largest m of the tile, be it of keys that this row does not
+        // see, stay below their bounds; else the row's own keys say.
         float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < BNK; i += 8)
@@ -482,34 +482,31 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
           for (int k = 0; k < 4; ++k) mxa[k] = max3(mxa[k], __uint_as_float(sv[i + 2 * k]), __uint_as_float(sv[i + 2 * k + 1]));
         const float2 m_most = *reinterpret_cast<const float2*>(numbers + st * kNumbers + 1024 + 256);
         const float high = max3(fmaxf(mxa[0], mxa[1]), mxa[2], mxa[3]);          // -inf: no key, or only NaN rows
-        if (__any_sync(0xffffffffu, high + (fmaxf(m_most.x, m_most.y) - m_ref) > kRescaleThreshold)) {
+        if (__any_sync(0xffffffffu, (high - x_ref) + fmaxf(fmaxf(m_most.x, m_most.y) - m_ref, kRescaleThreshold - kScoreRoom) > kRescaleThreshold)) {
+          const float x_new = fmaxf(x_ref, high), dx = x_new - x_ref;
           const ulonglong2* lg = num + 64;
+          const f2 nx2 = pk(-x_new, -x_new);
           float top[2] = {-INFINITY, -INFINITY};
-          const float less = high > -INFINITY ? -high : 0.f;           // what a new x_ref changes
-          const f2 nh2 = pk(less, less);
 #pragma unroll
           for (int i = 0; i < BNK; i += 4) {
             const ulonglong2 m = lg[i / 4];
             float x0, x1, x2, x3;
-            upk(add2(add2(pk(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), nh2), m.x), x0, x1);
-            upk(add2(add2(pk(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), nh2), m.y), x2, x3);
+            upk(add2(add2(pk(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), nx2), m.x), x0, x1);
+            upk(add2(add2(pk(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), nx2), m.y), x2, x3);
             top[i / 4 & 1] = max3(max3(top[i / 4 & 1], x0, x1), x2, x3);
           }
-          const float m_new = fmaxf(top[0], top[1]), up = high + (m_new - m_ref);
-          const bool grow = up > kRescaleThreshold;
+          const float m_new = max3(top[0], top[1], m_ref - dx), up = dx + (m_new - m_ref);
+          const bool grow = up > kRescaleThreshold || dx > kScoreRoom;
           if (__any_sync(0xffffffffu, grow)) {
-            float alpha = 1.f, by = 0.f;
+            float alpha = 1.f;
             if (grow) {
-              const float half = exp2f(-0.5f * up);                    // twice the half: the sums may be as large as the change
-              alpha = half * half;
-              l = l * half * half;
-              zs = zs * half * half;
-              x_ref += high;
+              alpha = exp2f(-up);
+              l *= exp2f(-dx);
+              zs *= alpha;
+              x_ref = x_new;
               m_ref = m_new;
-              by = less;
+              g = exp2f(-m_new);
             }
-#pragma unroll
-            for (int i = 0; i < BNK; ++i) sv[i] = __float_as_uint(__uint_as_float(sv[i]) + by);
             if (j > 0) {
               mbar_wait(o_full(a, ns - 1), ((ns - 1) >> 1) & 1);       // P V of the tile before
               tc_after();
@@ -527,8 +524,8 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
             }
           }
         }
-        const float base = (m_ref == -INFINITY) ? 0.f : m_ref;
-        const f2 nb2 = pk(-base, -base);
+        const float base = (x_ref == -INFINITY) ? 0.f : x_ref;
+        const f2 nb2 = pk(-base, -base), g2 = pk(g, g);
         f2 rs[2] = {0, 0}, zr[2] = {0, 0};
         if (ns >= 2) { mbar_wait(o_full(a, ns), ((ns - 2) >> 1) & 1); tc_after(); }       // P V of two tiles before has read this buffer
         if (turns && j == 0 && a == 1) asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -543,8 +540,9 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
             const f2 e = pk(ex2_ftz(p0), ex2_ftz(p1));                 // masked: -inf -> 0
             const ulonglong2 sz = num[c + 2 * i + 1];
             rs[i & 1] = add2(rs[i & 1], e);
-            zr[i & 1] = fma2(e, sz.y, zr[i & 1]);
-            upk(mul2(e, sz.x), p0, p1);
+            const f2 eg = mul2(e, g2);
+            zr[i & 1] = fma2(eg, sz.y, zr[i & 1]);
+            upk(mul2(eg, sz.x), p0, p1);
             pkd[i] = pack_h2(p0, p1);
           }
           tmem_st16(t_p + c / 2, pkd);
@@ -567,17 +565,17 @@ attn_kv4_tc_kernel(const __grid_constant__ CUtensorMap tm_q8, const __grid_const
         asm volatile("bar.sync 2, 256;" ::: "memory");
         tc_after();
         if (!a) {
-          const float4 p1 = part[r];
-          const float up = (p1.x - x_ref) + (p1.y - m_ref);            // R of the other half less this one's
-          const float half0 = m_ref == -INFINITY ? (l == l ? 0.f : l) : exp2f(-0.5f * fmaxf(up, 0.f));      // (a half that saw nothing but NaN keeps it)
-          const float half1 = p1.y == -INFINITY ? (p1.z == p1.z ? 0.f : p1.z) : exp2f(0.5f * fminf(up, 0.f));
-          mine = half0 * half0;
-          other = half1 * half1;
-          l = l * half0 * half0 + p1.z * half1 * half1;
-          zs = zs * half0 * half0 + p1.w * half1 * half1;
+          const float4 p1 = part[r];                                   // (a half that saw nothing but NaN keeps it)
+          const bool none0 = x_ref == -INFINITY, none1 = p1.x == -INFINITY;
+          const float x_new = fmaxf(x_ref, p1.x), up = (p1.x - x_ref) + (p1.y - m_ref);       // X; the other half's X + M less this one's
+          mine = none0 ? 0.f : exp2f(-fmaxf(up, 0.f));
+          other = none1 ? 0.f : exp2f(fminf(up, 0.f));
+          l = (none0 ? (l == l ? 0.f : l) : l * exp2f(x_ref - x_new)) + (none1 ? (p1.z == p1.z ? 0.f : p1.z) : p1.z * exp2f(p1.x - x_new));
+          zs = zs * mine + p1.w * other;
+          g = exp2f(none0 || up > 0.f ? (x_new - p1.x) - p1.y : (x_new - x_ref) - m_ref);
         }
       }
-      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+      const float inv = l > 0.f ? 1.f / (l * g) : l == l ? 0.f : l;
       // a warp turns its 32 rows in shared memory, 64 columns at a time, and stores 128 contiguous bytes of four rows at once
       uint8_t* stage = stage_out + warp * 4096;
       const int srow = lane >> 3, schunk = lane & 7;

@@ -185,10 +185,10 @@ def attention_terms(cache, q, table, lens, qsl, H, scale, window=0, first=0, dev
     """attention() for finite rows, with what its errors are measured by: with z = low + 8 s of a row, a sum of 16-bit weights is off by their
     rounding times sum p s |code - 8|, sums in 32 bits by theirs times that and sum p |z|, and a score by theirs times reach, the largest visible
     scale (s sum |q| |code - 8| + |z| sum |q|).  most: the largest p s / sum p.  square: of p s |code - 8|, the root of the sum of
-    squares.  Returns (out, codes, rest, most, reach, keys, square), [T, H, hd] or 1."""
+    squares.  whole: the visible rows' sum of |v|.  Returns (out, codes, rest, most, reach, keys, whole, square), [T, H, hd] or 1."""
     T, KV, hd, bs = q.shape[0], cache.KV, cache.hd, cache.bs
     G = H // KV
-    out, codes, rest, square = (torch.zeros(T, H, hd, dtype=torch.float64, device=device) for _ in range(4))
+    out, codes, rest, whole, square = (torch.zeros(T, H, hd, dtype=torch.float64, device=device) for _ in range(5))
     most, reach, keys = (torch.zeros(T, H, 1, dtype=torch.float64, device=device) for _ in range(3))
     for b, n in enumerate(lens):
         r0, r1 = int(qsl[b]), int(qsl[b + 1])
@@ -213,24 +213,25 @@ def attention_terms(cache, q, table, lens, qsl, H, scale, window=0, first=0, dev
             at = (slice(r0, r1), slice(h * G, (h + 1) * G))
             out[at] = (p @ (vl + vs * vc)).transpose(0, 1)
             codes[at] = ((p * vs.T) @ (vc - 8).abs()).transpose(0, 1)
+            whole[at] = (seen[0].double() @ (vl + vs * vc).abs())[:, None].expand(-1, G, -1)
             square[at] = ((p * vs.T) ** 2 @ (vc - 8) ** 2).sqrt().transpose(0, 1)
             rest[at] = (p @ (vl + 8 * vs).abs()).expand(-1, -1, hd).transpose(0, 1)
             most[at] = (p * vs.T).amax(-1, keepdim=True).transpose(0, 1)
             reach[at] = far.amax(-1, keepdim=True).transpose(0, 1)
             keys[at] = seen.sum(-1, keepdim=True).double().expand(G, -1, -1).transpose(0, 1)
-    return out, codes, rest, most, reach, keys, square
+    return out, codes, rest, most, reach, keys, whole, square
 
 
 def allowed(terms, dt):
     """How far a result may be from attention_terms(): its own rounding; weights rounded to float16, 2^-11 of each, or 2^-25 where they are smaller
     than its normal numbers (the largest is 2^0 or more, or the largest exponential is 2^90 or more, or there is a row 2^90 above the codes' steps);
     a score of hd + 8 roundings of 2^-23 of its reach, which stand in weights and in their sum; 2^-18 for sums, exponentials and the division in 32
-    bits; what 16 and 32 bits hold no more."""
-    out, codes, rest, most, reach, keys, square = terms
+    bits; what 16 and 32 bits hold no more, which for exponentials is 2^-126 of the largest."""
+    out, codes, rest, most, reach, keys, whole, square = terms
     hd = out.shape[-1]
     fp32 = 2.0 ** -18 + 2 * (hd + 8) * 2.0 ** -23 * reach
     small = 8 * 2.0 ** -25 * keys * (most + 2.0 ** -90 + 2.0 ** -90 * rest)
-    return half_step(dt) * out.abs() + 2.0 ** -11 * codes + fp32 * (codes + rest) + small + torch.finfo(dt).smallest_normal * half_step(dt) + 2.0 ** -126
+    return half_step(dt) * out.abs() + 2.0 ** -11 * codes + fp32 * (codes + rest) + small + 2.0 ** -126 * whole + torch.finfo(dt).smallest_normal * half_step(dt) + 2.0 ** -126
 
 
 def maps(table, cached, new, free, first, T, bs):

@@ -150,12 +150,47 @@ def test_constant_values_under_steep_scores(kge, L, dtype, hd, H, KV, lens, news
     s.check(out)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("hd,H,KV,lens,news", FAR)
+@pytest.mark.parametrize("steep", [5, 30, 65, 87])
+@pytest.mark.parametrize("small", [0.0, 1e-12, 1.0])
+def test_small_values_under_steep_scores_behind_large_ones(kge, L, dtype, hd, H, KV, lens, news, steep, small):
+    """The first third of a context has values of 10^30 (float16: 10^4), the rest small ones whose weights are up to e^87 times theirs: results from
+    the one to the other, by scores alone."""
+    s = Batch(dtype, hd, H, KV, 16, lens, news, seed=8)
+    for b, n in enumerate(lens):
+        s.k[b] *= 0.05
+        s.k[b][..., 0] = 0
+        s.k[b][n // 3:, :, 0] = steep * hd ** 0.5 / 8 * torch.linspace(0.2, 1, n - n // 3)[:, None]
+        s.v[b][:n // 3] *= 1e4 if dtype == "fp16" else 1e30
+        s.v[b][n // 3:] *= small
+    s.q[..., 0] = 8
+    out = s.fill().run(kge)
+    assert torch.isfinite(out).all()
+    s.check(out)
+
+
 @pytest.mark.parametrize("hd,H,KV,lens,news", FAR)
 @pytest.mark.parametrize("size", [1e-30, 1e-18, 1e18, 1e36])
 def test_values_near_the_ends_of_their_type(kge, L, hd, H, KV, lens, news, size):
     s = Batch("bf16", hd, H, KV, 16, lens, news, seed=4)
     for b in range(len(lens)):
         s.v[b] *= size
+    s.check(s.fill().run(kge))
+
+
+@pytest.mark.parametrize("hd,H,KV,lens,news", FAR)
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e37])
+@pytest.mark.parametrize("above", [8.2, 13.0])
+def test_many_small_weights_beside_a_large_one(kge, L, hd, H, KV, lens, news, size, above):
+    """One key lies e^8 or e^13 above all others, whose weights together still count, whatever the values' size."""
+    s = Batch("bf16", hd, H, KV, 16, lens, news, seed=10)
+    for b in range(len(lens)):
+        s.k[b] *= 0.05
+        s.k[b][..., 0] = 0
+        s.k[b][min(3, lens[b] - 1), :, 0] = above * hd ** 0.5 / 8
+        s.v[b] *= size
+    s.q[..., 0] = 8
     s.check(s.fill().run(kge))
 
 
