@@ -13,6 +13,9 @@
 //   Weights: w = e s_v with e = 2^(x - R), rounded to float16; R is a reference per head, such that the largest w of a warp lies between 1 and
 //   2^14.  It moves only when a weight would pass that, so most tiles rescale nothing and need no shuffles.  What is taken off for centring, 8
 //   times the sum of the weights, is the sum of the ROUNDED ones (a product with ones), so a rounding's error meets |n - 8| and not n.
+//   Weights say nothing of e where a row's values are one constant (s_v = 0) or nearly, e ends before it counts for nothing where s_v is 2^80 and
+//   more, and a score of 2^20 and more leaves a sum with log2(s_v) little of that.  Such units and heads take a path of their own (Core::hard), which
+//   looks at the sums of e and e z_v too, keeps R in two parts and lets e become denormal.
 //   scores come out as (key, head) fragments; movmatrix turns a packed 8 x 8 of weights into the B operand of the second product
 #include <algorithm>
 
@@ -30,8 +33,10 @@ __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; 
 __host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 3 : 4; }
 __host__ __device__ constexpr int shares_of(int nt) { return 148 * ctas_per_sm(nt); }
 constexpr int kMaxShares = 148 * 3;
-constexpr float kLog2e = 1.4426950408889634f, kNoRef = -1e30f;
-constexpr float kExpRoom = 40.f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRoom = 90.f, kRoomDown = 0x1p-90f;      // log2 of what e and e z_v may be when a reference is set; the least s_v that keeps them there
+constexpr float kSumMost = 0x1p100f;           // what a unit's sums of e and e z_v may be
+constexpr float kDeep = 80.f, kDeepMost = 0x1p80f, kSteep = 0x1p20f;      // a reference this far above its largest score, or this large, is for the hard path
 constexpr uint32_t kWeightMost = 0x7400;       // 2^14 in float16
 
 struct Args {
@@ -39,7 +44,7 @@ struct Args {
   const bf16* q;
   const uint8_t* cache;
   const int32_t *table, *lens, *qsl;
-  float* part;                                 // outputs of the pieces of cut groups: [2 per share][G][HD], then [2 per share][G] (R, l)
+  float* part;                                 // outputs of the pieces of cut groups: [2 per share][G][HD], then [2 per share][G] Parts of 16 bytes
   int4* desc;                                  // per share: the group that begins in it and ends in a later one's: (row of q, kv head, last share, slot)
   int q_stride, max_blocks, B, H, KV, bs_shift, window, first;
   float scale_log2;
@@ -72,6 +77,7 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t v) {
   return r;
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float ex2_all(float x) { float y; asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }      // (denormal results too)
 __device__ __forceinline__ float lg2(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   uint32_t r;
@@ -112,7 +118,7 @@ struct Core {
   float qs[NT][2], fs;                         // scale log2(e) sum(q) of the two columns; what scores are multiplied with
   float o[NM][NT][4], ws[NT][4];               // outputs; sums of the rounded weights, from a product with ones
   float ref[NT][2], l[NT][2], zs[NT][2];
-  bool fresh;                                  // the first unit sets the references
+  bool fresh, hard;                            // the first unit sets the references; `lo` holds a part of them, or e may be denormal
 
   __device__ __forceinline__ void start(const bf16* q, int G, float scale_log2, int lane) {
     const int g = lane >> 2, t = lane & 3;
@@ -158,11 +164,85 @@ struct Core {
       for (int h = 0; h < 2; ++h) ref[nt][h] = l[nt][h] = zs[nt][h] = ws[nt][h] = ws[nt][2 + h] = 0.f;
     }
     fresh = true;
+    hard = false;
+  }
+
+  // The hard path: weights and exponentials of any finite rows, references in two parts.
+  __device__ __forceinline__ void reweigh(float (&x)[2][NT][4], const float (&sv)[2][2], const float (&zv)[2][2], float (&e)[2][NT][4], uint32_t (&wt)[2][NT][2], int t, int lane,
+                                          float* lows) {
+    bool harder = hard;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float* low_at = lows + 8 * nt + 2 * t + h;
+        float low = hard ? *low_at : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { x[i][nt][h] -= low; x[i][nt][2 + h] -= low; }
+        auto weigh = [&]() {                   // true: does not fit
+          float sum_e = 0.f, sum_z = 0.f, w_most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float v = ex2_all(x[i][nt][2 * r + h]);
+              e[i][nt][2 * r + h] = v;
+              sum_e += v;
+              sum_z = fmaf(v, zv[i][r], sum_z);
+              w_most = fmaxf(w_most, v * sv[i][r]);
+            }
+          return !(fmaxf(sum_e, fabsf(sum_z)) < kSumMost && w_most < 16384.f);
+        };
+        // only a column that has passed a bound moves
+        const bool over = __ballot_sync(0xffffffffu, weigh()) & (0x11111111u << t);
+        float high = -INFINITY, top = -INFINITY;                  // of the column's scores; of what they are with their rows' numbers, less that
+#pragma unroll
+        for (int i = 0; i < 2; ++i) high = fmaxf(high, fmaxf(x[i][nt][h], x[i][nt][2 + h]));
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, m));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            top = fmaxf(top, x[i][nt][2 * r + h] - high + fmaxf(lg2(sv[i][r]), fmaxf(lg2(fabsf(zv[i][r])) - kRoom, -kRoom)));
+#pragma unroll
+        for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+        const float up = high + top;                              // how far the reference goes up (the first: or down)
+        if (fabsf(up) < INFINITY && (fresh || (over && up > 0.f))) {       // (not: only NaN rows)
+          const bool steep = hard || fabsf(ref[nt][h]) + fabsf(up) > kSteep;
+          ref[nt][h] += steep ? high : up;
+          low += steep ? top : 0.f;
+          harder |= steep || top > kDeep;
+          const float f = fresh ? 1.f : ex2(-0.5f * up);          // twice the half: the sums may be as large as the change
+          l[nt][h] = l[nt][h] * f * f;
+          zs[nt][h] = zs[nt][h] * f * f;
+          ws[nt][h] = ws[nt][h] * f * f;
+#pragma unroll
+          for (int i = 0; i < NM; ++i) { o[i][nt][h] = o[i][nt][h] * f * f; o[i][nt][2 + h] = o[i][nt][2 + h] * f * f; }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] = x[i][nt][2 * r + h] - high - top;
+          weigh();
+        }
+        __syncwarp();
+        if ((lane >> 2) == 0) *low_at = low;
+      }
+    fresh = false;
+    hard = __any_sync(0xffffffffu, harder);
+    __syncwarp();                                                 // (`lows`)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) wt[i][nt][r] = pack_h2(e[i][nt][2 * r] * sv[i][r], e[i][nt][2 * r + 1] * sv[i][r]);
   }
 
   // A unit whose two groups lie at shared address `at`.  edge: some of its keys are not visible - those from `len` on, and those below `lo` but
   // the first `first` ones.
-  __device__ __forceinline__ void unit(uint32_t at, int lane, bool edge, int key0, int len, int lo, int first) {
+  // lows: the warp's 8 NT numbers of shared memory for the references' other parts, R = ref + low.
+  __device__ __forceinline__ void unit(uint32_t at, int lane, bool edge, int key0, int len, int lo, int first, float* lows) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t k_at = at + g * (HD / 2) + t * (HD / 8), n_at = at + 16 * HD + kv4::key_token(g) * 4;
     // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
@@ -211,7 +291,8 @@ struct Core {
         for (int r = 0; r < 2; ++r) {
           const int key = mine + 16 * i + 8 * r;
           if (!(key < len && (key >= lo || key < first))) {       // its numbers may be anything
-            sv[i][r] = zv[i][r] = 0.f;
+            sv[i][r] = 1.f;                      // (which makes nothing of a weight of zero)
+            zv[i][r] = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) x[i][nt][2 * r] = x[i][nt][2 * r + 1] = -INFINITY;
           }
@@ -236,38 +317,52 @@ struct Core {
       return most < (kWeightMost << 16) && (most & 0xffffu) < kWeightMost;
     };
     const bool fits = weigh();
-    if (fresh || !__all_sync(0xffffffffu, fits)) {
+    // Small weights say that e and e z_v are small where no s_v is zero (it is 2^-16 |z_v| then, or more) or next to it.
+    const bool plain = fminf(fminf(sv[0][0], sv[0][1]), fminf(sv[1][0], sv[1][1])) >= kRoomDown;
+    if (fresh || hard || !__all_sync(0xffffffffu, fits && plain)) {
+      bool wide = hard || !plain || fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1])) > kDeepMost;      // for the hard path
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          // only a column that has passed the bound moves: what a head gets does not hang on its neighbours
-          uint32_t most = 0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i) most = max_u16x2(most, max_u16x2(wt[i][nt][0], wt[i][nt][1]));
-          const bool over = __ballot_sync(0xffffffffu, (h ? most >> 16 : most & 0xffffu) >= kWeightMost) & (0x11111111u << t);
-          float top = fresh ? -INFINITY : 0.f;                    // how far the reference goes up (the first: or down)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) top = fmaxf(top, fmaxf(x[i][nt][2 * r + h] + lg2(sv[i][r]), x[i][nt][2 * r + h] - kExpRoom));
-#pragma unroll
-          for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-          if (top == -INFINITY || !(fresh || over)) top = 0.f;    // (the first: only NaN rows)
-          const float f = fresh ? 1.f : ex2(-top);                // (2^-top may be infinite where the first one goes down, and the sums are zeros)
-          ref[nt][h] += top;
-          l[nt][h] *= f;
-          zs[nt][h] *= f;
-          ws[nt][h] *= f;
-#pragma unroll
-          for (int i = 0; i < NM; ++i) { o[i][nt][h] *= f; o[i][nt][2 + h] *= f; }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] -= top;
+          const float high = fmaxf(fmaxf(x[0][nt][h], x[0][nt][2 + h]), fmaxf(x[1][nt][h], x[1][nt][2 + h]));
+          wide |= fabsf(ref[nt][h]) > kSteep || (fabsf(high) > kSteep && fabsf(high) < INFINITY);
         }
-      weigh();
-      fresh = false;
+      if (__any_sync(0xffffffffu, wide)) {
+        reweigh(x, sv, zv, e, wt, t, lane, lows);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            // only a column that has passed the bound moves: what a head gets does not hang on its neighbours
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) most = max_u16x2(most, max_u16x2(wt[i][nt][0], wt[i][nt][1]));
+            const bool over = __ballot_sync(0xffffffffu, (h ? most >> 16 : most & 0xffffu) >= kWeightMost) & (0x11111111u << t);
+            float top = fresh ? -INFINITY : 0.f;                    // how far the reference goes up (the first: or down)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) top = fmaxf(top, x[i][nt][2 * r + h] + lg2(sv[i][r]));
+#pragma unroll
+            for (int m = 4; m < 32; m <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+            if (top == -INFINITY || !(fresh || over)) top = 0.f;    // (the first: only NaN rows)
+            const float f = fresh ? 1.f : ex2(-top);                // (2^-top may be infinite where the first one goes down, and the sums are zeros)
+            ref[nt][h] += top;
+            l[nt][h] *= f;
+            zs[nt][h] *= f;
+            ws[nt][h] *= f;
+#pragma unroll
+            for (int i = 0; i < NM; ++i) { o[i][nt][h] *= f; o[i][nt][2 + h] *= f; }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) x[i][nt][2 * r + h] -= top;
+          }
+        weigh();
+        fresh = false;
+      }
     }
     uint32_t pb[2][NT][2];
 #pragma unroll
@@ -335,9 +430,16 @@ struct Core {
 __device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 128;" ::: "memory"); }      // the computing warps
 template <int HD> __host__ __device__ constexpr int red_floats() { return NW * 4 * (HD + 4); }
 
-// The four warps' sums of one (request, kv head) in shared memory, four heads at a time: write(row, first of four dimensions, reference, sum, values)
+// Part of a head's keys: R = x + m (m -inf: no keys) and the sum of e.  Parts are joined in units of the largest R.
+struct Part { float x, m, l; };
+__device__ __forceinline__ Part no_part() { return {0.f, -INFINITY, 0.f}; }
+__device__ __forceinline__ bool above(const Part& a, const Part& b) { return a.m > -INFINITY && (b.m == -INFINITY || (a.x - b.x) + (a.m - b.m) > 0.f); }
+// 2^((a - b) / 2) of their R: a sum of e may be as large as the difference is, so it is multiplied twice
+__device__ __forceinline__ float half_of(const Part& a, const Part& b) { return a.m == -INFINITY ? 0.f : ex2(0.5f * ((a.x - b.x) + (a.m - b.m))); }
+
+// The four warps' sums of one (request, kv head) in shared memory, four heads at a time: write(row, first of four dimensions, part, values)
 template <int HD, int NT, typename F>
-__device__ __forceinline__ void combine(Core<HD, NT>& core, float* red, int warp, int lane, int G, F write) {
+__device__ __forceinline__ void combine(Core<HD, NT>& core, const float* lows, float* red, int warp, int lane, int G, F write) {
   constexpr int RS = HD + 4, NV = HD / 64;
   const int t = lane & 3;
   core.sums();
@@ -349,7 +451,8 @@ __device__ __forceinline__ void combine(Core<HD, NT>& core, float* red, int warp
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int m = 0; m < NV; ++m) core.rows(nt, h, m, lane, v[h][m]);
-#pragma unroll
+    // (not unrolled: what a CTA runs once costs it the way of its code from the L2; 16 requests of 2048 keys, 16 heads to a kv head, 26.7 us against 23.0)
+#pragma unroll 1
     for (int half = 0; half < 2; ++half) {               // heads 8 nt + 4 half .. + 3: threads t = 2 half and 2 half + 1 of a quad
       const int r0 = 8 * nt + 4 * half;
       if (r0 >= G) break;
@@ -364,26 +467,32 @@ __device__ __forceinline__ void combine(Core<HD, NT>& core, float* red, int warp
             at[0] = make_float4(v[h][m][0], v[h][m][1], v[h][m][2], v[h][m][3]);
             at[1] = make_float4(v[h][m][4], v[h][m][5], v[h][m][6], v[h][m][7]);
           }
-          if (lane < 4) { dst[HD] = core.fresh ? kNoRef : core.ref[nt][h]; dst[HD + 1] = core.l[nt][h]; }      // (a warp without a unit)
+          if (lane < 4) {
+            dst[HD] = core.ref[nt][h];
+            dst[HD + 1] = core.fresh ? -INFINITY : core.hard ? lows[8 * nt + 2 * t + h] : 0.f;      // (fresh: a warp without a unit)
+            dst[HD + 2] = core.l[nt][h];
+          }
         }
       bar_compute();
       for (int it = warp * 32 + lane; it < HD; it += NW * 32) {       // (row, 4 dimensions)
         const int r = it / (HD / 4), c = it % (HD / 4);
         if (r0 + r >= G) break;
-        float mm = kNoRef;
+        auto part_of = [&](int w) { const float* src = red + (w * 4 + r) * RS + HD; return Part{src[0], src[1], src[2]}; };
+        Part all = no_part();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) mm = fmaxf(mm, red[(w * 4 + r) * RS + HD]);
+        for (int w = 0; w < NW; ++w)
+          if (above(part_of(w), all)) all = part_of(w);
+        all.l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float ll = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          const float* src = red + (w * 4 + r) * RS;
-          const float f = ex2(src[HD] - mm);
-          const float4 u = *reinterpret_cast<const float4*>(src + 4 * c);
+          const Part p = part_of(w);
+          const float half = half_of(p, all), f = half * half;
+          const float4 u = *reinterpret_cast<const float4*>(red + (w * 4 + r) * RS + 4 * c);
           acc.x = fmaf(f, u.x, acc.x); acc.y = fmaf(f, u.y, acc.y); acc.z = fmaf(f, u.z, acc.z); acc.w = fmaf(f, u.w, acc.w);
-          ll = fmaf(f, src[HD + 1], ll);
+          all.l = fmaf(half, half * p.l, all.l);
         }
-        write(r0 + r, 4 * c, mm, ll, acc);
+        write(r0 + r, 4 * c, all, acc);
       }
     }
   }
@@ -410,7 +519,9 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(const Args a) {
   constexpr int ST = 3, GB = kv4::group_bytes(HD);
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float all_lows[NW][8 * NT];
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  float* lows = all_lows[warp];
   const uint32_t ring = s_addr(smem) + warp * ST * 2 * GB, bars = s_addr(smem) + NW * ST * 2 * GB + warp * ST * 8;
   if (lane == 0)
     for (int s = 0; s < ST; ++s) mbar_init(bars + 8 * s, 1);
@@ -453,13 +564,13 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(cons
   for (int u = warp; u < sp.n; u += NW) {
     const int key0 = sp.key0(u), next = block_of(u + ST * NW);
     mbar_wait(bars + 8 * stage, parity);
-    if (sp.len > 0) core.unit(ring + stage * 2 * GB, lane, key0 + WK > sp.len || (key0 < sp.lo && key0 + WK > a.first), key0, sp.len, sp.lo, a.first);
+    if (sp.len > 0) core.unit(ring + stage * 2 * GB, lane, key0 + WK > sp.len || (key0 < sp.lo && key0 + WK > a.first), key0, sp.len, sp.lo, a.first, lows);
     __syncwarp();
     ask(u + ST * NW, stage, next);
     if (++stage == ST) { stage = 0; parity ^= 1; }
   }
-  combine<HD, NT>(core, reinterpret_cast<float*>(smem), warp, lane, G, [&](int r, int d, float, float l, float4 v) {      // over the rings, which are read
-    *reinterpret_cast<uint2*>(a.out + ((int64_t)qrow * a.H + kvh * G + r) * HD + d) = divided(v, l);
+  combine<HD, NT>(core, lows, reinterpret_cast<float*>(smem), warp, lane, G, [&](int r, int d, const Part& p, float4 v) {      // over the rings, which are read
+    *reinterpret_cast<uint2*>(a.out + ((int64_t)qrow * a.H + kvh * G + r) * HD + d) = divided(v, p.l);
   });
 }
 
@@ -481,6 +592,7 @@ __global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_
   uint8_t* sq = smem + ST * STAGE;                       // query heads of a piece, two buffers
   float* red = reinterpret_cast<float*>(sq + q_bytes<HD, NT>());
   Piece* pieces = reinterpret_cast<Piece*>(red + red_floats<HD>());
+  __shared__ float all_lows[NW][8 * NT];
   const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, G = a.H / a.KV;
   const uint32_t ring = s_addr(smem), bar0 = s_addr(pieces + 2);
   // full(s), p_full(i): the producer's arrival and its copies' bytes; empty(s), p_empty(i): the computing warps.  A wait for one comes before
@@ -579,6 +691,7 @@ __global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_
   }
 
   const uint32_t own = ring + warp * 2 * GB;
+  float* lows = all_lows[warp];
   while (true) {
     mbar_wait(p_full(pi), p_parity);
     const Piece p = pieces[pi];
@@ -593,21 +706,21 @@ __global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_
       mbar_wait(full(stage), parity);
       if (u + warp < p.t1 && p.span.len > 0) {
         const int key0 = p.span.key0(u + warp);
-        core.unit(own + stage * STAGE, lane, key0 + WK > p.span.len || (key0 < p.span.lo && key0 + WK > a.first), key0, p.span.len, p.span.lo, a.first);
+        core.unit(own + stage * STAGE, lane, key0 + WK > p.span.len || (key0 < p.span.lo && key0 + WK > a.first), key0, p.span.len, p.span.lo, a.first, lows);
       }
       __syncwarp();                                      // the stage is read
       if (lane == 0) mbar_arrive(empty(stage));
       if (++stage == ST) { stage = 0; parity ^= 1; }
     }
     if (p.slot < 0) {
-      combine<HD, NT>(core, red, warp, lane, G, [&](int r, int d, float, float l, float4 v) {
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)p.row * a.H + p.kvh * G + r) * HD + d) = divided(v, l);
+      combine<HD, NT>(core, lows, red, warp, lane, G, [&](int r, int d, const Part& all, float4 v) {
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)p.row * a.H + p.kvh * G + r) * HD + d) = divided(v, all.l);
       });
     } else {
-      combine<HD, NT>(core, red, warp, lane, G, [&](int r, int d, float m, float l, float4 v) {
+      combine<HD, NT>(core, lows, red, warp, lane, G, [&](int r, int d, const Part& all, float4 v) {
         const int64_t at = (int64_t)p.slot * G + r;
         *reinterpret_cast<float4*>(a.part + at * HD + d) = v;
-        if (d == 0) *reinterpret_cast<float2*>(a.part + (int64_t)2 * kMaxShares * G * HD + at * 2) = make_float2(m, l);
+        if (d == 0) *reinterpret_cast<float4*>(a.part + (int64_t)2 * kMaxShares * G * HD + at * 4) = make_float4(all.x, all.m, all.l, 0.f);
       });
     }
   }
@@ -620,53 +733,53 @@ template <int HD>
 __global__ void __launch_bounds__(MW * 32) attn_kv4_merge_kernel(bf16* __restrict__ out, const float* __restrict__ part, const int4* __restrict__ desc, int H, int G, int shares) {
   constexpr int C = HD / 4;                    // lanes of a row (the others of a warp idle along)
   __shared__ float4 sh[MW][C];
-  __shared__ float2 sl[MW];
+  __shared__ Part sp[MW];
   __shared__ int4 sd[MW];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y, c = lane % C;
-  const float2* ml = reinterpret_cast<const float2*>(part + (int64_t)2 * kMaxShares * G * HD);
+  const float4* ml = reinterpret_cast<const float4*>(part + (int64_t)2 * kMaxShares * G * HD);
   const int4 mine = blockIdx.x * MW + warp < shares ? desc[blockIdx.x * MW + warp] : make_int4(-1, 0, 0, 0);
-  // pieces first .. n - 1 of the group of d that begins in share s, by steps; a running reference and sum
-  auto merge = [&](int s, const int4& d, int first, int step, float& mm, float& ll, float4& acc) {
+  // pieces first .. n - 1 of the group of d that begins in share s, by steps
+  auto merge = [&](int s, const int4& d, int first, int step, Part& all, float4& acc) {
     const int n = d.z - s + 1;
     constexpr int AT_ONCE = 8;
     for (int i0 = first; i0 < n; i0 += AT_ONCE * step) {
-      float2 p[AT_ONCE];
+      Part p[AT_ONCE];
       float4 v[AT_ONCE];
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k) {
         const int i = min(i0 + k * step, n - 1);
         const int64_t row = (int64_t)(2 * (s + i) + (i == 0)) * G + r;      // slot 1 of the first share, slot 0 of the others
-        p[k] = ml[row];
+        const float4 u = ml[row];
+        p[k] = {u.x, i0 + k * step < n ? u.y : -INFINITY, u.z};
         v[k] = *reinterpret_cast<const float4*>(part + row * HD + 4 * c);
       }
-      float m = mm;
+      const Part was = all;
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k)
-        if (i0 + k * step < n) m = fmaxf(m, p[k].x);
-      const float old = ex2(mm - m);
-      mm = m;
-      acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old; ll *= old;
+        if (above(p[k], all)) all = p[k];
+      const float old_half = half_of(was, all), old = old_half * old_half;
+      acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+      all.l = was.l * old_half * old_half;
 #pragma unroll
       for (int k = 0; k < AT_ONCE; ++k)
         if (i0 + k * step < n) {
-          const float f = ex2(p[k].x - m);
+          const float half = half_of(p[k], all), f = half * half;
           acc.x = fmaf(f, v[k].x, acc.x); acc.y = fmaf(f, v[k].y, acc.y); acc.z = fmaf(f, v[k].z, acc.z); acc.w = fmaf(f, v[k].w, acc.w);
-          ll = fmaf(f, p[k].y, ll);
+          all.l = fmaf(half, half * p[k].l, all.l);
         }
     }
   };
-  auto write = [&](const int4& d, float ll, const float4& acc) {
-    const float inv = ll != 0.f ? 1.f / ll : 0.f;
-    *reinterpret_cast<uint2*>(out + ((int64_t)d.x * H + d.y * G + r) * HD + 4 * c) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+  auto write = [&](const int4& d, float l, const float4& acc) {
+    *reinterpret_cast<uint2*>(out + ((int64_t)d.x * H + d.y * G + r) * HD + 4 * c) = divided(acc, l);
   };
   const bool many = mine.x >= 0 && mine.z - (int)(blockIdx.x * MW + warp) >= kFewPieces;
   if (mine.x >= 0 && !many) {
-    float mm = kNoRef, ll = 0.f;
+    Part all = no_part();
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    merge(blockIdx.x * MW + warp, mine, 0, 1, mm, ll, acc);
-    if (lane < C) write(mine, ll, acc);
+    merge(blockIdx.x * MW + warp, mine, 0, 1, all, acc);
+    if (lane < C) write(mine, all.l, acc);
   }
   if (!__syncthreads_or(many)) return;
   if (lane == 0) sd[warp] = many ? mine : make_int4(-1, 0, 0, 0);
@@ -674,33 +787,34 @@ __global__ void __launch_bounds__(MW * 32) attn_kv4_merge_kernel(bf16* __restric
   for (int w = 0; w < MW; ++w) {
     const int4 d = sd[w];
     if (d.x < 0) continue;                     // (the same for the block)
-    float mm = kNoRef, ll = 0.f;
+    Part all = no_part();
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    merge(blockIdx.x * MW + w, d, warp, MW, mm, ll, acc);
+    merge(blockIdx.x * MW + w, d, warp, MW, all, acc);
     if (lane < C) sh[warp][c] = acc;
-    if (lane == 0) sl[warp] = make_float2(mm, ll);
+    if (lane == 0) sp[warp] = all;
     __syncthreads();
     if (warp == 0) {
-      float m = kNoRef;
+      all = no_part();
 #pragma unroll
-      for (int k = 0; k < MW; ++k) m = fmaxf(m, sl[k].x);
+      for (int k = 0; k < MW; ++k)
+        if (above(sp[k], all)) all = sp[k];
       acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      ll = 0.f;
+      float l = 0.f;
 #pragma unroll
       for (int k = 0; k < MW; ++k) {
-        const float f = ex2(sl[k].x - m);
+        const float half = half_of(sp[k], all), f = half * half;
         const float4 v = sh[k][c];
         acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
-        ll = fmaf(f, sl[k].y, ll);
+        l = fmaf(half, half * sp[k].l, l);
       }
-      if (lane < C) write(d, ll, acc);
+      if (lane < C) write(d, l, acc);
     }
     __syncthreads();
   }
 }
 
 constexpr int kDescBytes = kMaxShares * 16;    // the workspace's start
-constexpr int64_t workspace_bytes(int G, int hd) { return kDescBytes + (int64_t)2 * kMaxShares * G * (hd + 2) * 4; }
+constexpr int64_t workspace_bytes(int G, int hd) { return kDescBytes + (int64_t)2 * kMaxShares * G * (hd + 4) * 4; }
 constexpr int kMaxRequests = 1024;             // requests of one launch (every warp reads their lengths)
 
 // Which kernel.  A CTA per (request, kv head) has four CTAs an SM, which cover each other's starts and ends, and the hardware's queue; shares have
