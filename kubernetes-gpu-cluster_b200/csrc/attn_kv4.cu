@@ -9,7 +9,8 @@
 // 8 heads leaves few empty, half the products that heads as the M side cost.  Both operands are float16 in either build.
 //   Codes: the bits n in the low half-byte of a float16 are the number n 2^-24 (its denormals), in the next one n 2^-20, so a code costs half an
 //   AND and no arithmetic; powers of two are put right in q (scores) and in the outputs.  (As 1024 + n less 1032: 2.6 instructions a pair.)
-//   q: a power of two moves the largest number of the group's heads to 2^14; exact but for what lies 2^-24 below that.
+//   q: a power of two moves the largest number of the group's heads to 2^14, or of each head where they lie 2^10 apart; exact but for what lies
+//   2^-24 below that.
 //   Weights: w = e s_v with e = 2^(x - R), rounded to float16; R is a reference per head, such that the largest w of a warp lies between 1 and
 //   2^14.  It moves only when a weight would pass that, so most tiles rescale nothing and need no shuffles.  What is taken off for centring, 8
 //   times the sum of the weights, is the sum of the ROUNDED ones (a product with ones), so a rounding's error meets |n - 8| and not n.
@@ -118,17 +119,18 @@ struct Core {
   float qs[NT][2], fs;                         // scale log2(e) sum(q) of the two columns; what scores are multiplied with
   float o[NM][NT][4], ws[NT][4];               // outputs; sums of the rounded weights, from a product with ones
   float ref[NT][2], l[NT][2], zs[NT][2];
-  bool fresh, hard;                            // the first unit sets the references; `lo` holds a part of them, or e may be denormal
+  bool fresh, hard, uneven;                    // the first unit sets the references; they have two parts, or e may be denormal; heads have an fs each
 
-  __device__ __forceinline__ void start(const bf16* q, int G, float scale_log2, int lane) {
+  __device__ __forceinline__ void start(const bf16* q, int G, float scale_log2, int lane, float* lows) {
     const int g = lane >> 2, t = lane & 3;
     uint4 raw[NT][W];
-    float mx = 0.f;
+    float mx[NT], most = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int head = nt * 8 + g;
       const uint4* src = reinterpret_cast<const uint4*>(q + min(head, G - 1) * HD + t * (HD / 4));
       float sum = 0.f;
+      mx[nt] = 0.f;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         raw[nt][i] = head < G ? src[i] : make_uint4(0, 0, 0, 0);
@@ -137,21 +139,42 @@ struct Core {
         for (int k = 0; k < 4; ++k) {
           const float x = bf_lo(u[k]), y = bf_hi(u[k]);
           sum += x + y;
-          mx = fmaxf(mx, fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f));
+          mx[nt] = fmaxf(mx[nt], fmaxf(fabsf(x) <= 3.402823466e38f ? fabsf(x) : 0.f, fabsf(y) <= 3.402823466e38f ? fabsf(y) : 0.f));
         }
       }
+      most = fmaxf(most, mx[nt]);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       qs[nt][0] = scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t);
       qs[nt][1] = scale_log2 * __shfl_sync(0xffffffffu, sum, 8 * t + 4);
     }
-    // 2^e brings the largest finite number to 2^14 (e from -100 to 100); high nibbles count 16 times, so what they meet is q 2^(e - 4)
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
-    const int e = top ? min(max(141 - (int)(top >> 23), -100), 100) : 0;
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23), up4 = __uint_as_float((uint32_t)(123 + e) << 23);
-    fs = scale_log2 * __uint_as_float((uint32_t)(151 - e) << 23);
+    // 2^e brings the largest finite number to 2^14 (e from -100 to 100), of all heads or, where these lie 2^10 apart, of each; high nibbles count 16
+    // times, so what they meet is q 2^(e - 4)
+    auto exponent = [](uint32_t top) { return top ? min(max(141 - (int)(top >> 23), -100), 100) : 0; };
+    auto factor = [&](int e) { return scale_log2 * __uint_as_float((uint32_t)(151 - e) << 23); };
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    int es[NT];
+    uneven = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      es[nt] = exponent(top);
+      auto heads = [](uint32_t lanes) { return (lanes | lanes >> 1 | lanes >> 2 | lanes >> 3) & 0x11111111u; };
+      uneven |= (heads(__ballot_sync(0xffffffffu, mx[nt] > 0.f)) & ~heads(__ballot_sync(0xffffffffu, mx[nt] >= __uint_as_float(top) * 0x1p-10f))) != 0;
+    }
+    fs = factor(es[0]);
+    if (uneven) {                              // the same for the warp
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], 1));
+        mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], 2));
+        es[nt] = exponent(__float_as_uint(mx[nt]));
+        if (t == 0) lows[8 * (NT + nt) + g] = factor(es[nt]);
+      }
+      __syncwarp();
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float up = __uint_as_float((uint32_t)(127 + es[nt]) << 23), up4 = __uint_as_float((uint32_t)(123 + es[nt]) << 23);
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const uint32_t* u = &raw[nt][i].x;
@@ -241,7 +264,7 @@ struct Core {
 
   // A unit whose two groups lie at shared address `at`.  edge: some of its keys are not visible - those from `len` on, and those below `lo` but
   // the first `first` ones.
-  // lows: the warp's 8 NT numbers of shared memory for the references' other parts, R = ref + low.
+  // lows: numbers of the warp's own in shared memory, 8 NT for the references' other parts, R = ref + low, and an fs for each of 8 NT heads.
   __device__ __forceinline__ void unit(uint32_t at, int lane, bool edge, int key0, int len, int lo, int first, float* lows) {
     const int g = lane >> 2, t = lane & 3;
     const uint32_t k_at = at + g * (HD / 2) + t * (HD / 8), n_at = at + 16 * HD + kv4::key_token(g) * 4;
@@ -282,6 +305,16 @@ struct Core {
 #pragma unroll
           for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
       }
+      if (uneven)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t pk = lds32(n_at + i * GB + 32 * r);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], lows[8 * (NT + nt) + 2 * t + h] * bf_lo(pk), fmaf(qs[nt][h], bf_hi(pk), -ref[nt][h]));
+        }
     }
     if (edge) {                                // the same for the warp
       const int mine = key0 + kv4::key_token(g);
@@ -519,7 +552,7 @@ template <int HD, int NT>
 __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(const Args a) {
   constexpr int ST = 3, GB = kv4::group_bytes(HD);
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float all_lows[NW][8 * NT];
+  __shared__ float all_lows[NW][2 * 8 * NT];
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   float* lows = all_lows[warp];
   const uint32_t ring = s_addr(smem) + warp * ST * 2 * GB, bars = s_addr(smem) + NW * ST * 2 * GB + warp * ST * 8;
@@ -558,7 +591,7 @@ __global__ void __launch_bounds__(NW * 32, NT == 1 ? 4 : 3) attn_kv4_kernel(cons
 #pragma unroll
   for (int s = 0; s < ST; ++s) ask(warp + s * NW, s, blk[s]);
   Core<HD, NT> core;
-  core.start(a.q + (int64_t)qrow * a.q_stride + kvh * G * HD, G, a.scale_log2, lane);
+  core.start(a.q + (int64_t)qrow * a.q_stride + kvh * G * HD, G, a.scale_log2, lane, lows);
   int stage = 0;
   uint32_t parity = 0;
   for (int u = warp; u < sp.n; u += NW) {
@@ -592,7 +625,7 @@ __global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_
   uint8_t* sq = smem + ST * STAGE;                       // query heads of a piece, two buffers
   float* red = reinterpret_cast<float*>(sq + q_bytes<HD, NT>());
   Piece* pieces = reinterpret_cast<Piece*>(red + red_floats<HD>());
-  __shared__ float all_lows[NW][8 * NT];
+  __shared__ float all_lows[NW][2 * 8 * NT];
   const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31, G = a.H / a.KV;
   const uint32_t ring = s_addr(smem), bar0 = s_addr(pieces + 2);
   // full(s), p_full(i): the producer's arrival and its copies' bytes; empty(s), p_empty(i): the computing warps.  A wait for one comes before
@@ -697,7 +730,7 @@ __global__ void __launch_bounds__(NW * 32 + 32, ctas_per_sm(NT)) attn_kv4_share_
     const Piece p = pieces[pi];
     if (p.t0 == p.t1) break;
     Core<HD, NT> core;
-    core.start(reinterpret_cast<const bf16*>(sq + pi * (q_bytes<HD, NT>() / 2)), G, a.scale_log2, lane);
+    core.start(reinterpret_cast<const bf16*>(sq + pi * (q_bytes<HD, NT>() / 2)), G, a.scale_log2, lane, lows);
     __syncwarp();
     if (lane == 0) mbar_arrive(p_empty(pi));
     pi ^= 1;

@@ -98,8 +98,8 @@ def test_later_rows_leave_earlier_queries_alone(kge, L, dtype, hd, H, KV, lens, 
 
 # ------------------------------------------------------------------------------------------------------ rows far apart
 
-FAR = [(128, 4, 1, [150, 90, 64], [1, 1, 1]), (64, 12, 1, [900, 33], [1, 1]), (128, 16, 1, [70, 500], [1, 1]), (128, 32, 8, [1500, 700], [1, 1]),
-       (128, 4, 1, [150, 90, 64], [64, 90, 7]), (64, 40, 2, [150, 90, 64], [1, 90, 1]), (128, 32, 8, [300] * 6, [300] * 6)]
+SINGLE = [(128, 4, 1, [150, 90, 64], [1, 1, 1]), (64, 12, 1, [900, 33], [1, 1]), (128, 16, 1, [70, 500], [1, 1]), (128, 32, 8, [1500, 700], [1, 1])]
+FAR = SINGLE + [(128, 4, 1, [150, 90, 64], [64, 90, 7]), (64, 40, 2, [150, 90, 64], [1, 90, 1]), (128, 32, 8, [300] * 6, [300] * 6)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
@@ -178,6 +178,19 @@ def test_values_near_the_ends_of_their_type(kge, L, hd, H, KV, lens, news, size)
     for b in range(len(lens)):
         s.v[b] *= size
     s.check(s.fill().run(kge))
+
+
+@pytest.mark.parametrize("hd,H,KV,lens,news", SINGLE)
+def test_heads_of_one_group_far_apart(kge, L, hd, H, KV, lens, news):
+    """Single-token requests whose heads' q lie 10^12 apart: each is as exact as alone, and has the same bits."""
+    s = Batch("bf16", hd, H, KV, 16, lens, news, seed=5).fill()
+    s.q[:, 0] *= 1e12
+    s.q[:, 2] *= 1e-12
+    out = s.run(kge)
+    s.check(out)
+    s.q[:, 0] *= 1e-12
+    again = s.run(kge)
+    assert torch.equal(again[:, 1:], out[:, 1:])
 
 
 @pytest.mark.parametrize("hd,H,KV,lens,news", FAR)
