@@ -872,7 +872,7 @@ static int launch(const Args& a, int max_seq_len, cudaStream_t st) {
   if (cta_each((int64_t)a.B * a.KV, keys)) {
     constexpr int ring = NW * 3 * 2 * kv4::group_bytes(HD) + NW * 3 * 8, smem = ring > red_floats<HD>() * 4 ? ring : red_floats<HD>() * 4;
     auto kern = attn_kv4_kernel<HD, NT>;
-    if (smem > 48 * 1024) KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (smem > (int)kPlainShared) KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     KGE_CUDA_OK(launch_pdl(kern, dim3(a.KV, a.B), dim3(NW * 32), smem, st, a));
     return 0;
   }

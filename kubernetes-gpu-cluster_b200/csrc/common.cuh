@@ -149,6 +149,9 @@ __device__ __forceinline__ uint32_t mapa_u32(uint32_t local, uint32_t rank) {   
   return r;
 }
 
+// Dynamic shared memory that a launch has without opting in, beside 8 KB of its kernel's own: both together may be 48 KB.
+constexpr size_t kPlainShared = 40 * 1024;
+
 // Every kernel of a step asks for the same L1 / shared-memory split (all shared memory): the GEMM and attention kernels
 // need ~200 KB per SM anyway, and an SM that has to change its split between two kernels must drain first, which
 // serialises exactly the kernel boundaries that programmatic dependent launch is there to overlap.  (Knob

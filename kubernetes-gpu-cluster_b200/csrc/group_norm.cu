@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256) silu_mul_halves_kernel(E* y, const E* gu,
 
 template <typename K>
 int opt_in_smem(K kern, size_t smem) {
-  if (smem > 48 * 1024) KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > kPlainShared) KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return 0;
 }
 

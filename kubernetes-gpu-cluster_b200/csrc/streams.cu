@@ -183,16 +183,16 @@ int stream_norm(const StreamNormArgs& a, cudaStream_t st) {
   KGE_REQUIRE(a.S >= 1 && a.S <= SMAX && a.d > 0 && (size_t)a.d * 4 <= 200 * 1024, "stream_norm: %d streams of %d columns", a.S, a.d);
   const size_t smem = (size_t)a.d * 4;
   static size_t smem_set = 0;
-  if (smem > 48 * 1024 && smem > smem_set) {
+  if (smem > kPlainShared && smem > smem_set) {
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_norm_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_norm_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   const bool vec = a.d % 8 == 0 && al16(a.xs) && al16(a.y) && al16(a.w) && al16(a.sum_out);
-  if (vec && smem > 48 * 1024 && smem > smem_set) {
+  if (vec && smem > kPlainShared && smem > smem_set) {
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_norm_vec_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_norm_vec_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
-  if (smem > 48 * 1024 && smem > smem_set) smem_set = smem;
+  if (smem > kPlainShared && smem > smem_set) smem_set = smem;
   cudaError_t ce;
   if (vec) ce = a.elt == KGE_ELT_F32 ? launch_pdl(stream_norm_vec_kernel<float>, dim3(a.R), dim3(256), smem, st, a)
                                      : launch_pdl(stream_norm_vec_kernel<__nv_bfloat16>, dim3(a.R), dim3(256), smem, st, a);
@@ -249,17 +249,17 @@ int stream_combine(const StreamCombineArgs& a, cudaStream_t st) {
   const size_t smem = a.next_y ? (size_t)a.d * 4 : 0;
   KGE_REQUIRE(smem <= 200 * 1024, "stream_combine: rows of %d columns", a.d);
   static size_t smem_set = 0;
-  if (smem > 48 * 1024 && smem > smem_set) {
+  if (smem > kPlainShared && smem > smem_set) {
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_combine_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_combine_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   bool vec = a.d % 8 == 0 && al16(a.xs) && al16(a.y32) && al16(a.col_scale) && al16(a.next_y) && al16(a.next_w);
   for (int i = 0; i < a.src.n; ++i) vec = vec && al16(a.src.src[i]) && a.src.ld[i] % 8 == 0;
-  if (vec && smem > 48 * 1024 && smem > smem_set) {
+  if (vec && smem > kPlainShared && smem > smem_set) {
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_combine_vec_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     KGE_CUDA_OK(cudaFuncSetAttribute(stream_combine_vec_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
-  if (smem > 48 * 1024 && smem > smem_set) smem_set = smem;
+  if (smem > kPlainShared && smem > smem_set) smem_set = smem;
   cudaError_t ce;
   if (vec) ce = a.elt == KGE_ELT_F32 ? launch_pdl(stream_combine_vec_kernel<float>, dim3(a.T), dim3(256), smem, st, a)
                                      : launch_pdl(stream_combine_vec_kernel<__nv_bfloat16>, dim3(a.T), dim3(256), smem, st, a);

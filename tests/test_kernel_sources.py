@@ -71,3 +71,20 @@ def test_tensor_memory_is_allocated_before_the_next_kernel_may_start(file, kerne
     alloc, start = body.index("tcgen05.alloc"), body.index("pdl_launch_dependents")
     assert alloc < start, (file, kernel)
     assert "__syncthreads()" in body[alloc:start], (file, kernel)      # by one warp: the others may not announce it earlier
+
+
+def test_shared_memory_of_a_kernels_own_counts_towards_what_needs_no_opt_in():
+    """48 KB go without the attribute, of dynamic and static shared memory together: where kernels have both, the dynamic part alone is compared
+    with a bound that leaves room for the other."""
+    names = {"GN_MAX_GROUPS": 1024, "SMAX": 8}
+    room = 48 * 1024 - eval(re.search(r"kPlainShared = ([\d* ]+);", open(os.path.join(CSRC, "common.cuh")).read()).group(1))
+    found = 0
+    for f, kernel, body in kernels():
+        if f in ("group_norm.cu", "streams.cu") and "extern __shared__" in body:
+            sizes = re.findall(r"\w+\[([^\]]+)\]", " ".join(re.findall(r"(?<!extern )__shared__ float ([^;]*);", body)))
+            assert sum(4 * eval(n, dict(names)) for n in sizes) <= room, (f, kernel)
+            found += 1
+    assert found >= 6
+    for f in ("group_norm.cu", "streams.cu"):
+        src = open(os.path.join(CSRC, f)).read()
+        assert "48 * 1024" not in src and "> kPlainShared" in src, f
