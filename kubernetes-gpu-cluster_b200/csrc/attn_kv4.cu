@@ -19,6 +19,7 @@
 //   looks at the sums of e and e z_v too, keeps R in two parts and lets e become denormal.
 //   scores come out as (key, head) fragments; movmatrix turns a packed 8 x 8 of weights into the B operand of the second product
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kge.h"
@@ -270,52 +271,46 @@ struct Core {
     const uint32_t k_at = at + g * (HD / 2) + t * (HD / 8), n_at = at + 16 * HD + kv4::key_token(g) * 4;
     // ---- scores in units of log 2, less the reference: rows g and g + 8 of group i are keys key0 + 16 i + key_token(g) and 8 further
     float x[2][NT][4], zv[2][2], sv[2][2];
+    auto scores = [&](auto each) {             // each: heads have an fs of their own (a path of its own: 2 % of long batches' time in the other)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t ka[W], kb[W];
-      if (HD == 128) {
-        const uint4 u = lds128(k_at + i * GB), v = lds128(k_at + i * GB + 512);
-        ka[0] = u.x; ka[1] = u.y; ka[W - 2] = u.z; ka[W - 1] = u.w;
-        kb[0] = v.x; kb[1] = v.y; kb[W - 2] = v.z; kb[W - 1] = v.w;
-      } else {
-        const uint2 u = lds64(k_at + i * GB), v = lds64(k_at + i * GB + 256);
-        ka[0] = u.x; ka[1] = u.y;
-        kb[0] = v.x; kb[1] = v.y;
-      }
-      float c[NT][4];
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const uint32_t a0 = ka[j], b0 = kb[j], a1 = a0 >> 8, b1 = b0 >> 8;
-        const uint32_t f0[4] = {codes_lo(a0), codes_lo(b0), codes_hi(a0), codes_hi(b0)}, f1[4] = {codes_lo(a1), codes_lo(b1), codes_hi(a1), codes_hi(b1)};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (j == 0) mma_f16_first(c[nt], f0, qb[nt][0][0], qb[nt][0][1]);
-          else mma_f16(c[nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
-          mma_f16(c[nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+      for (int i = 0; i < 2; ++i) {
+        uint32_t ka[W], kb[W];
+        if (HD == 128) {
+          const uint4 u = lds128(k_at + i * GB), v = lds128(k_at + i * GB + 512);
+          ka[0] = u.x; ka[1] = u.y; ka[W - 2] = u.z; ka[W - 1] = u.w;
+          kb[0] = v.x; kb[1] = v.y; kb[W - 2] = v.z; kb[W - 1] = v.w;
+        } else {
+          const uint2 u = lds64(k_at + i * GB), v = lds64(k_at + i * GB + 256);
+          ka[0] = u.x; ka[1] = u.y;
+          kb[0] = v.x; kb[1] = v.y;
         }
-      }
+        float c[NT][4];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t pk = lds32(n_at + i * GB + 32 * r), pv = lds32(n_at + i * GB + 64 + 32 * r);
-        const float lk = bf_hi(pk), f = fs * bf_lo(pk);
-        sv[i][r] = bf_lo(pv);
-        zv[i][r] = fmaf(8.f, sv[i][r], bf_hi(pv));
+        for (int j = 0; j < W; ++j) {
+          const uint32_t a0 = ka[j], b0 = kb[j], a1 = a0 >> 8, b1 = b0 >> 8;
+          const uint32_t f0[4] = {codes_lo(a0), codes_lo(b0), codes_hi(a0), codes_hi(b0)}, f1[4] = {codes_lo(a1), codes_lo(b1), codes_hi(a1), codes_hi(b1)};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], f, fmaf(qs[nt][h], lk, -ref[nt][h]));
-      }
-      if (uneven)
+          for (int nt = 0; nt < NT; ++nt) {
+            if (j == 0) mma_f16_first(c[nt], f0, qb[nt][0][0], qb[nt][0][1]);
+            else mma_f16(c[nt], f0, qb[nt][2 * j][0], qb[nt][2 * j][1]);
+            mma_f16(c[nt], f1, qb[nt][2 * j + 1][0], qb[nt][2 * j + 1][1]);
+          }
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t pk = lds32(n_at + i * GB + 32 * r);
+          const uint32_t pk = lds32(n_at + i * GB + 32 * r), pv = lds32(n_at + i * GB + 64 + 32 * r);
+          const float lk = bf_hi(pk), f = fs * bf_lo(pk);
+          sv[i][r] = bf_lo(pv);
+          zv[i][r] = fmaf(8.f, sv[i][r], bf_hi(pv));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], lows[8 * (NT + nt) + 2 * t + h] * bf_lo(pk), fmaf(qs[nt][h], bf_hi(pk), -ref[nt][h]));
+            for (int h = 0; h < 2; ++h) x[i][nt][2 * r + h] = fmaf(c[nt][2 * r + h], decltype(each)::value ? lows[8 * (NT + nt) + 2 * t + h] * bf_lo(pk) : f, fmaf(qs[nt][h], lk, -ref[nt][h]));
         }
-    }
+      }
+    };
+    if (uneven) scores(std::true_type());      // the same for the warp
+    else scores(std::false_type());
     if (edge) {                                // the same for the warp
       const int mine = key0 + kv4::key_token(g);
 #pragma unroll
@@ -352,7 +347,7 @@ struct Core {
     const bool fits = weigh();
     // Small weights say that e and e z_v are small where no s_v is zero (it is 2^-16 |z_v| then, or more) or next to it.
     const bool plain = fminf(fminf(sv[0][0], sv[0][1]), fminf(sv[1][0], sv[1][1])) >= kRoomDown;
-    if (fresh || hard || !__all_sync(0xffffffffu, fits && plain)) {
+    if (!__all_sync(0xffffffffu, fits & plain & !fresh & !hard)) {
       bool wide = hard || !plain || fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1])) > kDeepMost;      // for the hard path
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -850,16 +845,23 @@ constexpr int kDescBytes = kMaxShares * 16;    // the workspace's start
 constexpr int64_t workspace_bytes(int G, int hd) { return kDescBytes + (int64_t)2 * kMaxShares * G * (hd + 4) * 4; }
 constexpr int kMaxRequests = 1024;             // requests of one launch (every warp reads their lengths)
 
-// Which kernel.  A CTA per (request, kv head) has four CTAs an SM, which cover each other's starts and ends, and the hardware's queue; shares have
-// three, a producer and a merge behind them (4 us), but every SM has work whatever the lengths are.  us with a CTA each / with shares, 32 / 8
-// heads of 128:           1024 keys     1500         2048         2900         4096         6000
-//      8 requests (64 groups)  8.2 / 10.8  11.1 / 11.6  14.0 / 12.0  19.5 / 13.5  27.6 / 16.8  38.9 / 19.2
-//     48 (384)                19.0 / 20.2  24.9 / 24.8  31.1 / 28.8  41.4 / 36.3  55.3 / 45.3  78.4 / 60.5
-//     72 (576)                20.6 / 26.8  26.2 / 35.0  32.6 / 39.0  43.1 / 49.9  57.4 / 63.8  80.9 / 85.1
-//    100 (800)                27.4 / 32.6  36.1 / 40.7  45.7 / 49.1  61.4 / 63.3  82.4 / 82.9   117 / 115
-//    150 (1200)               37.7 / 43.9  50.2 / 55.8  64.2 / 68.2  87.4 / 89.4   118 / 118    170 / 168
+// Which kernel.  A CTA per (request, kv head) has four CTAs an SM (three for groups of 9 to 16), which cover each other's starts and ends, and the
+// hardware's queue; shares have three (two), a producer and a merge behind them (4 us), but every SM has work whatever the lengths are.  us with a
+// CTA each / with shares, 32 / 8 heads of 128:
+//                             1024 keys     1500         2048         2900         4096         6000
+//      8 requests (64 groups)  8.9 / 11.3  12.0 / 12.3  15.0 / 12.7  20.7 / 14.2  29.2 / 17.3  41.1 / 19.4
+//     48 (384)                19.5 / 20.9  25.5 / 25.4  31.9 / 29.2  42.6 / 36.4  56.9 / 45.5  80.5 / 60.3
+//     72 (576)                20.8 / 27.7  26.7 / 33.6  33.3 / 39.2  44.2 / 50.2  59.0 / 64.2  83.0 / 88.1
+//    100 (800)                28.2 / 32.6  37.3 / 41.2  47.3 / 49.1  63.5 / 63.6  85.2 / 83.0   122 / 117
+//    150 (1200)               38.8 / 44.6  52.3 / 56.7  67.0 / 69.2  90.8 / 90.7   123 / 122    179 / 173
+//                   32 / 8 heads of 64                      128 / 8 heads of 128
+//                   1024 keys    2048         4096          1024         2048         4096
+//      8 (64)        7.4 /  9.8  12.2 / 10.7  22.0 / 13.0   14.4 / 20.1  23.1 / 22.0  42.7 / 27.4
+//     48 (384)      15.0 / 15.9  26.0 / 22.3  46.5 / 34.2   25.0 / 37.9  40.0 / 50.6  68.9 / 77.4
+//    100 (800)      21.2 / 25.0  34.5 / 36.7  61.6 / 60.5   46.3 / 58.3  74.9 / 84.7   132 / 138
 // so: up to 1024 keys, or six groups for every 32 keys; and up to 8192 keys, since one long context among many short ones is a single CTA's
-// work (0.35 us for 128 keys).
+// work (0.35 us for 128 keys).  How evenly the groups fall on the SMs is not looked at: that gives up 9 % at 384 groups of 2048 keys (17 % with
+// heads of 64) and at 576 of 4096, 6 % at 576 of 6000, 12 % at 384 groups of 16 heads and 4096 keys, and up to 4 % in other cells.
 static bool cta_each(int64_t groups, int keys) {
   const int units = (keys + WK - 1) / WK;
   return units <= 32 || (units <= 256 && groups >= 6 * units);
