@@ -637,7 +637,16 @@ static int launch(bf16* out, const bf16* q, int q_stride, KvArgs ka, int B, int 
   ka.per = 2;
   dim3 grid = tc_grid(B, T, max_q_len, ka.per * TT, ka.KV, by_request);
   auto items = [&] { return by_request ? ka.KV * ((int64_t)T / (ka.per * TT) + B) : (int64_t)grid.x * grid.y * grid.z; };
-  if (items() <= 74 || (items() <= 148 && max_seq_len >= 512)) {       // one query tile an item and its key tiles shared out (attn_pair.cuh)
+  // One query tile an item and its key tiles shared out (attn_pair.cuh), where items of two tiles leave SMs without work.  us of an item each / two tiles
+  // an item, 32 / 8 heads of 128, bfloat16 (float16 within 1 %), requests x rows behind cached keys, items of two tiles:
+  //    1 x 64    (8)    9.4 / 10.5      4 x 192 (96)  17.4 / 13.2      1 x 256 + 2000  (32)  45.9 / 62.4
+  //    1 x 256  (32)   12.3 / 14.1      4 x 256 (128) 18.5 / 14.5      1 x 512 + 2000  (64)  50.4 / 68.6
+  //    1 x 640  (80)   18.4 / 22.5      8 x 128 (128) 17.7 / 12.4      1 x 1024 + 2000 (128) 92.6 / 81.5
+  //    1 x 1024 (128)  27.9 / 31.6      4 x 300 (160) 25.8 / 18.1      2 x 512 + 4000  (128)  147 / 116
+  //    1 x 1184 (152)  37.2 / 37.1      1 x 2048 (256) 81.4 / 58.7     5 x 256 + 600   (160) 50.5 / 45.4
+  // so: up to 74 of them, and up to 148 where contexts are long enough that the last rows' items decide.  Rows behind many more cached keys have items
+  // alike: there the second half of that gives up 14 to 27 %.
+  if (items() <= 74 || (items() <= 148 && max_seq_len >= 512)) {
     ka.per = 1;
     grid = tc_grid(B, T, max_q_len, ka.per * TT, ka.KV, by_request);
   }
