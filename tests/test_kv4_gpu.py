@@ -6,8 +6,7 @@ Tolerances.  u is half a step of the 16-bit type relative to the value, eps / 2 
   are rounded once, to float16 (2^-11) in single-token requests and at most to the 16-bit type (u) in prompts; what they are multiplied with is
   |n - 8| <= 8, so that costs 8 max s of it at most.  The result is rounded once, u |out|.  Scores and sums are in fp32: their errors stay below
   2^-13 of the weights here.
-  Prompts in bfloat16 round keys, values and weights to float16, 2^-11 = u / 8 each: with scores of sum |q k| scale < 10 in the numbers of these
-  tests, 2^-11 (2 + 2 x 10) sum p |v| < 0.011 sum p |v|, below the u 8 max s = 0.012 that is allowed for weights rounded to u.
+  (Prompts round them to float16 too, which is less than u 8 max s; test_kv4_rows_gpu.py holds both to the roundings alone.)
   In the 2-norm the roundings are independent, each of at most u / sqrt(3) in the mean square: result and weights together sqrt(2 / 3) u =
   0.82 u where s (n - 8) is as large as the values (their ends lie about zero), held to 1.2 (u + 2^-11).
 """
