@@ -98,7 +98,8 @@ def test_later_rows_leave_earlier_queries_alone(kge, L, dtype, hd, H, KV, lens, 
 
 # ------------------------------------------------------------------------------------------------------ rows far apart
 
-SINGLE = [(128, 4, 1, [150, 90, 64], [1, 1, 1]), (64, 12, 1, [900, 33], [1, 1]), (128, 16, 1, [70, 500], [1, 1]), (128, 32, 8, [1500, 700], [1, 1])]
+SINGLE = [(128, 4, 1, [150, 90, 64], [1, 1, 1]), (64, 12, 1, [900, 33], [1, 1]), (128, 16, 1, [70, 500], [1, 1]), (128, 32, 8, [1500, 700], [1, 1]),
+          (128, 16, 1, [2000, 40], [1, 1]), (64, 10, 1, [1300], [1]), (128, 3, 1, [3100], [1])]      # the last three: shares of one group, many pieces
 FAR = SINGLE + [(128, 4, 1, [150, 90, 64], [64, 90, 7]), (64, 40, 2, [150, 90, 64], [1, 90, 1]), (128, 32, 8, [300] * 6, [300] * 6)]
 
 
