@@ -243,6 +243,47 @@ int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32_t* seq_len
                   int64_t* slot_mapping, int32_t* counts, const int32_t* cached_lens, const int32_t* new_lens, const int32_t* free_blocks,
                   int num_free, const int32_t* free_first, int B, int T, int block_size, void* stream);
 
+/* 8-bit floating point with a scale for each block of 128 (vllm:model_executor/layers/quantization/fp8.py with weight_block_size [128, 128],
+ * quantization/utils/fp8_utils.py): half the bytes of a weight and twice the rate of the matrix units.
+ *
+ * Codes are e4m3 (4 bits of exponent, 3 of mantissa, largest number 448), one byte each, in the order of the 16-bit numbers that they stand for; a
+ * number is scale * code.  A block with the largest magnitude m has the scale s = max(m / 448, 2^-126) in fp32, and a number x of it the code nearest
+ * to 448 x / m (2^126 x where m is below 448 2^-126), ties to even.  A block with an infinity or NaN has the scale NaN and codes of zero.
+ *   rows (activations)  a block is 128 columns of a row (the last one what is left); scales [ceil(K / 128)][scales_stride], block by block: those of
+ *                       neighbouring rows lie together, and a slice of rows t0 .. is (codes + t0 * K, scales + t0) with the same stride
+ *   matrices (weights)  a block is 128 rows x 128 columns; scales [ceil(N / 128), ceil(K / 128)] (a checkpoint's weight_scale_inv)
+ * K is a multiple of 16; N and the number of rows are any.  Codes, x and w are 16-byte aligned.
+ *
+ * kge_fp8_quant: T rows of x (x_stride elements apart, a multiple of 8) to codes [T, K] and scales.  rows (may be NULL) gathers: row t is x's row
+ * rows[t] (tokens sorted by expert), zeros where rows[t] < 0. */
+int kge_fp8_quant(void* codes, float* scales, int scales_stride, const void* x, int x_stride, const int32_t* rows, int T, int K, void* stream);
+
+/* E matrices w [E, N, K] to codes [E, N, K] and scales [E, ceil(N / 128), ceil(K / 128)]: a 16-bit checkpoint's weights. */
+int kge_fp8_quant_weight(void* codes, float* scales, const void* w, int E, int N, int K, void* stream);
+
+/* y[T, N] = x w^T (+ bias[N], 16 bits, may be NULL) from codes and scales of x [T, K] and of w [N, K]: products of a block of K are summed in fp32, times
+ * the two scales added up over the blocks in fp32, and rounded once.  Scales that are infinite or NaN make what they touch so.
+ * `workspace`: device scratch of kge_gemm_fp8_workspace_bytes(T) bytes, 16-byte aligned, whose first 1024 bytes are ZERO before the first call that
+ * uses it (every call leaves them zero again).  Calls that share a workspace must not overlap on the GPU.  Weights may be read before the kernel
+ * before on the stream has ended (kge_set_tunable "pdl"). */
+int kge_gemm_fp8(void* y, const void* x, const float* x_scales, int x_scales_stride, const void* w, const float* w_scales, const void* bias, int T, int N,
+                 int K, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t kge_gemm_fp8_workspace_bytes(int T);
+
+/* The gated front half: h = silu(x w[:f]^T) * (x w[f:]^T), w = [gate | up] [2f, K], f a multiple of 128, quantised as kge_fp8_quant does - codes [T, f] and
+ * scales [f / 128][scales_stride] for the product behind it.  Everything between the sums and the codes is in fp32. */
+int kge_gemm_fp8_silu_gate(void* codes, float* scales, int scales_stride, const void* x, const float* x_scales, int x_scales_stride,
+                           const void* w_gate_up, const float* w_scales, int T, int f, int K, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Both with rows in E groups of ragged sizes, each with a matrix of its own (the experts of a mixture): group e has the rows offsets[e] .. offsets[e + 1]
+ * (device, [E + 1], not falling; a group may be empty) and w[e], w_scales[e].  T: rows of x, y, codes, an upper bound of offsets[E]; rows outside
+ * of all groups are left as they were.  E up to 1024.  No size of a group has to be known to the host. */
+int kge_gemm_fp8_grouped(void* y, const void* x, const float* x_scales, int x_scales_stride, const void* w, const float* w_scales, const int32_t* offsets,
+                         int E, int T, int N, int K, void* workspace, int64_t workspace_bytes, void* stream);
+int kge_gemm_fp8_grouped_silu_gate(void* codes, float* scales, int scales_stride, const void* x, const float* x_scales, int x_scales_stride,
+                                   const void* w_gate_up, const float* w_scales, const int32_t* offsets, int E, int T, int f, int K, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
 /* Greedy sampling, vllm:v1/sample/sampler.py:91,235-236: argmax over fp32(bf16 logits),
  * lowest index wins ties.  logits [B, ld] bf16 (ld >= V: padded vocab columns ignored). */
 int kge_argmax(int32_t* out_ids, const void* logits, int B, int V, int ld, void* stream);
@@ -301,6 +342,12 @@ int kge_paged_attn_kv4_f16(void* out, const void* q, int q_stride, const void* k
                            int max_blocks_per_seq, const int32_t* seq_lens, const int32_t* query_start_loc, int B, int T, int max_q_len,
                            int max_seq_len, int H, int KV, int hd, int block_size, float scale, int window, int first, void* workspace,
                            int64_t workspace_bytes, void* stream);
+int kge_fp8_quant_f16(void* codes, float* scales, int scales_stride, const void* x, int x_stride, const int32_t* rows, int T, int K, void* stream);
+int kge_fp8_quant_weight_f16(void* codes, float* scales, const void* w, int E, int N, int K, void* stream);
+int kge_gemm_fp8_f16(void* y, const void* x, const float* x_scales, int x_scales_stride, const void* w, const float* w_scales, const void* bias, int T,
+                     int N, int K, void* workspace, int64_t workspace_bytes, void* stream);
+int kge_gemm_fp8_grouped_f16(void* y, const void* x, const float* x_scales, int x_scales_stride, const void* w, const float* w_scales,
+                             const int32_t* offsets, int E, int T, int N, int K, void* workspace, int64_t workspace_bytes, void* stream);
 int kge_argmax_f16(int32_t* out_ids, const void* logits, int B, int V, int ld, void* stream);
 int kge_sample_f16(int32_t* out_ids, const void* logits, int B, int V, int ld, const float* temperature,
                    const int32_t* top_k, const float* top_p, const float* exp_noise, const uint64_t* seeds, uint64_t step,

@@ -97,6 +97,13 @@ SIGNATURES = {
     "kge_paged_attn_kv4": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _L, _P]),
     "kge_attn_kv4_workspace_bytes": (_L, [_I, _I, _I]),
     "kge_step_maps": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P]),
+    "kge_fp8_quant": (_I, [_P, _P, _I, _P, _I, _P, _I, _I, _P]),
+    "kge_fp8_quant_weight": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "kge_gemm_fp8": (_I, [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _L, _P]),
+    "kge_gemm_fp8_workspace_bytes": (_L, [_I]),
+    "kge_gemm_fp8_silu_gate": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _I, _I, _I, _P, _L, _P]),
+    "kge_gemm_fp8_grouped": (_I, [_P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P]),
+    "kge_gemm_fp8_grouped_silu_gate": (_I, [_P, _P, _I, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P]),
     "kge_argmax": (_I, [_P, _P, _I, _I, _I, _P]),
     "kge_sample": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P, _P, C.c_uint64, _P, _L, _P]),
     "kge_sample_workspace_bytes": (_L, [_I, _I]),
@@ -181,7 +188,8 @@ for _n, _t in {"kge_embed": "kge_embed_f16", "kge_rmsnorm": "kge_rmsnorm_f16", "
                "kge_gemm_silu_gate_ws_bf16": "kge_gemm_silu_gate_ws_f16", "kge_gemm_clamped_glu_bf16": "kge_gemm_clamped_glu_f16",
                "kge_rope_kvwrite": "kge_rope_kvwrite_f16", "kge_rope_cache_host": "kge_rope_cache_host_f16",
                "kge_paged_attn": "kge_paged_attn_f16", "kge_rope_kv4write": "kge_rope_kv4write_f16", "kge_kv4_read": "kge_kv4_read_f16",
-               "kge_paged_attn_kv4": "kge_paged_attn_kv4_f16", "kge_argmax": "kge_argmax_f16", "kge_sample": "kge_sample_f16",
+               "kge_paged_attn_kv4": "kge_paged_attn_kv4_f16", "kge_fp8_quant": "kge_fp8_quant_f16",
+               "kge_fp8_quant_weight": "kge_fp8_quant_weight_f16", "kge_gemm_fp8": "kge_gemm_fp8_f16", "kge_gemm_fp8_grouped": "kge_gemm_fp8_grouped_f16", "kge_argmax": "kge_argmax_f16", "kge_sample": "kge_sample_f16",
                "kge_logprobs": "kge_logprobs_f16", "kge_tp_reduce_add_norm": "kge_tp_reduce_add_norm_f16"}.items():
     SIGNATURES[_t] = SIGNATURES[_n]
 

@@ -1,0 +1,32 @@
+// 8-bit floating point (e4m3: 4 bits of exponent, 3 of mantissa, largest number 448) with a scale for each block of 128.
+//
+// A block with the largest magnitude m has the scale s = max(m / 448, 2^-126) in fp32, and a number x of it the code nearest to 448 x / m (to
+// 2^126 x below that), ties to even.  A block with an infinity or NaN has the scale NaN and codes of zero, so every product with it is NaN.
+#pragma once
+#include "common.cuh"
+
+namespace kge {
+namespace fp8 {
+constexpr int kBlock = 128;
+constexpr float kMax = 448.f;
+constexpr float kLeast = 1.17549435e-38f;                  // 2^-126
+inline int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+#ifdef __CUDACC__
+// two numbers as codes, the first in the low byte
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack2(a, b) | pack2(c, d) << 16; }
+
+// A block's scale and what its numbers are multiplied with, from its largest magnitude; an infinity or NaN gives NaN and zero.
+__device__ __forceinline__ void scale_of(float m, float& scale, float& factor) {
+  const bool fine = m <= 3.402823466e38f;
+  scale = fine ? fmaxf(__fdiv_rn(m, kMax), kLeast) : __int_as_float(0x7fffffff);
+  factor = fine ? __fdiv_rn(kMax, fmaxf(m, kMax * kLeast)) : 0.f;
+}
+#endif
+}  // namespace fp8
+}  // namespace kge
