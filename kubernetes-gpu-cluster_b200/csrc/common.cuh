@@ -125,6 +125,12 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity) {
   while (!mbar_try(bar, parity))
     if (clock64() - t0 > kBarrierCycles) __trap();
 }
+// Whether it has, without waiting: a thread that paces others asks for its next barrier early and looks at the answer when it gets there.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 // The same for a warp that runs ahead of others and only feeds them: every arrival wakes a waiter, and its tries take issue slots from those
 // that compute (a fifth of a decode attention's instructions), so it sleeps in between.
 __device__ __forceinline__ void mbar_wait_idle(uint32_t bar, uint32_t parity) {

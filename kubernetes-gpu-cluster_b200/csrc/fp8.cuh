@@ -22,10 +22,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) { return pack2(a, b) | pack2(c, d) << 16; }
 
 // A block's scale and what its numbers are multiplied with, from its largest magnitude; an infinity or NaN gives NaN and zero.
+// The scale is m / 448 rounded once: a product with 1 / 448 and what is left of m, which one fma gives exactly.  The factor is off by 2^-22 at most (a
+// reciprocal within a last place of m / 16, which keeps both of them normal numbers).  Two divisions were two thirds of an eight-lane block's instructions.
 __device__ __forceinline__ void scale_of(float m, float& scale, float& factor) {
   const bool fine = m <= 3.402823466e38f;
-  scale = fine ? fmaxf(__fdiv_rn(m, kMax), kLeast) : __int_as_float(0x7fffffff);
-  factor = fine ? __fdiv_rn(kMax, fmaxf(m, kMax * kLeast)) : 0.f;
+  constexpr float c = 1.f / kMax;
+  float q = m * c;
+  q = fmaf(fmaf(-kMax, q, m), c, q);
+  float inv;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(fmaxf(m, kMax * kLeast) * 0.0625f));
+  scale = fine ? fmaxf(q, kLeast) : __int_as_float(0x7fffffff);
+  factor = fine ? inv * (kMax * 0.0625f) : 0.f;
 }
 #endif
 }  // namespace fp8

@@ -4,8 +4,7 @@
 //
 // Orientation: the MMA's M rows are TOKENS and its N columns weight rows, so that what a thread reads back of tensor memory (one lane) belongs to one
 // token and, within 128 columns, to one scale of the weights: a single factor for all of them.  tcgen05.mma sums a block of K (four instructions of
-// 32) in fp32 in tensor memory, and eight warps add it, times its factor, to accumulators in registers: TM += factor * D, two numbers an
-// instruction.  Tensor memory holds several blocks, so that the next ones are multiplied meanwhile.
+// 32) in fp32 in tensor memory, and eight warps add it, times its factor, to accumulators in registers.  Tensor memory holds several blocks, so that the next ones are multiplied meanwhile.
 //
 // Two kernels.
 //  fp8_stream_kernel: tiles of 128 tokens x NT weight rows by single CTAs, one an SM; the (tile, block of K) units of the whole problem are laid end
@@ -15,7 +14,6 @@
 //    shared memory, 32 KB a block of K, where its MMA takes 512 cycles.
 #include <cuda.h>
 
-#include "f32x2.cuh"
 #include "fp8.cuh"
 #include "kge.h"
 
@@ -24,12 +22,22 @@ inline namespace KGE_ELT_NS {
 
 constexpr int kRows = 128;                        // tokens of a CTA's tile
 constexpr int kSlab = 128 * 128;                  // bytes of 128 rows of a block of K
-constexpr int kThreads = 384;                     // producer, MMA, tensor memory, table; eight warps that add up
+#ifndef FP8_CHUNK
+#define FP8_CHUNK 32
+#define FP8_UP 216
+#define FP8_DOWN 72
+#endif
+constexpr int kSumWarps = 8;                      // warps that add up: a token of 128 and 64 columns of each 128 a thread
+constexpr int kThreads = 128 + 32 * kSumWarps;    // producer, MMA, tensor memory, factors; those
+constexpr int kChunk = FP8_CHUNK;                 // columns that a warp reads of tensor memory at a time
 constexpr int kCounters = 256;                    // arrival counters at the head of the workspace
 constexpr int kMaxCtas = 160;
 constexpr int kMaxGroups = 1024;
 constexpr int kSmem = 226 * 1024;
 constexpr int kPairStages = 6;
+constexpr int kPairSlots = kPairStages + 2;
+constexpr int kPairBatch = 4, kBatch = 2;         // blocks that a warp prepares factors of at a time
+static_assert(kPairStages > kPairBatch, "");
 constexpr int kPairBand = 8;                      // 74 pairs at work: 8 x 9 tiles share 17 slabs a block of K, 32 x 2.3 would 34
 
 struct Fp8Params {
@@ -45,6 +53,7 @@ struct Fp8Params {
   int E, T, N, KB, n_tiles, w_rows, w_blocks;     // w_rows, w_blocks: of one group's matrix (2 N when gated)
   float* part;                                    // stream: partial sums
   unsigned int* count;
+  int wide;                                       // pairs: y's rows are 16-byte aligned
   int quarters, stages, x_bytes, min_units;       // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, least units of a share
 };
 
@@ -54,7 +63,9 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// On a barrier of the pair's leader.  What it tells is that tensor memory has been read (tcgen05.wait::ld, the fence before): nothing in memory is
+// published, and a release for the whole cluster would wait for all of a thread's stores, every block of K (2048 x 9472 x 4096: 194 us with it).
+__device__ __forceinline__ void bar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
@@ -77,13 +88,21 @@ __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_
 __device__ __forceinline__ void mma8x2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-// 32 columns of this warp's 32 lanes; the caller waits (tmem_wait_ld)
-__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&r)[32]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(at));
+// N columns of this warp's 32 lanes; the caller waits (tmem_wait_ld)
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[N]) {
+  static_assert(N == 16 || N == 32, "");
+  if constexpr (N == 32)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+  else
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
 }
 // K-major tile of 128-byte rows with 128-byte swizzle, atoms of 8 rows 1024 bytes apart
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at) {
@@ -102,23 +121,27 @@ __device__ __forceinline__ void group_rows(const Fp8Params& p, int e, int& r0, i
   r0 = min(max(p.offsets[e], 0), p.T);
   r1 = max(r0, min(p.offsets[e + 1], p.T));
 }
-// One warp: starts[e] = tiles of the groups before e.
-__device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, int* starts, int lane) {
-  int total = 0;
-  for (int e0 = 0; e0 < p.E; e0 += 32) {
-    int n = 0;
-    if (e0 + lane < p.E) {
-      int r0, r1;
-      group_rows(p, e0 + lane, r0, r1);
-      n = (r1 - r0 + tile_rows - 1) / tile_rows * p.n_tiles;
-    }
-    int s = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += v; }
-    if (e0 + lane < p.E) starts[e0 + lane] = total + s - n;
-    total += __shfl_sync(0xffffffffu, s, 31);
+// starts[e] = tiles of the groups before e.  By all threads of the CTA.
+__device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, int* starts) {
+  for (int e = threadIdx.x; e < p.E; e += kThreads) {
+    int r0, r1;
+    group_rows(p, e, r0, r1);
+    starts[e] = (r1 - r0 + tile_rows - 1) / tile_rows * p.n_tiles;
   }
-  if (lane == 0) starts[p.E] = total;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    int total = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + threadIdx.x, n = e < p.E ? starts[e] : 0;
+      int s = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, s, o); if ((int)threadIdx.x >= o) s += v; }
+      if (e < p.E) starts[e] = total + s - n;
+      total += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (threadIdx.x == 0) starts[p.E] = total;
+  }
+  __syncthreads();
 }
 
 // A tile: rows [row, row + rows) of the tokens and column tile n of group e.
@@ -148,78 +171,86 @@ __device__ __forceinline__ int first_group(const Fp8Params& p, const int* starts
 // The running sums of a thread: one token, C columns.
 template <int C>
 struct Sums {
-  f2 v[C / 2];
+  float v[C];
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < C / 2; ++i) v[i] = 0ull;
+    for (int i = 0; i < C; ++i) v[i] = 0.f;
   }
-  // += factor * D of 32 columns at c
-  __device__ __forceinline__ void add(int c, const uint32_t (&r)[32], float factor) {
-    const f2 s = pk(factor, factor);
+  // += factor * D of kChunk columns at c
+  __device__ __forceinline__ void add(int c, const uint32_t (&r)[kChunk], float factor) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[c / 2 + i] = fma2(pk(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), s, v[c / 2 + i]);
+    for (int i = 0; i < kChunk; ++i) asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(v[c + i]) : "f"(__uint_as_float(r[i])), "f"(factor));
   }
-  __device__ __forceinline__ void at(int c, float& a, float& b) const { upk(v[c / 2], a, b); }
+  __device__ __forceinline__ void at(int c, float& a, float& b) const { a = v[c]; b = v[c + 1]; }
 };
 
-// A block of K, at tensor memory address `at`: columns below C / 2 times f0, the others times f1 (the same but for gate and up).
-template <int C>
-__device__ __forceinline__ void add_block(Sums<C>& s, uint32_t at, float f0, float f1) {
-  uint32_t r[2][32];
-  tmem_ld32(at, r[0]);
+// Adds up `blocks` blocks of K.  wait(): the address of the next block's columns in tensor memory and its factors, when they are there; read(): they are
+// in registers.  A thread's second 64 columns (if it has them) lie SKIP columns behind its first, with a factor of their own.  The next block is waited
+// for, and its first columns asked for, before the last ones of this block are added, so that the way to tensor memory and back passes under arithmetic.
+template <int C, int SKIP, typename W, typename R>
+__device__ __forceinline__ void add_blocks(Sums<C>& s, int blocks, W wait, R read) {
+  uint32_t r[2][kChunk], at;
+  float f0, f1;
+  wait(at, f0, f1);
+  tmem_ld(at, r[0]);
+#pragma unroll 1
+  for (; blocks > 0; --blocks) {
+    const float g0 = f0, g1 = f1;
 #pragma unroll
-  for (int c = 0; c < C; c += 32) {
-    tmem_wait_ld(r[(c / 32) & 1]);
-    if (c + 32 < C) tmem_ld32(at + c + 32, r[(c / 32 + 1) & 1]);
-    s.add(c, r[(c / 32) & 1], c < C / 2 ? f0 : f1);
+    for (int c = 0; c < C; c += kChunk) {
+      uint32_t (&now)[kChunk] = r[(c / kChunk) & 1], (&then)[kChunk] = r[(c / kChunk + 1) & 1];
+      tmem_wait_ld(now);
+      if (c + kChunk < C) {
+        tmem_ld(at + c + kChunk + (c + kChunk >= 64 ? SKIP : 0), then);
+      } else {
+        read();
+        if (blocks > 1) {
+          wait(at, f0, f1);
+          tmem_ld(at, then);
+        }
+      }
+      s.add(c, now, c < 64 ? g0 : g1);
+    }
   }
 }
 
-// Factors of the blocks of K for a thread's token and its columns, asked for three blocks ahead.
-template <bool GATED>
+// The factors of a tile's rows, block of K by block of K: xs ws for the 128 rows and its first (gate) and second (up) 128 columns, by two warps for
+// those that add up, in a ring in shared memory, BATCH blocks of one and BATCH of the other.  A warp sees every barrier of the stages' ring at least once a
+// round, as a wait by parity needs it, where there are more stages than the other's blocks.  (A thread's own loads, two blocks ahead, came too late: with the copies at full rate a load takes
+// more than 1000 cycles, and 190 to 230 cycles of every block went into waiting for it.)
+template <int SETS, int BATCH>
 struct Factors {
-  const float *xs, *w0, *w1;
-  int64_t stride;
-  int kb, end;
-  float x[3], a[3], b[3];
-  __device__ __forceinline__ void ask(int i) {
-    const bool in = kb < end;
-    x[i] = xs && in ? __ldg(xs) : 0.f;
-    a[i] = in ? __ldg(w0 + kb) : 0.f;
-    if (GATED) b[i] = in ? __ldg(w1 + kb) : 0.f;
-    if (xs) xs += stride;
-    ++kb;
-  }
-  __device__ __forceinline__ void start(const Fp8Params& p, int row, bool there, int64_t block0, int64_t block1, int kb0, int kb1) {
-    stride = p.xs_stride;
-    xs = there ? p.xs + kb0 * stride + row : nullptr;
-    w0 = p.ws + block0 * p.KB;
-    w1 = p.ws + block1 * p.KB;
-    kb = kb0; end = kb1;
+  float x[BATCH][4], w[BATCH][SETS];
+  // asks for n <= BATCH blocks from kb on
+  __device__ __forceinline__ void ask(const Fp8Params& p, int row, int rows, int64_t block0, int64_t block1, int kb, int n, int lane) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) ask(i);
+    for (int i = 0; i < BATCH; ++i) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[i][q] = i < n && q * 32 + lane < rows ? __ldg(p.xs + (kb + i) * p.xs_stride + row + q * 32 + lane) : 0.f;
+      w[i][0] = i < n ? __ldg(p.ws + block0 * p.KB + kb + i) : 0.f;
+      if (SETS == 2) w[i][SETS - 1] = i < n ? __ldg(p.ws + block1 * p.KB + kb + i) : 0.f;
+    }
   }
-  __device__ __forceinline__ void next(float& f0, float& f1) {
-    f0 = x[0] * a[0];
-    f1 = GATED ? x[0] * b[0] : f0;
-    x[0] = x[1]; x[1] = x[2]; a[0] = a[1]; a[1] = a[2];
-    if (GATED) { b[0] = b[1]; b[1] = b[2]; }
-    ask(2);
+  __device__ __forceinline__ void put(float* slot, int i, int lane) const {
+#pragma unroll
+    for (int s = 0; s < SETS; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) slot[s * 128 + q * 32 + lane] = x[i][q] * w[i][s];
   }
 };
 
-// One row's C columns from n0 on, rounded once.
+// 64 columns of a row from n0 on, rounded once; c0: where their sums begin.
 template <int C>
-__device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, int row, int n0) {
+__device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, int c0, int row, int n0) {
   bf16* dst = p.y + (int64_t)row * p.N + n0;
-  if (n0 + C <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
+  if (n0 + 64 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
 #pragma unroll
-    for (int c = 0; c < C; c += 8) {
+    for (int c = 0; c < 64; c += 8) {
       uint32_t u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float a, b;
-        s.at(c + 2 * i, a, b);
+        s.at(c0 + c + 2 * i, a, b);
         if (p.bias) { a += bf2f(p.bias[n0 + c + 2 * i]); b += bf2f(p.bias[n0 + c + 2 * i + 1]); }
         u[i] = pack_bf2(a, b);
       }
@@ -227,63 +258,114 @@ __device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, 
     }
   } else {
 #pragma unroll
-    for (int c = 0; c < C; c += 2) {
+    for (int c = 0; c < 64; c += 2) {
       float a, b;
-      s.at(c, a, b);
+      s.at(c0 + c, a, b);
       if (n0 + c < p.N) dst[c] = f2bf(p.bias ? a + bf2f(p.bias[n0 + c]) : a);
       if (n0 + c + 1 < p.N) dst[c + 1] = f2bf(p.bias ? b + bf2f(p.bias[n0 + c + 1]) : b);
     }
   }
 }
 
-// Gated: a thread has 64 columns of the gate and the same 64 of up, its counterpart in the other warpgroup the block's other 64.  The block's largest
-// magnitude goes through shared memory (two rows of 128 words).  Called by all 256 threads.
-__device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>& s, int row, bool there, int n, uint32_t* both, int half, int lane128) {
-  float h[64];
+// A warp's 32 rows (from `row` on, `rows` of them there) of C columns, 32 at a time through 2 KB of its own in shared memory: rows of 64 bytes, whose
+// 16-byte pieces are exchanged by two bits of the row, so that neither side meets in a bank.  A lane then stores 16 bytes beside its neighbour's.
+template <int C>
+__device__ __forceinline__ void store_rows(const Fp8Params& p, const Sums<C>& s, int row, int rows, int n0, uint32_t buffer, int lane) {
+  const int j = lane & 3, r = lane >> 2;
+  const uint32_t put = buffer + lane * 64, get = buffer + r * 64 + ((j ^ ((r >> 1) & 3)) << 4);
+  bf16* dst = p.y + (int64_t)(row + r) * p.N + n0 + j * 8;
+#pragma unroll
+  for (int c0 = 0; c0 < C; c0 += 32) {
+    if (n0 + c0 >= p.N) break;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + k * 8 + 2 * i;
+        float a, b;
+        s.at(c, a, b);
+        if (p.bias) {
+          const int at = n0 + c;
+          if (at < p.N) a += bf2f(p.bias[at]);
+          if (at + 1 < p.N) b += bf2f(p.bias[at + 1]);
+        }
+        u[i] = pack_bf2(a, b);
+      }
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(put + ((k ^ ((lane >> 1) & 3)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[4];
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(get + i * 512) : "memory");
+      if (r + i * 8 < rows && n0 + c0 + j * 8 < p.N) *reinterpret_cast<uint4*>(dst + (int64_t)i * 8 * p.N + c0) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+
+// Gated: a thread has 64 columns of the gate and the same of up, the block's other 64 are another warp's; its largest magnitude goes through shared
+// memory (two rows of 128 words).  Called by all warps that add up.
+__device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>& s, int row, bool there, int n, uint32_t* tops, int part, int lane128) {
+  constexpr int H = 64;
+  float h[H];
   uint32_t m = 0;
 #pragma unroll
-  for (int c = 0; c < 64; c += 2) {
+  for (int c = 0; c < H; c += 2) {
     float g[2], u[2];
     s.at(c, g[0], g[1]);
-    s.at(64 + c, u[0], u[1]);
+    s.at(H + c, u[0], u[1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       h[c + i] = __fdividef(g[i], 1.f + __expf(-g[i])) * u[i];
       m = max(m, __float_as_uint(h[c + i]) & 0x7fffffffu);       // (NaN above all)
     }
   }
-  both[half * 128 + lane128] = m;
+  tops[part * 128 + lane128] = m;
   sums_sync();
-  m = max(m, both[(half ^ 1) * 128 + lane128]);
+  m = max(m, tops[(part ^ 1) * 128 + lane128]);
   sums_sync();                                                   // (the next tile writes there)
   if (!there) return;
   float scale, factor;
   fp8::scale_of(__uint_as_float(m), scale, factor);
-  uint8_t* dst = p.codes + (int64_t)row * p.N + n * 128 + half * 64;
+  uint8_t* dst = p.codes + (int64_t)row * p.N + n * 128 + part * H;
 #pragma unroll
-  for (int c = 0; c < 64; c += 16) {
+  for (int c = 0; c < H; c += 16) {
     uint32_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       q[i] = factor > 0.f ? fp8::pack4(h[c + 4 * i] * factor, h[c + 4 * i + 1] * factor, h[c + 4 * i + 2] * factor, h[c + 4 * i + 3] * factor) : 0u;
     *reinterpret_cast<uint4*>(dst + c) = make_uint4(q[0], q[1], q[2], q[3]);
   }
-  if (half == 0) p.out_scales[n * p.out_stride + row] = scale;
+  if (part == 0) p.out_scales[n * p.out_stride + row] = scale;
 }
 
 // ----------------------------------------------------------------------------------------------------- equal shares of all units
 
+// U units in G equal shares: share c begins at floor(U c / G) (one 32-bit quotient of small numbers).
+struct Shares {
+  uint32_t U, G, q, r;
+  __device__ __forceinline__ Shares(uint32_t units, uint32_t shares) : U(units), G(shares), q(units / shares), r(units - units / shares * shares) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return q * c + r * c / G; }
+  // the share with unit x
+  __device__ __forceinline__ uint32_t of(uint32_t x) const {
+    uint32_t c = min(G - 1, (uint32_t)((float)x * ((float)G / (float)U)));
+    while (begin(c) > x) --c;
+    while (c + 1 < G && begin(c + 1) <= x) ++c;
+    return c;
+  }
+};
 // A share as pieces of tiles: blocks of K [kb0, kb1) of tile `tile`.
 struct Pieces {
-  int64_t cur, end;
-  int KB;
-  __device__ __forceinline__ bool next(int& tile, int& kb0, int& kb1) {
+  int cur, end, KB, tile, kb;
+  __device__ __forceinline__ Pieces(int u0, int u1, int KB_, int tile0) : cur(u0), end(u1), KB(KB_), tile(tile0), kb(u0 - tile0 * KB_) {}
+  __device__ __forceinline__ bool next(int& t, int& kb0, int& kb1) {
     if (cur >= end) return false;
-    tile = (int)(cur / KB);
-    kb0 = (int)(cur - (int64_t)tile * KB);
-    const int64_t left = end - cur;
-    kb1 = left < KB - kb0 ? kb0 + (int)left : KB;
+    t = tile; kb0 = kb;
+    kb1 = min(KB, kb + end - cur);
     cur += kb1 - kb0;
+    ++tile; kb = 0;
     return true;
   }
 };
@@ -291,14 +373,14 @@ struct Pieces {
 template <int NT, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  constexpr int C = NT / 2, BUFS = 512 / NT;
+  constexpr int C = NT / 2, BUFS = 512 / NT, SETS = NT / 128;
   static_assert(!GATED || NT == 256, "a gated tile holds 128 columns of each");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * 32 + 2 * BUFS];
   __shared__ uint32_t tmem_slot;
   __shared__ int last_flag;
-  __shared__ uint32_t both[256];
+  __shared__ uint32_t tops[256];
   __shared__ int starts[kMaxGroups + 1];
   const int stages = p.stages;
   const uint32_t stage_bytes = (uint32_t)p.x_bytes + NT * 128;
@@ -314,15 +396,15 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
   }
   if (warp == 1 && lane == 0) {
-    for (int s = 0; s < stages; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    for (int b = 0; b < BUFS; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), 8); }
+    for (int s = 0; s < stages; ++s) { bar_init(full(s), 2); bar_init(empty(s), 1); }
+    for (int b = 0; b < BUFS; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), kSumWarps); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 3 && !p.offsets) count_tiles(p, kRows, starts, lane);
+  if (!p.offsets && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
   fence_before();
   __syncthreads();
   fence_after();
@@ -330,33 +412,28 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   pdl_launch_dependents();
   if (p.offsets) {                                  // which tiles there are is the kernel before's output
     pdl_wait();
-    if (warp == 3) count_tiles(p, kRows, starts, lane);
-    __syncthreads();
+    count_tiles(p, kRows, starts);
   }
   const int KB = p.KB;
-  const int64_t U = (int64_t)starts[p.E] * KB;
-  const int64_t G = max((int64_t)1, min((int64_t)gridDim.x, U / p.min_units)), me = blockIdx.x;
-  const int64_t u0 = me < G ? U * me / G : U, u1 = me < G ? U * (me + 1) / G : U;
-  const int e_first = u0 < u1 ? first_group(p, starts, (int)(u0 / KB)) : 0;
+  const uint32_t U = (uint32_t)starts[p.E] * KB;
+  const Shares shares(U, max(1u, min(gridDim.x, U / p.min_units)));
+  const uint32_t me = blockIdx.x, u0 = me < shares.G ? shares.begin(me) : U, u1 = me < shares.G ? shares.begin(me + 1) : U;
+  const int tile0 = u0 < u1 ? (int)(u0 / (uint32_t)KB) : 0, e_first = u0 < u1 ? first_group(p, starts, tile0) : 0;
+  // A slot of the ring is free again when its block is added up.  The block `stages` further is then at the earliest on its way (its stage was freed by an
+  // MMA that began after the sums BUFS blocks before had been read).
+  float* factors = reinterpret_cast<float*>(smem + stages * stage_bytes);
+  const int slots = stages + BUFS;
 
   if (warp == 0) {
-    regs_down<72>();
+    regs_down<FP8_DOWN>();
     if (elect_one()) {
       int stage = 0;
       uint32_t phase = 0;
       auto load_w = [&](int s, const Tile& t, int kb) {
         const uint32_t dst = base + s * stage_bytes + p.x_bytes;
         const int row = t.e * p.w_rows;
-        if (GATED) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            load_box(dst + h * kSlab, &map_w, full(s), kb * 128, row + t.n * 128 + h * 64);
-            load_box(dst + h * kSlab + kSlab / 2, &map_w, full(s), kb * 128, row + p.N + t.n * 128 + h * 64);
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < NT / 128; ++h) load_box(dst + h * kSlab, &map_w, full(s), kb * 128, row + t.n * NT + h * 128);
-        }
+        for (int h = 0; h < NT / 128; ++h) load_box(dst + h * kSlab, &map_w, full(s), kb * 128, row + (GATED ? t.n * 128 + h * p.N : t.n * NT + h * 128));
       };
       auto load_x = [&](int s, const Tile& t, int kb) {
         for (int r = 0; r < t.rows; r += 32) load_box(base + s * stage_bytes + r * 128, &map_x, full(s), kb * 128, t.row + r);
@@ -365,7 +442,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       // What the weights are is known before the kernel before has ended: its first tile's, as many as there are stages.
       int tile, kb0, kb1, ahead = 0, e = e_first;
       if (!p.offsets) {
-        Pieces it{u0, u1, KB};
+        Pieces it(u0, u1, KB, tile0);
         if (it.next(tile, kb0, kb1)) {
           const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
           ahead = min(stages, kb1 - kb0);
@@ -373,7 +450,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
         pdl_wait();
       }
-      Pieces it{u0, u1, KB};
+      Pieces it(u0, u1, KB, tile0);
       while (it.next(tile, kb0, kb1)) {
         const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -390,14 +467,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       }
     }
   } else if (warp == 1) {
-    regs_down<72>();
+    regs_down<FP8_DOWN>();
     if (elect_one()) {
       constexpr uint32_t idesc = instr_desc(kRows, NT);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       const uint64_t a0 = tile_desc(base), b0 = tile_desc(base + p.x_bytes);
       uint64_t a = a0, b = b0;
-      for (int64_t u = u0; u < u1; ++u) {
+      for (uint32_t u = u0; u < u1; ++u) {
         mbar_wait(tempty(buf), buf_phase ^ 1);
         mbar_wait(full(stage), phase);
         fence_after();
@@ -411,43 +488,75 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       }
     }
   } else if (warp < 4) {
-    regs_down<72>();
-  } else {
-    regs_up<216>();
-    const int q = warp & 3, half = (warp - 4) >> 2, tid = threadIdx.x - 128, lane128 = q * 32 + lane;
+    regs_down<FP8_DOWN>();
     pdl_wait();
-    int buf = 0, tile, kb0, kb1, e = e_first;
+    int stage = 0, slot = 0, tile, kb0, kb1, e = e_first, turn = warp & 1;
+    uint32_t phase = 0;
+    Pieces it(u0, u1, KB, tile0);
+    while (it.next(tile, kb0, kb1)) {
+      const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
+      const int64_t wb = (int64_t)t.e * p.w_blocks + (GATED ? t.n : t.n * SETS);
+      Factors<SETS, kBatch> f;
+      for (int kb = kb0; kb < kb1; kb += kBatch) {
+        turn ^= 1;
+        if (turn) {                                  // the other warp's
+          const int n = min(kBatch, kb1 - kb);
+          for (stage += n; stage >= stages; stage -= stages) phase ^= 1;
+          for (slot += n; slot >= slots; slot -= slots) {}
+          continue;
+        }
+        f.ask(p, t.row, t.rows, wb, GATED ? wb + p.N / 128 : wb + (t.n * SETS + 1 < p.w_blocks), kb, min(kBatch, kb1 - kb), lane);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (kb + i >= kb1) break;
+          mbar_wait(empty(stage), phase ^ 1);
+          f.put(factors + slot * SETS * 128, i, lane);
+          __syncwarp();
+          if (lane == 0) bar_arrive(full(stage));
+          if (++stage == stages) { stage = 0; phase ^= 1; }
+          if (++slot == slots) slot = 0;
+        }
+      }
+    }
+  } else {
+    regs_up<FP8_UP>();
+    const int q = warp & 3, part = (warp - 4) >> 2, tid = threadIdx.x - 128, lane128 = q * 32 + lane;
+    pdl_wait();
+    int buf = 0, slot = 0, tile, kb0, kb1, e = e_first;
     uint32_t buf_phase = 0;
-    Pieces it{u0, u1, KB};
+    Pieces it(u0, u1, KB, tile0);
     while (it.next(tile, kb0, kb1)) {
       const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
       const bool some = q * 32 < t.rows, there = lane128 < t.rows;
-      const int row = t.row + lane128, n0 = t.n * NT + half * C;
-      const int64_t wb = (int64_t)t.e * p.w_blocks;
+      const int row = t.row + lane128, n0 = t.n * NT + part * 64;
       Sums<C> s;
       s.clear();
-      Factors<GATED> f;
-      f.start(p, row, there, wb + (GATED ? t.n : min(n0 / 128, p.w_blocks - 1)), wb + (GATED ? p.N / 128 + t.n : 0), kb0, kb1);
-      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + half * C;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        float f0, f1;
-        f.next(f0, f1);
-        mbar_wait(tfull(buf), buf_phase);
-        if (some) {
-          fence_after();
-          add_block<C>(s, at + buf * NT, f0, f1);
-          fence_before();
-        }
-        __syncwarp();
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 64;
+      auto read = [&] {
+        fence_before();
         if (lane == 0) bar_arrive(tempty(buf));
         if (++buf == BUFS) { buf = 0; buf_phase ^= 1; }
+        if (++slot == slots) slot = 0;
+      };
+      auto wait = [&](uint32_t& from, float& f0, float& f1) {
+        mbar_wait(tfull(buf), buf_phase);
+        fence_after();
+        const float* f = factors + slot * SETS * 128 + lane128;
+        f0 = f[0];
+        f1 = f[SETS == 2 ? 128 : 0];
+        from = at + buf * NT;
+      };
+      if (some) {
+        add_blocks<C, 64>(s, kb1 - kb0, wait, read);
+      } else {
+        for (int kb = kb0; kb < kb1; ++kb) { mbar_wait(tfull(buf), buf_phase); read(); }
       }
       if (kb1 - kb0 != KB) {
-        // A part of the tile's sum: to the workspace, [slot][quarter][half][column / 4][lane] of 16 bytes.  A share has at most two such pieces: slot 0
+        // A part of the tile's sum: to the workspace, [slot][quarter][part][column / 4][lane] of 16 bytes.  A share has at most two such pieces: slot 0
         // the one that it begins with.
-        constexpr int kPer = 2 * (C / 4) * 32;          // float4 of a quarter
-        const int64_t x0 = (int64_t)tile * KB;
-        auto slot_of = [&](int64_t cta, int slot) { return reinterpret_cast<float4*>(p.part) + ((cta * 2 + slot) * p.quarters + q) * kPer + half * (C / 4) * 32 + lane; };
+        constexpr int kPer = (NT / 4) * 32;          // float4 of a quarter
+        const uint32_t x0 = (uint32_t)tile * KB;
+        auto slot_of = [&](uint32_t cta, int slot) { return reinterpret_cast<float4*>(p.part) + ((cta * 2 + slot) * p.quarters + q) * kPer + part * (C / 4) * 32 + lane; };
         if (some) {
           float4* dst = slot_of(me, x0 + kb0 == u0 ? 0 : 1);
 #pragma unroll
@@ -458,34 +567,39 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             __stcg(dst + c / 4 * 32, v);
           }
         }
-        __threadfence();
         sums_sync();
         // its CTAs: from the one with its first unit to the one with its last; they count in the first one's counter
-        const int64_t c0 = ((x0 + 1) * G + U - 1) / U - 1, c1 = ((x0 + KB) * G + U - 1) / U - 1;
+        const uint32_t c0 = shares.of(x0), c1 = shares.of(x0 + KB - 1);
         if (tid == 0) {
-          const bool mine = atomicAdd(p.count + c0, 1u) == (unsigned)(c1 - c0);
+          __threadfence();                              // (of what all threads of the barrier have stored)
+          const bool mine = atomicAdd(p.count + c0, 1u) == c1 - c0;
           if (mine) p.count[c0] = 0;                    // ready for the next launch
+          __threadfence();
           last_flag = mine;
         }
         sums_sync();
         const bool last = last_flag != 0;
         sums_sync();                                    // (the next piece writes there)
         if (!last) continue;
-        __threadfence();
         s.clear();
         if (some)
-          for (int64_t c = c0; c <= c1; ++c) {
-            const float4* src = slot_of(c, U * c / G >= x0 ? 0 : 1);
 #pragma unroll
-            for (int i = 0; i < C / 4; ++i) {
-              const float4 v = __ldcg(src + i * 32);
-              s.v[2 * i] = add2(s.v[2 * i], pk(v.x, v.y));
-              s.v[2 * i + 1] = add2(s.v[2 * i + 1], pk(v.z, v.w));
+          for (int h = 0; h < C; h += 64)
+            for (uint32_t c = c0; c <= c1; ++c) {
+              const float4* src = slot_of(c, shares.begin(c) >= x0 ? 0 : 1) + h / 4 * 32;
+              float4 v[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __ldcg(src + i * 32);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) { s.v[h + 4 * i] += v[i].x; s.v[h + 4 * i + 1] += v[i].y; s.v[h + 4 * i + 2] += v[i].z; s.v[h + 4 * i + 3] += v[i].w; }
             }
-          }
       }
-      if constexpr (GATED) store_gated(p, s, row, there, t.n, both, half, lane128);
-      else if (there) store_row<C>(p, s, row, n0);
+      if constexpr (GATED) {
+        store_gated(p, s, row, there, t.n, tops, part, lane128);
+      } else if (there) {
+#pragma unroll
+        for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
+      }
     }
   }
   fence_before();
@@ -505,15 +619,16 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   constexpr uint32_t kStage = 2 * kSlab;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * STAGES + 4];
+  __shared__ uint64_t bars[2 * STAGES + 8];
   __shared__ uint32_t tmem_slot;
-  __shared__ uint32_t both[256];
+  __shared__ uint32_t tops[256];
+  __shared__ int4 tiles[16];                        // n, row, rows of the tiles under way: at most one a block of K of the rings, and the last one
   __shared__ int starts[kMaxGroups + 1];
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 2 + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 4 + b); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31, rank = (int)cluster_ctarank();
 
   if (warp == 0 && lane == 0) {
@@ -521,15 +636,15 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
   }
   if (warp == 1 && lane == 0) {
-    for (int s = 0; s < STAGES; ++s) { bar_init(full(s), 1); bar_init(empty(s), 1); }
-    for (int b = 0; b < 2; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), 16); }
+    for (int s = 0; s < STAGES; ++s) { bar_init(full(s), 3); bar_init(empty(s), 2); }       // (full: the leader's copies, both CTAs' factors)
+    for (int b = 0; b < 4; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), kSumWarps); }       // (of two blocks, the first and the second 128 columns)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  if (warp == 3 && !p.offsets) count_tiles(p, 2 * kRows, starts, lane);
+  if (!p.offsets && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + 2 * kRows - 1) / (2 * kRows) * p.n_tiles; }
   fence_before();
   __syncthreads();
   fence_after();
@@ -537,93 +652,127 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   pdl_launch_dependents();
   cluster_arrive(); cluster_wait();                 // the peer's barriers are there
   pdl_wait();
-  if (p.offsets) {
-    if (warp == 3) count_tiles(p, 2 * kRows, starts, lane);
-    __syncthreads();
-  }
+  if (p.offsets) count_tiles(p, 2 * kRows, starts);
   const int KB = p.KB, total = starts[p.E], first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
   const int e_first = first < total ? first_group(p, starts, first) : 0;
+  float* factors = reinterpret_cast<float*>(smem + STAGES * kStage + (GATED ? 0 : kSumWarps * 2048));
 
-  if (warp == 0) {
-    regs_down<72>();
-    if (elect_one()) {
-      int stage = 0, e = e_first;
-      uint32_t phase = 0;
-      const uint32_t lead0 = mapa_u32(full(0), 0);
-      for (int w = first; w < total; w += step) {
-        const Tile t = find_tile<2 * kRows, kPairBand>(p, starts, w, e);
-        const int wr = t.e * p.w_rows + (GATED ? t.n * 128 + rank * 64 : t.n * 256 + rank * 128), xr = t.row + rank * kRows;
-        for (int kb = 0; kb < KB; ++kb) {
-          mbar_wait(empty(stage), phase ^ 1);
-          if (rank == 0) bar_expect(full(stage), 2 * kStage);
-          const uint32_t dst = base + stage * kStage, lead = lead0 + 8u * stage;
-          load_box2(dst, &map_x, lead, kb * 128, xr);
-          if (GATED) {
-            load_box2(dst + kSlab, &map_w, lead, kb * 128, wr);
-            load_box2(dst + kSlab + kSlab / 2, &map_w, lead, kb * 128, wr + p.N);
-          } else {
-            load_box2(dst + kSlab, &map_w, lead, kb * 128, wr);
-          }
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    regs_down<72>();
-    if (rank == 0 && elect_one()) {                 // the leader issues for both
-      constexpr uint32_t idesc = instr_desc(2 * kRows, 256);
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, buf_phase = 0;
-      const uint64_t a0 = tile_desc(base), b0 = tile_desc(base + kSlab);
-      uint64_t a = a0, b = b0;
-      for (int w = first; w < total; w += step)
-        for (int kb = 0; kb < KB; ++kb) {
-          mbar_wait(tempty(buf), buf_phase ^ 1);
-          mbar_wait(full(stage), phase);
-          fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma8x2(tmem + buf * 256, a + 2 * k, b + 2 * k, idesc, k > 0);
-          commit2(empty(stage), 3);
-          commit2(tfull(buf), 3);
-          a += kStage >> 4; b += kStage >> 4;
-          if (++stage == STAGES) { stage = 0; phase ^= 1; a = a0; b = b0; }
-          if (++buf == 2) { buf = 0; buf_phase ^= 1; }
-        }
-    }
-  } else if (warp < 4) {
-    regs_down<72>();
-  } else {
-    regs_up<216>();
-    const int q = warp & 3, half = (warp - 4) >> 2, lane128 = q * 32 + lane;
-    const uint32_t lead_tempty = mapa_u32(tempty(0), 0);
-    int buf = 0, e = e_first;
-    uint32_t buf_phase = 0;
+  if (warp == 0 || warp == 3) {
+    // the copies and factors of kPairBatch blocks of K by one of the two, of as many by the other
+    regs_down<FP8_DOWN>();
+    int stage = 0, slot = 0, tile = 0, e = e_first, turn = 1 - (warp & 1);
+    uint32_t phase = 0;
+    const uint32_t lead0 = mapa_u32(full(0), 0);
     for (int w = first; w < total; w += step) {
       const Tile t = find_tile<2 * kRows, kPairBand>(p, starts, w, e);
+      const int64_t wb = (int64_t)t.e * p.w_blocks + (GATED ? t.n : t.n * 2);
+      // 64 weight rows for the first 128 columns, 64 for the second: half of each block or, gated, the leader's of the gate and the other's of up
+      const int wr = t.e * p.w_rows + (GATED ? t.n * 128 + rank * p.N : t.n * 256 + rank * 64), xr = t.row + rank * kRows;
+      Factors<2, kPairBatch> f;
+      if (turn && lane == 0) tiles[tile & 15] = make_int4(t.n, t.row, t.rows, 0);      // (the first batch is this warp's)
+      ++tile;
+      for (int kb = 0; kb < KB; kb += kPairBatch) {
+        const int n = min(kPairBatch, KB - kb);
+        turn ^= 1;
+        if (turn) {                                  // the other warp's
+          for (stage += n; stage >= STAGES; stage -= STAGES) phase ^= 1;
+          slot = (slot + n) % kPairSlots;
+          continue;
+        }
+        f.ask(p, xr, t.rows - rank * kRows, wb, GATED ? wb + p.N / 128 : wb + (t.n * 2 + 1 < p.w_blocks), kb, n, lane);
+#pragma unroll
+        for (int i = 0; i < kPairBatch; ++i) {
+          if (i >= n) break;
+          mbar_wait(empty(stage), phase ^ 1);
+          const uint32_t lead = lead0 + 8u * stage;
+          if (elect_one()) {
+            if (rank == 0) bar_expect(full(stage), 2 * kStage);
+            const uint32_t dst = base + stage * kStage;
+            load_box2(dst, &map_x, lead, (kb + i) * 128, xr);
+            load_box2(dst + kSlab, &map_w, lead, (kb + i) * 128, wr);
+            load_box2(dst + kSlab + kSlab / 2, &map_w, lead, (kb + i) * 128, wr + (GATED ? 64 : 128));
+          }
+          __syncwarp();
+          f.put(factors + slot * 256, i, lane);
+          __syncwarp();
+          if (lane == 0) bar_arrive_at(lead);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (++slot == kPairSlots) slot = 0;
+        }
+      }
+    }
+  } else if (warp < 4) {
+    regs_down<FP8_DOWN>();
+    if (rank == 0 && elect_one()) {                 // the leader issues for both, the first 128 columns by one thread and the second by another
+      constexpr uint32_t idesc = instr_desc(2 * kRows, 128);
+      const int h = warp - 1;
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      const uint64_t a0 = tile_desc(base), b0 = tile_desc(base + kSlab + h * (kSlab / 2));
+      uint64_t a = a0, b = b0;
+      const uint32_t d = tmem + h * 128;
+      const int tiles = first < total ? (total - 1 - first) / step + 1 : 0;
+      bool f_there = false, t_there = false;
+      for (int64_t n = (int64_t)tiles * KB; n > 0; --n) {
+        if (!f_there) mbar_wait(full(stage), phase);
+        if (!t_there) mbar_wait(tempty(2 * buf + h), buf_phase ^ 1);
+        const int s1 = stage + 1 == STAGES ? 0 : stage + 1, v1 = buf ^ 1;
+        const uint32_t p1 = stage + 1 == STAGES ? phase ^ 1 : phase, w1 = buf_phase ^ buf;
+        f_there = mbar_test(full(s1), p1);
+        t_there = mbar_test(tempty(2 * v1 + h), w1 ^ 1);
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma8x2(d + buf * 256, a + 2 * k, b + 2 * k, idesc, k > 0);
+        commit2(tfull(2 * buf + h), 3);
+        commit2(empty(stage), 3);
+        a += kStage >> 4; b += kStage >> 4;
+        if (s1 == 0) { a = a0; b = b0; }
+        stage = s1; phase = p1; buf = v1; buf_phase = w1;
+      }
+    }
+  } else {
+    regs_up<FP8_UP>();
+    const int q = warp & 3, part = (warp - 4) >> 2, lane128 = q * 32 + lane;
+    const uint32_t lead_tempty = mapa_u32(tempty(part), 0);
+    int buf = 0, slot = 0, tile = 0;
+    uint32_t buf_phase = 0;
+    for (int w = first; w < total; w += step) {
+      mbar_wait(tfull(2 * buf + part), buf_phase);
+      const int4 found = tiles[tile++ & 15];
+      const Tile t = {0, found.x, found.y, found.z};
       const int mine = rank * kRows + lane128;
       const bool some = rank * kRows + q * 32 < t.rows, there = mine < t.rows;
-      const int row = t.row + mine, n0 = t.n * 256 + half * C;
-      const int64_t wb = (int64_t)t.e * p.w_blocks;
+      const int row = t.row + mine, n0 = t.n * 256 + part * 128;
       Sums<C> s;
       s.clear();
-      Factors<GATED> f;
-      f.start(p, row, there, wb + (GATED ? t.n : min(n0 / 128, p.w_blocks - 1)), wb + (GATED ? p.N / 128 + t.n : 0), 0, KB);
-      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + half * C;
-      for (int kb = 0; kb < KB; ++kb) {
-        float f0, f1;
-        f.next(f0, f1);
-        mbar_wait(tfull(buf), buf_phase);
-        if (some) {
-          fence_after();
-          add_block<C>(s, at + buf * 256, f0, f1);
-          fence_before();
-        }
-        __syncwarp();
-        if (lane == 0) bar_arrive_cluster(lead_tempty + 8u * buf);
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 128;
+      auto read = [&] {
+        fence_before();
+        if (lane == 0) bar_arrive_at(lead_tempty + 16u * buf);
         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+        if (++slot == kPairSlots) slot = 0;
+      };
+      auto wait = [&](uint32_t& from, float& f0, float& f1) {
+        mbar_wait(tfull(2 * buf + part), buf_phase);
+        fence_after();
+        const float* f = factors + slot * 256 + lane128;
+        f0 = f[GATED ? 0 : part * 128];
+        f1 = GATED ? f[128] : f0;
+        from = at + buf * 256;
+      };
+      if (some) {
+        add_blocks<C, 0>(s, KB, wait, read);
+      } else {
+        for (int kb = 0; kb < KB; ++kb) { mbar_wait(tfull(2 * buf + part), buf_phase); read(); }
       }
-      if constexpr (GATED) store_gated(p, s, row, there, t.n, both, half, lane128);
-      else if (there) store_row<C>(p, s, row, n0);
+      if constexpr (GATED) {
+        store_gated(p, s, row, there, t.n, tops, part, lane128);
+      } else if (p.wide) {
+        if (some) store_rows<C>(p, s, row - lane, t.rows - (mine - lane), n0, base + STAGES * kStage + (warp - 4) * 2048, lane);
+      } else if (there) {
+#pragma unroll
+        for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 64);
+      }
     }
   }
   fence_before();
@@ -656,6 +805,8 @@ static int encode_map(CUtensorMap* m, const void* ptr, int64_t rows, int64_t col
   return 0;
 }
 
+static bool aligned_to(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
 static int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
@@ -664,20 +815,21 @@ static int sm_count() {
 
 template <int NT, bool GATED>
 static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cudaStream_t st) {
-  constexpr int box = GATED ? 64 : 128;
   const int widest = p.T < kRows ? p.T : kRows;
   p.quarters = (widest + 31) / 32;
   p.x_bytes = p.quarters * 4096;
   p.n_tiles = (p.N + (GATED ? 128 : NT) - 1) / (GATED ? 128 : NT);
   constexpr int own = 8 * 1024;                            // the kernel's own shared memory, and rounding up to 1024
-  p.stages = (kSmem - own) / (p.x_bytes + NT * 128);
+  constexpr int slot_bytes = NT / 128 * 512, more = 512 / NT;
+  p.stages = (kSmem - own - more * slot_bytes) / (p.x_bytes + NT * 128 + slot_bytes);
   if (p.stages > 16) p.stages = 16;
+  static_assert((kSmem - own - more * slot_bytes) / (kRows * 128 + NT * 128 + slot_bytes) > kBatch, "");
   p.min_units = 2;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");
-  const int smem = p.stages * (p.x_bytes + NT * 128) + 1024;
+  const int smem = p.stages * (p.x_bytes + NT * 128 + slot_bytes) + more * slot_bytes + 1024;
   CUtensorMap mw, mx;
-  if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, box)) return rc;
+  if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
   auto kern = fp8_stream_kernel<NT, GATED>;
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -685,8 +837,10 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   KGE_REQUIRE(sms > 0, "kge_gemm_fp8: no CUDA device");
   int64_t ctas = sms;
   if (!p.offsets) {
-    const int64_t units = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles * p.KB / p.min_units;
-    ctas = units < 1 ? 1 : units < ctas ? units : ctas;
+    // Whole numbers of CTAs a tile cost each of them one partial sum in place of two: worth up to a tenth of the SMs.
+    const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles, most = tiles * p.KB / p.min_units, even = tiles < sms ? sms / tiles * tiles : sms;
+    if (even * 10 >= sms * 9) ctas = even;
+    if (ctas > most) ctas = most < 1 ? 1 : most;
   }
   KGE_CUDA_OK(launch_pdl(kern, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, st, mw, mx, p));
   return 0;
@@ -695,10 +849,11 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
 template <bool GATED>
 static int launch_pairs(Fp8Params& p, const void* x, const void* w, int K, cudaStream_t st) {
   p.n_tiles = (p.N + (GATED ? 128 : 256) - 1) / (GATED ? 128 : 256);
-  const int smem = kPairStages * 2 * kSlab + 1024;
+  const int smem = kPairStages * 2 * kSlab + kPairSlots * 1024 + (GATED ? 0 : kSumWarps * 2048) + 1024;
   CUtensorMap mw, mx;
-  if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, GATED ? 64 : 128)) return rc;
+  if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 64)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 128)) return rc;
+  p.wide = !GATED && p.N % 8 == 0 && aligned_to(p.y, 16);
   auto kern = fp8_pair_kernel<GATED>;
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   prefer_max_shared(kern);
@@ -727,7 +882,6 @@ static int64_t workspace_bytes_of(int T) {
   return kCounters * 4 + (int64_t)kMaxCtas * 2 * quarters * 256 * 128;
 }
 
-static bool aligned_to(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // What all four have in common; N: columns of the result.
 static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, int x_scales_stride, const void* w, int K, void* workspace, int64_t workspace_bytes, cudaStream_t st) {
@@ -747,12 +901,12 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
   p.w_rows = (int)rows;
   p.w_blocks = (int)fp8::blocks(rows);
   const int64_t tiles = ((int64_t)p.T / kRows + p.E) * p.w_blocks;
-  KGE_REQUIRE(tiles < (1ll << 31), "%s: %lld tiles in one call", name, (long long)tiles);
+  KGE_REQUIRE(tiles * p.KB < (1ll << 31), "%s: %lld tiles of %d blocks in one call", name, (long long)tiles, p.KB);
   KGE_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(p.T) && aligned_to(workspace, 16), "%s: needs a workspace of %lld bytes, 16-byte aligned", name,
               (long long)workspace_bytes_of(p.T));
   p.count = (unsigned int*)workspace;
   p.part = (float*)((uint8_t*)workspace + kCounters * 4);
-  const bool pairs = p.T / p.E > 256;
+  const bool pairs = p.T / p.E > 96;
 #ifndef KGE_HALF
   if (gated) return pairs ? launch_pairs<true>(p, x, w, K, st) : launch_stream<256, true>(p, x, w, K, st);
 #endif
