@@ -14,6 +14,8 @@
 //    shared memory, 32 KB a block of K, where its MMA takes 512 cycles.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "fp8.cuh"
 #include "kge.h"
 
@@ -33,10 +35,13 @@ constexpr int kChunk = FP8_CHUNK;                 // columns that a warp reads o
 constexpr int kCounters = 256;                    // arrival counters at the head of the workspace
 constexpr int kMaxCtas = 160;
 constexpr int kMaxGroups = 1024;
+constexpr int kMaxStages = 16;
+constexpr int kMaxSplits = 8;                     // CTAs of a cluster
 constexpr int kSmem = 226 * 1024;
+constexpr int kOwn = 14 * 1024;                   // of it, at most, a kernel's own
 constexpr int kPairStages = 6;
 constexpr int kPairSlots = kPairStages + 2;
-constexpr int kPairBatch = 4, kBatch = 2;         // blocks that a warp prepares factors of at a time
+constexpr int kPairBatch = 4;                     // blocks of K that a warp brings in at a time
 static_assert(kPairStages > kPairBatch, "");
 constexpr int kPairBand = 8;                      // 74 pairs at work: 8 x 9 tiles share 17 slabs a block of K, 32 x 2.3 would 34
 
@@ -54,7 +59,8 @@ struct Fp8Params {
   float* part;                                    // stream: partial sums
   unsigned int* count;
   int wide;                                       // pairs: y's rows are 16-byte aligned
-  int quarters, stages, x_bytes, min_units;       // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, least units of a share
+  int quarters, stages, x_bytes, ahead;           // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, stages filled early
+  int splits;                                     // stream, dense: shares of K that a tile is cut into
 };
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -239,6 +245,24 @@ struct Factors {
   }
 };
 
+__device__ __forceinline__ float gated(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
+
+// 8 columns of a row from n0 on, rounded once.
+__device__ __forceinline__ void store_group(const Fp8Params& p, float (&v)[8], int row, int n0) {
+  if (p.bias)
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + j < p.N) v[j] += bf2f(p.bias[n0 + j]);
+  bf16* dst = p.y + (int64_t)row * p.N + n0;
+  if (n0 + 8 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (n0 + j < p.N) dst[j] = f2bf(v[j]);
+  }
+}
+
 // 64 columns of a row from n0 on, rounded once; c0: where their sums begin.
 template <int C>
 __device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, int c0, int row, int n0) {
@@ -318,7 +342,7 @@ __device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>&
     s.at(H + c, u[0], u[1]);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      h[c + i] = __fdividef(g[i], 1.f + __expf(-g[i])) * u[i];
+      h[c + i] = gated(g[i], u[i]);
       m = max(m, __float_as_uint(h[c + i]) & 0x7fffffffu);       // (NaN above all)
     }
   }
@@ -341,54 +365,55 @@ __device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>&
   if (part == 0) p.out_scales[n * p.out_stride + row] = scale;
 }
 
-// ----------------------------------------------------------------------------------------------------- equal shares of all units
+// -------------------------------------------------------------------------------------------------- tiles by single CTAs
 
-// U units in G equal shares: share c begins at floor(U c / G) (one 32-bit quotient of small numbers).
-struct Shares {
-  uint32_t U, G, q, r;
-  __device__ __forceinline__ Shares(uint32_t units, uint32_t shares) : U(units), G(shares), q(units / shares), r(units - units / shares * shares) {}
-  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return q * c + r * c / G; }
-  // the share with unit x
-  __device__ __forceinline__ uint32_t of(uint32_t x) const {
-    uint32_t c = min(G - 1, (uint32_t)((float)x * ((float)G / (float)U)));
-    while (begin(c) > x) --c;
-    while (c + 1 < G && begin(c + 1) <= x) ++c;
-    return c;
+// What a CTA does: blocks of K [kb0, kb1) of tiles [tile0, tile1).  With at least half as many tiles as SMs each is one CTA's, and as many CTAs work as make
+// all have the same number (a weight stream needs bytes under way, not SMs); fewer are cut along K, into `splits` shares.
+struct Work { int tile0, tile1, kb0, kb1, splits; };
+__device__ __forceinline__ Work work_of(int tiles, int KB, int splits, int me, int sms) {
+  if (splits == 0) splits = tiles == 0 || 2 * tiles >= sms ? 1 : max(1, min(min(sms / tiles, KB / 2), kMaxSplits));
+  if (splits > 1) {
+    const int tile = me / splits, piece = me - tile * splits;
+    if (tile >= tiles) return Work{0, 0, 0, 0, splits};
+    return Work{tile, tile + 1, KB * piece / splits, KB * (piece + 1) / splits, splits};
   }
-};
-// A share as pieces of tiles: blocks of K [kb0, kb1) of tile `tile`.
-struct Pieces {
-  int cur, end, KB, tile, kb;
-  __device__ __forceinline__ Pieces(int u0, int u1, int KB_, int tile0) : cur(u0), end(u1), KB(KB_), tile(tile0), kb(u0 - tile0 * KB_) {}
-  __device__ __forceinline__ bool next(int& t, int& kb0, int& kb1) {
-    if (cur >= end) return false;
-    t = tile; kb0 = kb;
-    kb1 = min(KB, kb + end - cur);
-    cur += kb1 - kb0;
-    ++tile; kb = 0;
-    return true;
-  }
-};
+  const int rounds = (tiles + sms - 1) / sms;
+  if (rounds <= 1) return me < tiles ? Work{me, me + 1, 0, KB, 1} : Work{0, 0, 0, 0, 1};
+  const int ctas = (tiles + rounds - 1) / rounds;
+  if (me >= ctas) return Work{0, 0, 0, 0, 1};
+  const int each = tiles / ctas, more = tiles - each * ctas;
+  return Work{each * me + min(me, more), each * (me + 1) + min(me + 1, more), 0, KB, 1};
+}
 
-template <int NT, bool GATED>
+__device__ __forceinline__ void copy4(uint32_t dst, const float* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void push4(uint32_t dst, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+// CLUSTER: the shares of a tile are a cluster's CTAs.  Each finishes its part of the tile's columns, groups of 8, and gets the others' sums of them through
+// distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
+// Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
+template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  constexpr int C = NT / 2, BUFS = 512 / NT, SETS = NT / 128;
+  constexpr int C = NT / 2, BUFS = 512 / NT, SETS = NT / 128, SLOT = 136;
   static_assert(!GATED || NT == 256, "a gated tile holds 128 columns of each");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * 32 + 2 * BUFS];
+  __shared__ uint64_t bars[2 * kMaxStages + 2 * BUFS];
   __shared__ uint32_t tmem_slot;
   __shared__ int last_flag;
-  __shared__ uint32_t tops[256];
-  __shared__ int starts[kMaxGroups + 1];
+  __shared__ uint32_t tops[(CLUSTER ? 2 * kMaxSplits : 2) * 128];
+  __shared__ int starts[CLUSTER ? 2 : kMaxGroups + 1];
   const int stages = p.stages;
   const uint32_t stage_bytes = (uint32_t)p.x_bytes + NT * 128;
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
-  auto empty = [&](int s) { return bar0 + 8u * (32 + s); };
-  auto tfull = [&](int b) { return bar0 + 8u * (64 + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (64 + BUFS + b); };
+  auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  auto tfull = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + BUFS + b); };
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
 
   if (warp == 0 && lane == 0) {
@@ -396,7 +421,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
   }
   if (warp == 1 && lane == 0) {
-    for (int s = 0; s < stages; ++s) { bar_init(full(s), 2); bar_init(empty(s), 1); }
+    for (int s = 0; s < stages; ++s) { bar_init(full(s), 33); bar_init(empty(s), 1); }      // (full: the tiles' copies, the factors' by 32 lanes)
     for (int b = 0; b < BUFS; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), kSumWarps); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -404,30 +429,29 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (!p.offsets && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
+  if ((CLUSTER || !p.offsets) && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_launch_dependents();
-  if (p.offsets) {                                  // which tiles there are is the kernel before's output
+  if (CLUSTER) cluster_arrive_relaxed();
+  if (!CLUSTER && p.offsets) {                      // which tiles there are is the kernel before's output
     pdl_wait();
     count_tiles(p, kRows, starts);
   }
   const int KB = p.KB;
-  const uint32_t U = (uint32_t)starts[p.E] * KB;
-  const Shares shares(U, max(1u, min(gridDim.x, U / p.min_units)));
-  const uint32_t me = blockIdx.x, u0 = me < shares.G ? shares.begin(me) : U, u1 = me < shares.G ? shares.begin(me + 1) : U;
-  const int tile0 = u0 < u1 ? (int)(u0 / (uint32_t)KB) : 0, e_first = u0 < u1 ? first_group(p, starts, tile0) : 0;
-  // A slot of the ring is free again when its block is added up.  The block `stages` further is then at the earliest on its way (its stage was freed by an
-  // MMA that began after the sums BUFS blocks before had been read).
+  const Work work = work_of(starts[p.E], KB, p.splits, (int)blockIdx.x, (int)gridDim.x);
+  const int e_first = work.tile0 < work.tile1 ? first_group(p, starts, work.tile0) : 0;
+  // xs of the rows and ws of the columns, block of K by block of K, in a ring.  A slot is free again when its block is added up.  The block `stages` further
+  // is then at the earliest on its way (its stage was freed by an MMA that began after the sums BUFS blocks before had been read).
   float* factors = reinterpret_cast<float*>(smem + stages * stage_bytes);
   const int slots = stages + BUFS;
 
   if (warp == 0) {
     regs_down<FP8_DOWN>();
     if (elect_one()) {
-      int stage = 0;
+      int stage = 0, e = e_first;
       uint32_t phase = 0;
       auto load_w = [&](int s, const Tile& t, int kb) {
         const uint32_t dst = base + s * stage_bytes + p.x_bytes;
@@ -439,21 +463,17 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         for (int r = 0; r < t.rows; r += 32) load_box(base + s * stage_bytes + r * 128, &map_x, full(s), kb * 128, t.row + r);
       };
       auto bytes_of = [&](const Tile& t) { return (uint32_t)(NT * 128 + (t.rows + 31) / 32 * 4096); };
-      // What the weights are is known before the kernel before has ended: its first tile's, as many as there are stages.
-      int tile, kb0, kb1, ahead = 0, e = e_first;
-      if (!p.offsets) {
-        Pieces it(u0, u1, KB, tile0);
-        if (it.next(tile, kb0, kb1)) {
-          const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
-          ahead = min(stages, kb1 - kb0);
-          for (int i = 0; i < ahead; ++i) { bar_expect(full(i), bytes_of(t)); load_w(i, t, kb0 + i); }
-        }
-        pdl_wait();
+      // What the weights are is known before the kernel before has ended: the first tile's first blocks.
+      int ahead = 0;
+      if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
+        const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
+        ahead = min(p.ahead, work.kb1 - work.kb0);
+        for (int i = 0; i < ahead; ++i) { bar_expect(full(i), bytes_of(t)); load_w(i, t, work.kb0 + i); }
       }
-      Pieces it(u0, u1, KB, tile0);
-      while (it.next(tile, kb0, kb1)) {
+      pdl_wait();
+      for (int tile = work.tile0; tile < work.tile1; ++tile) {
         const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = work.kb0; kb < work.kb1; ++kb) {
           if (ahead > 0) {
             --ahead;
           } else {
@@ -474,58 +494,63 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       uint32_t phase = 0, buf_phase = 0;
       const uint64_t a0 = tile_desc(base), b0 = tile_desc(base + p.x_bytes);
       uint64_t a = a0, b = b0;
-      for (uint32_t u = u0; u < u1; ++u) {
+      for (int64_t n = (int64_t)(work.tile1 - work.tile0) * (work.kb1 - work.kb0); n > 0; --n) {
         mbar_wait(tempty(buf), buf_phase ^ 1);
         mbar_wait(full(stage), phase);
         fence_after();
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma8(tmem + buf * NT, a + 2 * k, b + 2 * k, idesc, k > 0);
-        commit(empty(stage));
         commit(tfull(buf));
+        commit(empty(stage));
         a += stage_bytes >> 4; b += stage_bytes >> 4;
         if (++stage == stages) { stage = 0; phase ^= 1; a = a0; b = b0; }
         if (++buf == BUFS) { buf = 0; buf_phase ^= 1; }
       }
     }
-  } else if (warp < 4) {
+  } else if (warp == 2) {
     regs_down<FP8_DOWN>();
-    pdl_wait();
-    int stage = 0, slot = 0, tile, kb0, kb1, e = e_first, turn = warp & 1;
+    int stage = 0, slot = 0, e = e_first;
     uint32_t phase = 0;
-    Pieces it(u0, u1, KB, tile0);
-    while (it.next(tile, kb0, kb1)) {
+    auto column = [&](const Tile& t, int kb) {           // of a tile's ws: lanes 0 (and 1) have a block of its columns each
+      const int64_t block = (int64_t)t.e * p.w_blocks + (GATED ? t.n + lane * (p.N / 128) : min(t.n * SETS + lane, p.w_blocks - 1));
+      return p.ws + block * p.KB + kb;
+    };
+    auto to = [&](int s, int i) { return s_addr(factors + s * SLOT + i); };
+    int early = 0;
+    if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
+      const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
+      early = min(p.ahead, work.kb1 - work.kb0);
+      for (int i = 0; i < early; ++i)
+        if (lane < SETS) copy4(to(i, 128 + lane), column(t, work.kb0 + i), true);
+    }
+    pdl_wait();
+    for (int tile = work.tile0; tile < work.tile1; ++tile) {
       const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
-      const int64_t wb = (int64_t)t.e * p.w_blocks + (GATED ? t.n : t.n * SETS);
-      Factors<SETS, kBatch> f;
-      for (int kb = kb0; kb < kb1; kb += kBatch) {
-        turn ^= 1;
-        if (turn) {                                  // the other warp's
-          const int n = min(kBatch, kb1 - kb);
-          for (stage += n; stage >= stages; stage -= stages) phase ^= 1;
-          for (slot += n; slot >= slots; slot -= slots) {}
-          continue;
+      const float* xs = p.xs + work.kb0 * p.xs_stride + t.row + lane;
+      for (int kb = work.kb0; kb < work.kb1; ++kb) {
+        mbar_wait(empty(stage), phase ^ 1);
+        for (int q = 0; q * 32 < t.rows; ++q) {
+          const bool there = q * 32 + lane < t.rows;
+          copy4(to(slot, q * 32 + lane), there ? xs + q * 32 : p.xs, there);
         }
-        f.ask(p, t.row, t.rows, wb, GATED ? wb + p.N / 128 : wb + (t.n * SETS + 1 < p.w_blocks), kb, min(kBatch, kb1 - kb), lane);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          if (kb + i >= kb1) break;
-          mbar_wait(empty(stage), phase ^ 1);
-          f.put(factors + slot * SETS * 128, i, lane);
-          __syncwarp();
-          if (lane == 0) bar_arrive(full(stage));
-          if (++stage == stages) { stage = 0; phase ^= 1; }
-          if (++slot == slots) slot = 0;
-        }
+        if (early > 0) --early;
+        else if (lane < SETS) copy4(to(slot, 128 + lane), column(t, kb), true);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(stage)) : "memory");
+        xs += p.xs_stride;
+        if (++stage == stages) { stage = 0; phase ^= 1; }
+        if (++slot == slots) slot = 0;
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == 3) {
+    regs_down<FP8_DOWN>();
   } else {
     regs_up<FP8_UP>();
     const int q = warp & 3, part = (warp - 4) >> 2, tid = threadIdx.x - 128, lane128 = q * 32 + lane;
     pdl_wait();
-    int buf = 0, slot = 0, tile, kb0, kb1, e = e_first;
+    int buf = 0, slot = 0, e = e_first;
     uint32_t buf_phase = 0;
-    Pieces it(u0, u1, KB, tile0);
-    while (it.next(tile, kb0, kb1)) {
+    for (int tile = work.tile0; tile < work.tile1; ++tile) {
       const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
       const bool some = q * 32 < t.rows, there = lane128 < t.rows;
       const int row = t.row + lane128, n0 = t.n * NT + part * 64;
@@ -541,66 +566,148 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       auto wait = [&](uint32_t& from, float& f0, float& f1) {
         mbar_wait(tfull(buf), buf_phase);
         fence_after();
-        const float* f = factors + slot * SETS * 128 + lane128;
-        f0 = f[0];
-        f1 = f[SETS == 2 ? 128 : 0];
+        const float* f = factors + slot * SLOT;
+        f0 = f[lane128] * f[128];
+        f1 = SETS == 2 ? f[lane128] * f[129] : f0;
         from = at + buf * NT;
       };
       if (some) {
-        add_blocks<C, 64>(s, kb1 - kb0, wait, read);
+        add_blocks<C, 64>(s, work.kb1 - work.kb0, wait, read);
       } else {
-        for (int kb = kb0; kb < kb1; ++kb) { mbar_wait(tfull(buf), buf_phase); read(); }
+        for (int kb = work.kb0; kb < work.kb1; ++kb) { mbar_wait(tfull(buf), buf_phase); read(); }
       }
-      if (kb1 - kb0 != KB) {
-        // A part of the tile's sum: to the workspace, [slot][quarter][part][column / 4][lane] of 16 bytes.  A share has at most two such pieces: slot 0
-        // the one that it begins with.
-        constexpr int kPer = (NT / 4) * 32;          // float4 of a quarter
-        const uint32_t x0 = (uint32_t)tile * KB;
-        auto slot_of = [&](uint32_t cta, int slot) { return reinterpret_cast<float4*>(p.part) + ((cta * 2 + slot) * p.quarters + q) * kPer + part * (C / 4) * 32 + lane; };
+      if constexpr (CLUSTER) {
+        // Groups of 8 columns of each set: this CTA finishes [g0, g1) of 16.  What it sends of another's lies there by sender (but the owner), set, group, half
+        // and row, 16 bytes each.
+        const int S = work.splits, me = (int)cluster_ctarank(), rows = p.quarters * 32, most = (16 + S - 1) / S;
+        const uint32_t sums = s_addr(factors + slots * SLOT);
+        auto place = [&](int sender, int set, int g, int half) { return sums + (uint32_t)((((sender * SETS + set) * most + g) * 2 + half) * rows + lane128) * 16u; };
+        cluster_wait();                                   // (all have begun)
+        const int g0 = 16 * me / S, g1 = 16 * (me + 1) / S;
         if (some) {
-          float4* dst = slot_of(me, x0 + kb0 == u0 ? 0 : 1);
 #pragma unroll
-          for (int c = 0; c < C; c += 4) {
-            float4 v;
-            s.at(c, v.x, v.y);
-            s.at(c + 2, v.z, v.w);
-            __stcg(dst + c / 4 * 32, v);
+          for (int i = 0; i < 8; ++i) {
+            const int g = part * 8 + i;
+            if (g >= g0 && g < g1) continue;
+            int owner = (g * S + S - 1) / 16;             // the last with 16 owner / S <= g
+            while (16 * owner / S > g) --owner;
+            while (16 * (owner + 1) / S <= g) ++owner;
+            const int sender = me - (me > owner), first = g - 16 * owner / S;
+#pragma unroll
+            for (int set = 0; set < SETS; ++set)
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const float* v = &s.v[set * 64 + i * 8 + half * 4];
+                push4(mapa_u32(place(sender, set, first, half), owner), v[0], v[1], v[2], v[3]);
+              }
           }
         }
-        sums_sync();
-        // its CTAs: from the one with its first unit to the one with its last; they count in the first one's counter
-        const uint32_t c0 = shares.of(x0), c1 = shares.of(x0 + KB - 1);
-        if (tid == 0) {
-          __threadfence();                              // (of what all threads of the barrier have stored)
-          const bool mine = atomicAdd(p.count + c0, 1u) == c1 - c0;
-          if (mine) p.count[c0] = 0;                    // ready for the next launch
-          __threadfence();
-          last_flag = mine;
-        }
-        sums_sync();
-        const bool last = last_flag != 0;
-        sums_sync();                                    // (the next piece writes there)
-        if (!last) continue;
-        s.clear();
-        if (some)
+        cluster_arrive(); cluster_wait();
+        uint32_t top = 0;
+        float h[GATED ? 64 : 1];
+        if (some) {
 #pragma unroll
-          for (int h = 0; h < C; h += 64)
-            for (uint32_t c = c0; c <= c1; ++c) {
-              const float4* src = slot_of(c, shares.begin(c) >= x0 ? 0 : 1) + h / 4 * 32;
-              float4 v[16];
+          for (int i = 0; i < 8; ++i) {
+            const int g = part * 8 + i;
+            if (g < g0 || g >= g1) continue;
+            float v[SETS][8];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __ldcg(src + i * 32);
+            for (int set = 0; set < SETS; ++set)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) { s.v[h + 4 * i] += v[i].x; s.v[h + 4 * i + 1] += v[i].y; s.v[h + 4 * i + 2] += v[i].z; s.v[h + 4 * i + 3] += v[i].w; }
+              for (int j = 0; j < 8; ++j) v[set][j] = 0.f;
+            for (int from = 0; from < S; ++from) {
+#pragma unroll
+              for (int set = 0; set < SETS; ++set)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const float* own = &s.v[set * 64 + i * 8 + half * 4];
+                  float4 f = make_float4(own[0], own[1], own[2], own[3]);
+                  if (from != me)
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(place(from - (from > me), set, g - g0, half)) : "memory");
+                  float* d = &v[set][half * 4];
+                  d[0] += f.x; d[1] += f.y; d[2] += f.z; d[3] += f.w;
+                }
             }
-      }
-      if constexpr (GATED) {
-        store_gated(p, s, row, there, t.n, tops, part, lane128);
-      } else if (there) {
+            if constexpr (GATED) {
 #pragma unroll
-        for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
+              for (int j = 0; j < 8; ++j) {
+                h[i * 8 + j] = gated(v[0][j], v[1][j]);
+                top = max(top, __float_as_uint(h[i * 8 + j]) & 0x7fffffffu);
+              }
+            } else if (there) {
+              store_group(p, v[0], row, t.n * NT + g * 8);
+            }
+          }
+        }
+        if constexpr (GATED) {
+          // the block's largest magnitude over all CTAs
+          for (int to = 0; to < S; ++to) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(s_addr(&tops[(me * 2 + part) * 128 + lane128]), to)), "r"(top) : "memory");
+          cluster_arrive(); cluster_wait();
+          for (int i = 0; i < 2 * S; ++i) top = max(top, tops[i * 128 + lane128]);
+          if (there) {
+            float scale, factor;
+            fp8::scale_of(__uint_as_float(top), scale, factor);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int g = part * 8 + i;
+              if (g < g0 || g >= g1) continue;
+              uint2 c = make_uint2(0, 0);
+              if (factor > 0.f) {
+                const float* v = &h[i * 8];
+                c.x = fp8::pack4(v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
+                c.y = fp8::pack4(v[4] * factor, v[5] * factor, v[6] * factor, v[7] * factor);
+              }
+              *reinterpret_cast<uint2*>(p.codes + (int64_t)row * p.N + t.n * 128 + g * 8) = c;
+            }
+            if (me == 0 && part == 0) p.out_scales[t.n * p.out_stride + row] = scale;
+          }
+        }
+      } else {
+        if (work.splits > 1) {
+          // To the workspace, [CTA][quarter][part][column / 4][lane] of 16 bytes.
+          constexpr int kPer = (NT / 4) * 32;          // float4 of a quarter
+          auto share_of = [&](int cta) { return reinterpret_cast<float4*>(p.part) + ((int64_t)cta * p.quarters + q) * kPer + part * (C / 4) * 32 + lane; };
+          if (some) {
+            float4* dst = share_of((int)blockIdx.x);
+#pragma unroll
+            for (int c = 0; c < C; c += 4) __stcg(dst + c / 4 * 32, make_float4(s.v[c], s.v[c + 1], s.v[c + 2], s.v[c + 3]));
+          }
+          sums_sync();
+          if (tid == 0) {
+            __threadfence();                              // (of what all threads of the barrier have stored)
+            const bool mine = atomicAdd(p.count + tile, 1u) == (unsigned)(work.splits - 1);
+            if (mine) p.count[tile] = 0;                  // ready for the next launch
+            __threadfence();
+            last_flag = mine;
+          }
+          sums_sync();
+          if (last_flag == 0) continue;                   // (a share is all that its CTA has)
+          s.clear();
+          if (some)
+#pragma unroll
+            for (int h = 0; h < C; h += 64)
+              for (int c = tile * work.splits; c < (tile + 1) * work.splits; ++c) {
+                const float4* src = share_of(c) + h / 4 * 32;
+                float4 v[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = __ldcg(src + i * 32);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { s.v[h + 4 * i] += v[i].x; s.v[h + 4 * i + 1] += v[i].y; s.v[h + 4 * i + 2] += v[i].z; s.v[h + 4 * i + 3] += v[i].w; }
+              }
+        }
+        if constexpr (GATED) {
+          store_gated(p, s, row, there, t.n, tops, part, lane128);
+        } else if (there) {
+#pragma unroll
+          for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
+        }
       }
     }
+  }
+  if (CLUSTER && warp < 4) {                        // the barriers that the others take, for all threads take part
+    cluster_wait();
+    cluster_arrive(); cluster_wait();
+    if (GATED) { cluster_arrive(); cluster_wait(); }
   }
   fence_before();
   __syncthreads();
@@ -813,36 +920,70 @@ static int sm_count() {
   return n < kMaxCtas ? n : kMaxCtas;
 }
 
+// How many clusters of `size` CTAs, one an SM, run at once.
+static int max_clusters(int size) {
+  static std::atomic<int> cache[kMaxSplits + 1];
+  int n = cache[size].load(std::memory_order_relaxed);
+  if (n == 0) {
+    auto kern = fp8_stream_kernel<128, false, true>;
+    int got = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem - kOwn) == cudaSuccess) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(size * 64); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = kSmem - kOwn;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&got, kern, &cfg) != cudaSuccess) { (void)cudaGetLastError(); got = 0; }
+    }
+    n = got + 1;
+    cache[size].store(n, std::memory_order_relaxed);
+  }
+  return n - 1;
+}
+
 template <int NT, bool GATED>
 static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cudaStream_t st) {
+  constexpr int BUFS = 512 / NT, SETS = NT / 128, kSlot = 136 * 4;
   const int widest = p.T < kRows ? p.T : kRows;
   p.quarters = (widest + 31) / 32;
   p.x_bytes = p.quarters * 4096;
   p.n_tiles = (p.N + (GATED ? 128 : NT) - 1) / (GATED ? 128 : NT);
-  constexpr int own = 8 * 1024;                            // the kernel's own shared memory, and rounding up to 1024
-  constexpr int slot_bytes = NT / 128 * 512, more = 512 / NT;
-  p.stages = (kSmem - own - more * slot_bytes) / (p.x_bytes + NT * 128 + slot_bytes);
-  if (p.stages > 16) p.stages = 16;
-  static_assert((kSmem - own - more * slot_bytes) / (kRows * 128 + NT * 128 + slot_bytes) > kBatch, "");
-  p.min_units = 2;
+  const int sms = sm_count();
+  KGE_REQUIRE(sms > 0, "kge_gemm_fp8: no CUDA device");
+  const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles;
+  p.splits = 0;                                            // grouped: by the number of tiles, on the device
+  if (!p.offsets) {
+    p.splits = 1;
+    if (2 * tiles < sms)
+      for (int s = kMaxSplits; s > 1; --s)
+        if (tiles * s <= sms && p.KB >= 2 * s && tiles <= max_clusters(s)) { p.splits = s; break; }
+  }
+  const bool cluster = p.splits > 1;
+  const int sums = cluster ? (p.splits - 1) * ((16 + p.splits - 1) / p.splits) * SETS * 2 * p.quarters * 32 * 16 : 0;
+  const int stage = p.x_bytes + NT * 128 + kSlot;
+  p.stages = (kSmem - kOwn - 1024 - BUFS * kSlot - sums) / stage;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  KGE_REQUIRE(p.stages >= 2, "kge_gemm_fp8: internal: %d stages", p.stages);
+  p.ahead = p.stages;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");
-  const int smem = p.stages * (p.x_bytes + NT * 128 + slot_bytes) + more * slot_bytes + 1024;
+  const int smem = p.stages * stage + BUFS * kSlot + sums + 1024;
   CUtensorMap mw, mx;
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
-  auto kern = fp8_stream_kernel<NT, GATED>;
+  auto kern = cluster ? fp8_stream_kernel<NT, GATED, true> : fp8_stream_kernel<NT, GATED, false>;
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int sms = sm_count();
-  KGE_REQUIRE(sms > 0, "kge_gemm_fp8: no CUDA device");
-  int64_t ctas = sms;
-  if (!p.offsets) {
-    // Whole numbers of CTAs a tile cost each of them one partial sum in place of two: worth up to a tenth of the SMs.
-    const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles, most = tiles * p.KB / p.min_units, even = tiles < sms ? sms / tiles * tiles : sms;
-    if (even * 10 >= sms * 9) ctas = even;
-    if (ctas > most) ctas = most < 1 ? 1 : most;
-  }
-  KGE_CUDA_OK(launch_pdl(kern, dim3((unsigned)ctas), dim3(kThreads), (size_t)smem, st, mw, mx, p));
+  prefer_max_shared(kern);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(cluster ? tiles * p.splits : sms)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_for_this_launch() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = cluster ? 2 : 1;
+  KGE_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, mw, mx, p));
   return 0;
 }
 
@@ -879,7 +1020,7 @@ static int launch_pairs(Fp8Params& p, const void* x, const void* w, int K, cudaS
 static int64_t workspace_bytes_of(int T) {
   if (T <= 0) return 0;
   const int64_t quarters = ((T < kRows ? T : kRows) + 31) / 32;
-  return kCounters * 4 + (int64_t)kMaxCtas * 2 * quarters * 256 * 128;
+  return kCounters * 4 + (int64_t)kMaxCtas * quarters * 256 * 128;
 }
 
 
