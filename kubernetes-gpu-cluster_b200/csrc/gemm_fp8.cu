@@ -61,6 +61,8 @@ struct Fp8Params {
   int wide;                                       // pairs: y's rows are 16-byte aligned
   int quarters, stages, x_bytes, ahead;           // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, stages filled early
   int splits;                                     // stream, dense: shares of K that a tile is cut into
+  int most;                                       // of a cluster: column groups that a CTA finishes at most,
+  uint8_t first[kMaxSplits + 1], owner[16];       // the first of 16 that each finishes, which CTA finishes each
 };
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -370,6 +372,9 @@ __device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>&
 // What a CTA does: blocks of K [kb0, kb1) of tiles [tile0, tile1).  With at least half as many tiles as SMs each is one CTA's, and as many CTAs work as make
 // all have the same number (a weight stream needs bytes under way, not SMs); fewer are cut along K, into `splits` shares.
 struct Work { int tile0, tile1, kb0, kb1, splits; };
+// Blocks of K of a stage: the thread that issues the MMAs takes some 600 cycles from one pair of barriers to the next, and tiles of 128 columns have their
+// data in 370; besides, boxes of 128 bytes a row are read at 5.7 TB/s and two neighbouring ones at 6.35.
+__host__ __device__ constexpr int stream_sub(int nt) { return nt == 128 ? 2 : 1; }
 __device__ __forceinline__ Work work_of(int tiles, int KB, int splits, int me, int sms) {
   if (splits == 0) splits = tiles == 0 || 2 * tiles >= sms ? 1 : max(1, min(min(sms / tiles, KB / 2), kMaxSplits));
   if (splits > 1) {
@@ -392,23 +397,29 @@ __device__ __forceinline__ void push4(uint32_t dst, float a, float b, float c, f
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
 
+__device__ __forceinline__ float4 lds4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
 // CLUSTER: the shares of a tile are a cluster's CTAs.  Each finishes its part of the tile's columns, groups of 8, and gets the others' sums of them through
 // distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
 // Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
 template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  constexpr int C = NT / 2, BUFS = 512 / NT, SETS = NT / 128, SLOT = 136;
+  constexpr int C = NT / 2, SUB = stream_sub(NT), BUFS = 512 / (NT * SUB), SETS = NT / 128, SLOT = 136;
   static_assert(!GATED || NT == 256, "a gated tile holds 128 columns of each");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * kMaxStages + 2 * BUFS];
   __shared__ uint32_t tmem_slot;
   __shared__ int last_flag;
-  __shared__ uint32_t tops[(CLUSTER ? 2 * kMaxSplits : 2) * 128];
+  __shared__ uint32_t tops[(CLUSTER ? 1 + kMaxSplits : 2) * 128];
   __shared__ int starts[CLUSTER ? 2 : kMaxGroups + 1];
   const int stages = p.stages;
-  const uint32_t stage_bytes = (uint32_t)p.x_bytes + NT * 128;
+  const uint32_t block_bytes = (uint32_t)p.x_bytes + NT * 128, stage_bytes = SUB * block_bytes;
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
@@ -429,6 +440,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (CLUSTER && GATED && threadIdx.x < 128) tops[threadIdx.x] = 0;
   if ((CLUSTER || !p.offsets) && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
   fence_before();
   __syncthreads();
@@ -446,42 +458,51 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   // xs of the rows and ws of the columns, block of K by block of K, in a ring.  A slot is free again when its block is added up.  The block `stages` further
   // is then at the earliest on its way (its stage was freed by an MMA that began after the sums BUFS blocks before had been read).
   float* factors = reinterpret_cast<float*>(smem + stages * stage_bytes);
-  const int slots = stages + BUFS;
+  const int slots = (stages + BUFS) * SUB;
 
   if (warp == 0) {
     regs_down<FP8_DOWN>();
     if (elect_one()) {
       int stage = 0, e = e_first;
       uint32_t phase = 0;
-      auto load_w = [&](int s, const Tile& t, int kb) {
-        const uint32_t dst = base + s * stage_bytes + p.x_bytes;
+      auto load_w = [&](int s, const Tile& t, int kb, int n) {
         const int row = t.e * p.w_rows;
 #pragma unroll
-        for (int h = 0; h < NT / 128; ++h) load_box(dst + h * kSlab, &map_w, full(s), kb * 128, row + (GATED ? t.n * 128 + h * p.N : t.n * NT + h * 128));
+        for (int u = 0; u < SUB; ++u) {
+          if (u >= n) break;
+          const uint32_t dst = base + s * stage_bytes + u * block_bytes + p.x_bytes;
+#pragma unroll
+          for (int h = 0; h < NT / 128; ++h) load_box(dst + h * kSlab, &map_w, full(s), (kb + u) * 128, row + (GATED ? t.n * 128 + h * p.N : t.n * NT + h * 128));
+        }
       };
-      auto load_x = [&](int s, const Tile& t, int kb) {
-        for (int r = 0; r < t.rows; r += 32) load_box(base + s * stage_bytes + r * 128, &map_x, full(s), kb * 128, t.row + r);
+      auto load_x = [&](int s, const Tile& t, int kb, int n) {
+        for (int u = 0; u < n; ++u)
+          for (int r = 0; r < t.rows; r += 32) load_box(base + s * stage_bytes + u * block_bytes + r * 128, &map_x, full(s), (kb + u) * 128, t.row + r);
       };
-      auto bytes_of = [&](const Tile& t) { return (uint32_t)(NT * 128 + (t.rows + 31) / 32 * 4096); };
+      auto bytes_of = [&](const Tile& t, int n) { return (uint32_t)(n * (NT * 128 + (t.rows + 31) / 32 * 4096)); };
       // What the weights are is known before the kernel before has ended: the first tile's first blocks.
       int ahead = 0;
       if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
         const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
-        ahead = min(p.ahead, work.kb1 - work.kb0);
-        for (int i = 0; i < ahead; ++i) { bar_expect(full(i), bytes_of(t)); load_w(i, t, work.kb0 + i); }
+        for (int kb = work.kb0; ahead < p.ahead && kb < work.kb1; kb += SUB, ++ahead) {
+          const int n = min(SUB, work.kb1 - kb);
+          bar_expect(full(ahead), bytes_of(t, n));
+          load_w(ahead, t, kb, n);
+        }
       }
       pdl_wait();
       for (int tile = work.tile0; tile < work.tile1; ++tile) {
         const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
-        for (int kb = work.kb0; kb < work.kb1; ++kb) {
+        for (int kb = work.kb0; kb < work.kb1; kb += SUB) {
+          const int n = min(SUB, work.kb1 - kb);
           if (ahead > 0) {
             --ahead;
           } else {
             mbar_wait(empty(stage), phase ^ 1);
-            bar_expect(full(stage), bytes_of(t));
-            load_w(stage, t, kb);
+            bar_expect(full(stage), bytes_of(t, n));
+            load_w(stage, t, kb, n);
           }
-          load_x(stage, t, kb);
+          load_x(stage, t, kb, n);
           if (++stage == stages) { stage = 0; phase ^= 1; }
         }
       }
@@ -494,18 +515,30 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       uint32_t phase = 0, buf_phase = 0;
       const uint64_t a0 = tile_desc(base), b0 = tile_desc(base + p.x_bytes);
       uint64_t a = a0, b = b0;
-      for (int64_t n = (int64_t)(work.tile1 - work.tile0) * (work.kb1 - work.kb0); n > 0; --n) {
-        mbar_wait(tempty(buf), buf_phase ^ 1);
-        mbar_wait(full(stage), phase);
-        fence_after();
+      bool f_there = false, t_there = false;
+      for (int tile = work.tile0; tile < work.tile1; ++tile)
+        for (int kb = work.kb0; kb < work.kb1; kb += SUB) {
+          if (!f_there) mbar_wait(full(stage), phase);
+          if (!t_there) mbar_wait(tempty(buf), buf_phase ^ 1);
+          const int s1 = stage + 1 == stages ? 0 : stage + 1, v1 = buf + 1 == BUFS ? 0 : buf + 1;
+          const uint32_t p1 = s1 == 0 ? phase ^ 1 : phase, w1 = v1 == 0 ? buf_phase ^ 1 : buf_phase;
+          f_there = mbar_test(full(s1), p1);
+          t_there = mbar_test(tempty(v1), w1 ^ 1);
+          fence_after();
+          const uint32_t d = tmem + buf * (NT * SUB);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma8(tmem + buf * NT, a + 2 * k, b + 2 * k, idesc, k > 0);
-        commit(tfull(buf));
-        commit(empty(stage));
-        a += stage_bytes >> 4; b += stage_bytes >> 4;
-        if (++stage == stages) { stage = 0; phase ^= 1; a = a0; b = b0; }
-        if (++buf == BUFS) { buf = 0; buf_phase ^= 1; }
-      }
+          for (int u = 0; u < SUB; ++u) {
+            if (u > 0 && kb + u >= work.kb1) break;
+            const uint64_t off = (uint64_t)(u * (block_bytes >> 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma8(d + u * NT, a + off + 2 * k, b + off + 2 * k, idesc, k > 0);
+          }
+          commit(tfull(buf));
+          commit(empty(stage));
+          a += stage_bytes >> 4; b += stage_bytes >> 4;
+          if (s1 == 0) { a = a0; b = b0; }
+          stage = s1; phase = p1; buf = v1; buf_phase = w1;
+        }
     }
   } else if (warp == 2) {
     regs_down<FP8_DOWN>();
@@ -519,7 +552,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     int early = 0;
     if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
       const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
-      early = min(p.ahead, work.kb1 - work.kb0);
+      early = min(p.ahead * SUB, work.kb1 - work.kb0);
       for (int i = 0; i < early; ++i)
         if (lane < SETS) copy4(to(i, 128 + lane), column(t, work.kb0 + i), true);
     }
@@ -527,18 +560,25 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     for (int tile = work.tile0; tile < work.tile1; ++tile) {
       const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
       const float* xs = p.xs + work.kb0 * p.xs_stride + t.row + lane;
-      for (int kb = work.kb0; kb < work.kb1; ++kb) {
+      const float* ws = column(t, work.kb0);
+      for (int kb = work.kb0; kb < work.kb1; kb += SUB) {
         mbar_wait(empty(stage), phase ^ 1);
-        for (int q = 0; q * 32 < t.rows; ++q) {
-          const bool there = q * 32 + lane < t.rows;
-          copy4(to(slot, q * 32 + lane), there ? xs + q * 32 : p.xs, there);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+          if (kb + u < work.kb1) {
+            for (int q = 0; q * 32 < t.rows; ++q) {
+              const bool there = q * 32 + lane < t.rows;
+              copy4(to(slot + u, q * 32 + lane), there ? xs + q * 32 : p.xs, there);
+            }
+            if (early > 0) --early;
+            else if (lane < SETS) copy4(to(slot + u, 128 + lane), ws, true);
+            xs += p.xs_stride;
+            ++ws;
+          }
         }
-        if (early > 0) --early;
-        else if (lane < SETS) copy4(to(slot, 128 + lane), column(t, kb), true);
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full(stage)) : "memory");
-        xs += p.xs_stride;
         if (++stage == stages) { stage = 0; phase ^= 1; }
-        if (++slot == slots) slot = 0;
+        if ((slot += SUB) == slots) slot = 0;
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -557,109 +597,120 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       Sums<C> s;
       s.clear();
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 64;
+      int sub = 0, left = work.kb1 - work.kb0;
       auto read = [&] {
-        fence_before();
-        if (lane == 0) bar_arrive(tempty(buf));
-        if (++buf == BUFS) { buf = 0; buf_phase ^= 1; }
-        if (++slot == slots) slot = 0;
+        if (--left == 0 || ++sub == SUB) {
+          sub = 0;
+          fence_before();
+          if (lane == 0) bar_arrive(tempty(buf));
+          if (++buf == BUFS) { buf = 0; buf_phase ^= 1; }
+          if ((slot += SUB) == slots) slot = 0;
+        }
       };
       auto wait = [&](uint32_t& from, float& f0, float& f1) {
-        mbar_wait(tfull(buf), buf_phase);
-        fence_after();
-        const float* f = factors + slot * SLOT;
+        if (SUB == 1 || sub == 0) {
+          mbar_wait(tfull(buf), buf_phase);
+          fence_after();
+        }
+        const float* f = factors + (slot + sub) * SLOT;
         f0 = f[lane128] * f[128];
         f1 = SETS == 2 ? f[lane128] * f[129] : f0;
-        from = at + buf * NT;
+        from = at + buf * (NT * SUB) + sub * NT;
       };
       if (some) {
-        add_blocks<C, 64>(s, work.kb1 - work.kb0, wait, read);
+        add_blocks<C, 64>(s, left, wait, read);
       } else {
-        for (int kb = work.kb0; kb < work.kb1; ++kb) { mbar_wait(tfull(buf), buf_phase); read(); }
+        while (left > 0) {
+          if (sub == 0) mbar_wait(tfull(buf), buf_phase);
+          read();
+        }
       }
       if constexpr (CLUSTER) {
-        // Groups of 8 columns of each set: this CTA finishes [g0, g1) of 16.  What it sends of another's lies there by sender (but the owner), set, group, half
-        // and row, 16 bytes each.
-        const int S = work.splits, me = (int)cluster_ctarank(), rows = p.quarters * 32, most = (16 + S - 1) / S;
+        // Groups of 8 columns of each set: this CTA finishes [g0, g1) of 16.  Their sums lie there by sender, set, group, half and row, 16 bytes each; each is
+        // finished by a lane of its row.  (Everything here runs once a launch and costs its way from the L2: rolled loops, and all sums by one path.)
+        const int S = work.splits, me = (int)cluster_ctarank(), rows = p.quarters * 32, most = p.most;
         const uint32_t sums = s_addr(factors + slots * SLOT);
-        auto place = [&](int sender, int set, int g, int half) { return sums + (uint32_t)((((sender * SETS + set) * most + g) * 2 + half) * rows + lane128) * 16u; };
+        auto place = [&](int sender, int set, int g, int half, int r) { return sums + (uint32_t)((((sender * SETS + set) * most + g) * 2 + half) * rows + r) * 16u; };
         cluster_wait();                                   // (all have begun)
-        const int g0 = 16 * me / S, g1 = 16 * (me + 1) / S;
         if (some) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int g = part * 8 + i;
-            if (g >= g0 && g < g1) continue;
-            int owner = (g * S + S - 1) / 16;             // the last with 16 owner / S <= g
-            while (16 * owner / S > g) --owner;
-            while (16 * (owner + 1) / S <= g) ++owner;
-            const int sender = me - (me > owner), first = g - 16 * owner / S;
+            const int g = part * 8 + i, owner = p.owner[g];
+            const uint32_t to = mapa_u32(place(me, 0, g - p.first[owner], 0, lane128), owner);
 #pragma unroll
             for (int set = 0; set < SETS; ++set)
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
                 const float* v = &s.v[set * 64 + i * 8 + half * 4];
-                push4(mapa_u32(place(sender, set, first, half), owner), v[0], v[1], v[2], v[3]);
+                push4(to + (uint32_t)((set * most * 2 + half) * rows) * 16u, v[0], v[1], v[2], v[3]);
               }
           }
         }
         cluster_arrive(); cluster_wait();
-        uint32_t top = 0;
-        float h[GATED ? 64 : 1];
-        if (some) {
+        const int g0 = p.first[me], items = (p.first[me + 1] - g0) * p.quarters;
+        auto item = [&](int n, int& r, int& g) {          // a warp's n-th quarter of the rows and group
+          g = n / p.quarters;
+          r = (n - g * p.quarters) * 32 + lane;
+        };
+        auto sum_of = [&](int set, int g, int r, float (&v)[8]) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int g = part * 8 + i;
-            if (g < g0 || g >= g1) continue;
-            float v[SETS][8];
+          for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll 1
+          for (int from = 0; from < S; ++from)
 #pragma unroll
-            for (int set = 0; set < SETS; ++set)
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[set][j] = 0.f;
-            for (int from = 0; from < S; ++from) {
-#pragma unroll
-              for (int set = 0; set < SETS; ++set)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                  const float* own = &s.v[set * 64 + i * 8 + half * 4];
-                  float4 f = make_float4(own[0], own[1], own[2], own[3]);
-                  if (from != me)
-                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(place(from - (from > me), set, g - g0, half)) : "memory");
-                  float* d = &v[set][half * 4];
-                  d[0] += f.x; d[1] += f.y; d[2] += f.z; d[3] += f.w;
-                }
+            for (int half = 0; half < 2; ++half) {
+              const float4 f = lds4(place(from, set, g, half, r));
+              v[half * 4] += f.x; v[half * 4 + 1] += f.y; v[half * 4 + 2] += f.z; v[half * 4 + 3] += f.w;
             }
-            if constexpr (GATED) {
+        };
+#pragma unroll 1
+        for (int n = warp - 4; n < items; n += kSumWarps) {
+          int r, g;
+          item(n, r, g);
+          float v[8];
+          sum_of(0, g, r, v);
+          if constexpr (GATED) {
+            float u[8];
+            sum_of(1, g, r, u);
+            uint32_t top = 0;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                h[i * 8 + j] = gated(v[0][j], v[1][j]);
-                top = max(top, __float_as_uint(h[i * 8 + j]) & 0x7fffffffu);
-              }
-            } else if (there) {
-              store_group(p, v[0], row, t.n * NT + g * 8);
+            for (int j = 0; j < 8; ++j) {
+              v[j] = gated(v[j], u[j]);
+              top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
             }
+            atomicMax(&tops[r], top);
+            push4(mapa_u32(place(0, 0, g, 0, r), me), v[0], v[1], v[2], v[3]);      // (in the place of the first sender's sums)
+            push4(mapa_u32(place(0, 0, g, 1, r), me), v[4], v[5], v[6], v[7]);
+          } else if (r < t.rows) {
+            store_group(p, v, t.row + r, t.n * NT + (g0 + g) * 8);
           }
         }
         if constexpr (GATED) {
           // the block's largest magnitude over all CTAs
-          for (int to = 0; to < S; ++to) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(s_addr(&tops[(me * 2 + part) * 128 + lane128]), to)), "r"(top) : "memory");
+          sums_sync();
+          if (tid < 128)
+#pragma unroll 1
+            for (int to = 0; to < S; ++to)
+              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_u32(s_addr(&tops[(1 + me) * 128 + tid]), to)), "r"(tops[tid]) : "memory");
           cluster_arrive(); cluster_wait();
-          for (int i = 0; i < 2 * S; ++i) top = max(top, tops[i * 128 + lane128]);
-          if (there) {
+#pragma unroll 1
+          for (int n = warp - 4; n < items; n += kSumWarps) {
+            int r, g;
+            item(n, r, g);
+            uint32_t top = 0;
+            for (int c = 1; c <= S; ++c) top = max(top, tops[c * 128 + r]);
             float scale, factor;
             fp8::scale_of(__uint_as_float(top), scale, factor);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int g = part * 8 + i;
-              if (g < g0 || g >= g1) continue;
-              uint2 c = make_uint2(0, 0);
-              if (factor > 0.f) {
-                const float* v = &h[i * 8];
-                c.x = fp8::pack4(v[0] * factor, v[1] * factor, v[2] * factor, v[3] * factor);
-                c.y = fp8::pack4(v[4] * factor, v[5] * factor, v[6] * factor, v[7] * factor);
-              }
-              *reinterpret_cast<uint2*>(p.codes + (int64_t)row * p.N + t.n * 128 + g * 8) = c;
+            const float4 a = lds4(place(0, 0, g, 0, r)), b = lds4(place(0, 0, g, 1, r));
+            uint2 c = make_uint2(0, 0);
+            if (factor > 0.f) {
+              c.x = fp8::pack4(a.x * factor, a.y * factor, a.z * factor, a.w * factor);
+              c.y = fp8::pack4(b.x * factor, b.y * factor, b.z * factor, b.w * factor);
             }
-            if (me == 0 && part == 0) p.out_scales[t.n * p.out_stride + row] = scale;
+            if (r < t.rows) {
+              *reinterpret_cast<uint2*>(p.codes + (int64_t)(t.row + r) * p.N + t.n * 128 + (g0 + g) * 8) = c;
+              if (me == 0 && g == 0) p.out_scales[t.n * p.out_stride + t.row + r] = scale;
+            }
           }
         }
       } else {
@@ -944,7 +995,7 @@ static int max_clusters(int size) {
 
 template <int NT, bool GATED>
 static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cudaStream_t st) {
-  constexpr int BUFS = 512 / NT, SETS = NT / 128, kSlot = 136 * 4;
+  constexpr int SUB = stream_sub(NT), BUFS = 512 / (NT * SUB), SETS = NT / 128, kSlot = 136 * 4;
   const int widest = p.T < kRows ? p.T : kRows;
   p.quarters = (widest + 31) / 32;
   p.x_bytes = p.quarters * 4096;
@@ -960,15 +1011,21 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
         if (tiles * s <= sms && p.KB >= 2 * s && tiles <= max_clusters(s)) { p.splits = s; break; }
   }
   const bool cluster = p.splits > 1;
-  const int sums = cluster ? (p.splits - 1) * ((16 + p.splits - 1) / p.splits) * SETS * 2 * p.quarters * 32 * 16 : 0;
-  const int stage = p.x_bytes + NT * 128 + kSlot;
-  p.stages = (kSmem - kOwn - 1024 - BUFS * kSlot - sums) / stage;
+  if (cluster) {
+    p.most = (16 + p.splits - 1) / p.splits;
+    for (int c = 0; c <= p.splits; ++c) p.first[c] = (uint8_t)(16 * c / p.splits);
+    for (int c = 0; c < p.splits; ++c)
+      for (int g = p.first[c]; g < p.first[c + 1]; ++g) p.owner[g] = (uint8_t)c;
+  }
+  const int sums = cluster ? p.splits * p.most * SETS * 2 * p.quarters * 32 * 16 : 0;
+  const int stage = SUB * (p.x_bytes + NT * 128 + kSlot);
+  p.stages = (kSmem - kOwn - 1024 - BUFS * SUB * kSlot - sums) / stage;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   KGE_REQUIRE(p.stages >= 2, "kge_gemm_fp8: internal: %d stages", p.stages);
   p.ahead = p.stages;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");
-  const int smem = p.stages * stage + BUFS * kSlot + sums + 1024;
+  const int smem = p.stages * stage + BUFS * SUB * kSlot + sums + 1024;
   CUtensorMap mw, mx;
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
