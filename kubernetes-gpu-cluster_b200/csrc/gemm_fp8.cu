@@ -24,14 +24,9 @@ inline namespace KGE_ELT_NS {
 
 constexpr int kRows = 128;                        // tokens of a CTA's tile
 constexpr int kSlab = 128 * 128;                  // bytes of 128 rows of a block of K
-#ifndef FP8_CHUNK
-#define FP8_CHUNK 32
-#define FP8_UP 216
-#define FP8_DOWN 72
-#endif
 constexpr int kSumWarps = 8;                      // warps that add up: a token of 128 and 64 columns of each 128 a thread
 constexpr int kThreads = 128 + 32 * kSumWarps;    // producer, MMA, tensor memory, factors; those
-constexpr int kChunk = FP8_CHUNK;                 // columns that a warp reads of tensor memory at a time
+constexpr int kSumRegs = 216, kOtherRegs = 72;    // registers of those and of the others: 256 x 216 + 128 x 72 = 384 x 168, what the block is launched with
 constexpr int kCounters = 256;                    // arrival counters at the head of the workspace
 constexpr int kMaxCtas = 160;
 constexpr int kMaxGroups = 1024;
@@ -96,21 +91,13 @@ __device__ __forceinline__ void mma8(uint32_t d, uint64_t a, uint64_t b, uint32_
 __device__ __forceinline__ void mma8x2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-// N columns of this warp's 32 lanes; the caller waits (tmem_wait_ld)
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[N]) {
-  static_assert(N == 16 || N == 32, "");
-  if constexpr (N == 32)
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(at));
-  else
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(at));
+// 32 columns of this warp's 32 lanes; the caller waits (tmem_wait_ld)
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+               "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+               "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(at));
 }
 // K-major tile of 128-byte rows with 128-byte swizzle, atoms of 8 rows 1024 bytes apart
 __device__ __forceinline__ uint64_t tile_desc(uint32_t at) {
@@ -184,10 +171,11 @@ struct Sums {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = 0.f;
   }
-  // += factor * D of kChunk columns at c
-  __device__ __forceinline__ void add(int c, const uint32_t (&r)[kChunk], float factor) {
+  // += factor * D of N columns at c
+  template <int N>
+  __device__ __forceinline__ void add(int c, const uint32_t (&r)[N], float factor) {
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(v[c + i]) : "f"(__uint_as_float(r[i])), "f"(factor));
+    for (int i = 0; i < N; ++i) asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(v[c + i]) : "f"(__uint_as_float(r[i])), "f"(factor));
   }
   __device__ __forceinline__ void at(int c, float& a, float& b) const { a = v[c]; b = v[c + 1]; }
 };
@@ -195,9 +183,11 @@ struct Sums {
 // Adds up `blocks` blocks of K.  wait(): the address of the next block's columns in tensor memory and its factors, when they are there; read(): they are
 // in registers.  A thread's second 64 columns (if it has them) lie SKIP columns behind its first, with a factor of their own.  The next block is waited
 // for, and its first columns asked for, before the last ones of this block are added, so that the way to tensor memory and back passes under arithmetic.
+// (All 64 columns of threads that have no more at once: 4096 x 14336, one token, 15.6 us against 14.8.)
 template <int C, int SKIP, typename W, typename R>
 __device__ __forceinline__ void add_blocks(Sums<C>& s, int blocks, W wait, R read) {
-  uint32_t r[2][kChunk], at;
+  constexpr int N = 32;
+  uint32_t r[2][N], at;
   float f0, f1;
   wait(at, f0, f1);
   tmem_ld(at, r[0]);
@@ -205,11 +195,11 @@ __device__ __forceinline__ void add_blocks(Sums<C>& s, int blocks, W wait, R rea
   for (; blocks > 0; --blocks) {
     const float g0 = f0, g1 = f1;
 #pragma unroll
-    for (int c = 0; c < C; c += kChunk) {
-      uint32_t (&now)[kChunk] = r[(c / kChunk) & 1], (&then)[kChunk] = r[(c / kChunk + 1) & 1];
+    for (int c = 0; c < C; c += N) {
+      uint32_t (&now)[N] = r[(c / N) & 1], (&then)[N] = r[(c / N + 1) & 1];
       tmem_wait_ld(now);
-      if (c + kChunk < C) {
-        tmem_ld(at + c + kChunk + (c + kChunk >= 64 ? SKIP : 0), then);
+      if (c + N < C) {
+        tmem_ld(at + c + N + (c + N >= 64 ? SKIP : 0), then);
       } else {
         read();
         if (blocks > 1) {
@@ -247,7 +237,13 @@ struct Factors {
   }
 };
 
-__device__ __forceinline__ float gated(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
+// silu(gate) up, with the unit's own exponential and reciprocal: e^-gate is infinite below -88, and the result then zero
+__device__ __forceinline__ float gated(float gate, float up) {
+  float e, inv;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(gate * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.f + e));
+  return gate * inv * up;
+}
 
 // 8 columns of a row from n0 on, rounded once.
 __device__ __forceinline__ void store_group(const Fp8Params& p, float (&v)[8], int row, int n0) {
@@ -461,7 +457,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   const int slots = (stages + BUFS) * SUB;
 
   if (warp == 0) {
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
     if (elect_one()) {
       int stage = 0, e = e_first;
       uint32_t phase = 0;
@@ -508,7 +504,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       }
     }
   } else if (warp == 1) {
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
     if (elect_one()) {
       constexpr uint32_t idesc = instr_desc(kRows, NT);
       int stage = 0, buf = 0;
@@ -541,7 +537,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
     }
   } else if (warp == 2) {
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
     int stage = 0, slot = 0, e = e_first;
     uint32_t phase = 0;
     auto column = [&](const Tile& t, int kb) {           // of a tile's ws: lanes 0 (and 1) have a block of its columns each
@@ -583,9 +579,9 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 3) {
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
   } else {
-    regs_up<FP8_UP>();
+    regs_up<kSumRegs>();
     const int q = warp & 3, part = (warp - 4) >> 2, tid = threadIdx.x - 128, lane128 = q * 32 + lane;
     pdl_wait();
     int buf = 0, slot = 0, e = e_first;
@@ -817,7 +813,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
   if (warp == 0 || warp == 3) {
     // the copies and factors of kPairBatch blocks of K by one of the two, of as many by the other
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
     int stage = 0, slot = 0, tile = 0, e = e_first, turn = 1 - (warp & 1);
     uint32_t phase = 0;
     const uint32_t lead0 = mapa_u32(full(0), 0);
@@ -860,7 +856,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       }
     }
   } else if (warp < 4) {
-    regs_down<FP8_DOWN>();
+    regs_down<kOtherRegs>();
     if (rank == 0 && elect_one()) {                 // the leader issues for both, the first 128 columns by one thread and the second by another
       constexpr uint32_t idesc = instr_desc(2 * kRows, 128);
       const int h = warp - 1;
@@ -889,7 +885,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       }
     }
   } else {
-    regs_up<FP8_UP>();
+    regs_up<kSumRegs>();
     const int q = warp & 3, part = (warp - 4) >> 2, lane128 = q * 32 + lane;
     const uint32_t lead_tempty = mapa_u32(tempty(part), 0);
     int buf = 0, slot = 0, tile = 0;
@@ -1006,7 +1002,7 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   p.splits = 0;                                            // grouped: by the number of tiles, on the device
   if (!p.offsets) {
     p.splits = 1;
-    if (2 * tiles < sms)
+    if ((GATED || NT == 128) && 2 * tiles < sms)
       for (int s = kMaxSplits; s > 1; --s)
         if (tiles * s <= sms && p.KB >= 2 * s && tiles <= max_clusters(s)) { p.splits = s; break; }
   }
@@ -1029,7 +1025,10 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   CUtensorMap mw, mx;
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
-  auto kern = cluster ? fp8_stream_kernel<NT, GATED, true> : fp8_stream_kernel<NT, GATED, false>;
+  auto kern = fp8_stream_kernel<NT, GATED, false>;
+  if constexpr (GATED || NT == 128) {
+    if (cluster) kern = fp8_stream_kernel<NT, GATED, true>;
+  }
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   prefer_max_shared(kern);
   cudaLaunchConfig_t cfg = {};
@@ -1108,7 +1107,11 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
 #ifndef KGE_HALF
   if (gated) return pairs ? launch_pairs<true>(p, x, w, K, st) : launch_stream<256, true>(p, x, w, K, st);
 #endif
-  return pairs ? launch_pairs<false>(p, x, w, K, st) : launch_stream<128, false>(p, x, w, K, st);
+  if (pairs) return launch_pairs<false>(p, x, w, K, st);
+  // Tiles of 256 columns where they are enough for whole tiles a CTA: 64 tokens, us with 128 and 256, 28672 x 4096 27.5 and 25.9, 128256 x 4096 96.5 and 97.4,
+  // 128 experts of 2048 x 768, 512 rows, 39.2 and 38.6.  Cut along K they have less to show (4096 x 4096 8.8 and 10.3).
+  const int64_t groups = p.offsets && p.T < p.E ? p.T : p.E, wide = ((int64_t)(p.T / p.E + kRows - 1) / kRows + (p.T < p.E)) * groups * ((p.N + 255) / 256);
+  return 2 * wide >= sm_count() ? launch_stream<256, false>(p, x, w, K, st) : launch_stream<128, false>(p, x, w, K, st);
 }
 
 }  // namespace KGE_ELT_NS
