@@ -31,12 +31,13 @@ constexpr int kCounters = 256;                    // arrival counters at the hea
 constexpr int kMaxCtas = 160;
 constexpr int kMaxGroups = 1024;
 constexpr int kMaxStages = 16;
+constexpr int kSlotBytes = 136 * 4;               // factors of a block of K: of 128 rows, of up to two sets of columns
 constexpr int kMaxSplits = 8;                     // CTAs of a cluster
 constexpr int kSmem = 226 * 1024;
 constexpr int kOwn = 14 * 1024;                   // of it, at most, a kernel's own
 constexpr int kPairStages = 6;
 constexpr int kPairSlots = kPairStages + 2;
-constexpr int kPairBatch = 4;                     // blocks of K that a warp brings in at a time
+constexpr int kPairBatch = 2;                     // blocks of K that a warp brings in at a time
 static_assert(kPairStages > kPairBatch, "");
 constexpr int kPairBand = 8;                      // 74 pairs at work: 8 x 9 tiles share 17 slabs a block of K, 32 x 2.3 would 34
 
@@ -405,7 +406,7 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
 template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
-  constexpr int C = NT / 2, SUB = stream_sub(NT), BUFS = 512 / (NT * SUB), SETS = NT / 128, SLOT = 136;
+  constexpr int C = NT / 2, SUB = stream_sub(NT), BUFS = 512 / (NT * SUB), SETS = NT / 128, SLOT = kSlotBytes / 4;
   static_assert(!GATED || NT == 256, "a gated tile holds 128 columns of each");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -989,23 +990,47 @@ static int max_clusters(int size) {
   return n - 1;
 }
 
+static int quarters_of(int T) { return ((T < kRows ? T : kRows) + 31) / 32; }
+// What the sums of a cluster's shares take of shared memory, and how many stages are left.
+static int sums_bytes(int splits, int sets, int quarters) { return splits > 1 ? splits * ((16 + splits - 1) / splits) * sets * 2 * quarters * 32 * 16 : 0; }
+static int stage_bytes_of(int nt, int quarters) { return stream_sub(nt) * (quarters * 4096 + nt * 128 + kSlotBytes); }
+static int stream_stages(int nt, int splits, int quarters) {
+  const int n = (kSmem - kOwn - 1024 - 512 / nt * kSlotBytes - sums_bytes(splits, nt / 128, quarters)) / stage_bytes_of(nt, quarters);
+  return n < kMaxStages ? n : kMaxStages;
+}
+// Shares of K of a dense problem's tiles: the most that run at once and leave two stages.
+static int plan_splits(int64_t tiles, int nt, int quarters, int KB, int sms) {
+  if (2 * tiles >= sms) return 1;
+  for (int s = kMaxSplits; s > 1; --s)
+    if (tiles * s <= sms && KB >= 2 * s && tiles <= max_clusters(s) && stream_stages(nt, s, quarters) >= 2) return s;
+  return 1;
+}
+// Which kernel a dense problem takes, by what each is measured to need: a block of K 0.37 us a tile of the pair kernel and 1.8 for the tile's end; 0.38 a
+// tile of 128 columns of the other (0.45 of a share, for there the rings are not yet full), 0.70 of 256, and 1.5 for its end; 5 us for start and end.  us by pairs and by single CTAs: 128
+// x 28672 x 4096 37.2 and 29.1, 256 38.2 and 51.5, 512 64 and 98; 256 x 4096 x 4096 18.7 and 13.0, 512 19.4 and 16.7, 1024 20.4 and 23.0; 333 x 2504 x 2064
+// 15.4 and 10.8; gated 128 x 28672 x 4096 36.5 and 26.8, 256 37.6 and 47.2.
+static bool use_pairs(int T, int N, int KB, bool gated, int sms) {
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t wide = up(N, gated ? 128 : 256);
+  const double pairs = up(up(T, 2 * kRows) * wide, sms / 2) * (KB * 0.37 + 1.8);
+  double single = up(up(T, kRows) * wide, sms) * (KB * 0.70 + 1.5);
+  const int64_t tiles = up(T, kRows) * (gated ? wide : up(N, 128));
+  const int splits = plan_splits(tiles, gated ? 256 : 128, quarters_of(T), KB, sms);
+  if (splits > 1) single = up(KB, splits) * (gated ? 0.70 : 0.45) + 1.5;
+  else if (!gated && 2 * up(T, kRows) * wide < sms) single = up(tiles, sms) * (KB * 0.38 + 1.5);
+  return pairs < single;
+}
+
 template <int NT, bool GATED>
 static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cudaStream_t st) {
-  constexpr int SUB = stream_sub(NT), BUFS = 512 / (NT * SUB), SETS = NT / 128, kSlot = 136 * 4;
-  const int widest = p.T < kRows ? p.T : kRows;
-  p.quarters = (widest + 31) / 32;
+  p.quarters = quarters_of(p.T);
   p.x_bytes = p.quarters * 4096;
   p.n_tiles = (p.N + (GATED ? 128 : NT) - 1) / (GATED ? 128 : NT);
   const int sms = sm_count();
   KGE_REQUIRE(sms > 0, "kge_gemm_fp8: no CUDA device");
   const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles;
   p.splits = 0;                                            // grouped: by the number of tiles, on the device
-  if (!p.offsets) {
-    p.splits = 1;
-    if ((GATED || NT == 128) && 2 * tiles < sms)
-      for (int s = kMaxSplits; s > 1; --s)
-        if (tiles * s <= sms && p.KB >= 2 * s && tiles <= max_clusters(s)) { p.splits = s; break; }
-  }
+  if (!p.offsets) p.splits = GATED || NT == 128 ? plan_splits(tiles, NT, p.quarters, p.KB, sms) : 1;
   const bool cluster = p.splits > 1;
   if (cluster) {
     p.most = (16 + p.splits - 1) / p.splits;
@@ -1013,15 +1038,12 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
     for (int c = 0; c < p.splits; ++c)
       for (int g = p.first[c]; g < p.first[c + 1]; ++g) p.owner[g] = (uint8_t)c;
   }
-  const int sums = cluster ? p.splits * p.most * SETS * 2 * p.quarters * 32 * 16 : 0;
-  const int stage = SUB * (p.x_bytes + NT * 128 + kSlot);
-  p.stages = (kSmem - kOwn - 1024 - BUFS * SUB * kSlot - sums) / stage;
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  p.stages = stream_stages(NT, p.splits, p.quarters);
   KGE_REQUIRE(p.stages >= 2, "kge_gemm_fp8: internal: %d stages", p.stages);
   p.ahead = p.stages;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");
-  const int smem = p.stages * stage + BUFS * SUB * kSlot + sums + 1024;
+  const int smem = p.stages * stage_bytes_of(NT, p.quarters) + 512 / NT * kSlotBytes + sums_bytes(p.splits, NT / 128, p.quarters) + 1024;
   CUtensorMap mw, mx;
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
@@ -1103,7 +1125,11 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
               (long long)workspace_bytes_of(p.T));
   p.count = (unsigned int*)workspace;
   p.part = (float*)((uint8_t*)workspace + kCounters * 4);
-  const bool pairs = p.T / p.E > 96;
+  const int sms = sm_count();
+  KGE_REQUIRE(sms > 1, "%s: no CUDA device", name);
+  // Groups: by their mean size.  64 of 2048 x 1408, us by pairs and by single CTAs: 96 rows each 59.3 and 59.7, 192 71.5 and 85.9; 16 of 2048 x 2048: 128 25.7
+  // and 30.8, 256 33.5 and 44.2.
+  const bool pairs = p.offsets ? p.T / p.E > 96 : use_pairs(p.T, p.N, p.KB, gated, sms);
 #ifndef KGE_HALF
   if (gated) return pairs ? launch_pairs<true>(p, x, w, K, st) : launch_stream<256, true>(p, x, w, K, st);
 #endif
@@ -1111,7 +1137,7 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
   // Tiles of 256 columns where they are enough for whole tiles a CTA: 64 tokens, us with 128 and 256, 28672 x 4096 27.5 and 25.9, 128256 x 4096 96.5 and 97.4,
   // 128 experts of 2048 x 768, 512 rows, 39.2 and 38.6.  Cut along K they have less to show (4096 x 4096 8.8 and 10.3).
   const int64_t groups = p.offsets && p.T < p.E ? p.T : p.E, wide = ((int64_t)(p.T / p.E + kRows - 1) / kRows + (p.T < p.E)) * groups * ((p.N + 255) / 256);
-  return 2 * wide >= sm_count() ? launch_stream<256, false>(p, x, w, K, st) : launch_stream<128, false>(p, x, w, K, st);
+  return 2 * wide >= sms ? launch_stream<256, false>(p, x, w, K, st) : launch_stream<128, false>(p, x, w, K, st);
 }
 
 }  // namespace KGE_ELT_NS
