@@ -290,3 +290,268 @@ def test_offsets_that_are_none_stay_within_the_rows(kge, L, off):
          work, work.numel())
     torch.cuda.synchronize()
     assert (whole[:100] == 7).all() and (whole[100 + T:] == 7).all() and (work[:1024] == 0).all()
+
+
+TILES = [  # T, N, K: whole tiles of 256 columns, one and several a CTA; tiles of 128 columns cut along K over 2 to 8 CTAs; pairs, whole and ragged
+    (5, 19000, 272), (3, 40000, 144), (130, 19000, 144), (40, 30000, 1424), (1, 6016, 2048), (64, 4096, 528), (9, 2048, 1040), (33, 384, 2064), (97, 256, 4096), (128, 128, 4112),
+    (65, 1536, 1296), (120, 9500, 400), (1030, 4104, 272), (2050, 2056, 528), (3000, 600, 144), (520, 8200, 400)]
+
+
+@pytest.mark.parametrize("T,N,K", TILES)
+def test_product_in_every_kind_of_tile(kge, L, T, N, K):
+    g = torch.Generator().manual_seed(T + N)
+    x, xs, xn = quantised(g, T, K, 1)
+    w, ws, wn = quantised(g, N, K, 128)
+    y = torch.full((T + 1, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    work = workspace(L, T)
+    call(kge, "kge_gemm_fp8", y, x.cuda(), xs.t().contiguous().cuda(), T, w.cuda(), ws.cuda(), None, T, N, K, work, work.numel())
+    xn, wn = xn.cuda(), wn.cuda()
+    z, a = (xn @ wn.t()).cpu(), (xn.abs() @ wn.abs().t()).cpu()
+    held(y[:T].cpu(), z, a, K, fo.half_step(torch.bfloat16))
+    assert (y[T] == 7).all() and (work[:1024] == 0).all()
+
+
+@pytest.mark.parametrize("K", [128, 400])
+def test_every_number_of_rows_and_columns(kge, L, K):
+    """1 to 140 rows of 72 columns and 1 to 140 columns of 3 rows: sentinels around the result stay."""
+    g = torch.Generator().manual_seed(K)
+    x, xs, xn = quantised(g, 140, K, 1)
+    w, ws, wn = quantised(g, 140, K, 128)
+    xd, xsd, wd, wsd = x.cuda(), xs.t().contiguous().cuda(), w.cuda(), ws.cuda()
+    z, a = xn @ wn.t(), xn.abs() @ wn.abs().t()
+    work = workspace(L, 140)
+    for T, N in [(t, 72) for t in range(1, 141)] + [(3, n) for n in range(1, 141)]:
+        y = torch.full((T * N + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+        call(kge, "kge_gemm_fp8", y[32:], xd, xsd, 140, wd, wsd, None, T, N, K, work, work.numel())
+        got = y.cpu()
+        assert (got[:32] == 7).all() and (got[32 + T * N:] == 7).all(), (T, N)
+        held(got[32:32 + T * N].view(T, N), z[:T, :N], a[:T, :N], K, fo.half_step(torch.bfloat16))
+
+
+def test_what_is_no_number_stays_in_its_row_or_columns(kge, L):
+    """A row's NaN scale, NaN code or infinite scale makes its own results NaN or infinite; a block of weights its 128 columns; nothing else changes."""
+    T, N, K, g = 40, 400, 528, torch.Generator().manual_seed(5)
+    x, xs, _ = quantised(g, T, K, 1)
+    w, ws, _ = quantised(g, N, K, 128)
+    work = workspace(L, T)
+
+    def run(x, xs, w, ws):
+        y = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+        call(kge, "kge_gemm_fp8", y, x.cuda(), xs.t().contiguous().cuda(), T, w.cuda(), ws.cuda(), None, T, N, K, work, work.numel())
+        return y.cpu()
+    want = run(x, xs, w, ws)
+    xs2, ws2, x2 = xs.clone(), ws.clone(), x.clone()
+    xs2[3, 1], xs2[7, 0], ws2[1, 2] = math.nan, math.inf, math.nan
+    x2.view(torch.uint8)[33, 17] = 0x7f
+    got = run(x2, xs2, w, ws2)
+    bad = torch.zeros(T, N, dtype=torch.bool)
+    bad[[3, 33]], bad[:, 128:256] = True, True
+    assert got[bad].isnan().all() and not got[7].isfinite().any()
+    bad[7] = True
+    assert torch.equal(got[~bad], want[~bad])
+    # and through the gated pair: the row's blocks are NaN, with codes of zero
+    wg, wgs, _ = quantised(g, 512, K, 128)
+    codes, scales = torch.full((T, 256), 0x55, dtype=torch.uint8, device="cuda"), torch.zeros(2, T, device="cuda")
+    call(kge, "kge_gemm_fp8_silu_gate", codes, scales, T, x2.cuda(), xs2.t().contiguous().cuda(), T, wg.cuda(), wgs.cuda(), T, 256, K, work, work.numel())
+    rows = torch.zeros(T, dtype=torch.bool)
+    rows[[3, 7, 33]] = True
+    assert scales.cpu()[:, rows].isnan().all() and (codes.cpu()[rows] == 0).all() and scales.cpu()[:, ~rows].isfinite().all()
+
+
+def test_zero_and_extreme_scales(kge, L):
+    """Rows of zeros, scales of 2^-126 and 2^120: sums neither vanish nor overflow before they have to."""
+    T, N, K, g = 8, 136, 256, torch.Generator().manual_seed(6)
+    x, xs, _ = quantised(g, T, K, 1)
+    w, ws, _ = quantised(g, N, K, 128)
+    xs[0], xs[1], xs[2] = 2.0 ** -126, 2.0 ** 100, 0.0
+    x.view(torch.uint8)[3] = 0
+    ws = ws * 2.0 ** 10
+    y = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+    work = workspace(L, T)
+    call(kge, "kge_gemm_fp8", y, x.cuda(), xs.t().contiguous().cuda(), T, w.cuda(), ws.cuda(), None, T, N, K, work, work.numel())
+    xn, wn = fo.numbers(x.double(), xs, 1), fo.numbers(w.double(), ws, 128)
+    held(y.cpu(), xn @ wn.t(), xn.abs() @ wn.abs().t() + 2.0 ** -126 * 448 * 448 * K, K, fo.half_step(torch.bfloat16))
+    assert (y[2:4] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------- as they are used together
+
+def experts64(x, wg, wd, chosen, share):
+    """A mixture in 64 bits over the quantised numbers, and what the result is held to (see below)."""
+    out, mag = torch.zeros(x.shape[0], wd[0].shape[0], dtype=torch.float64), torch.zeros(x.shape[0], dtype=torch.float64)
+    for t in range(x.shape[0]):
+        for k, e in enumerate(chosen[t].tolist()):
+            h = fo.silu_gate((x[t] @ wg[e].t())[None])[0]
+            out[t] += share[t, k] * (wd[e] @ h)
+            mag[t] += share[t, k] * wd[e].norm(dim=1).max() * h.norm()
+    return out, mag
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tokens,E,top,d,f", [(1, 4, 2, 256, 128), (9, 16, 4, 512, 256), (200, 8, 2, 384, 256), (900, 4, 2, 256, 384)])
+def test_a_mixture_of_experts(kge, L, dtype, tokens, E, top, d, f):
+    """Weights quantised, tokens gathered by expert and quantised, gate and up, down: one stream, nothing waits for the host.  Against the experts over the
+    numbers that the codes stand for.  Between the products h has 8 bits: each number off by 2^-4 of it at most, in the mean square 2^-4 / sqrt(3) of it and
+    2^-5 where significands are spread; a result, a sum of f of them, is off by the norm of the weights' row times that of h times 2^-5 / sqrt(3) or so in
+    the mean square, held to 2^-4 of the two norms (codes below the normal range, 2^-10 of a block's scale, are less)."""
+    dt, g = fo.DT[dtype], torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, d, generator=g).to(dt)
+    wg, wd = (torch.randn(E, 2 * f, d, generator=g) * d ** -0.5).to(dt), (torch.randn(E, d, f, generator=g) * f ** -0.5).to(dt)
+    chosen = torch.stack([torch.randperm(E, generator=g)[:top] for _ in range(tokens)])
+    share = torch.softmax(torch.randn(tokens, top, generator=g), -1).double()
+    pair = chosen.flatten().sort(stable=True)
+    T = tokens * top
+    rows, off = (pair.indices // top).int().cuda(), torch.cat([torch.zeros(1, dtype=torch.long), torch.bincount(pair.values, minlength=E).cumsum(0)]).int().cuda()
+    u8, f32 = dict(dtype=torch.uint8, device="cuda"), dict(device="cuda")
+    cg, sg, cd, sd = torch.empty(E, 2 * f, d, **u8), torch.empty(E, -(-2 * f // 128), -(-d // 128), **f32), torch.empty(E, d, f, **u8), torch.empty(E, -(-d // 128), f // 128, **f32)
+    cx, sx, ch, sh = torch.empty(T, d, **u8), torch.empty(-(-d // 128), T, **f32), torch.empty(T, f, **u8), torch.empty(f // 128, T, **f32)
+    y, work = torch.empty(T, d, dtype=dt, device="cuda"), workspace(L, T)
+    xd, wgd, wdd = x.cuda(), wg.cuda(), wd.cuda()
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    call(kge, name("kge_fp8_quant_weight", dt), cg, sg, wgd, E, 2 * f, d, stream=st)
+    call(kge, name("kge_fp8_quant_weight", dt), cd, sd, wdd, E, d, f, stream=st)
+    call(kge, name("kge_fp8_quant", dt), cx, sx, T, xd, d, rows, T, d, stream=st)
+    call(kge, "kge_gemm_fp8_grouped_silu_gate", ch, sh, T, cx, sx, T, cg, sg, off, E, T, f, d, work, work.numel(), stream=st)
+    call(kge, name("kge_gemm_fp8_grouped", dt), y, ch, sh, T, cd, sd, off, E, T, d, f, work, work.numel(), stream=st)
+    st.synchronize()
+    pairs = torch.empty(T, d, dtype=torch.float64)
+    pairs[pair.indices] = y.double().cpu()
+    got = (pairs.view(tokens, top, d) * share[..., None]).sum(1)
+    num = lambda c, s, r: fo.numbers(c.cpu().view(fo.E4M3).double(), s.cpu(), r)
+    xn, xscale = fo.quantise(x, 1)
+    want, mag = experts64(fo.numbers(xn, xscale.float(), 1), [num(cg[e], sg[e], 128) for e in range(E)], [num(cd[e], sd[e], 128) for e in range(E)], chosen, share)
+    assert ((got - want).abs() <= 2.0 ** -4 * mag[:, None]).all()
+    assert (got - want).norm() <= (2.0 ** -4 / math.sqrt(3) + fo.half_step(dt)) * want.norm()
+
+
+def test_a_captured_step_over_changing_groups(kge, L):
+    """Two graphs that share a workspace, replayed in turn with other rows, offsets and numbers of rows: each gives what calls of the time give."""
+    E, T, d, f, g = 6, 70, 256, 128, torch.Generator().manual_seed(11)
+    w, ws, _ = quantised(g, E * 2 * f, d, 128)
+    w2, ws2, _ = quantised(g, E * d, f, 128)
+    w, ws, w2, ws2 = w.cuda(), ws.cuda(), w2.cuda(), ws2.cuda()
+    x, off = torch.zeros(T, d, dtype=torch.bfloat16, device="cuda"), torch.zeros(E + 1, **I32)
+    u8, f32 = dict(dtype=torch.uint8, device="cuda"), dict(device="cuda")
+    work = workspace(L, T)
+
+    def buffers():
+        return (torch.zeros(T, d, **u8), torch.zeros(2, T, **f32), torch.zeros(T, f, **u8), torch.zeros(1, T, **f32), torch.zeros(T, d, dtype=torch.bfloat16, device="cuda"))
+
+    def step(b):
+        cx, sx, ch, sh, y = b
+        call(kge, "kge_fp8_quant", cx, sx, T, x, d, None, T, d)
+        call(kge, "kge_gemm_fp8_grouped_silu_gate", ch, sh, T, cx, sx, T, w, ws, off, E, T, f, d, work, work.numel())
+        call(kge, "kge_gemm_fp8_grouped", y, ch, sh, T, w2, ws2, off, E, T, d, f, work, work.numel())
+
+    def dense(b):
+        cx, sx, ch, sh, y = b
+        call(kge, "kge_gemm_fp8_silu_gate", ch, sh, T, cx, sx, T, w, ws, T, f, d, work, work.numel())
+        call(kge, "kge_gemm_fp8", y, ch, sh, T, w2, ws2, None, T, d, f, work, work.numel())
+    eager, a, b = buffers(), buffers(), buffers()
+    step(eager), dense(eager)
+    torch.cuda.synchronize()
+    graphs = []
+    for fn, buf in ((step, a), (dense, b)):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            fn(buf)
+        graphs.append(gr)
+    for turn in range(6):
+        x.copy_(torch.randn(T, d, generator=g) * 10 ** (turn - 2))
+        sizes = torch.randint(0, 12, (E,), generator=g)
+        sizes[turn] = 0
+        off.copy_(torch.cat([torch.zeros(1, dtype=torch.long), sizes.cumsum(0)]))
+        for t in (*eager, *a, *b):
+            t.zero_()
+        b[0].copy_(a[0])
+        graphs[0].replay()
+        step(eager)
+        torch.cuda.synchronize()
+        for s, t in zip(a, eager):
+            assert torch.equal(s.view(torch.uint8), t.view(torch.uint8)), turn
+        b[0].copy_(a[0]), b[1].copy_(a[1])
+        graphs[1].replay()
+        eager2 = [a[0], a[1], *(torch.zeros_like(t) for t in a[2:])]
+        dense(eager2)
+        torch.cuda.synchronize()
+        for s, t in zip(b, eager2):
+            assert torch.equal(s.view(torch.uint8), t.view(torch.uint8)), turn
+    assert (work[:1024] == 0).all()
+
+
+def test_two_streams_at_once(kge, L):
+    """Calls on two streams with a workspace each, many times: the bits that each gives alone."""
+    g = torch.Generator().manual_seed(12)
+    jobs = []
+    for T, N, K in ((3, 640, 2064), (300, 776, 528)):
+        x, xs, _ = quantised(g, T, K, 1)
+        w, ws, _ = quantised(g, N, K, 128)
+        y = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+        work = workspace(L, T)
+        off = torch.tensor([0, T // 3, T // 3, T], **I32)
+        args = x.cuda(), xs.t().contiguous().cuda(), T, torch.stack([w] * 3).cuda(), torch.stack([ws] * 3).cuda(), off, 3, T, N, K, work, work.numel()
+        call(kge, "kge_gemm_fp8_grouped", y, *args)
+        torch.cuda.synchronize()
+        jobs.append((torch.cuda.Stream(), args, y.clone(), [torch.zeros_like(y) for _ in range(20)]))
+    for i in range(20):
+        for st, args, _, ys in jobs:
+            call(kge, "kge_gemm_fp8_grouped", ys[i], *args, stream=st)
+    torch.cuda.synchronize()
+    for _, _, want, ys in jobs:
+        assert all(torch.equal(y, want) for y in ys)
+
+
+def test_a_slice_of_a_batch(kge, L):
+    """Rows t0 .. of a quantised batch: codes and scales from there on, with the batch's stride."""
+    T, N, K, g = 50, 200, 272, torch.Generator().manual_seed(13)
+    x, xs, _ = quantised(g, T, K, 1)
+    w, ws, _ = quantised(g, N, K, 128)
+    xd, xsd, wd, wsd, work = x.cuda(), xs.t().contiguous().cuda(), w.cuda(), ws.cuda(), workspace(L, T)
+    whole = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+    call(kge, "kge_gemm_fp8", whole, xd, xsd, T, wd, wsd, None, T, N, K, work, work.numel())
+    for t0, n in ((1, 3), (17, 33), (49, 1)):
+        y = torch.zeros(n, N, dtype=torch.bfloat16, device="cuda")
+        call(kge, "kge_gemm_fp8", y, xd[t0:], xsd.flatten()[t0:], T, wd, wsd, None, n, N, K, work, work.numel())
+        assert torch.equal(y, whole[t0:t0 + n])
+
+
+def test_more_than_32_bits_of_elements(kge, L):
+    """A result of 2^31 numbers and more, weights of 2^31 bytes and more, rows beyond 2^31 numbers: the last of each are right."""
+    g = torch.Generator().manual_seed(14)
+    T, N, K = 66000, 33024, 128
+    x, xs, xn = quantised(g, 512, K, 1)
+    w, ws, wn = quantised(g, 256, K, 128)
+    xd, xsd = x.view(torch.uint8).cuda().repeat(T // 512 + 1, 1)[:T].contiguous(), xs.t().contiguous().cuda().repeat(1, T // 512 + 1)[:, :T].contiguous()
+    wd, wsd = w.view(torch.uint8).cuda().repeat(N // 256, 1).contiguous(), ws.cuda().repeat(N // 256, 1).contiguous()
+    y, work = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda"), workspace(L, T)
+    call(kge, "kge_gemm_fp8", y, xd, xsd, T, wd, wsd, None, T, N, K, work, work.numel())
+    z, a = xn @ wn.t(), xn.abs() @ wn.abs().t()
+    at = torch.arange(T - 300, T) % 512
+    for n in (0, N - 256):
+        held(y[T - 300:, n:n + 256].cpu(), z[at], a[at], K, fo.half_step(torch.bfloat16))
+    del y, wd
+    E = 2                                                    # the second group's matrix begins behind 2^31 bytes
+    K2 = 65664
+    w2 = torch.zeros(E, 33024, K2, dtype=torch.uint8, device="cuda")
+    w2[1, -256:, :128] = w.view(torch.uint8).cuda()
+    s2 = torch.ones(E, 258, K2 // 128, device="cuda")
+    s2[1, -2:, 0] = ws.cuda()[:, 0]
+    x2 = torch.zeros(300, K2, dtype=torch.uint8, device="cuda")
+    x2[:, :128] = xd[:300]
+    xs2 = torch.ones(K2 // 128, 300, device="cuda")
+    xs2[0] = xsd[0, :300]
+    y2 = torch.zeros(300, 33024, dtype=torch.bfloat16, device="cuda")
+    call(kge, "kge_gemm_fp8_grouped", y2, x2, xs2, 300, w2, s2, torch.tensor([0, 150, 300], **I32), E, 300, 33024, K2, work, work.numel())
+    held(y2[150:, -256:].cpu(), z[150:300], a[150:300], K2, fo.half_step(torch.bfloat16))
+    assert (y2[:150] == 0).all() and (y2[150:, :-256] == 0).all()
+    del w2
+    # rows quantised from beyond 2^31 numbers
+    K3, T3 = 131072, 16600
+    big = torch.zeros(T3, K3, dtype=torch.bfloat16, device="cuda")
+    big[-1] = torch.randn(K3, generator=g).to(torch.bfloat16)
+    codes, scales = torch.zeros(T3, K3, dtype=torch.uint8, device="cuda"), torch.zeros(K3 // 128, T3, device="cuda")
+    call(kge, "kge_fp8_quant", codes, scales, T3, big, K3, None, T3, K3)
+    code, scale = fo.quantise(big[-1:].cpu(), 1)
+    assert torch.equal(codes[-1].cpu().view(fo.E4M3).double(), code[0]) and torch.equal(scales[:, -1].cpu(), scale[0].float())
+    assert not codes[:-1].any()
