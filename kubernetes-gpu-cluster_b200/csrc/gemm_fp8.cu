@@ -29,7 +29,7 @@ constexpr int kThreads = 128 + 32 * kSumWarps;    // producer, MMA, tensor memor
 constexpr int kSumRegs = 216, kOtherRegs = 72;    // registers of those and of the others: 256 x 216 + 128 x 72 = 384 x 168, what the block is launched with
 constexpr int kCounters = 256;                    // arrival counters at the head of the workspace
 constexpr int kMaxCtas = 160;
-constexpr int kMaxGroups = 1024;
+constexpr int kMaxGroups = 1024, kNearGroups = 256;      // groups; those whose rows are kept in shared memory
 constexpr int kMaxStages = 16;
 constexpr int kSlotBytes = 136 * 4;               // factors of a block of K: of 128 rows, of up to two sets of columns
 constexpr int kMaxSplits = 8;                     // CTAs of a cluster
@@ -111,18 +111,26 @@ template <int REGS> __device__ __forceinline__ void regs_up() { asm volatile("se
 template <int REGS> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
 __device__ __forceinline__ void sums_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Rows of group e, whatever the table holds.
-__device__ __forceinline__ void group_rows(const Fp8Params& p, int e, int& r0, int& r1) {
-  if (!p.offsets) { r0 = 0; r1 = p.T; return; }
-  r0 = min(max(p.offsets[e], 0), p.T);
-  r1 = max(r0, min(p.offsets[e + 1], p.T));
+// Which rows and tiles the groups have, in shared memory: starts[e] = tiles of the groups before e, near[e] = {first row, behind the last}.
+template <int GROUPS>
+struct Groups {
+  int starts[GROUPS + 1];
+  int2 near[GROUPS < kNearGroups ? GROUPS : kNearGroups];
+};
+// Rows of group e, whatever the table of offsets holds.
+__device__ __forceinline__ int2 rows_of(const Fp8Params& p, int e) {
+  if (!p.offsets) return make_int2(0, p.T);
+  const int r0 = min(max(p.offsets[e], 0), p.T);
+  return make_int2(r0, max(r0, min(p.offsets[e + 1], p.T)));
 }
-// starts[e] = tiles of the groups before e.  By all threads of the CTA.
-__device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, int* starts) {
+// Fills them, by all threads of the CTA.
+template <int GROUPS>
+__device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, Groups<GROUPS>& groups) {
+  int* starts = groups.starts;
   for (int e = threadIdx.x; e < p.E; e += kThreads) {
-    int r0, r1;
-    group_rows(p, e, r0, r1);
-    starts[e] = (r1 - r0 + tile_rows - 1) / tile_rows * p.n_tiles;
+    const int2 r = rows_of(p, e);
+    starts[e] = (r.y - r.x + tile_rows - 1) / tile_rows * p.n_tiles;
+    if (e < kNearGroups) groups.near[e] = r;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -144,23 +152,29 @@ __device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, i
 struct Tile { int e, n, row, rows; };
 // From a tile's number; the group is looked for from `e` on (numbers come in rising order).  Tiles of a group run over BAND token tiles (0: all), then
 // the next column tile: neighbours share weights, and a band's tokens stay in the L2 meanwhile.
-template <int TILE_ROWS, int BAND>
-__device__ __forceinline__ Tile find_tile(const Fp8Params& p, const int* starts, int tile, int& e) {
-  while (e + 1 < p.E && tile >= starts[e + 1]) ++e;
-  int r0, r1;
-  group_rows(p, e, r0, r1);
-  const int m_tiles = (r1 - r0 + TILE_ROWS - 1) / TILE_ROWS, local = tile - starts[e], band = BAND ? BAND : m_tiles;
-  const int g = local / (band * p.n_tiles), first = g * band, width = min(band, m_tiles - first), in = local - g * band * p.n_tiles;
+template <int TILE_ROWS, int BAND, int GROUPS>
+__device__ __forceinline__ Tile find_tile(const Fp8Params& p, const Groups<GROUPS>& groups, int tile, int& e) {
+  while (e + 1 < p.E && tile >= groups.starts[e + 1]) ++e;
+  const int2 r = e < (GROUPS < kNearGroups ? GROUPS : kNearGroups) ? groups.near[e] : rows_of(p, e);
+  const int m_tiles = (r.y - r.x + TILE_ROWS - 1) / TILE_ROWS, local = tile - groups.starts[e];
   Tile t;
   t.e = e;
-  t.n = in / width;
-  t.row = r0 + (first + in - t.n * width) * TILE_ROWS;
-  t.rows = min(TILE_ROWS, r1 - t.row);
+  int m = 0;
+  if (m_tiles == 1) {
+    t.n = local;
+  } else {
+    const int band = BAND ? BAND : m_tiles, g = BAND ? local / (band * p.n_tiles) : 0, first = g * band, width = min(band, m_tiles - first), in = local - g * band * p.n_tiles;
+    t.n = in / width;
+    m = first + in - t.n * width;
+  }
+  t.row = r.x + m * TILE_ROWS;
+  t.rows = min(TILE_ROWS, r.y - t.row);
   return t;
 }
-__device__ __forceinline__ int first_group(const Fp8Params& p, const int* starts, int tile) {
+template <int GROUPS>
+__device__ __forceinline__ int first_group(const Fp8Params& p, const Groups<GROUPS>& groups, int tile) {
   int lo = 0, hi = p.E - 1;
-  while (lo < hi) { const int mid = (lo + hi + 1) / 2; if (starts[mid] <= tile) lo = mid; else hi = mid - 1; }
+  while (lo < hi) { const int mid = (lo + hi + 1) / 2; if (groups.starts[mid] <= tile) lo = mid; else hi = mid - 1; }
   return lo;
 }
 
@@ -270,26 +284,20 @@ __device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, 
   bf16* dst = p.y + (int64_t)row * p.N + n0;
   if (n0 + 64 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
 #pragma unroll
-    for (int c = 0; c < 64; c += 8) {
-      uint32_t u[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float a, b;
-        s.at(c0 + c + 2 * i, a, b);
-        if (p.bias) { a += bf2f(p.bias[n0 + c + 2 * i]); b += bf2f(p.bias[n0 + c + 2 * i + 1]); }
-        u[i] = pack_bf2(a, b);
-      }
-      *reinterpret_cast<uint4*>(dst + c) = make_uint4(u[0], u[1], u[2], u[3]);
-    }
+    for (int c = c0; c < c0 + 64; c += 8)
+      *reinterpret_cast<uint4*>(dst + c - c0) = make_uint4(pack_bf2(s.v[c], s.v[c + 1]), pack_bf2(s.v[c + 2], s.v[c + 3]), pack_bf2(s.v[c + 4], s.v[c + 5]), pack_bf2(s.v[c + 6], s.v[c + 7]));
   } else {
 #pragma unroll
-    for (int c = 0; c < 64; c += 2) {
-      float a, b;
-      s.at(c0 + c, a, b);
-      if (n0 + c < p.N) dst[c] = f2bf(p.bias ? a + bf2f(p.bias[n0 + c]) : a);
-      if (n0 + c + 1 < p.N) dst[c + 1] = f2bf(p.bias ? b + bf2f(p.bias[n0 + c + 1]) : b);
-    }
+    for (int c = 0; c < 64; ++c)
+      if (n0 + c < p.N) dst[c] = f2bf(s.v[c0 + c]);
   }
+}
+// The bias of 64 columns from n0 on, to the sums from c0 on.
+template <int C>
+__device__ __forceinline__ void add_bias(const Fp8Params& p, Sums<C>& s, int c0, int n0) {
+#pragma unroll
+  for (int c = 0; c < 64; ++c)
+    if (n0 + c < p.N) s.v[c0 + c] += bf2f(p.bias[n0 + c]);
 }
 
 // A warp's 32 rows (from `row` on, `rows` of them there) of C columns, 32 at a time through 2 KB of its own in shared memory: rows of 64 bytes, whose
@@ -309,14 +317,7 @@ __device__ __forceinline__ void store_rows(const Fp8Params& p, const Sums<C>& s,
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = c0 + k * 8 + 2 * i;
-        float a, b;
-        s.at(c, a, b);
-        if (p.bias) {
-          const int at = n0 + c;
-          if (at < p.N) a += bf2f(p.bias[at]);
-          if (at + 1 < p.N) b += bf2f(p.bias[at + 1]);
-        }
-        u[i] = pack_bf2(a, b);
+        u[i] = pack_bf2(s.v[c], s.v[c + 1]);
       }
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(put + ((k ^ ((lane >> 1) & 3)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
     }
@@ -416,7 +417,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   __shared__ uint32_t tmem_slot;
   __shared__ int last_flag;
   __shared__ uint32_t tops[(CLUSTER ? 1 + kMaxSplits : 2) * 128];
-  __shared__ int starts[CLUSTER ? 2 : kMaxGroups + 1];
+  __shared__ Groups<CLUSTER ? 1 : kMaxGroups> groups;
   const int stages = p.stages;
   const uint32_t block_bytes = (uint32_t)p.x_bytes + NT * 128, stage_bytes = SUB * block_bytes;
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
@@ -440,7 +441,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (CLUSTER && GATED && threadIdx.x < 128) tops[threadIdx.x] = 0;
-  if ((CLUSTER || !p.offsets) && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
+  if ((CLUSTER || !p.offsets) && threadIdx.x == 0) { groups.starts[0] = 0; groups.near[0] = make_int2(0, p.T); groups.starts[1] = (p.T + kRows - 1) / kRows * p.n_tiles; }
   fence_before();
   __syncthreads();
   fence_after();
@@ -449,11 +450,11 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   if (CLUSTER) cluster_arrive_relaxed();
   if (!CLUSTER && p.offsets) {                      // which tiles there are is the kernel before's output
     pdl_wait();
-    count_tiles(p, kRows, starts);
+    count_tiles(p, kRows, groups);
   }
   const int KB = p.KB;
-  const Work work = work_of(starts[p.E], KB, p.splits, (int)blockIdx.x, (int)gridDim.x);
-  const int e_first = work.tile0 < work.tile1 ? first_group(p, starts, work.tile0) : 0;
+  const Work work = work_of(groups.starts[p.E], KB, p.splits, (int)blockIdx.x, (int)gridDim.x);
+  const int e_first = work.tile0 < work.tile1 ? first_group(p, groups, work.tile0) : 0;
   // xs of the rows and ws of the columns, block of K by block of K, in a ring.  A slot is free again when its block is added up.  The block `stages` further
   // is then at the earliest on its way (its stage was freed by an MMA that began after the sums BUFS blocks before had been read).
   float* factors = reinterpret_cast<float*>(smem + stages * stage_bytes);
@@ -482,7 +483,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       // What the weights are is known before the kernel before has ended: the first tile's first blocks.
       int ahead = 0;
       if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
-        const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
+        const Tile t = find_tile<kRows, 0>(p, groups, work.tile0, e);
         for (int kb = work.kb0; ahead < p.ahead && kb < work.kb1; kb += SUB, ++ahead) {
           const int n = min(SUB, work.kb1 - kb);
           bar_expect(full(ahead), bytes_of(t, n));
@@ -491,7 +492,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       }
       pdl_wait();
       for (int tile = work.tile0; tile < work.tile1; ++tile) {
-        const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
+        const Tile t = find_tile<kRows, 0>(p, groups, tile, e);
         for (int kb = work.kb0; kb < work.kb1; kb += SUB) {
           const int n = min(SUB, work.kb1 - kb);
           if (ahead > 0) {
@@ -550,14 +551,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     auto to = [&](int s, int i) { return s_addr(factors + s * SLOT + i); };
     int early = 0;
     if ((CLUSTER || !p.offsets) && work.tile0 < work.tile1) {
-      const Tile t = find_tile<kRows, 0>(p, starts, work.tile0, e);
+      const Tile t = find_tile<kRows, 0>(p, groups, work.tile0, e);
       early = min(p.ahead * SUB, work.kb1 - work.kb0);
       for (int i = 0; i < early; ++i)
         if (lane < SETS) copy4(to(i, 128 + lane), column(t, work.kb0 + i), true);
     }
     pdl_wait();
     for (int tile = work.tile0; tile < work.tile1; ++tile) {
-      const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
+      const Tile t = find_tile<kRows, 0>(p, groups, tile, e);
       const float* xs = p.xs + work.kb0 * p.xs_stride + t.row + lane;
       const float* ws = column(t, work.kb0);
       for (int kb = work.kb0; kb < work.kb1; kb += SUB) {
@@ -590,7 +591,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     int buf = 0, slot = 0, e = e_first;
     uint32_t buf_phase = 0;
     for (int tile = work.tile0; tile < work.tile1; ++tile) {
-      const Tile t = find_tile<kRows, 0>(p, starts, tile, e);
+      const Tile t = find_tile<kRows, 0>(p, groups, tile, e);
       const bool some = q * 32 < t.rows, there = lane128 < t.rows;
       const int row = t.row + lane128, n0 = t.n * NT + part * 64;
       Sums<C> s;
@@ -749,6 +750,9 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
           store_gated(p, s, row, there, t.n, tops, part, lane128);
         } else if (there) {
 #pragma unroll
+          for (int h = 0; h < C / 64; ++h)
+            if (p.bias) add_bias<C>(p, s, h * 64, n0 + h * 128);
+#pragma unroll
           for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
         }
       }
@@ -780,7 +784,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t tops[256];
   __shared__ int4 tiles[16];                        // n, row, rows of the tiles under way: at most one a block of K of the rings, and the last one
-  __shared__ int starts[kMaxGroups + 1];
+  __shared__ Groups<kMaxGroups> groups;
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
@@ -801,7 +805,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&tmem_slot)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
-  if (!p.offsets && threadIdx.x == 0) { starts[0] = 0; starts[1] = (p.T + 2 * kRows - 1) / (2 * kRows) * p.n_tiles; }
+  if (!p.offsets && threadIdx.x == 0) { groups.starts[0] = 0; groups.near[0] = make_int2(0, p.T); groups.starts[1] = (p.T + 2 * kRows - 1) / (2 * kRows) * p.n_tiles; }
   fence_before();
   __syncthreads();
   fence_after();
@@ -809,9 +813,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   pdl_launch_dependents();
   cluster_arrive(); cluster_wait();                 // the peer's barriers are there
   pdl_wait();
-  if (p.offsets) count_tiles(p, 2 * kRows, starts);
-  const int KB = p.KB, total = starts[p.E], first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
-  const int e_first = first < total ? first_group(p, starts, first) : 0;
+  if (p.offsets) count_tiles(p, 2 * kRows, groups);
+  const int KB = p.KB, total = groups.starts[p.E], first = (int)blockIdx.x >> 1, step = (int)gridDim.x >> 1;
+  const int e_first = first < total ? first_group(p, groups, first) : 0;
   float* factors = reinterpret_cast<float*>(smem + STAGES * kStage + (GATED ? 0 : kSumWarps * 2048));
 
   if (warp == 0 || warp == 3) {
@@ -821,7 +825,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     uint32_t phase = 0;
     const uint32_t lead0 = mapa_u32(full(0), 0);
     for (int w = first; w < total; w += step) {
-      const Tile t = find_tile<2 * kRows, kPairBand>(p, starts, w, e);
+      const Tile t = find_tile<2 * kRows, kPairBand>(p, groups, w, e);
       const int64_t wb = (int64_t)t.e * p.w_blocks + (GATED ? t.n : t.n * 2);
       // 64 weight rows for the first 128 columns, 64 for the second: half of each block or, gated, the leader's of the gate and the other's of up
       const int wr = t.e * p.w_rows + (GATED ? t.n * 128 + rank * p.N : t.n * 256 + rank * 64), xr = t.row + rank * kRows;
@@ -921,6 +925,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         add_blocks<C, 0>(s, KB, wait, read);
       } else {
         for (int kb = 0; kb < KB; ++kb) { mbar_wait(tfull(2 * buf + part), buf_phase); read(); }
+      }
+      if (!GATED && p.bias) {
+        add_bias<C>(p, s, 0, n0);
+        add_bias<C>(p, s, 64, n0 + 64);
       }
       if constexpr (GATED) {
         store_gated(p, s, row, there, t.n, tops, part, lane128);
@@ -1029,7 +1037,6 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   p.x_bytes = p.quarters * 4096;
   p.n_tiles = (p.N + (GATED ? 128 : NT) - 1) / (GATED ? 128 : NT);
   const int sms = sm_count();
-  KGE_REQUIRE(sms > 0, "kge_gemm_fp8: no CUDA device");
   const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles;
   p.splits = 0;                                            // grouped: by the number of tiles, on the device
   if (!p.offsets) p.splits = GATED || NT == 128 ? plan_splits(tiles, NT, p.quarters, p.KB, sms) : 1;
@@ -1079,7 +1086,6 @@ static int launch_pairs(Fp8Params& p, const void* x, const void* w, int K, cudaS
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   prefer_max_shared(kern);
   const int sms = sm_count();
-  KGE_REQUIRE(sms > 1, "kge_gemm_fp8: no CUDA device");
   int64_t pairs = sms / 2;
   if (!p.offsets) {
     const int64_t tiles = (int64_t)((p.T + 2 * kRows - 1) / (2 * kRows)) * p.n_tiles;
@@ -1128,7 +1134,10 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
   p.count = (unsigned int*)workspace;
   p.part = (float*)((uint8_t*)workspace + kCounters * 4);
   const int sms = sm_count();
-  KGE_REQUIRE(sms > 1, "%s: no CUDA device", name);
+  if (sms < 2) {
+    set_error("%s: no CUDA device", name);
+    return -2;
+  }
   // Groups: by their mean size.  64 of 2048 x 1408, us by pairs and by single CTAs: 96 rows each 59.3 and 59.7, 192 71.5 and 85.9; 16 of 2048 x 2048: 128 25.7
   // and 30.8, 256 33.5 and 44.2.
   const bool pairs = p.offsets ? p.T / p.E > 96 : use_pairs(p.T, p.N, p.KB, gated, sms);
