@@ -30,7 +30,7 @@ __device__ __forceinline__ void scale_of(float m, float& scale, float& factor) {
   float q = m * c;
   q = fmaf(fmaf(-kMax, q, m), c, q);
   float inv;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(fmaxf(m, kMax * kLeast) * 0.0625f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaxf(m, kMax * kLeast) * 0.0625f));
   scale = fine ? fmaxf(q, kLeast) : __int_as_float(0x7fffffff);
   factor = fine ? inv * (kMax * 0.0625f) : 0.f;
 }

@@ -30,65 +30,120 @@ __device__ __forceinline__ uint2 codes8(uint4 v, float factor) {
   return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
 
-// Eight lanes have a block of a row, 16 numbers each, and go on to another 32 blocks a CTA further: the next block's numbers and the one after's row are
-// under way meanwhile.  Bound by instructions (13 a number), not by the bytes: 16384 rows of 2048 gathered from 2048 (43 MB, 6.6 us) 22.9 us, 8192 rows of
-// 4096 (101 MB, 15.5 us) 27.1; a block a thread and no more 24.9 and 30.8, two blocks at a time in 64 registers 24.3 and 28.6.
-__global__ void __launch_bounds__(256, 6)
-fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_stride, const bf16* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ rows,
-                 uint32_t units, int K, uint32_t blocks) {
+// (zeros where the factor is zero: a block with an infinity or NaN)
+__device__ __forceinline__ uint4 codes16(const uint4 (&v)[2], float factor) {
+  if (!(factor > 0.f)) return make_uint4(0, 0, 0, 0);
+  const uint2 lo = codes8(v[0], factor), hi = codes8(v[1], factor);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// Few rows: eight lanes have a block of a row, 16 numbers each.
+__global__ void __launch_bounds__(256)
+fp8_quant_few_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_stride, const bf16* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ rows,
+                     uint32_t units, int K, uint32_t blocks) {
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t step = gridDim.x * 32, step_t = step / blocks, step_b = step - step_t * blocks;
-  const int lane_k = (threadIdx.x & 7) * 16;
-  struct Place { uint32_t at, t, b; int row; };            // block number, row, block of the row; the row of x, below 0 for zeros
-  auto look = [&](Place& p) {
-    if (p.at < units) p.row = rows ? rows[p.t] : (int)p.t;
-  };
-  auto on = [&](const Place& p) {
-    Place n{p.at + step, p.t + step_t, p.b + step_b, -1};
-    if (n.b >= blocks) { n.b -= blocks; ++n.t; }
-    return n;
-  };
-  auto load = [&](const Place& p, uint4 (&v)[2]) {
-    v[0] = v[1] = make_uint4(0, 0, 0, 0);
-    const int k = p.b * fp8::kBlock + lane_k;
-    if (p.at < units && p.row >= 0 && k < K) {
-      const bf16* src = x + p.row * x_stride + k;
+  const uint32_t at = blockIdx.x * 32 + (threadIdx.x >> 3), t = at / blocks, b = at - t * blocks;
+  const int k = b * fp8::kBlock + (threadIdx.x & 7) * 16;
+  const bool there = at < units && k < K;
+  uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (there) {
+    const int r = rows ? rows[t] : (int)t;
+    if (r >= 0) {
+      const bf16* src = x + r * x_stride + k;
       v[0] = ld_nc_v4(src);
       v[1] = ld_nc_v4(src + 8);
     }
+  }
+  uint32_t m2 = max2(mag2(v[0]), mag2(v[1]));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) m2 = max2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+  if (!there) return;
+  float scale, factor;
+  fp8::scale_of(mag(m2), scale, factor);
+  *reinterpret_cast<uint4*>(codes + (int64_t)t * K + k) = codes16(v, factor);
+  if ((threadIdx.x & 7) == 0) scales[b * scales_stride + t] = scale;
+}
+
+// Many rows: a warp takes 512 columns of a row at a time, eight lanes a block as above, one piece after the other of an equal share of all, copied kAheadRows
+// pieces ahead into a ring of its own in shared memory; a lane reads back what it has copied itself, so nothing is waited for but the copies.  Bound by
+// instructions, 12 a number, at half to two thirds of what the schedulers issue: 8192 rows of 4096 (101 MB, 15.5 us) 22.1 us, 16384 rows of 2048 gathered
+// from 2048 (43 MB, 6.6 us) 19.1; with 16 warps 22.9 and 20.1; a block a thread 30.8 and 24.9; loads into registers one block ahead 27.1 and 22.9 (the use
+// of one waits for all that share its counter).
+constexpr int kRowWarps = 32, kAheadRows = 6, kPiece = 1024;
+__global__ void __launch_bounds__(kRowWarps * 32, 1)
+fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_stride, const bf16* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ rows,
+                 uint32_t pieces, int K, uint32_t per_row) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t warps = gridDim.x * kRowWarps, me = blockIdx.x * kRowWarps + warp, each = pieces / warps, more = pieces - each * warps;
+  const uint32_t first = each * me + min(me, more);
+  int n = (int)(each + (me < more));
+  if (n == 0) return;
+  const uint32_t t0 = first / per_row, last = (first + n - 1) / per_row;
+  const int k0 = (int)(first - t0 * per_row) * 512 + lane * 16;
+  uint8_t* mine = smem + warp * (kAheadRows * kPiece) + lane * 32;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine), to_end = to + kAheadRows * kPiece;
+  auto row_of = [&](uint32_t t) { return rows && t <= last ? rows[t] : (int)t; };
+  // the copies' way through the share: row, column, source; and the row after that, asked for a row ahead
+  uint32_t t = t0, slot_in = to;
+  int k = k0, r = row_of(t0), r_next = row_of(t0 + 1), left = n;
+  const bf16* src = x + r * x_stride + k;
+  auto copy = [&] {
+    if (left > 0) {
+      --left;
+      const bool there = r >= 0 && k < K;
+      const uint32_t size = there ? 16u : 0u;
+      const bf16* from = there ? src : x;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in), "l"(from), "r"(size) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in + 16), "l"(there ? from + 8 : x), "r"(size) : "memory");
+      k += 512;
+      src += 512;
+      if (k - lane * 16 >= K) {
+        ++t;
+        k = lane * 16;
+        r = r_next;
+        r_next = row_of(t + 1);
+        src = x + r * x_stride + k;
+      }
+      if ((slot_in += kPiece) == to_end) slot_in = to;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  Place now{blockIdx.x * 32 + (threadIdx.x >> 3), 0, 0, -1};
-  now.t = now.at / blocks;
-  now.b = now.at - now.t * blocks;
-  look(now);
-  Place next = on(now);
-  look(next);
-  uint4 v[2];
-  load(now, v);
-  while (__any_sync(0xffffffffu, now.at < units)) {
-    uint4 w[2];
-    load(next, w);
-    Place then = on(next);
-    look(then);
+#pragma unroll 1
+  for (int i = 0; i < kAheadRows; ++i) copy();
+  int at = k0, slot = 0;
+  const int64_t blocks_on = 4 * scales_stride, row_on = 1 - (int64_t)(per_row - 1) * blocks_on;      // from one piece's scales to the next's, to the next row's first
+  uint8_t* dst = codes + (int64_t)t0 * K + k0;
+  float* sc = scales + (int64_t)(k0 / 128) * scales_stride + t0;
+#pragma unroll 1
+  for (; n > 0; --n) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAheadRows - 1) : "memory");
+    const uint4 v[2] = {*reinterpret_cast<const uint4*>(mine + slot), *reinterpret_cast<const uint4*>(mine + slot + 16)};
+    copy();
+    if ((slot += kPiece) == kAheadRows * kPiece) slot = 0;
     uint32_t m2 = max2(mag2(v[0]), mag2(v[1]));
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) m2 = max2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
     float scale, factor;
     fp8::scale_of(mag(m2), scale, factor);
-    const int k = now.b * fp8::kBlock + lane_k;
-    if (now.at < units && k < K) {
-      uint4 c = make_uint4(0, 0, 0, 0);
-      if (factor > 0.f) {
-        const uint2 lo = codes8(v[0], factor), hi = codes8(v[1], factor);
-        c = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      }
-      *reinterpret_cast<uint4*>(codes + (int64_t)now.t * K + k) = c;
-      if ((threadIdx.x & 7) == 0) scales[now.b * scales_stride + now.t] = scale;
+    if (at < K) {
+      *reinterpret_cast<uint4*>(dst) = codes16(v, factor);
+      if ((lane & 7) == 0) *sc = scale;
     }
-    v[0] = w[0]; v[1] = w[1];
-    now = next; next = then;
+    at += 512;
+    dst += 512;
+    if (at - lane * 16 < K) {
+      sc += blocks_on;
+    } else {
+      dst += K - (at - lane * 16);
+      at = lane * 16;
+      sc += row_on;
+    }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // A CTA takes steps of 128 rows x 256 columns (two blocks), copied three steps ahead into shared memory: every access to memory is a whole 512-byte piece
@@ -176,9 +231,16 @@ extern "C" int KGE_API(kge_fp8_quant)(void* codes, float* scales, int scales_str
   const int blocks = (int)fp8::blocks(K);
   const int64_t units = (int64_t)T * blocks;
   KGE_REQUIRE(units < (1ll << 31) - 64 * 148 * 32, "kge_fp8_quant: %d rows of %d in one call", T, K);
-  const int64_t ctas = (units + 31) / 32, most = 148 * 6;
-  KGE_CUDA_OK(launch_pdl(fp8_quant_kernel, dim3((unsigned)(ctas < most ? ctas : most)), dim3(256), 0, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride,
-                         (const bf16*)x, (int64_t)x_stride, rows, (uint32_t)units, K, (uint32_t)blocks));
+  const int64_t per_row = (K + 511) / 512, pieces = T * per_row;
+  if (pieces < 2 * 148 * kRowWarps) {
+    KGE_CUDA_OK(launch_pdl(fp8_quant_few_kernel, dim3((unsigned)((units + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride,
+                           (const bf16*)x, (int64_t)x_stride, rows, (uint32_t)units, K, (uint32_t)blocks));
+    return 0;
+  }
+  const int smem = kRowWarps * kAheadRows * kPiece;
+  KGE_CUDA_OK(cudaFuncSetAttribute(fp8_quant_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  KGE_CUDA_OK(launch_pdl(fp8_quant_kernel, dim3(148), dim3(kRowWarps * 32), (size_t)smem, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride, (const bf16*)x,
+                         (int64_t)x_stride, rows, (uint32_t)pieces, K, (uint32_t)per_row));
   return 0;
 }
 

@@ -23,15 +23,13 @@ def quantise(x, rows):
     x = x.double()
     N, K = x.shape
     code, scale = torch.zeros_like(x), torch.empty(-(-N // rows), -(-K // 128), dtype=torch.float64)
-    for n in range(0, N, rows):
-        for k in range(0, K, 128):
-            part = x[n:n + rows, k:k + 128]
-            if torch.isfinite(part).all():
-                m = part.abs().max()
-                scale[n // rows, k // 128] = max(m.item() / 448, LEAST)
-                code[n:n + rows, k:k + 128] = nearest(448 * part / m) if m >= 448 * LEAST else nearest(part / LEAST)
-            else:
-                scale[n // rows, k // 128] = math.nan
+    for k in range(0, K, 128):
+        part = torch.nn.functional.pad(x[:, k:k + 128], (0, 0, 0, -N % rows)).unflatten(0, (-1, rows))
+        m = part.abs().amax((1, 2), keepdim=True)                          # (NaN where one is)
+        fine = torch.isfinite(m)
+        c = nearest(torch.where(fine, torch.where(m >= 448 * LEAST, 448 * part / m, part / LEAST), 0.0))
+        code[:, k:k + 128] = c.flatten(0, 1)[:N]
+        scale[:, k // 128] = torch.where(fine, torch.clamp(m / 448, min=LEAST), math.nan)[:, 0, 0]
     return code, scale
 
 

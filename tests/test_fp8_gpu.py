@@ -59,7 +59,7 @@ def quantised(g, T, K, rows):
 
 # ---------------------------------------------------------------------------------------------------------------- quantising
 
-QUANT = [("bf16", 1, 16), ("fp16", 1, 128), ("bf16", 3, 144), ("fp16", 33, 1424), ("bf16", 64, 4096), ("fp16", 200, 272), ("bf16", 7, 14336)]
+QUANT = [("bf16", 1, 16), ("fp16", 1, 128), ("bf16", 3, 144), ("fp16", 33, 1424), ("bf16", 64, 4096), ("fp16", 200, 272), ("bf16", 7, 14336), ("bf16", 9700, 528), ("fp16", 4800, 1040)]
 
 
 @pytest.mark.parametrize("dtype,T,K", QUANT)
