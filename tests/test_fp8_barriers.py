@@ -1,0 +1,294 @@
+"""The barrier protocols of the 8-bit products (csrc/gemm_fp8.cu), run on the CPU many times with their roles, copies and MMAs in random order.  Barriers know
+phases and parities alone, as the hardware's do; what lies in stages, factor slots and tensor memory is tracked by block: whoever reads finds the block that it
+is about, nothing is written that is still to be read, and nobody waits for ever."""
+import os
+import random
+import re
+
+import pytest
+
+SRC = open(os.path.join(os.path.dirname(__file__), "..", "kubernetes-gpu-cluster_b200", "csrc", "gemm_fp8.cu")).read()
+
+# every barrier operation of the roles, in the order of the source: what the programs below transcribe
+STREAM_OPS = [
+    "expect full(ahead), bytes_of(t, n)", "wait empty(stage), phase ^ 1", "expect full(stage), bytes_of(t, n)",
+    "wait full(stage), phase", "wait tempty(buf), buf_phase ^ 1", "test full(s1), p1", "test tempty(v1), w1 ^ 1", "commit tfull(buf)", "commit empty(stage)",
+    "wait empty(stage), phase ^ 1",
+    "arrive tempty(buf)", "wait tfull(buf), buf_phase", "wait tfull(buf), buf_phase"]
+PAIR_OPS = [
+    "wait empty(stage), phase ^ 1", "expect full(stage), 2 * kStage", "arrive lead",
+    "wait full(stage), phase", "wait tempty(2 * buf + h), buf_phase ^ 1", "test full(s1), p1", "test tempty(2 * v1 + h), w1 ^ 1", "commit tfull(2 * buf + h), 3",
+    "commit empty(stage), 3",
+    "wait tfull(2 * buf + part), buf_phase", "arrive lead_tempty + 16u * buf", "wait tfull(2 * buf + part), buf_phase", "wait tfull(2 * buf + part), buf_phase"]
+CALLS = {"mbar_wait": "wait", "mbar_test": "test", "bar_expect": "expect", "bar_arrive": "arrive", "bar_arrive_at": "arrive", "commit": "commit", "commit2": "commit"}
+
+
+def operations(kernel, begin):
+    body = SRC[SRC.index(kernel + "(const __grid"):]
+    body = body[body.index(begin):]
+    body = re.sub(r"//[^\n]*", "", body[:re.search(r"\n}\n", body).start()])
+    out = []
+    for m in re.finditer(r"\b(" + "|".join(CALLS) + r")\(", body):
+        depth, i = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(body[i], 0)
+            i += 1
+        out.append(CALLS[m.group(1)] + " " + body[m.end():i - 1])
+    return out
+
+
+def constant(name):
+    return int(re.search(r"\b%s = (\d+)\b" % name, SRC).group(1))
+
+
+def test_transcriptions_match_the_kernels():
+    assert operations("fp8_stream_kernel", "  if (warp == 0) {\n    regs_down") == STREAM_OPS
+    assert operations("fp8_pair_kernel", "  if (warp == 0 || warp == 3) {") == PAIR_OPS
+    assert constant("kPairStages") > constant("kPairBatch") and "kPairSlots = kPairStages + 2;" in SRC and "slots = (stages + BUFS) * SUB;" in SRC
+    for count in ("bar_init(full(s), 33); bar_init(empty(s), 1);", "bar_init(tfull(b), 1); bar_init(tempty(b), kSumWarps);", "bar_init(full(s), 3); bar_init(empty(s), 2);"):
+        assert count in SRC
+
+
+class Barrier:
+    def __init__(self, need):
+        self.need, self.got, self.done = need, 0, 0
+
+    def arrive(self):
+        self.got += 1
+        assert self.got <= self.need
+        if self.got == self.need:
+            self.got, self.done = 0, self.done + 1
+
+    def passed(self, parity):                             # of a phase that the caller names by its parity
+        return (self.done & 1) != (parity & 1)
+
+
+def run(roles, flights, rng):
+    """Roles are generators that yield a condition to wait for (or None); flights: functions that return what may complete now (lists of callables)."""
+    waiting = [next(r, "end") for r in roles]
+    quiet = 0
+    while any(w != "end" for w in waiting):
+        ready = [("role", i) for i, w in enumerate(waiting) if w != "end" and (w is None or w())]
+        ready += [("flight", f) for group in flights for f in group()]
+        assert ready, "waits for ever"
+        kind, what = rng.choice(ready)
+        if kind == "role":
+            waiting[what] = next(roles[what], "end")
+        else:
+            what()
+        quiet += 1
+        assert quiet < 100000
+
+
+class Copies:
+    """Copies in flight: any of them may arrive next."""
+
+    def __init__(self):
+        self.todo = []
+
+    def start(self, fn):
+        self.todo.append(fn)
+
+    def ready(self):
+        def take(fn):
+            self.todo.remove(fn)
+            fn()
+        return [lambda fn=fn: take(fn) for fn in self.todo]
+
+
+class Tensor(Copies):
+    """MMAs complete in the order of issue."""
+
+    def ready(self):
+        return super().ready()[:1]
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("tiles,KB", [(1, 1), (1, 7), (5, 1), (4, 2), (3, 5), (2, 11), (3, 16)])
+def test_pairs(seed, tiles, KB):
+    """Two CTAs: two producers and two groups of sums each, two threads that issue."""
+    S, BATCH = constant("kPairStages"), constant("kPairBatch")
+    SLOTS, rng = S + 2, random.Random(seed * 1000 + tiles * 50 + KB)
+    full = [Barrier(3 + 2) for _ in range(S)]             # (and both CTAs' copies, which the hardware counts in bytes)
+    empty = [[Barrier(2) for _ in range(S)] for _ in range(2)]
+    tfull = [[Barrier(1) for _ in range(4)] for _ in range(2)]
+    tempty = [Barrier(4) for _ in range(4)]               # (two groups of two CTAs; a group's four warps here in two halves)
+    stage_of, factor, acc, info = [[None] * S for _ in range(2)], [[None] * SLOTS for _ in range(2)], [None] * 4, [[None] * 16 for _ in range(2)]
+    copies, tensor, left = Copies(), Tensor(), {}
+    total = tiles * KB
+
+    def producer(cta, warp):
+        stage, slot, phase, turn = 0, 0, 0, 1 - warp
+        for tile in range(tiles):
+            if turn:
+                info[cta][tile & 15] = tile
+            for kb in range(0, KB, BATCH):
+                n = min(BATCH, KB - kb)
+                turn ^= 1
+                if turn:
+                    stage += n
+                    while stage >= S:
+                        stage, phase = stage - S, phase ^ 1
+                    slot = (slot + n) % SLOTS
+                    continue
+                for i in range(n):
+                    block = tile * KB + kb + i
+                    b, p = empty[cta][stage], phase ^ 1
+                    yield lambda b=b, p=p: b.passed(p)
+                    assert b.done >= block // S, "the stage is not free"
+                    if cta == 0:
+                        full[stage].arrive()
+
+                    def land(stage=stage, block=block):
+                        assert left.get(("stage", cta, stage), 0) == 0, "a stage is overwritten"
+                        stage_of[cta][stage] = block
+                        left[("stage", cta, stage)] = 2
+                        full[stage].arrive()
+                    copies.start(land)
+                    yield None
+                    assert left.get(("factor", cta, slot), 0) == 0, "factors are overwritten"
+                    factor[cta][slot] = block
+                    left[("factor", cta, slot)] = 4
+                    full[stage].arrive()
+                    yield None
+                    stage, phase = (0, phase ^ 1) if stage + 1 == S else (stage + 1, phase)
+                    slot = (slot + 1) % SLOTS
+
+    def issuer(h):
+        stage, buf, phase, buf_phase, f_there, t_there = 0, 0, 0, 0, False, False
+        for block in range(total):
+            if not f_there:
+                yield lambda: full[stage].passed(phase)
+            if not t_there:
+                yield lambda: tempty[2 * buf + h].passed(buf_phase ^ 1)
+            assert full[stage].done == block // S + 1 and tempty[2 * buf + h].done == block // 2
+            s1, v1 = (stage + 1) % S, buf ^ 1
+            p1, w1 = phase ^ (s1 == 0), buf_phase ^ buf
+            f_there, t_there = full[s1].passed(p1), tempty[2 * v1 + h].passed(w1 ^ 1)
+            yield None
+
+            def mma(stage=stage, buf=buf, block=block):
+                for cta in range(2):
+                    assert stage_of[cta][stage] == block
+                    left[("stage", cta, stage)] -= 1
+                assert left.get(("acc", 2 * buf + h), 0) == 0, "sums are overwritten"
+                acc[2 * buf + h] = block
+                left[("acc", 2 * buf + h)] = 4
+                for cta in range(2):
+                    tfull[cta][2 * buf + h].arrive()
+                    empty[cta][stage].arrive()
+            tensor.start(mma)
+            yield None
+            stage, phase, buf, buf_phase = s1, p1, v1, w1
+
+    def sums(cta, part):
+        buf, slot, buf_phase = 0, 0, 0
+        for block in range(total):
+            yield lambda: tfull[cta][2 * buf + part].passed(buf_phase)
+            assert info[cta][block // KB & 15] == block // KB and factor[cta][slot] == block and acc[2 * buf + part] == block
+            yield None
+            left[("factor", cta, slot)] -= 1
+            left[("acc", 2 * buf + part)] -= 1
+            tempty[2 * buf + part].arrive()
+            buf, buf_phase = buf ^ 1, buf_phase ^ buf
+            slot = (slot + 1) % SLOTS
+    roles = [producer(c, w) for c in range(2) for w in range(2)] + [issuer(h) for h in range(2)] + [sums(c, p) for c in range(2) for p in range(2) for _ in range(2)]
+    run(roles, [copies.ready, tensor.ready], rng)
+
+
+@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("stages,sub", [(2, 1), (3, 1), (5, 1), (2, 2), (3, 2), (8, 2)])
+@pytest.mark.parametrize("tiles,KB,ahead", [(1, 1, 1), (1, 9, 2), (1, 16, 8), (3, 5, 0), (4, 3, 2), (5, 8, 0)])
+def test_single_ctas(seed, stages, sub, tiles, KB, ahead):
+    """A producer (whose first tile's weights are under way early), a warp that copies factors, an issuing thread, groups of sums."""
+    rng = random.Random(seed * 1000 + stages * 100 + tiles * 10 + KB)
+    bufs, slots = 2, (stages + 2) * sub
+    full, empty = [Barrier(3) for _ in range(stages)], [Barrier(1) for _ in range(stages)]      # (full: the producer, its copies, the factors' copies)
+    tfull, tempty = [Barrier(1) for _ in range(bufs)], [Barrier(2) for _ in range(bufs)]
+    held, factor, acc, left = [None] * stages, [None] * slots, [None] * bufs, {}
+    copies, tensor = Copies(), Tensor()
+    steps = [(t, kb, min(sub, KB - kb)) for t in range(tiles) for kb in range(0, KB, sub)]
+    per = -(-KB // sub)
+
+    def land(stage, n):
+        def fn():
+            assert left.get(("stage", stage), 0) == 0, "a stage is overwritten"
+            held[stage] = n
+            left[("stage", stage)] = 1
+            full[stage].arrive()
+        return fn
+
+    def producer():
+        early = min(ahead, stages, per)
+        for n in range(early):
+            full[n].arrive()
+        stage, phase = 0, 0
+        yield None
+        for n in range(len(steps)):
+            if n >= early:
+                yield lambda: empty[stage].passed(phase ^ 1)
+                full[stage].arrive()
+            copies.start(land(stage, n))
+            yield None
+            stage, phase = (0, phase ^ 1) if stage + 1 == stages else (stage + 1, phase)
+
+    def helper():
+        stage, phase, slot = 0, 0, 0
+        for n, (_, _, k) in enumerate(steps):
+            yield lambda: empty[stage].passed(phase ^ 1)
+            assert empty[stage].done >= n // stages
+
+            def fn(n=n, k=k, slot=slot, stage=stage):
+                for u in range(k):
+                    assert left.get(("factor", slot + u), 0) == 0, "factors are overwritten"
+                    factor[slot + u] = (n, u)
+                    left[("factor", slot + u)] = 2
+                full[stage].arrive()
+            copies.start(fn)
+            yield None
+            stage, phase = (0, phase ^ 1) if stage + 1 == stages else (stage + 1, phase)
+            slot = (slot + sub) % slots
+
+    def issuer():
+        stage, buf, phase, buf_phase, f_there, t_there = 0, 0, 0, 0, False, False
+        for n in range(len(steps)):
+            if not f_there:
+                yield lambda: full[stage].passed(phase)
+            if not t_there:
+                yield lambda: tempty[buf].passed(buf_phase ^ 1)
+            assert full[stage].done == n // stages + 1 and tempty[buf].done == n // bufs
+            s1, v1 = (stage + 1) % stages, (buf + 1) % bufs
+            p1, w1 = phase ^ (s1 == 0), buf_phase ^ (v1 == 0)
+            f_there, t_there = full[s1].passed(p1), tempty[v1].passed(w1 ^ 1)
+            yield None
+
+            def mma(stage=stage, buf=buf, n=n):
+                assert held[stage] == n and left.get(("acc", buf), 0) == 0
+                left[("stage", stage)] -= 1
+                acc[buf], left[("acc", buf)] = n, 2
+                tfull[buf].arrive()
+                empty[stage].arrive()
+            tensor.start(mma)
+            yield None
+            stage, phase, buf, buf_phase = s1, p1, v1, w1
+
+    def sums():
+        buf, slot, buf_phase, at = 0, 0, 0, 0
+        for n, (t, kb, k) in enumerate(steps):
+            yield lambda: tfull[buf].passed(buf_phase)
+            for u in range(k):
+                assert acc[buf] == n and factor[slot + u] == (n, u)
+                yield None
+                left[("factor", slot + u)] -= 1
+            left[("acc", buf)] -= 1
+            tempty[buf].arrive()
+            buf, buf_phase = (0, buf_phase ^ 1) if buf + 1 == bufs else (buf + 1, buf_phase)
+            slot = (slot + sub) % slots
+    run([producer(), helper(), issuer(), sums(), sums()], [copies.ready, tensor.ready], rng)
+
+
+def test_registers_add_up():
+    """What the groups take on and give up is no more than the block is launched with."""
+    threads, sums, others = 384, constant("kSumRegs"), constant("kOtherRegs")
+    launched = 65536 // threads // 8 * 8
+    assert 256 * sums + 128 * others <= threads * launched and sums <= 232
