@@ -255,7 +255,8 @@ int kge_step_maps(int32_t* block_table, int max_blocks_per_seq, int32_t* seq_len
  * K is a multiple of 16; N and the number of rows are any.  Codes, x and w are 16-byte aligned.
  *
  * kge_fp8_quant: T rows of x (x_stride elements apart, a multiple of 8) to codes [T, K] and scales.  rows (may be NULL) gathers: row t is x's row
- * rows[t] (tokens sorted by expert), zeros where rows[t] < 0. */
+ * rows[t] (tokens sorted by expert; the same row may be taken more than once), zeros where rows[t] < 0.  What rows of x there are the call does not
+ * know: an index beyond the last one reads beyond x. */
 int kge_fp8_quant(void* codes, float* scales, int scales_stride, const void* x, int x_stride, const int32_t* rows, int T, int K, void* stream);
 
 /* E matrices w [E, N, K] to codes [E, N, K] and scales [E, ceil(N / 128), ceil(K / 128)]: a 16-bit checkpoint's weights. */

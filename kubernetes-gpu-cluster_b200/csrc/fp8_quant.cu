@@ -226,11 +226,12 @@ extern "C" int KGE_API(kge_fp8_quant)(void* codes, float* scales, int scales_str
   KGE_REQUIRE(K > 0 && K % 16 == 0, "kge_fp8_quant: K=%d must be a positive multiple of 16", K);
   KGE_REQUIRE(x_stride >= K && x_stride % 8 == 0, "kge_fp8_quant: rows of x %d apart (a multiple of 8, at least K = %d)", x_stride, K);
   KGE_REQUIRE(scales_stride >= T, "kge_fp8_quant: scales_stride=%d for %d rows", scales_stride, T);
-  KGE_REQUIRE(aligned16(codes) && aligned16(x) && ((uintptr_t)scales & 3) == 0, "kge_fp8_quant: codes and x must be 16-byte aligned");
+  KGE_REQUIRE(aligned16(codes) && aligned16(x) && ((uintptr_t)scales & 3) == 0 && ((uintptr_t)rows & 3) == 0,
+              "kge_fp8_quant: codes and x must be 16-byte aligned, scales and rows to their types");
   if (T <= 0) return 0;
   const int blocks = (int)fp8::blocks(K);
   const int64_t units = (int64_t)T * blocks;
-  KGE_REQUIRE(units < (1ll << 31) - 64 * 148 * 32, "kge_fp8_quant: %d rows of %d in one call", T, K);
+  KGE_REQUIRE(units < (1ll << 31) - 64 * 148 * 32 && K < 0x7fffffff - 1024, "kge_fp8_quant: %d rows of %d in one call", T, K);      // (columns are counted beyond K)
   const int64_t per_row = (K + 511) / 512, pieces = T * per_row;
   if (pieces < 2 * 148 * kRowWarps) {
     KGE_CUDA_OK(launch_pdl(fp8_quant_few_kernel, dim3((unsigned)((units + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride,

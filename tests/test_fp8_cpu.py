@@ -61,6 +61,13 @@ def test_gated_refusals(kge, grouped, change, words):
         refused(kge, kge.lib().kge_gemm_fp8_silu_gate(*[v for k, v in a.items() if k not in ("off", "E")], None), words)
 
 
+@pytest.mark.parametrize("f16", ["", "_f16"])
+@pytest.mark.parametrize("change,words", [(dict(rows=P + 2), "aligned"), (dict(K=2 ** 31 - 16, xst=2 ** 31 - 8), "in one call")])
+def test_row_refusals_of_indexes_and_long_rows(kge, f16, change, words):
+    a = dict(codes=P, scales=P, sst=3, x=P, xst=128, rows=None, T=3, K=128) | change
+    refused(kge, getattr(kge.lib(), "kge_fp8_quant" + f16)(*a.values(), None), words)
+
+
 def test_calls_without_rows_do_nothing(kge):
     L = kge.lib()
     assert L.kge_fp8_quant(P, P, 3, P, 128, None, 0, 128, None) == 0
