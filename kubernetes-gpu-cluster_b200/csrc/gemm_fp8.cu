@@ -7,9 +7,9 @@
 // 32) in fp32 in tensor memory, and eight warps add it, times its factor, to accumulators in registers.  Tensor memory holds several blocks, so that the next ones are multiplied meanwhile.
 //
 // Two kernels.
-//  fp8_stream_kernel: tiles of 128 tokens x NT weight rows by single CTAs, one an SM; the (tile, block of K) units of the whole problem are laid end
-//    to end and cut into equal shares, so every SM reads the same number of weight bytes whatever the sizes are.  A tile that a share's end cuts is
-//    summed by the last of its CTAs to arrive, from fp32 partial sums in the workspace and in the order of K: the same bits each time.
+//  fp8_stream_kernel: tiles of 128 tokens x 128 or 256 weight rows by single CTAs, one an SM, for calls that a pass over the weights bounds.  With at least
+//    half as many tiles as SMs a CTA has whole tiles; fewer tiles are cut along K, over the CTAs of a cluster where the host knows their number, and
+//    else (few rows in groups) over CTAs that meet in the workspace.  Shares are added in the order of K: the same bits each time.
 //  fp8_pair_kernel: tiles of 256 x 256 by pairs of CTAs (cta_group::2), for many tokens: a CTA has its own 128 tokens and half of the weight rows in
 //    shared memory, 32 KB a block of K, where its MMA takes 512 cycles.
 #include <cuda.h>
@@ -406,6 +406,9 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
 // CLUSTER: the shares of a tile are a cluster's CTAs.  Each finishes its part of the tile's columns, groups of 8, and gets the others' sums of them through
 // distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
 // Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
+// Bound by the weights' way from memory, and at one or two tiles a CTA by what is before and behind it: about 2 us from the launch to the first bytes and 2
+// to 3 for the last tile's sums, exchange and stores.  64 tokens: eight each of 128 experts, gated 1536 x 2048 (376 MB) 69.4 us, 5.4 TB/s; gated 28672 x 4096
+// (119 MB) 25.4 us; 4096 x 6144 (26 MB) 10.5 us; one token, 4096 x 14336 (59 MB) 14.7 us.
 template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
@@ -773,6 +776,12 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 
 // -------------------------------------------------------------------------------------------------------------- pairs
 
+// A block of K is 32 KB of codes and 512 cycles of MMAs a CTA; its 128 x 256 sums are 256 cycles of the fp32 pipe.  Both run side by side: tensor memory holds
+// two blocks, and the first and the second 128 columns of each are handed over apart, as soon as their four warps have read them.  Six stages and 2 KB a warp
+// through which rows are stored; four stages and a whole tile stored by copies from shared memory took 410 us where this took 399.
+// Bound by the power limit when it runs over and over, else by the 573 cycles that a block of K takes and by a tile's end (3000 cycles, gated 3400, under which
+// two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 385 us (2.5 PFLOP/s; over and over 441; copies and MMAs alone 334), gated 28672 x
+// 4096 796 us (2.4 PFLOP/s; 895; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 67.6 us.
 template <bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
