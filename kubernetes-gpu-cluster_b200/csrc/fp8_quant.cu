@@ -4,6 +4,7 @@
 // codes, 5 bits) are integers of at most 17 bits on one grid: 448 x / m either is t or misses it by 2^-17 and more.  x times the factor is off by less
 // than 2^-21, hence rounding it to 20 bits gives t where the quotient is t, and leaves it on its side of t elsewhere: one product and two integer
 // operations in place of a division.
+#include "f32x2.cuh"
 #include "fp8.cuh"
 #include "kge.h"
 
@@ -20,13 +21,16 @@ __device__ __forceinline__ uint32_t mag2(uint4 v) { return max2(max2(v.x, v.y), 
 // the largest magnitude of a block from that of its halves
 __device__ __forceinline__ float mag(uint32_t m2) { return fabsf(bf_lo(max2(m2, m2 >> 16))); }
 
-// x factor, rounded to 20 bits
-__device__ __forceinline__ float scaled(float x, float factor) { return __uint_as_float((__float_as_uint(x * factor) + 8u) & ~15u); }
+__device__ __forceinline__ float to_20_bits(float x) { return __uint_as_float((__float_as_uint(x) + 8u) & ~15u); }
 __device__ __forceinline__ uint2 codes8(uint4 v, float factor) {
   const uint32_t u[4] = {v.x, v.y, v.z, v.w};
   uint32_t c[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) c[k] = fp8::pack2(scaled(bf_lo(u[k]), factor), scaled(bf_hi(u[k]), factor));
+  for (int k = 0; k < 4; ++k) {
+    float a, b;
+    upk(mul2(pk(bf_lo(u[k]), bf_hi(u[k])), pk(factor, factor)), a, b);
+    c[k] = fp8::pack2(to_20_bits(a), to_20_bits(b));
+  }
   return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
 }
 
@@ -66,10 +70,11 @@ fp8_quant_few_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, in
 }
 
 // Many rows: a warp takes 512 columns of a row at a time, eight lanes a block as above, one piece after the other of an equal share of all, copied kAheadRows
-// pieces ahead into a ring of its own in shared memory; a lane reads back what it has copied itself, so nothing is waited for but the copies.  Bound by
-// instructions, 12 a number, at half to two thirds of what the schedulers issue: 8192 rows of 4096 (101 MB, 15.5 us) 22.1 us, 16384 rows of 2048 gathered
-// from 2048 (43 MB, 6.6 us) 19.1; with 16 warps 22.9 and 20.1; a block a thread 30.8 and 24.9; loads into registers one block ahead 27.1 and 22.9 (the use
-// of one waits for all that share its counter).
+// pieces ahead into a ring of its own in shared memory.  A copy is 512 bytes one behind the other; a lane reads back the 32 that it turns into codes, whose
+// halves are exchanged in every second group of four lanes, so that eight lanes meet in no bank.  (Where a lane copied its own 32 bytes every sector was
+// fetched twice: 18.3 us where this takes 16.)  16384 rows of 2048 gathered from 2048 (43 MB, 6.6 us) 16 us, bound by instructions; 8192 rows of 4096
+// (101 MB, 15.5 us) 21.3, 20000 of 7168 (434 MB) 84.5, 5.1 TB/s, by memory; two pieces a step 15.7, 21.4 and 84.8, but 1200 rows of 4096 6.0 for 5.4; 16, 24
+// and 28 warps and as many more pieces ahead within 4 % of it.
 constexpr int kRowWarps = 32, kAheadRows = 6, kPiece = 1024;
 __global__ void __launch_bounds__(kRowWarps * 32, 1)
 fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_stride, const bf16* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ rows,
@@ -84,26 +89,27 @@ fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_
   if (n == 0) return;
   const uint32_t t0 = first / per_row, last = (first + n - 1) / per_row;
   const int k0 = (int)(first - t0 * per_row) * 512 + lane * 16;
-  uint8_t* mine = smem + warp * (kAheadRows * kPiece) + lane * 32;
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(mine), to_end = to + kAheadRows * kPiece;
+  // a piece's 16 bytes number c lie at c ^ (c / 8 & 1)
+  const uint8_t* ring = smem + warp * (kAheadRows * kPiece);
+  const int turned = (lane >> 2) & 1;
+  const uint8_t *lo = ring + (2 * lane + turned) * 16, *hi = ring + (2 * lane + 1 - turned) * 16;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring) + ((lane ^ ((lane >> 3) & 1)) << 4), to_end = to + kAheadRows * kPiece;
   auto row_of = [&](uint32_t t) { return rows && t <= last ? rows[t] : (int)t; };
   // the copies' way through the share: row, column, source; and the row after that, asked for a row ahead
   uint32_t t = t0, slot_in = to;
-  int k = k0, r = row_of(t0), r_next = row_of(t0 + 1), left = n;
+  int k = k0 - lane * 8, r = row_of(t0), r_next = row_of(t0 + 1), left = n;
   const bf16* src = x + r * x_stride + k;
   auto copy = [&] {
     if (left > 0) {
       --left;
-      const bool there = r >= 0 && k < K;
-      const uint32_t size = there ? 16u : 0u;
-      const bf16* from = there ? src : x;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in), "l"(from), "r"(size) : "memory");
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in + 16), "l"(there ? from + 8 : x), "r"(size) : "memory");
+      const bool a = r >= 0 && k < K, b = r >= 0 && k + 256 < K;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in), "l"(a ? src : x), "r"(a ? 16u : 0u) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in + 512), "l"(b ? src + 256 : x), "r"(b ? 16u : 0u) : "memory");
       k += 512;
       src += 512;
-      if (k - lane * 16 >= K) {
+      if (k - lane * 8 >= K) {
         ++t;
-        k = lane * 16;
+        k = lane * 8;
         r = r_next;
         r_next = row_of(t + 1);
         src = x + r * x_stride + k;
@@ -121,7 +127,9 @@ fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_
 #pragma unroll 1
   for (; n > 0; --n) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kAheadRows - 1) : "memory");
-    const uint4 v[2] = {*reinterpret_cast<const uint4*>(mine + slot), *reinterpret_cast<const uint4*>(mine + slot + 16)};
+    __syncwarp();                                    // (a lane reads what others have copied)
+    const uint4 v[2] = {*reinterpret_cast<const uint4*>(lo + slot), *reinterpret_cast<const uint4*>(hi + slot)};
+    __syncwarp();
     copy();
     if ((slot += kPiece) == kAheadRows * kPiece) slot = 0;
     uint32_t m2 = max2(mag2(v[0]), mag2(v[1]));
