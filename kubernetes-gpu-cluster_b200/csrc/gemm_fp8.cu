@@ -54,7 +54,7 @@ struct Fp8Params {
   int E, T, N, KB, n_tiles, w_rows, w_blocks;     // w_rows, w_blocks: of one group's matrix (2 N when gated)
   float* part;                                    // stream: partial sums
   unsigned int* count;
-  int wide;                                       // pairs: y's rows are 16-byte aligned
+  int wide;                                       // plain: y's rows are 16-byte aligned
   int quarters, stages, x_bytes, ahead;           // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, stages filled early
   int splits;                                     // stream, dense: shares of K that a tile is cut into
   int most;                                       // of a cluster: column groups that a CTA finishes at most,
@@ -262,42 +262,97 @@ __device__ __forceinline__ float gated(float gate, float up) {
   return gate * inv * up;
 }
 
-// 8 columns of a row from n0 on, rounded once.
-__device__ __forceinline__ void store_group(const Fp8Params& p, float (&v)[8], int row, int n0) {
-  if (p.bias)
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n0 + j < p.N) v[j] += bf2f(p.bias[n0 + j]);
-  bf16* dst = p.y + (int64_t)row * p.N + n0;
-  if (n0 + 8 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (n0 + j < p.N) dst[j] = f2bf(v[j]);
-  }
-}
-
-// 64 columns of a row from n0 on, rounded once; c0: where their sums begin.
+// 64 columns of a row from n0 on, rounded once, where its rows are 16-byte aligned; c0: where their sums begin.
 template <int C>
 __device__ __forceinline__ void store_row(const Fp8Params& p, const Sums<C>& s, int c0, int row, int n0) {
   bf16* dst = p.y + (int64_t)row * p.N + n0;
-  if (n0 + 64 <= p.N && (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0) {
 #pragma unroll
-    for (int c = c0; c < c0 + 64; c += 8)
+  for (int c = c0; c < c0 + 64; c += 8)
+    if (n0 + c - c0 < p.N)
       *reinterpret_cast<uint4*>(dst + c - c0) = make_uint4(pack_bf2(s.v[c], s.v[c + 1]), pack_bf2(s.v[c + 2], s.v[c + 3]), pack_bf2(s.v[c + 4], s.v[c + 5]), pack_bf2(s.v[c + 6], s.v[c + 7]));
-  } else {
+}
+
+// The bias of SETS x 64 columns, SKIP apart, from n0 (even) on to a warp's own words in shared memory, two columns a word: asked for when a tile begins, there
+// when it ends.  (Loads by each thread when it ends, 9472 x 4096 x 1408: 18 us of 74.)
+template <int SETS, int SKIP>
+__device__ __forceinline__ void ask_bias(const Fp8Params& p, uint32_t* own, int n0, int lane) {
 #pragma unroll
-    for (int c = 0; c < 64; ++c)
-      if (n0 + c < p.N) dst[c] = f2bf(s.v[c0 + c]);
+  for (int h = 0; h < SETS; ++h) {
+    const int n = n0 + h * SKIP + 2 * lane, left = min(max(p.N - n, 0), 2);
+    const bf16* src = p.bias + (left ? n : 0);
+    uint32_t* dst = own + h * 32 + lane;
+    if ((reinterpret_cast<uintptr_t>(p.bias) & 3) == 0) {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(s_addr(dst)), "l"(src), "r"(2 * left) : "memory");
+    } else {
+      uint32_t v = 0;
+      if (left > 0) v = *reinterpret_cast<const uint16_t*>(src);
+      if (left > 1) v |= (uint32_t)*reinterpret_cast<const uint16_t*>(src + 1) << 16;
+      *dst = v;
+    }
   }
 }
-// The bias of 64 columns from n0 on, to the sums from c0 on.
 template <int C>
-__device__ __forceinline__ void add_bias(const Fp8Params& p, Sums<C>& s, int c0, int n0) {
+__device__ __forceinline__ void add_bias(Sums<C>& s, const uint32_t* own) {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
 #pragma unroll
-  for (int c = 0; c < 64; ++c)
-    if (n0 + c < p.N) s.v[c0 + c] += bf2f(p.bias[n0 + c]);
+  for (int c = 0; c < C; c += 8) {
+    const uint4 b = *reinterpret_cast<const uint4*>(own + c / 2);
+    s.v[c] += bf_lo(b.x); s.v[c + 1] += bf_hi(b.x); s.v[c + 2] += bf_lo(b.y); s.v[c + 3] += bf_hi(b.y);
+    s.v[c + 4] += bf_lo(b.z); s.v[c + 5] += bf_hi(b.z); s.v[c + 6] += bf_lo(b.w); s.v[c + 7] += bf_hi(b.w);
+  }
+  __syncwarp();
+}
+
+// Rows that are not 16-byte aligned: a warp's 32 rows (from `row` on, `rows` of them there) of C columns, the second 64 of them SKIP behind the first.  8 rows
+// of 64 columns at a time go through shared memory, in words as memory has them: a row that begins in the middle of a word has its columns one half further.
+// A row's whole words go out at once, and the halves at its ends, of 8 rows at once: what is written piece by piece costs the L2 by the piece (from registers,
+// a column of 32 rows at a time, 2048 x 4095 x 4096 took 105 us; 16 columns of two rows at a time 43).
+constexpr int kNarrowRow = 144, kNarrow = 8 * kNarrowRow;      // bytes of a row (33 words, and none that meets another row's in a bank) and of a warp
+template <int C, int SKIP>
+__device__ __forceinline__ void store_narrow(const Fp8Params& p, const Sums<C>& s, int row, int rows, int n0, uint32_t buffer, int lane) {
+  auto at = [&](int r, int n) { return reinterpret_cast<uint16_t*>(p.y) + (int64_t)(row + r) * p.N + n; };
+  auto is_odd = [](const uint16_t* dst) { return (int)(reinterpret_cast<uintptr_t>(dst) >> 1) & 1; };
+#pragma unroll
+  for (int c0 = 0; c0 < C; c0 += 64) {
+    const int n = n0 + c0 / 64 * SKIP, columns = min(p.N - n, 64);
+    if (columns <= 0) break;
+    uint32_t u[33];
+    const bool half = is_odd(at(lane, n));
+    u[0] = pack_bf2(half ? 0.f : s.v[c0], half ? s.v[c0] : s.v[c0 + 1]);
+#pragma unroll
+    for (int w = 1; w < 32; ++w) u[w] = pack_bf2(half ? s.v[c0 + 2 * w - 1] : s.v[c0 + 2 * w], half ? s.v[c0 + 2 * w] : s.v[c0 + 2 * w + 1]);
+    u[32] = pack_bf2(s.v[c0 + 63], 0.f);
+#pragma unroll 1
+    for (int g = 0; g < 32 && g < rows; g += 8) {
+      __syncwarp();
+      if ((lane & 24) == g) {
+        const uint32_t put = buffer + (lane & 7) * kNarrowRow;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(put + k * 16), "r"(u[4 * k]), "r"(u[4 * k + 1]), "r"(u[4 * k + 2]), "r"(u[4 * k + 3]) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(put + 128), "r"(u[32]) : "memory");
+      }
+      __syncwarp();
+      uint32_t v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[r]) : "r"(buffer + r * kNarrowRow + lane * 4) : "memory");
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        uint16_t* dst = at(g + r, n);
+        const int c = 2 * lane - is_odd(dst);
+        if (g + r < rows && c >= 0 && c + 1 < columns) *reinterpret_cast<uint32_t*>(dst + c) = v[r];
+      }
+      // the first column of a row that begins in a word's middle; the last of one that ends there
+      const int r = (lane >> 1) & 7, c = lane & 1 ? columns - 1 : 0;
+      uint16_t* dst = at(g + r, n);
+      const int odd = is_odd(dst);
+      if (lane < 16 && g + r < rows && ((c + odd) & 1) == 1 - (lane & 1)) {
+        uint16_t e;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(e) : "r"(buffer + r * kNarrowRow + (c + odd) * 2) : "memory");
+        dst[c] = e;
+      }
+    }
+  }
 }
 
 // A warp's 32 rows (from `row` on, `rows` of them there) of C columns, 32 at a time through 2 KB of its own in shared memory: rows of 64 bytes, whose
@@ -403,6 +458,12 @@ __device__ __forceinline__ float4 lds4(uint32_t at) {
   return v;
 }
 
+__device__ __forceinline__ float lds1(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // CLUSTER: the shares of a tile are a cluster's CTAs.  Each finishes its part of the tile's columns, groups of 8, and gets the others' sums of them through
 // distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
 // Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
@@ -419,7 +480,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   __shared__ uint64_t bars[2 * kMaxStages + 2 * BUFS];
   __shared__ uint32_t tmem_slot;
   __shared__ int last_flag;
-  __shared__ uint32_t tops[(CLUSTER ? 1 + kMaxSplits : 2) * 128];
+  __shared__ uint32_t tops[GATED ? (CLUSTER ? 1 + kMaxSplits : 2) * 128 : 1];
+  __shared__ __align__(16) uint32_t biases[GATED ? 4 : kSumWarps * 64];       // of each warp that adds up; of all columns
   __shared__ Groups<CLUSTER ? 1 : kMaxGroups> groups;
   const int stages = p.stages;
   const uint32_t block_bytes = (uint32_t)p.x_bytes + NT * 128, stage_bytes = SUB * block_bytes;
@@ -587,6 +649,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 3) {
     regs_down<kOtherRegs>();
+    if constexpr (CLUSTER && !GATED) {               // (the others see it behind the cluster's barriers)
+      if (p.bias) {
+        pdl_wait();
+        int e = 0;
+        ask_bias<NT / 64, 64>(p, biases, find_tile<kRows, 0>(p, groups, work.tile0, e).n * NT, lane);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      }
+    }
   } else {
     regs_up<kSumRegs>();
     const int q = warp & 3, part = (warp - 4) >> 2, tid = threadIdx.x - 128, lane128 = q * 32 + lane;
@@ -599,6 +669,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
       const int row = t.row + lane128, n0 = t.n * NT + part * 64;
       Sums<C> s;
       s.clear();
+      uint32_t* own = biases + (GATED ? 0 : (warp - 4) * 64);
+      if (!GATED && !CLUSTER && p.bias) ask_bias<C / 64, 128>(p, own, n0, lane);
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 64;
       int sub = 0, left = work.kb1 - work.kb0;
       auto read = [&] {
@@ -666,6 +738,21 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
               v[half * 4] += f.x; v[half * 4 + 1] += f.y; v[half * 4 + 2] += f.z; v[half * 4 + 3] += f.w;
             }
         };
+        if (!GATED && !p.wide) {
+          // rows that are not 16-byte aligned: four rows of a group at a time, a column a lane
+          const int j = lane & 7;
+#pragma unroll 1
+          for (int r = (warp - 4) * 4 + (lane >> 3); r < t.rows; r += 4 * kSumWarps)
+#pragma unroll 1
+            for (int g = 0; g < p.first[me + 1] - g0; ++g) {
+              const int c = (g0 + g) * 8 + j;
+              float v = 0.f;
+#pragma unroll 1
+              for (int from = 0; from < S; ++from) v += lds1(place(from, 0, g, j >> 2, r) + (j & 3) * 4);
+              if (p.bias) v += bf2f(reinterpret_cast<const bf16*>(biases)[c]);
+              if (t.n * NT + c < p.N) p.y[(int64_t)(t.row + r) * p.N + t.n * NT + c] = f2bf(v);
+            }
+        } else
 #pragma unroll 1
         for (int n = warp - 4; n < items; n += kSumWarps) {
           int r, g;
@@ -684,8 +771,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
             atomicMax(&tops[r], top);
             push4(mapa_u32(place(0, 0, g, 0, r), me), v[0], v[1], v[2], v[3]);      // (in the place of the first sender's sums)
             push4(mapa_u32(place(0, 0, g, 1, r), me), v[4], v[5], v[6], v[7]);
-          } else if (r < t.rows) {
-            store_group(p, v, t.row + r, t.n * NT + (g0 + g) * 8);
+          } else if (r < t.rows && t.n * NT + (g0 + g) * 8 < p.N) {
+            if (p.bias) {
+              const uint4 b = *reinterpret_cast<const uint4*>(biases + (g0 + g) * 4);
+              v[0] += bf_lo(b.x); v[1] += bf_hi(b.x); v[2] += bf_lo(b.y); v[3] += bf_hi(b.y);
+              v[4] += bf_lo(b.z); v[5] += bf_hi(b.z); v[6] += bf_lo(b.w); v[7] += bf_hi(b.w);
+            }
+            *reinterpret_cast<uint4*>(p.y + (int64_t)(t.row + r) * p.N + t.n * NT + (g0 + g) * 8) =
+                make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
           }
         }
         if constexpr (GATED) {
@@ -751,12 +844,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         }
         if constexpr (GATED) {
           store_gated(p, s, row, there, t.n, tops, part, lane128);
-        } else if (there) {
+        } else {
+          if (p.bias) add_bias<C>(s, own);
+          if (!p.wide) {
+            if (some) store_narrow<C, 128>(p, s, row - lane, t.rows - q * 32, n0, s_addr(factors + slots * SLOT) + (warp - 4) * kNarrow, lane);
+          } else if (there) {
 #pragma unroll
-          for (int h = 0; h < C / 64; ++h)
-            if (p.bias) add_bias<C>(p, s, h * 64, n0 + h * 128);
-#pragma unroll
-          for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
+            for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 128);
+          }
         }
       }
     }
@@ -782,7 +877,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // Bound by the power limit when it runs over and over, else by the 573 cycles that a block of K takes and by a tile's end (3000 cycles, gated 3400, under which
 // two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 385 us (2.5 PFLOP/s; over and over 441; copies and MMAs alone 334), gated 28672 x
 // 4096 796 us (2.4 PFLOP/s; 895; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 67.6 us.
-template <bool GATED>
+template <bool GATED, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
   constexpr int C = 128, STAGES = kPairStages;
@@ -791,7 +886,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t bars[2 * STAGES + 8];
   __shared__ uint32_t tmem_slot;
-  __shared__ uint32_t tops[256];
+  __shared__ uint32_t tops[GATED ? 256 : 1];
+  __shared__ __align__(16) uint32_t biases[GATED ? 4 : kSumWarps * 64];       // of each warp that adds up
   __shared__ int4 tiles[16];                        // n, row, rows of the tiles under way: at most one a block of K of the rings, and the last one
   __shared__ Groups<kMaxGroups> groups;
   const uint32_t base = s_addr(smem), bar0 = s_addr(bars);
@@ -915,6 +1011,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       const int row = t.row + mine, n0 = t.n * 256 + part * 128;
       Sums<C> s;
       s.clear();
+      uint32_t* own = biases + (GATED ? 0 : (warp - 4) * 64);
+      if (!GATED && p.bias) ask_bias<2, 64>(p, own, n0, lane);
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 128;
       auto read = [&] {
         fence_before();
@@ -935,17 +1033,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       } else {
         for (int kb = 0; kb < KB; ++kb) { mbar_wait(tfull(2 * buf + part), buf_phase); read(); }
       }
-      if (!GATED && p.bias) {
-        add_bias<C>(p, s, 0, n0);
-        add_bias<C>(p, s, 64, n0 + 64);
-      }
+      if (!GATED && p.bias) add_bias<C>(s, own);
       if constexpr (GATED) {
         store_gated(p, s, row, there, t.n, tops, part, lane128);
-      } else if (p.wide) {
-        if (some) store_rows<C>(p, s, row - lane, t.rows - (mine - lane), n0, base + STAGES * kStage + (warp - 4) * 2048, lane);
-      } else if (there) {
-#pragma unroll
-        for (int h = 0; h < C / 64; ++h) store_row<C>(p, s, h * 64, row, n0 + h * 64);
+      } else if (some) {
+        const uint32_t buffer = base + STAGES * kStage + (warp - 4) * 2048;
+        if constexpr (WIDE) store_rows<C>(p, s, row - lane, t.rows - (mine - lane), n0, buffer, lane);
+        else store_narrow<C, 64>(p, s, row - lane, t.rows - (mine - lane), n0, buffer, lane);
       }
     }
   }
@@ -1013,15 +1107,17 @@ static int quarters_of(int T) { return ((T < kRows ? T : kRows) + 31) / 32; }
 // What the sums of a cluster's shares take of shared memory, and how many stages are left.
 static int sums_bytes(int splits, int sets, int quarters) { return splits > 1 ? splits * ((16 + splits - 1) / splits) * sets * 2 * quarters * 32 * 16 : 0; }
 static int stage_bytes_of(int nt, int quarters) { return stream_sub(nt) * (quarters * 4096 + nt * 128 + kSlotBytes); }
-static int stream_stages(int nt, int splits, int quarters) {
-  const int n = (kSmem - kOwn - 1024 - 512 / nt * kSlotBytes - sums_bytes(splits, nt / 128, quarters)) / stage_bytes_of(nt, quarters);
+// (without shares through a cluster, rows that are not 16-byte aligned go through 9 KB)
+static int end_bytes(int nt, int splits, int quarters, int wide) { return splits > 1 ? sums_bytes(splits, nt / 128, quarters) : wide ? 0 : kSumWarps * kNarrow; }
+static int stream_stages(int nt, int splits, int quarters, int wide) {
+  const int n = (kSmem - kOwn - 1024 - 512 / nt * kSlotBytes - end_bytes(nt, splits, quarters, wide)) / stage_bytes_of(nt, quarters);
   return n < kMaxStages ? n : kMaxStages;
 }
 // Shares of K of a dense problem's tiles: the most that run at once and leave two stages.
 static int plan_splits(int64_t tiles, int nt, int quarters, int KB, int sms) {
   if (2 * tiles >= sms) return 1;
   for (int s = kMaxSplits; s > 1; --s)
-    if (tiles * s <= sms && KB >= 2 * s && tiles <= max_clusters(s) && stream_stages(nt, s, quarters) >= 2) return s;
+    if (tiles * s <= sms && KB >= 2 * s && tiles <= max_clusters(s) && stream_stages(nt, s, quarters, 0) >= 2) return s;
   return 1;
 }
 // Which kernel a dense problem takes, by what each is measured to need: a block of K 0.37 us a tile of the pair kernel and 1.8 for the tile's end; 0.38 a
@@ -1056,12 +1152,13 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
     for (int c = 0; c < p.splits; ++c)
       for (int g = p.first[c]; g < p.first[c + 1]; ++g) p.owner[g] = (uint8_t)c;
   }
-  p.stages = stream_stages(NT, p.splits, p.quarters);
+  p.wide = GATED || (p.N % 8 == 0 && aligned_to(p.y, 16));
+  p.stages = stream_stages(NT, p.splits, p.quarters, p.wide);
   KGE_REQUIRE(p.stages >= 2, "kge_gemm_fp8: internal: %d stages", p.stages);
   p.ahead = p.stages;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");
-  const int smem = p.stages * stage_bytes_of(NT, p.quarters) + 512 / NT * kSlotBytes + sums_bytes(p.splits, NT / 128, p.quarters) + 1024;
+  const int smem = p.stages * stage_bytes_of(NT, p.quarters) + 512 / NT * kSlotBytes + end_bytes(NT, p.splits, p.quarters, p.wide) + 1024;
   CUtensorMap mw, mx;
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 128)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 32)) return rc;
@@ -1091,7 +1188,10 @@ static int launch_pairs(Fp8Params& p, const void* x, const void* w, int K, cudaS
   if (int rc = encode_map(&mw, w, (int64_t)p.E * p.w_rows, K, 64)) return rc;
   if (int rc = encode_map(&mx, x, p.T, K, 128)) return rc;
   p.wide = !GATED && p.N % 8 == 0 && aligned_to(p.y, 16);
-  auto kern = fp8_pair_kernel<GATED>;
+  auto kern = fp8_pair_kernel<GATED, true>;
+  if constexpr (!GATED) {
+    if (!p.wide) kern = fp8_pair_kernel<GATED, false>;
+  }
   KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   prefer_max_shared(kern);
   const int sms = sm_count();
