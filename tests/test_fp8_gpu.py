@@ -555,3 +555,56 @@ def test_more_than_32_bits_of_elements(kge, L):
     code, scale = fo.quantise(big[-1:].cpu(), 1)
     assert torch.equal(codes[-1].cpu().view(fo.E4M3).double(), code[0]) and torch.equal(scales[:, -1].cpu(), scale[0].float())
     assert not codes[:-1].any()
+
+
+ALIGNED = [  # T, N, K: tiles of 256 columns, several a CTA; tiles of 128 cut along K over a cluster; pairs, whole and ragged; a column more, then seven
+    (70, 19001, 144), (33, 19175, 144), (130, 30002, 144), (1, 4097, 2064), (64, 1001, 1040), (100, 3005, 1296), (9, 3, 528), (128, 6143, 528), (1030, 2049, 272), (2050, 1029, 400),
+    (777, 4095, 144)]
+
+
+@pytest.mark.parametrize("T,N,K", ALIGNED)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_results_and_biases_at_any_address(kge, L, T, N, K, dtype):
+    """y and the bias 0 to 7 elements behind a 16-byte boundary, rows of any alignment: sentinels around the result stay, and the bits do not depend on it."""
+    dt, g = fo.DT[dtype], torch.Generator().manual_seed(T + N)
+    x, xs, xn = quantised(g, T, K, 1)
+    w, ws, wn = quantised(g, N, K, 128)
+    b = torch.randn(N, generator=g).to(dt)
+    xn, wn = xn.cuda(), wn.cuda()
+    z, a = (xn @ wn.t()).cpu(), (xn.abs() @ wn.abs().t()).cpu()
+    args = xs.t().contiguous().cuda(), T, w.cuda(), ws.cuda()
+    xd, work = x.cuda(), workspace(L, T)
+    for bias in (False, True):
+        first = None
+        for off in ((0, 1, 2, 7) if bias else (0, 1, 6)):
+            room, broom = torch.full((T * N + 64,), 7.0, dtype=dt, device="cuda"), torch.full((N + 16,), math.nan, dtype=dt, device="cuda")
+            broom[off:off + N] = b.cuda()
+            call(kge, name("kge_gemm_fp8", dt), room[24 + off:], xd, *args, broom[off:] if bias else None, T, N, K, work, work.numel())
+            y = room[24 + off:24 + off + T * N].view(T, N)
+            assert (room[:24 + off] == 7).all() and (room[24 + off + T * N:] == 7).all()
+            if first is None:
+                first = y.clone()
+                held(first.cpu(), z + b.double() if bias else z, a + b.double().abs() if bias else a, K, fo.half_step(dt))
+            assert torch.equal(y, first), off
+
+
+@pytest.mark.parametrize("sizes,N,K", [([5, 0, 1, 33], 137, 528), ([300, 2, 0, 33, 129], 515, 400), ([1] * 40, 4098, 144), ([60] * 20, 1283, 272), ([200, 31, 0, 257], 1001, 656),
+                                       ([2, 1, 0, 3], 67, 2064)], ids=lambda v: str(v) if isinstance(v, int) else "x".join(map(str, v))[:24])
+@pytest.mark.parametrize("off", [0, 1, 6])
+def test_groups_with_rows_of_any_alignment(kge, L, sizes, N, K, off):
+    g, E, T = torch.Generator().manual_seed(N), len(sizes), sum(sizes)
+    x, xs, xn = quantised(g, T, K, 1)
+    w, ws, wn = quantised(g, E * 128 * -(-N // 128), K, 128)
+    w, wn = (v.unflatten(0, (E, -1))[:, :N].contiguous() for v in (w, wn))
+    offsets = np.concatenate([[0], np.cumsum(sizes)])
+    room = torch.full(((T + 9) * N + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    work = workspace(L, T + 9)
+    xd, xsd = torch.zeros(T + 9, K, dtype=torch.uint8, device="cuda"), torch.zeros(xs.shape[1], T + 9, device="cuda")
+    xd[:T], xsd[:, :T] = x.cuda().view(torch.uint8), xs.t().cuda()
+    call(kge, "kge_gemm_fp8_grouped", room[32 + off:], xd, xsd, T + 9, w.cuda(), ws.cuda(), torch.tensor(offsets, **I32), E, T + 9, N, K, work, work.numel())
+    y = room[32 + off:32 + off + T * N].view(T, N).cpu()
+    assert (room[:32 + off] == 7).all() and (room[32 + off + T * N:] == 7).all() and (work[:1024] == 0).all()
+    for e in range(E):
+        r = slice(offsets[e], offsets[e + 1])
+        if sizes[e]:
+            held(y[r], xn[r] @ wn[e].t(), xn[r].abs() @ wn[e].abs().t(), K, fo.half_step(torch.bfloat16))
