@@ -57,7 +57,8 @@ struct Fp8Params {
   int wide;                                       // plain: y's rows are 16-byte aligned
   int quarters, stages, x_bytes, ahead;           // stream: 32-row quarters that a tile can have, stages, bytes of a stage's tokens, stages filled early
   int splits;                                     // stream, dense: shares of K that a tile is cut into
-  int most;                                       // of a cluster: column groups that a CTA finishes at most,
+  int over;                                       // of a cluster: its sums are exchanged where the stages were
+  int most;                                       // column groups that a CTA finishes at most,
   uint8_t first[kMaxSplits + 1], owner[16];       // the first of 16 that each finishes, which CTA finishes each
 };
 
@@ -512,7 +513,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
   fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_launch_dependents();
-  if (CLUSTER) cluster_arrive_relaxed();
+  if (CLUSTER && !p.over) cluster_arrive_relaxed();
   if (!CLUSTER && p.offsets) {                      // which tiles there are is the kernel before's output
     pdl_wait();
     count_tiles(p, kRows, groups);
@@ -704,9 +705,10 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
         // Groups of 8 columns of each set: this CTA finishes [g0, g1) of 16.  Their sums lie there by sender, set, group, half and row, 16 bytes each; each is
         // finished by a lane of its row.  (Everything here runs once a launch and costs its way from the L2: rolled loops, and all sums by one path.)
         const int S = work.splits, me = (int)cluster_ctarank(), rows = p.quarters * 32, most = p.most;
-        const uint32_t sums = s_addr(factors + slots * SLOT);
+        const uint32_t sums = p.over ? base : s_addr(factors + slots * SLOT);
         auto place = [&](int sender, int set, int g, int half, int r) { return sums + (uint32_t)((((sender * SETS + set) * most + g) * 2 + half) * rows + r) * 16u; };
-        cluster_wait();                                   // (all have begun)
+        if (p.over) cluster_arrive();
+        cluster_wait();                                   // (all have begun; or their MMAs have read what the sums are laid over)
         if (some) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -722,7 +724,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
           }
         }
         cluster_arrive(); cluster_wait();
-        const int g0 = p.first[me], items = (p.first[me + 1] - g0) * p.quarters;
+        const int g0 = p.first[me], mine = p.first[me + 1] - g0, items = mine * p.quarters;
         auto item = [&](int n, int& r, int& g) {          // a warp's n-th quarter of the rows and group
           g = n / p.quarters;
           r = (n - g * p.quarters) * 32 + lane;
@@ -744,13 +746,18 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 #pragma unroll 1
           for (int r = (warp - 4) * 4 + (lane >> 3); r < t.rows; r += 4 * kSumWarps)
 #pragma unroll 1
-            for (int g = 0; g < p.first[me + 1] - g0; ++g) {
+            for (int g = 0; g < mine; g += 4) {      // (reading beyond the last group, but not beyond what lies there)
               const int c = (g0 + g) * 8 + j;
-              float v = 0.f;
+              const uint32_t from0 = place(0, 0, g, j >> 2, r) + (j & 3) * 4, group = 2 * rows * 16, sender = SETS * most * group;
+              float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-              for (int from = 0; from < S; ++from) v += lds1(place(from, 0, g, j >> 2, r) + (j & 3) * 4);
-              if (p.bias) v += bf2f(reinterpret_cast<const bf16*>(biases)[c]);
-              if (t.n * NT + c < p.N) p.y[(int64_t)(t.row + r) * p.N + t.n * NT + c] = f2bf(v);
+              for (int from = 0; from < S; ++from)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += lds1(from0 + from * sender + min(k, most - 1 - g) * group);
+              bf16* dst = p.y + (int64_t)(t.row + r) * p.N + t.n * NT + c;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (g + k < mine && t.n * NT + c + 8 * k < p.N) dst[8 * k] = f2bf(p.bias ? v[k] + bf2f(reinterpret_cast<const bf16*>(biases)[c + 8 * k]) : v[k]);
             }
         } else
 #pragma unroll 1
@@ -857,6 +864,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
   }
   if (CLUSTER && warp < 4) {                        // the barriers that the others take, for all threads take part
+    if (p.over) cluster_arrive();
     cluster_wait();
     cluster_arrive(); cluster_wait();
     if (GATED) { cluster_arrive(); cluster_wait(); }
@@ -1107,31 +1115,39 @@ static int quarters_of(int T) { return ((T < kRows ? T : kRows) + 31) / 32; }
 // What the sums of a cluster's shares take of shared memory, and how many stages are left.
 static int sums_bytes(int splits, int sets, int quarters) { return splits > 1 ? splits * ((16 + splits - 1) / splits) * sets * 2 * quarters * 32 * 16 : 0; }
 static int stage_bytes_of(int nt, int quarters) { return stream_sub(nt) * (quarters * 4096 + nt * 128 + kSlotBytes); }
-// (without shares through a cluster, rows that are not 16-byte aligned go through 9 KB)
-static int end_bytes(int nt, int splits, int quarters, int wide) { return splits > 1 ? sums_bytes(splits, nt / 128, quarters) : wide ? 0 : kSumWarps * kNarrow; }
-static int stream_stages(int nt, int splits, int quarters, int wide) {
-  const int n = (kSmem - kOwn - 1024 - 512 / nt * kSlotBytes - end_bytes(nt, splits, quarters, wide)) / stage_bytes_of(nt, quarters);
+static int stages_beside(int bytes, int nt, int quarters) {
+  const int n = (kSmem - kOwn - 1024 - 512 / nt * kSlotBytes - bytes) / stage_bytes_of(nt, quarters);
   return n < kMaxStages ? n : kMaxStages;
 }
-// Shares of K of a dense problem's tiles: the most that run at once and leave two stages.
-static int plan_splits(int64_t tiles, int nt, int quarters, int KB, int sms) {
+// What a tile's end takes of shared memory beside the stages: a cluster's sums, if two stages are left (else they lie over the stages: gated 128 rows); without
+// a cluster, 9 KB for rows that are not 16-byte aligned.
+static int end_bytes(int nt, int splits, int quarters, int wide) {
+  if (splits <= 1) return wide ? 0 : kSumWarps * kNarrow;
+  const int sums = sums_bytes(splits, nt / 128, quarters);
+  return stages_beside(sums, nt, quarters) >= 2 ? sums : 0;
+}
+static int stream_stages(int nt, int splits, int quarters, int wide) { return stages_beside(end_bytes(nt, splits, quarters, wide), nt, quarters); }
+// Shares of K of a dense problem's tiles: the most that run at once.
+static int plan_splits(int64_t tiles, int KB, int sms) {
   if (2 * tiles >= sms) return 1;
   for (int s = kMaxSplits; s > 1; --s)
-    if (tiles * s <= sms && KB >= 2 * s && tiles <= max_clusters(s) && stream_stages(nt, s, quarters, 0) >= 2) return s;
+    if (tiles * s <= sms && KB >= 2 * s && tiles <= max_clusters(s)) return s;
   return 1;
 }
-// Which kernel a dense problem takes, by what each is measured to need: a block of K 0.37 us a tile of the pair kernel and 1.8 for the tile's end; 0.38 a
-// tile of 128 columns of the other (0.45 of a share, for there the rings are not yet full), 0.70 of 256, and 1.5 for its end; 5 us for start and end.  us by pairs and by single CTAs: 128
-// x 28672 x 4096 37.2 and 29.1, 256 38.2 and 51.5, 512 64 and 98; 256 x 4096 x 4096 18.7 and 13.0, 512 19.4 and 16.7, 1024 20.4 and 23.0; 333 x 2504 x 2064
-// 15.4 and 10.8; gated 128 x 28672 x 4096 36.5 and 26.8, 256 37.6 and 47.2.
+// Which kernel a dense problem takes, by what each is measured to need: a block of K 0.37 us a tile of the pair kernel and 1.8 for the tile's end (4.4 where
+// rows are not 16-byte aligned); 0.38 a tile of 128 columns of the other and 0.70 of 256, and 1.5 for its end; 0.45 and 0.70 of a share, for there the rings
+// are not yet full, and 0.7 (gated 1.5) of every 32 rows for the exchange; 5 us for start and end.  us by pairs and by single CTAs: 128 x 28672 x 4096 37.2 and
+// 29.1, 256 38.2 and 51.5, 512 64 and 98; 256 x 4096 x 4096 18.7 and 13.0, 512 19.4 and 16.7, 1024 20.4 and 23.0; 898 x 491 x 512 11.0 and 8.4; gated 128 x
+// 28672 x 4096 36.5 and 26.8, 256 37.6 and 47.2; 1112 x 256 x 10240 31.5 and 16.9.  Of 45 dense shapes drawn at random the slower one was taken for three, by
+// 10 % and more: all of 12 us and less.
 static bool use_pairs(int T, int N, int KB, bool gated, int sms) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const int64_t wide = up(N, gated ? 128 : 256);
-  const double pairs = up(up(T, 2 * kRows) * wide, sms / 2) * (KB * 0.37 + 1.8);
+  const double pairs = up(up(T, 2 * kRows) * wide, sms / 2) * (KB * 0.37 + (gated || N % 8 == 0 ? 1.8 : 4.4));
   double single = up(up(T, kRows) * wide, sms) * (KB * 0.70 + 1.5);
   const int64_t tiles = up(T, kRows) * (gated ? wide : up(N, 128));
-  const int splits = plan_splits(tiles, gated ? 256 : 128, quarters_of(T), KB, sms);
-  if (splits > 1) single = up(KB, splits) * (gated ? 0.70 : 0.45) + 1.5;
+  const int splits = plan_splits(tiles, KB, sms);
+  if (splits > 1) single = up(KB, splits) * (gated ? 0.70 : 0.45) + (gated ? 1.5 : 0.7) * quarters_of(T);
   else if (!gated && 2 * up(T, kRows) * wide < sms) single = up(tiles, sms) * (KB * 0.38 + 1.5);
   return pairs < single;
 }
@@ -1144,7 +1160,7 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   const int sms = sm_count();
   const int64_t tiles = (int64_t)((p.T + kRows - 1) / kRows) * p.n_tiles;
   p.splits = 0;                                            // grouped: by the number of tiles, on the device
-  if (!p.offsets) p.splits = GATED || NT == 128 ? plan_splits(tiles, NT, p.quarters, p.KB, sms) : 1;
+  if (!p.offsets) p.splits = GATED || NT == 128 ? plan_splits(tiles, p.KB, sms) : 1;
   const bool cluster = p.splits > 1;
   if (cluster) {
     p.most = (16 + p.splits - 1) / p.splits;
@@ -1154,7 +1170,8 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   }
   p.wide = GATED || (p.N % 8 == 0 && aligned_to(p.y, 16));
   p.stages = stream_stages(NT, p.splits, p.quarters, p.wide);
-  KGE_REQUIRE(p.stages >= 2, "kge_gemm_fp8: internal: %d stages", p.stages);
+  p.over = cluster && end_bytes(NT, p.splits, p.quarters, p.wide) == 0;
+  KGE_REQUIRE(p.stages >= 2 && (!p.over || p.stages * stage_bytes_of(NT, p.quarters) >= sums_bytes(p.splits, NT / 128, p.quarters)), "kge_gemm_fp8: internal: %d stages", p.stages);
   p.ahead = p.stages;
   // an MMA reads 128 rows of tokens from where they begin, and finds others' bytes behind the last: never beyond the stage's weights
   static_assert(NT * 128 >= kRows * 128, "");

@@ -608,3 +608,22 @@ def test_groups_with_rows_of_any_alignment(kge, L, sizes, N, K, off):
         r = slice(offsets[e], offsets[e + 1])
         if sizes[e]:
             held(y[r], xn[r] @ wn[e].t(), xn[r].abs() @ wn[e].abs().t(), K, fo.half_step(torch.bfloat16))
+
+
+@pytest.mark.parametrize("T,f,K", [(97, 128, 272), (128, 1024, 1040), (97, 896, 2064), (370, 640, 2064), (1112, 128, 1040), (65, 256, 1424), (100, 2304, 528), (120, 2944, 400)])
+def test_gated_tiles_whose_sums_take_the_place_of_their_stages(kge, L, T, f, K):
+    """More than 96 rows in tiles cut along K over 2 to 8 CTAs (and one of fewer): twice over, and after itself, with the same bits."""
+    g = torch.Generator().manual_seed(T + f)
+    x, xs, xn = quantised(g, T, K, 1)
+    w, ws, wn = quantised(g, 2 * f, K, 128)
+    work = workspace(L, T)
+    args = x.cuda(), xs.t().contiguous().cuda(), T, w.cuda(), ws.cuda(), T, f, K, work, work.numel()
+    out = [(torch.full((T + 1, f), 0x55, dtype=torch.uint8, device="cuda"), torch.full((f // 128, T), 9.0, device="cuda")) for _ in range(5)]
+    for codes, scales in out:
+        call(kge, "kge_gemm_fp8_silu_gate", codes, scales, T, *args)
+    torch.cuda.synchronize()
+    xn, wn = xn.cuda(), wn.cuda()
+    codes, scales = out[0]
+    held_gated(codes[:T].cpu().view(fo.E4M3), scales.cpu().t(), (xn @ wn.t()).cpu(), (xn.abs() @ wn.abs().t()).cpu(), K)
+    for c, s in out:
+        assert (c[T] == 0x55).all() and torch.equal(c, codes) and torch.equal(s, scales)
