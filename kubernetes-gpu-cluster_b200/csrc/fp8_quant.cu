@@ -69,16 +69,19 @@ fp8_quant_few_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, in
   if ((threadIdx.x & 7) == 0) scales[b * scales_stride + t] = scale;
 }
 
-// Many rows: a warp takes 512 columns of a row at a time, eight lanes a block as above, one piece after the other of an equal share of all, copied kAheadRows
-// pieces ahead into a ring of its own in shared memory.  A copy is 512 bytes one behind the other; a lane reads back the 32 that it turns into codes, whose
-// halves are exchanged in every second group of four lanes, so that eight lanes meet in no bank.  (Where a lane copied its own 32 bytes every sector was
-// fetched twice: 18.3 us where this takes 16.)  16384 rows of 2048 gathered from 2048 (43 MB, 6.6 us) 16 us, bound by instructions; 8192 rows of 4096
-// (101 MB, 15.5 us) 21.3, 20000 of 7168 (434 MB) 84.5, 5.1 TB/s, by memory; two pieces a step 15.7, 21.4 and 84.8, but 1200 rows of 4096 6.0 for 5.4; 16, 24
-// and 28 warps and as many more pieces ahead within 4 % of it.
-constexpr int kRowWarps = 32, kAheadRows = 6, kPiece = 1024;
+// Many rows: a warp takes 512 W columns of a row at a time, 16 W numbers a lane, one piece after the other of an equal share of all, copied ahead into a ring
+// of its own in shared memory.  A copy is 512 bytes one behind the other; a lane reads back the 32 W that it turns into codes, from places exchanged so that
+// eight lanes meet in no bank.  (Where a lane copied its own 32 bytes every sector was fetched twice: 18.3 us for 16 of 16384 rows of 2048.)
+// Bound by instructions where rows lie in the L2, 12 a number with W = 1 and 9.5 with W = 2, else by memory.  us with W = 1 and 2: 16384 rows of 2048 gathered
+// from 2048 (43 MB, 6.6 us at the copy's rate) 15.9 and 13.8, 8192 of 4096 (101 MB, 15.5 us) 21.0 and 20.2, 20000 of 7168 (434 MB) 86.4 and 80.6 (5.4 TB/s), of
+// 2560 32.1 and 31.4, of 640 10.7 and 9.9; but where the last piece is half empty, 20000 of 512 7.6 and 9.3, 6000 of 1408 6.9 and 7.3: W = 2 with at most 5/8
+// as many pieces.  With 16, 24 and 28 warps and as many more pieces ahead within 4 % of it.
+constexpr int kRowWarps = 32, kRing = 6 * 1024;            // warps; bytes of a warp's ring
+template <int W>
 __global__ void __launch_bounds__(kRowWarps * 32, 1)
 fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_t scales_stride, const bf16* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ rows,
                  uint32_t pieces, int K, uint32_t per_row) {
+  constexpr int kColumns = 512 * W, kPiece = 2 * kColumns, kAhead = kRing / kPiece, kMine = 16 * W;      // of a piece: columns, bytes; pieces ahead; columns of a lane
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_launch_dependents();
   pdl_wait();
@@ -88,25 +91,29 @@ fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_
   int n = (int)(each + (me < more));
   if (n == 0) return;
   const uint32_t t0 = first / per_row, last = (first + n - 1) / per_row;
-  const int k0 = (int)(first - t0 * per_row) * 512 + lane * 16;
-  // a piece's 16 bytes number c lie at c ^ (c / 8 & 1)
-  const uint8_t* ring = smem + warp * (kAheadRows * kPiece);
-  const int turned = (lane >> 2) & 1;
-  const uint8_t *lo = ring + (2 * lane + turned) * 16, *hi = ring + (2 * lane + 1 - turned) * 16;
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring) + ((lane ^ ((lane >> 3) & 1)) << 4), to_end = to + kAheadRows * kPiece;
+  const int k0 = (int)(first - t0 * per_row) * kColumns;
+  // a piece's 16 bytes number c lie at c ^ (c / 8 % 2W)
+  const uint8_t* ring = smem + warp * kRing;
+  const int turned = W == 1 ? (lane >> 2) & 1 : (lane >> 1) & 3;
+  const uint8_t* mine[2 * W];
+#pragma unroll
+  for (int j = 0; j < 2 * W; ++j) mine[j] = ring + (2 * W * lane + (j ^ turned)) * 16;
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring) + ((lane ^ ((lane >> 3) & (2 * W - 1))) << 4), to_end = to + kAhead * kPiece;
   auto row_of = [&](uint32_t t) { return rows && t <= last ? rows[t] : (int)t; };
   // the copies' way through the share: row, column, source; and the row after that, asked for a row ahead
   uint32_t t = t0, slot_in = to;
-  int k = k0 - lane * 8, r = row_of(t0), r_next = row_of(t0 + 1), left = n;
+  int k = k0 + lane * 8, r = row_of(t0), r_next = row_of(t0 + 1), left = n;
   const bf16* src = x + r * x_stride + k;
   auto copy = [&] {
     if (left > 0) {
       --left;
-      const bool a = r >= 0 && k < K, b = r >= 0 && k + 256 < K;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in), "l"(a ? src : x), "r"(a ? 16u : 0u) : "memory");
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in + 512), "l"(b ? src + 256 : x), "r"(b ? 16u : 0u) : "memory");
-      k += 512;
-      src += 512;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) {
+        const bool there = r >= 0 && k + i * 256 < K;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_in + i * 512), "l"(there ? src + i * 256 : x), "r"(there ? 16u : 0u) : "memory");
+      }
+      k += kColumns;
+      src += kColumns;
       if (k - lane * 8 >= K) {
         ++t;
         k = lane * 8;
@@ -119,35 +126,43 @@ fp8_quant_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales, int64_
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll 1
-  for (int i = 0; i < kAheadRows; ++i) copy();
-  int at = k0, slot = 0;
-  const int64_t blocks_on = 4 * scales_stride, row_on = 1 - (int64_t)(per_row - 1) * blocks_on;      // from one piece's scales to the next's, to the next row's first
-  uint8_t* dst = codes + (int64_t)t0 * K + k0;
-  float* sc = scales + (int64_t)(k0 / 128) * scales_stride + t0;
+  for (int i = 0; i < kAhead; ++i) copy();
+  int at = k0 + lane * kMine, slot = 0;
+  const int64_t blocks_on = 4 * W * scales_stride, row_on = 1 - (int64_t)(per_row - 1) * blocks_on;      // from one piece's scales to the next's, to the next row's first
+  uint8_t* dst = codes + (int64_t)t0 * K + at;
+  float* sc = scales + (int64_t)(at / 128) * scales_stride + t0;
 #pragma unroll 1
   for (; n > 0; --n) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kAheadRows - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
     __syncwarp();                                    // (a lane reads what others have copied)
-    const uint4 v[2] = {*reinterpret_cast<const uint4*>(lo + slot), *reinterpret_cast<const uint4*>(hi + slot)};
+    uint4 v[W][2];
+#pragma unroll
+    for (int j = 0; j < 2 * W; ++j) v[j / 2][j % 2] = *reinterpret_cast<const uint4*>(mine[j] + slot);
     __syncwarp();
     copy();
-    if ((slot += kPiece) == kAheadRows * kPiece) slot = 0;
-    uint32_t m2 = max2(mag2(v[0]), mag2(v[1]));
+    if ((slot += kPiece) == kAhead * kPiece) slot = 0;
+    uint32_t m2 = max2(mag2(v[0][0]), mag2(v[0][1]));
+    if (W == 2) m2 = max2(m2, max2(mag2(v[W - 1][0]), mag2(v[W - 1][1])));
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) m2 = max2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
+    for (int o = 4 / W; o > 0; o >>= 1) m2 = max2(m2, __shfl_xor_sync(0xffffffffu, m2, o));
     float scale, factor;
     fp8::scale_of(mag(m2), scale, factor);
     if (at < K) {
-      *reinterpret_cast<uint4*>(dst) = codes16(v, factor);
-      if ((lane & 7) == 0) *sc = scale;
+      if constexpr (W == 1) {
+        *reinterpret_cast<uint4*>(dst) = codes16(v[0], factor);
+      } else {
+        const uint4 a = codes16(v[0], factor), b = codes16(v[1], factor);
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
+      }
+      if (lane % (8 / W) == 0) *sc = scale;
     }
-    at += 512;
-    dst += 512;
-    if (at - lane * 16 < K) {
+    at += kColumns;
+    dst += kColumns;
+    if (at - lane * kMine < K) {
       sc += blocks_on;
     } else {
-      dst += K - (at - lane * 16);
-      at = lane * 16;
+      dst += K - (at - lane * kMine);
+      at = lane * kMine;
       sc += row_on;
     }
   }
@@ -240,16 +255,19 @@ extern "C" int KGE_API(kge_fp8_quant)(void* codes, float* scales, int scales_str
   const int blocks = (int)fp8::blocks(K);
   const int64_t units = (int64_t)T * blocks;
   KGE_REQUIRE(units < (1ll << 31) - 64 * 148 * 32 && K < 0x7fffffff - 1024, "kge_fp8_quant: %d rows of %d in one call", T, K);      // (columns are counted beyond K)
-  const int64_t per_row = (K + 511) / 512, pieces = T * per_row;
-  if (pieces < 2 * 148 * kRowWarps) {
+  const int64_t per_row = (K + 511) / 512;
+  if (T * per_row < 2 * 148 * kRowWarps) {
     KGE_CUDA_OK(launch_pdl(fp8_quant_few_kernel, dim3((unsigned)((units + 31) / 32)), dim3(256), 0, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride,
                            (const bf16*)x, (int64_t)x_stride, rows, (uint32_t)units, K, (uint32_t)blocks));
     return 0;
   }
-  const int smem = kRowWarps * kAheadRows * kPiece;
-  KGE_CUDA_OK(cudaFuncSetAttribute(fp8_quant_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  KGE_CUDA_OK(launch_pdl(fp8_quant_kernel, dim3(148), dim3(kRowWarps * 32), (size_t)smem, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride, (const bf16*)x,
-                         (int64_t)x_stride, rows, (uint32_t)pieces, K, (uint32_t)per_row));
+  const bool wide = K % 32 == 0 && ((uintptr_t)codes & 31) == 0 && 8 * ((per_row + 1) / 2) <= 5 * per_row;
+  const int64_t per = wide ? (per_row + 1) / 2 : per_row;
+  auto kern = wide ? fp8_quant_kernel<2> : fp8_quant_kernel<1>;
+  const int smem = kRowWarps * kRing;
+  KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  KGE_CUDA_OK(launch_pdl(kern, dim3(148), dim3(kRowWarps * 32), (size_t)smem, (cudaStream_t)stream, (uint8_t*)codes, scales, (int64_t)scales_stride, (const bf16*)x, (int64_t)x_stride,
+                         rows, (uint32_t)(T * per), K, (uint32_t)per));
   return 0;
 }
 

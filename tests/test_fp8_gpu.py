@@ -627,3 +627,21 @@ def test_gated_tiles_whose_sums_take_the_place_of_their_stages(kge, L, T, f, K):
     held_gated(codes[:T].cpu().view(fo.E4M3), scales.cpu().t(), (xn @ wn.t()).cpu(), (xn.abs() @ wn.abs().t()).cpu(), K)
     for c, s in out:
         assert (c[T] == 0x55).all() and torch.equal(c, codes) and torch.equal(s, scales)
+
+
+@pytest.mark.parametrize("dtype,T,K", [("bf16", 2400, 2080), ("fp16", 9500, 672), ("bf16", 4800, 1024), ("fp16", 1400, 3616), ("bf16", 9473, 544), ("bf16", 700, 7168)])
+@pytest.mark.parametrize("form", ["plain", "strided", "gathered"])
+def test_many_rows_bit_for_bit(kge, L, dtype, T, K, form):
+    test_rows_are_quantised_bit_for_bit(kge, L, dtype, T, K, form)
+
+
+@pytest.mark.parametrize("T,K", [(5, 4096), (2400, 2080), (9500, 672)])
+def test_codes_at_any_16_bytes(kge, L, T, K):
+    x = rows_of(torch.Generator().manual_seed(T), T, K, torch.bfloat16).cuda()
+    out = []
+    for off in (0, 16, 48):
+        room, scales = torch.full((T * K + 96,), 0x55, dtype=torch.uint8, device="cuda"), torch.zeros(-(-K // 128), T, device="cuda")
+        call(kge, "kge_fp8_quant", room[off:], scales, T, x, K, None, T, K)
+        out.append((room[off:off + T * K].clone(), scales))
+        assert (room[:off] == 0x55).all() and (room[off + T * K:] == 0x55).all()
+    assert all(torch.equal(c, out[0][0]) and torch.equal(s, out[0][1]) for c, s in out)
