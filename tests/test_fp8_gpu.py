@@ -645,3 +645,8 @@ def test_codes_at_any_16_bytes(kge, L, T, K):
         out.append((room[off:off + T * K].clone(), scales))
         assert (room[:off] == 0x55).all() and (room[off + T * K:] == 0x55).all()
     assert all(torch.equal(c, out[0][0]) and torch.equal(s, out[0][1]) for c, s in out)
+
+
+@pytest.mark.parametrize("dtype,E,N,K", [("bf16", 7, 700, 2320), ("fp16", 40, 130, 1296), ("bf16", 1, 3000, 2064), ("fp16", 300, 65, 48), ("bf16", 2, 10100, 528)])
+def test_weights_of_many_steps_bit_for_bit(kge, L, dtype, E, N, K):
+    test_weights_are_quantised_bit_for_bit(kge, L, dtype, E, N, K)
