@@ -426,13 +426,15 @@ __device__ __forceinline__ void store_gated(const Fp8Params& p, const Sums<128>&
 // -------------------------------------------------------------------------------------------------- tiles by single CTAs
 
 // What a CTA does: blocks of K [kb0, kb1) of tiles [tile0, tile1).  With at least half as many tiles as SMs each is one CTA's, and as many CTAs work as make
-// all have the same number (a weight stream needs bytes under way, not SMs); fewer are cut along K, into `splits` shares.
+// all have the same number (a weight stream needs bytes under way, not SMs); fewer are cut along K, into `splits` shares: of groups, where that saves more than
+// the way through the workspace costs, 5 us (gated 8).  us cut and whole: 16 rows in 8 groups of 1024 x 1024 8.8 and 5.9, 8 of 2048 x 4096 15.2 and 15.1, of 1024 x
+// 6144 14.4 and 15.7, 2 of 2048 x 14336 18.6 and 29.7; gated 256 x 1024 12.2 and 8.6, 256 x 3200 18.2 and 16.2, 1024 x 6144 20.4 and 25.3.
 struct Work { int tile0, tile1, kb0, kb1, splits; };
 // Blocks of K of a stage: the thread that issues the MMAs takes some 600 cycles from one pair of barriers to the next, and tiles of 128 columns have their
 // data in 370; besides, boxes of 128 bytes a row are read at 5.7 TB/s and two neighbouring ones at 6.35.
 __host__ __device__ constexpr int stream_sub(int nt) { return nt == 128 ? 2 : 1; }
 __device__ __forceinline__ Work work_of(int tiles, int KB, int splits, int me, int sms) {
-  if (splits == 0) splits = tiles == 0 || 2 * tiles >= sms ? 1 : max(1, min(min(sms / tiles, KB / 2), kMaxSplits));
+  if (splits == 0) splits = tiles == 0 || 2 * tiles >= sms || KB <= 32 ? 1 : max(1, min(min(sms / tiles, KB / 2), kMaxSplits));
   if (splits > 1) {
     const int tile = me / splits, piece = me - tile * splits;
     if (tile >= tiles) return Work{0, 0, 0, 0, splits};

@@ -650,3 +650,11 @@ def test_codes_at_any_16_bytes(kge, L, T, K):
 @pytest.mark.parametrize("dtype,E,N,K", [("bf16", 7, 700, 2320), ("fp16", 40, 130, 1296), ("bf16", 1, 3000, 2064), ("fp16", 300, 65, 48), ("bf16", 2, 10100, 528)])
 def test_weights_of_many_steps_bit_for_bit(kge, L, dtype, E, N, K):
     test_weights_are_quantised_bit_for_bit(kge, L, dtype, E, N, K)
+
+
+@pytest.mark.parametrize("sizes,N,K", [([1], 64, 4240), ([5, 0, 1, 0, 0, 40], 136, 5136), ([33, 70], 520, 8208), ([0, 128, 3], 384, 4112), ([97, 0, 2, 31], 640, 4224), ([7] * 12, 256, 4608)],
+                         ids=lambda v: str(v) if isinstance(v, int) else "x".join(map(str, v)))
+@pytest.mark.parametrize("form", ["bf16", "fp16", "gated"])
+@pytest.mark.parametrize("first,behind", [(0, 0), (3, 9)])
+def test_groups_cut_along_k(kge, L, sizes, N, K, form, first, behind):
+    test_grouped(kge, L, sizes, N, K, form, first, behind)
