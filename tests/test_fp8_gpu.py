@@ -559,7 +559,7 @@ def test_more_than_32_bits_of_elements(kge, L):
 
 ALIGNED = [  # T, N, K: tiles of 256 columns, several a CTA; tiles of 128 cut along K over a cluster; pairs, whole and ragged; a column more, then seven
     (70, 19001, 144), (33, 19175, 144), (130, 30002, 144), (1, 4097, 2064), (64, 1001, 1040), (100, 3005, 1296), (9, 3, 528), (128, 6143, 528), (1030, 2049, 272), (2050, 1029, 400),
-    (777, 4095, 144)]
+    (777, 4095, 144), (200, 1024, 400), (64, 2048, 528), (600, 4096, 144), (3, 40000, 144), (1, 4096, 2064)]
 
 
 @pytest.mark.parametrize("T,N,K", ALIGNED)
