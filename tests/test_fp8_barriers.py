@@ -20,7 +20,7 @@ PAIR_OPS = [
     "wait full(stage), phase", "wait tempty(2 * buf + h), buf_phase ^ 1", "test full(s1), p1", "test tempty(2 * v1 + h), w1 ^ 1", "commit tfull(2 * buf + h), 3",
     "commit empty(stage), 3",
     "wait tfull(2 * buf + part), buf_phase", "arrive lead_tempty + 16u * buf", "wait tfull(2 * buf + part), buf_phase", "wait tfull(2 * buf + part), buf_phase"]
-CALLS = {"mbar_wait": "wait", "mbar_test": "test", "bar_expect": "expect", "bar_arrive": "arrive", "bar_arrive_at": "arrive", "commit": "commit", "commit2": "commit"}
+CALLS = {"mbar_wait": "wait", "mbar_test": "test", "bar_expect": "expect", "bar_arrive": "arrive", "bar_arrive_at": "arrive", "bar_arrive_lane0": "arrive", "commit": "commit", "commit2": "commit"}
 
 
 def operations(kernel, begin):
@@ -33,7 +33,7 @@ def operations(kernel, begin):
         while depth:
             depth += {"(": 1, ")": -1}.get(body[i], 0)
             i += 1
-        out.append(CALLS[m.group(1)] + " " + body[m.end():i - 1])
+        out.append(CALLS[m.group(1)] + " " + body[m.end():i - 1].removesuffix(", lane"))
     return out
 
 
