@@ -479,8 +479,8 @@ __device__ __forceinline__ float lds1(uint32_t at) {
 // distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
 // Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
 // Bound by the weights' way from memory, and at one or two tiles a CTA by what is before and behind it: about 2 us from the launch to the first bytes and 2
-// to 3 for the last tile's sums, exchange and stores.  64 tokens: eight each of 128 experts, gated 1536 x 2048 (376 MB) 69.4 us, 5.4 TB/s; gated 28672 x 4096
-// (119 MB) 25.4 us; 4096 x 6144 (26 MB) 10.5 us; one token, 4096 x 14336 (59 MB) 14.7 us.
+// to 3 for the last tile's sums, exchange and stores.  64 tokens: eight each of 128 experts, gated 1536 x 2048 (376 MB) 69 us, 5.4 TB/s; gated 28672 x 4096
+// (119 MB) 25.0 us; 4096 x 6144 (26 MB) 10.5 us; one token, 4096 x 14336 (59 MB) 14.7 us.
 template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
@@ -893,8 +893,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // two blocks, and the first and the second 128 columns of each are handed over apart, as soon as their four warps have read them.  Six stages and 2 KB a warp
 // through which rows are stored; four stages and a whole tile stored by copies from shared memory took 410 us where this took 399.
 // Bound by the power limit when it runs over and over, else by the 573 cycles that a block of K takes and by a tile's end (3000 cycles, gated 3400, under which
-// two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 385 us (2.5 PFLOP/s; over and over 441; copies and MMAs alone 334), gated 28672 x
-// 4096 796 us (2.4 PFLOP/s; 895; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 67.6 us.
+// two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 380 us (2.5 PFLOP/s; over and over 430; copies and MMAs alone 334), gated 28672 x
+// 4096 796 us (2.4 PFLOP/s; 880; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 66 us.
 template <bool GATED, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
