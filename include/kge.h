@@ -273,7 +273,8 @@ int kge_gemm_fp8(void* y, const void* x, const float* x_scales, int x_scales_str
 int64_t kge_gemm_fp8_workspace_bytes(int T);
 
 /* The gated front half: h = silu(x w[:f]^T) * (x w[f:]^T), w = [gate | up] [2f, K], f a multiple of 128, quantised as kge_fp8_quant does - codes [T, f] and
- * scales [f / 128][scales_stride] for the product behind it.  Everything between the sums and the codes is in fp32. */
+ * scales [f / 128][scales_stride] for the product behind it.  h is in fp32, off by 2^-20 of silu(gate) up of the two sums at most (gates above -174), and of
+ * that h scales and codes are exactly what the definition says. */
 int kge_gemm_fp8_silu_gate(void* codes, float* scales, int scales_stride, const void* x, const float* x_scales, int x_scales_stride,
                            const void* w_gate_up, const float* w_scales, int T, int f, int K, void* workspace, int64_t workspace_bytes, void* stream);
 

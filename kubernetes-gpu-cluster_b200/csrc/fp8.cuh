@@ -34,6 +34,31 @@ __device__ __forceinline__ void scale_of(float m, float& scale, float& factor) {
   scale = fine ? fmaxf(q, kLeast) : __int_as_float(0x7fffffff);
   factor = fine ? inv * (kMax * 0.0625f) : 0.f;
 }
+
+// fp32 numbers of a block as codes.  A product with the factor is off by a few 2^-24 and may lie on the other side of half a step than 448 h / m does.  So a number's code
+// is taken from just below and just above it, and four numbers of which one has two codes (1 in 50000) are marked and settled exactly.
+struct Rows32 {
+  float m, factor, below, above;                             // (m: no less than the magnitude that has the smallest scale)
+  // The factor within a rounding, 2^-24, by a Newton step; with that of `below` and of the product, three together, 2^-22 is enough between them.
+  __device__ __forceinline__ Rows32(float top, float f) : m(fmaxf(top, kMax * kLeast)) {
+    factor = fmaf(fmaf(-m, f, kMax) * (1.f / kMax), f, f);
+    below = factor * (1.f - 0x1p-22f);
+    above = factor * (1.f + 0x1p-22f);
+  }
+  __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, uint32_t& marked, int at) const {
+    const uint32_t lo = pack4(a * below, b * below, c * below, d * below), hi = pack4(a * above, b * above, c * above, d * above);
+    if (lo != hi) marked |= 1u << at;
+    return lo;
+  }
+  // A number on h's side of every half step, or on it.  Those and the codes have four bits behind the first at most: of such numbers the product's nearest, t,
+  // is either no half step or the one next to 448 h / m, and 448 h - t m (33 and 29 bits) has the sign of what is between them.
+  __device__ __forceinline__ float settled(float h) const {
+    const uint32_t t = (__float_as_uint(h * factor) + 0x40000u) & ~0x7ffffu;
+    const double r = fma(-(double)fabsf(__uint_as_float(t)), (double)m, 448.0 * (double)fabsf(h));
+    return __uint_as_float(t + (r > 0.0) - (r < 0.0));
+  }
+  __device__ __forceinline__ uint32_t settled4(float a, float b, float c, float d) const { return pack4(settled(a), settled(b), settled(c), settled(d)); }
+};
 #endif
 }  // namespace fp8
 }  // namespace kge
