@@ -1213,7 +1213,8 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   if constexpr (GATED || NT == 128) {
     if (cluster) kern = fp8_stream_kernel<NT, GATED, true>;
   }
-  KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // the function's limit, for every size: one set for this call could be lowered by another thread's before the launch
+  KGE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem - kOwn));
   prefer_max_shared(kern);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(cluster ? tiles * p.splits : sms)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
