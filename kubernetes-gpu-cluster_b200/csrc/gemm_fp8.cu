@@ -67,14 +67,23 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) { asm vol
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void bar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// On a barrier of the pair's leader.  What it tells is that tensor memory has been read (tcgen05.wait::ld, the fence before): nothing in memory is
-// published, and a release for the whole cluster would wait for all of a thread's stores, every block of K (2048 x 9472 x 4096: 194 us with it).
+// On a barrier of the pair's leader.  What it tells is that tensor memory has been read (tcgen05.wait::ld, the fence before), or that factors are on their way (Told
+// publishes them): nothing in memory is published, and a release for the whole cluster is a fence every block of K (2048 x 9472 x 4096: 194 us with it by those
+// that add up, 85 with it by those that bring in, 66.5 without).
 __device__ __forceinline__ void bar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // The same by lane 0 of a warp, without a branch that the other lanes would have to wait behind (2 % of a block of K).
 __device__ __forceinline__ void bar_arrive_lane0(uint32_t bar, int lane) {
   asm volatile("{\n.reg .pred p;\nsetp.eq.s32 p, %1, 0;\n@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n}" ::"r"(bar), "r"(lane) : "memory");
 }
+// A barrier for each slot of a ring: who fills a slot tells the readers, all in its own CTA.  (The pair's stages go to the leader's threads and back; what the other CTA
+// stores would have to be released to the cluster on that way.)
+struct Told {
+  uint32_t bars;
+  __device__ __forceinline__ void init(int slots) const { for (int s = 0; s < slots; ++s) bar_init(bars + 8u * s, 1); }
+  __device__ __forceinline__ void tell(int slot) const { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bars + 8u * slot) : "memory"); }
+  __device__ __forceinline__ void wait(int slot, uint32_t phase) const { mbar_wait(bars + 8u * slot, phase); }
+  __device__ __forceinline__ bool test(int slot, uint32_t phase) const { return mbar_test(bars + 8u * slot, phase); }
+};
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
@@ -922,7 +931,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   constexpr uint32_t kStage = 2 * kSlab;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * STAGES + 8];
+  __shared__ uint64_t bars[2 * STAGES + 8 + kPairSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t tops[GATED ? 256 : 1];
   __shared__ __align__(16) uint32_t biases[GATED ? 4 : kSumWarps * 64];       // of each warp that adds up
@@ -933,6 +942,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto tfull = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
   auto tempty = [&](int b) { return bar0 + 8u * (2 * STAGES + 4 + b); };
+  const Told told{bar0 + 8u * (2 * STAGES + 8)};    // factors, and with a tile's first ones its place
   const int warp = uniform_warp(), lane = threadIdx.x & 31, rank = (int)cluster_ctarank();
 
   if (warp == 0 && lane == 0) {
@@ -942,6 +952,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (warp == 1 && lane == 0) {
     for (int s = 0; s < STAGES; ++s) { bar_init(full(s), 3); bar_init(empty(s), 2); }       // (full: the leader's copies, both CTAs' factors)
     for (int b = 0; b < 4; ++b) { bar_init(tfull(b), 1); bar_init(tempty(b), kSumWarps); }       // (of two blocks, the first and the second 128 columns)
+    told.init(kPairSlots);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -999,7 +1010,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           __syncwarp();
           f.put(factors + slot * 256, i, lane);
           __syncwarp();
-          if (lane == 0) bar_arrive_at(lead);
+          if (lane == 0) {
+            told.tell(slot);
+            bar_arrive_at(lead);                     // (so that when a block's sums are there its factors mostly are)
+          }
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
           if (++slot == kPairSlots) slot = 0;
         }
@@ -1039,8 +1053,9 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const int q = warp & 3, part = (warp - 4) >> 2, lane128 = q * 32 + lane;
     const uint32_t lead_tempty = mapa_u32(tempty(part), 0);
     int buf = 0, slot = 0, tile = 0;
-    uint32_t buf_phase = 0;
+    uint32_t buf_phase = 0, slot_phase = 0;
     for (int w = first; w < total; w += step) {
+      told.wait(slot, slot_phase);
       mbar_wait(tfull(2 * buf + part), buf_phase);
       const int4 found = tiles[tile++ & 15];
       const Tile t = same(Tile{0, found.x, found.y, found.z});
@@ -1052,18 +1067,22 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
       uint32_t* own = biases + (GATED ? 0 : (warp - 4) * 64);
       if (!GATED && p.bias) ask_bias<2, 64>(p, own, n0, lane);
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + part * 128;
+      bool seen = true;                               // a slot is asked for a block ahead (where it is wanted, 4 % more)
       auto read = [&] {
         fence_before();
         bar_arrive_lane0(lead_tempty + 16u * buf, lane);
         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
-        if (++slot == kPairSlots) slot = 0;
+        if (++slot == kPairSlots) { slot = 0; slot_phase ^= 1; }
       };
       auto wait = [&](uint32_t& from, float& f0, float& f1) {
-        mbar_wait(tfull(2 * buf + part), buf_phase);
-        fence_after();
+        if (!seen) told.wait(slot, slot_phase);
+        const bool last = slot + 1 == kPairSlots;
+        seen = told.test(last ? 0 : slot + 1, slot_phase ^ last);
         const float* f = factors + slot * 256 + lane128;
         f0 = f[GATED ? 0 : part * 128];
         f1 = GATED ? f[128] : f0;
+        mbar_wait(tfull(2 * buf + part), buf_phase);
+        fence_after();
         from = at + buf * 256;
       };
       if (some) {
