@@ -610,6 +610,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
     }
   } else if (warp == 1) {
     regs_down<kOtherRegs>();
+    pdl_wait();                                     // (nothing is there to multiply before; a wait at a barrier, limited in time, would span what is left of the kernel before)
     if (elect_one()) {
       constexpr uint32_t idesc = instr_desc(kRows, NT);
       int stage = 0, buf = 0;

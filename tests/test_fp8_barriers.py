@@ -374,3 +374,15 @@ def test_a_slot_is_told_before_it_is_read():
     assert re.search(r"told\.wait\(slot, slot_phase\);\s*mbar_wait\(tfull\(2 \* buf \+ part\), buf_phase\);\s*const int4 found = tiles", body)
     assert re.search(r"if \(!seen\) told\.wait\(slot, slot_phase\);\s*const bool last = [^;]*;\s*seen = told\.test\([^;]*;\s*const float\* f = factors", body)
     assert body.count("= factors + slot") == 1 and body.count("= tiles[") == 1
+
+
+@pytest.mark.parametrize("kernel,roles", [("fp8_stream_kernel", 4), ("fp8_pair_kernel", 3)])
+def test_no_barrier_wait_spans_the_kernel_before(kernel, roles):
+    """Waits at barriers are limited in time, and what the kernel before takes is not: whoever waits at one has waited for that kernel's end first."""
+    body = re.sub(r"//[^\n]*", "", SRC[SRC.index(kernel + "(const __grid"):])
+    body = body[:re.search(r"\n}\n", body).start()]
+    parts = re.split(r"\n  (?:\} else )?(?:if \(warp [^\n]*\) \{|else \{|\} else \{)\s*\n    regs_\w+<\w+>\(\);", body)
+    begin, waiting = parts[0], [r for r in parts[1:] if re.search(r"\bmbar_wait\(|\.wait\(", r)]
+    assert len(waiting) == roles and "mbar_wait(" not in begin
+    for role in waiting:
+        assert re.search(r"\n  pdl_wait\(\);", begin) or role.index("pdl_wait();") < re.search(r"\bmbar_wait\(|\.wait\(", role).start()
