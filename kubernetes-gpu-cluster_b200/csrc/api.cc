@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "fresh_weights.h"
 #include "half_bits.h"
 #include "kge.h"
 
@@ -36,6 +37,17 @@ bool pdl_for_this_launch() {
   const bool brk = g_pdl_break;
   g_pdl_break = false;
   return pdl_enabled() && !brk && g_pdl_suspended <= 0;
+}
+static FreshWeights g_fresh;
+void pdl_weights_written(cudaStream_t stream) { g_fresh.written(stream); }
+bool pdl_for_weights(cudaStream_t stream) {
+  const bool early = pdl_for_this_launch();
+  return !g_fresh.take(stream, [stream] {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &s) == cudaSuccess) return s != cudaStreamCaptureStatusNone;
+    (void)cudaGetLastError();
+    return true;
+  }) && early;
 }
 
 static std::atomic<int> g_tun[TUN_COUNT] = {{1}, {0}, {0}, {0}, {1}, {0}, {1}, {0}, {1}, {1}};   // even grid measured +6.5 % on the gate_up GEMM of Llama-3.1-8B

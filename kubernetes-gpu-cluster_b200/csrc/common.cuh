@@ -17,6 +17,10 @@ void pdl_set_enabled(bool on);
 // relies on griddepcontrol.wait).  Used right after a kernel that is not ours (NCCL).  pdl_for_this_launch() consumes it.
 void pdl_break_next();
 bool pdl_for_this_launch();
+// pdl_weights_written(stream): a kernel that writes weights has been launched on `stream`.  pdl_for_weights(stream) is pdl_for_this_launch() for a kernel that reads
+// weights before griddepcontrol.wait: the first one behind such a writer is an ordinary launch (fresh_weights.h).
+void pdl_weights_written(cudaStream_t stream);
+bool pdl_for_weights(cudaStream_t stream);
 // pdl_suspend(true) .. pdl_suspend(false): every launch of this thread in between is an ordinary stream-ordered launch.
 void pdl_suspend(bool on);
 // Launch-shape knobs behind kge_set_tunable() (api.cc): heuristics that only change HOW work is

@@ -287,6 +287,6 @@ extern "C" int KGE_API(kge_fp8_quant_weight)(void* codes, float* scales, const v
   KGE_CUDA_OK(cudaFuncSetAttribute(fp8_quant_weight_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   KGE_CUDA_OK(launch_pdl(fp8_quant_weight_kernel, dim3((unsigned)(steps < 148 ? steps : 148)), dim3(kWThreads), (size_t)smem, (cudaStream_t)stream, (uint8_t*)codes, scales,
                          (const bf16*)w, N, K, (uint32_t)steps, (uint32_t)steps_k, (uint32_t)steps_n));
-  pdl_break_next();        // a product that is launched early reads weights before it waits for the kernel before it
+  pdl_weights_written((cudaStream_t)stream);        // a product that is launched early reads weights before it waits for the kernel before it
   return 0;
 }

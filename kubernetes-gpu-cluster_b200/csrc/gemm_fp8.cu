@@ -1240,7 +1240,7 @@ static int launch_stream(Fp8Params& p, const void* x, const void* w, int K, cuda
   cfg.gridDim = dim3((unsigned)(cluster ? tiles * p.splits : sms)); cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = pdl_for_this_launch() ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = (p.offsets ? pdl_for_this_launch() : pdl_for_weights(st)) ? 1 : 0;      // (grouped rows wait before they read anything)
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = p.splits; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = cluster ? 2 : 1;
