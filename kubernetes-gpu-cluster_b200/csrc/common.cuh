@@ -171,6 +171,15 @@ inline void prefer_max_shared(K kern) {
   if (tunable(TUN_SMEM_CARVEOUT)) (void)cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
+// A driver call that needs the calling thread's context.  Calls of the runtime bind one to a thread that has none yet, the driver's do not: tried again then, behind a
+// question about a kernel of this library.
+template <typename R, typename K, typename F>
+inline R with_context(R no_context, K kern, F call) {
+  const R r = call();
+  cudaFuncAttributes a;
+  return r == no_context && cudaFuncGetAttributes(&a, kern) == cudaSuccess ? call() : r;
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
   prefer_max_shared(kern);
