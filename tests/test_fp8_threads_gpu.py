@@ -59,3 +59,33 @@ def test_two_threads(kge, L, form, N, K, one, two):
     torch.cuda.synchronize()
     assert not failed, (len(failed), failed[0])
     assert all(torch.equal(a, b) for (out, *_), want in zip(jobs, alone) for a, b in zip(out, want))
+
+
+def test_weights_written_by_one_thread_and_read_by_another(kge, L):
+    """A matrix is quantised anew on a stream, the same thread launches on another stream, and another thread makes the products on the first: each has this turn's weights."""
+    T, N, K, turns = 64, 4096, 1024, 60
+    g = torch.Generator().manual_seed(3)
+    x, xs, _ = quantised(g, T, K, 1)
+    x, xs = x.cuda(), xs.t().contiguous().cuda()
+    mats = [(torch.randn(N, K, generator=g) * 0.03 * (i + 1)).to(torch.bfloat16).cuda() for i in range(3)]
+    cw, sw, other = torch.zeros(N, K, dtype=torch.uint8, device="cuda"), torch.zeros(N // 128, K // 128, device="cuda"), [torch.zeros(T, K, dtype=torch.uint8, device="cuda"), torch.zeros(K // 128, T, device="cuda")]
+    rows, work = torch.randn(T, K, generator=g).to(torch.bfloat16).cuda(), workspace(L, T)
+    want = []
+    for m in mats:
+        y = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+        call(kge, "kge_fp8_quant_weight", cw, sw, m, 1, N, K)
+        torch.cuda.synchronize()
+        call(kge, "kge_gemm_fp8", y, x, xs, T, cw, sw, None, T, N, K, work, work.numel())
+        want.append(y)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    out = [torch.zeros(T, N, dtype=torch.bfloat16, device="cuda") for _ in range(turns)]
+    torch.cuda.synchronize()
+    for i in range(turns):
+        call(kge, "kge_fp8_quant_weight", cw, sw, mats[i % 3], 1, N, K, stream=a)
+        call(kge, "kge_fp8_quant", *other, T, rows, K, None, T, K, stream=b)
+        t = threading.Thread(target=call, args=(kge, "kge_gemm_fp8", out[i], x, xs, T, cw, sw, None, T, N, K, work, work.numel()), kwargs=dict(stream=a))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(out))
