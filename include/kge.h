@@ -263,7 +263,8 @@ int kge_fp8_quant(void* codes, float* scales, int scales_stride, const void* x, 
 int kge_fp8_quant_weight(void* codes, float* scales, const void* w, int E, int N, int K, void* stream);
 
 /* y[T, N] = x w^T (+ bias[N], 16 bits, may be NULL) from codes and scales of x [T, K] and of w [N, K]: products of a block of K are summed in fp32, times
- * the two scales added up over the blocks in fp32, and rounded once.  Scales that are infinite or NaN make what they touch so.  y and bias need no more
+ * the two scales added up over the blocks in fp32, and rounded once.  Scales that are infinite or NaN make what they touch so.  The two scales are multiplied first,
+ * in fp32: where their product is below 2^-126 it is off by up to 2^-150, from 2^128 on it is infinite.  y and bias need no more
  * alignment than their type's (rows that are 16-byte aligned, N % 8 == 0, are stored fastest); the result's bits are the same at any address and each time.
  * `workspace`: device scratch of kge_gemm_fp8_workspace_bytes(T) bytes, 16-byte aligned, whose first 1024 bytes are ZERO before the first call that
  * uses it (every call leaves them zero again; the grouped products' partial sums).  Calls that share a workspace must not overlap on the GPU.  Weights
