@@ -180,7 +180,7 @@ fp8_quant_weight_kernel(uint8_t* __restrict__ codes, float* __restrict__ scales,
   __shared__ uint32_t part[2][2][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
-  const int blocks_k = (K + 127) / 128, blocks_n = (N + 127) / 128;
+  const int blocks_k = (K - 1) / 128 + 1, blocks_n = (N - 1) / 128 + 1;
   // a step's matrix, block row and pair of block columns; the CTA's next step is gridDim.x further
   const uint32_t dk = gridDim.x % steps_k, dr = gridDim.x / steps_k, dn = dr % steps_n, de = dr / steps_n;
   struct At { uint32_t e, n, k; };
@@ -281,8 +281,8 @@ extern "C" int KGE_API(kge_fp8_quant_weight)(void* codes, float* scales, const v
   KGE_REQUIRE(E > 0 && N > 0, "kge_fp8_quant_weight: %d matrices of %d rows", E, N);
   KGE_REQUIRE(K > 0 && K % 16 == 0, "kge_fp8_quant_weight: K=%d must be a positive multiple of 16", K);
   KGE_REQUIRE(aligned16(codes) && aligned16(w) && ((uintptr_t)scales & 3) == 0, "kge_fp8_quant_weight: codes and w must be 16-byte aligned");
-  const int64_t steps_k = (K + 255) / 256, steps_n = fp8::blocks(N), steps = steps_k * steps_n * E;
-  KGE_REQUIRE(steps < (1ll << 31) - 4 * 148, "kge_fp8_quant_weight: %d matrices of %d x %d in one call", E, N, K);
+  const int64_t most = (1ll << 31) - 4 * 148, steps_k = ((int64_t)K + 255) / 256, steps_n = fp8::blocks(N), steps = steps_k * steps_n < most ? steps_k * steps_n * E : most;
+  KGE_REQUIRE(steps < most, "kge_fp8_quant_weight: %d matrices of %d x %d in one call", E, N, K);
   const int smem = kWStages * kWStage;
   KGE_CUDA_OK(cudaFuncSetAttribute(fp8_quant_weight_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   KGE_CUDA_OK(launch_pdl(fp8_quant_weight_kernel, dim3((unsigned)(steps < 148 ? steps : 148)), dim3(kWThreads), (size_t)smem, (cudaStream_t)stream, (uint8_t*)codes, scales,

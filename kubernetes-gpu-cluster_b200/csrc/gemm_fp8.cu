@@ -1307,7 +1307,7 @@ static int gemm_fp8(const char* name, Fp8Params& p, bool gated, const void* x, i
   p.w_rows = (int)rows;
   p.w_blocks = (int)fp8::blocks(rows);
   const int64_t tiles = ((int64_t)p.T / kRows + p.E) * p.w_blocks;
-  KGE_REQUIRE(tiles * p.KB < (1ll << 31), "%s: %lld tiles of %d blocks in one call", name, (long long)tiles, p.KB);
+  KGE_REQUIRE(tiles < (1ll << 31) && tiles * p.KB < (1ll << 31), "%s: %lld tiles of %d blocks in one call", name, (long long)tiles, p.KB);
   KGE_REQUIRE(workspace && workspace_bytes >= workspace_bytes_of(p.T) && aligned_to(workspace, 16), "%s: needs a workspace of %lld bytes, 16-byte aligned", name,
               (long long)workspace_bytes_of(p.T));
   p.count = (unsigned int*)workspace;

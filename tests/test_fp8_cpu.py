@@ -82,3 +82,21 @@ def test_workspace_sizes(kge):
     assert L.kge_gemm_fp8_workspace_bytes(0) == 0 and L.kge_gemm_fp8_workspace_bytes(-5) == 0
     sizes = [L.kge_gemm_fp8_workspace_bytes(t) for t in (1, 32, 33, 64, 128, 129, 8192, 2 ** 31 - 1)]
     assert sizes == sorted(sizes) and sizes[0] == sizes[1] and sizes[4] == sizes[-1] <= 64 << 20
+
+
+@pytest.mark.parametrize("f16", ["", "_f16"])
+@pytest.mark.parametrize("E,N,K", [(2 ** 30, 2 ** 31 - 100, 2 ** 18), (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 16), (2 ** 24, 2 ** 31 - 128, 2 ** 24)])
+def test_matrices_whose_steps_64_bits_do_not_count(kge, f16, E, N, K):
+    refused(kge, getattr(kge.lib(), "kge_fp8_quant_weight" + f16)(P, P, P, E, N, K, None), "in one call")
+
+
+@pytest.mark.parametrize("f16", ["", "_f16"])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_products_whose_tiles_64_bits_do_not_count(kge, f16, grouped):
+    T = N = 2 ** 31 - 257
+    args = [P, P, P, 2 ** 31 - 1, P, P, P] + ([1] if grouped else []) + [T, N, 2 ** 31 - 16, P, 1 << 30, None]
+    refused(kge, getattr(kge.lib(), "kge_gemm_fp8" + ("_grouped" if grouped else "") + f16)(*args), "in one call")
+    if not f16:
+        f = 2 ** 30 - 256
+        args = [P, P, 2 ** 31 - 1, P, P, 2 ** 31 - 1, P, P] + ([P, 1] if grouped else []) + [T, f, 2 ** 31 - 16, P, 1 << 30, None]
+        refused(kge, getattr(kge.lib(), "kge_gemm_fp8" + ("_grouped" if grouped else "") + "_silu_gate")(*args), "in one call")
