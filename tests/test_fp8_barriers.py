@@ -386,3 +386,91 @@ def test_no_barrier_wait_spans_the_kernel_before(kernel, roles):
     assert len(waiting) == roles and "mbar_wait(" not in begin
     for role in waiting:
         assert re.search(r"\n  pdl_wait\(\);", begin) or role.index("pdl_wait();") < re.search(r"\bmbar_wait\(|\.wait\(", role).start()
+
+
+def exchange(S, over, gated, rng, early=False):
+    """The end of a cluster's tile (fp8_stream_kernel, CLUSTER): S CTAs, in each the warps that add up and the others, who take the same barriers of the cluster."""
+    arrived, counts = [0] * 8, {}                             # phases of the cluster's barrier: two arrivals a CTA each
+    stages_read, begun, gone = [False] * S, [False] * S, [0] * S
+    sums, tops, kept = [set() for _ in range(S)], [set() for _ in range(S)], [False] * S
+
+    def arrive(who):
+        arrived[counts.setdefault(who, 0)] += 1
+        counts[who] += 1
+
+    def wait(who):
+        return lambda: arrived[counts[who] - 1] == 2 * S
+
+    def remote(c):
+        assert begun[c], "a CTA that may not have begun is written to"
+        assert gone[c] < 2, "a CTA that may be gone is written to"
+
+    def adding(c):
+        me = ("sums", c)
+        yield None
+        begun[c] = True
+        if not over:
+            arrive(me)
+        yield None
+        stages_read[c] = True                                  # (its last block's sums are there: the MMAs have read the stages)
+        if over and not early:
+            arrive(me)
+        if not early:
+            yield wait(me)
+        for to in range(S):
+            remote(to)
+            assert not over or stages_read[to], "sums are laid over stages that are still read"
+            assert c not in sums[to]
+            sums[to].add(c)
+            yield None
+        arrive(me)
+        yield wait(me)
+        assert len(sums[c]) == S, "sums are missing"
+        if gated:
+            kept[c] = True                                     # (h, in the place of the first sender's sums)
+            for to in range(S):
+                remote(to)
+                tops[to].add(c)
+                yield None
+            arrive(me)
+            yield wait(me)
+            assert len(tops[c]) == S and kept[c]
+        gone[c] += 1
+
+    def others(c):
+        me = ("others", c)
+        yield None
+        if not over:
+            arrive(me)
+        yield None
+        for n in range(1 + (over and not early) + gated):
+            if n == 0 and not over:
+                yield wait(me)
+            arrive(me)
+            yield wait(me)
+        gone[c] += 1
+    run([r for c in range(S) for r in (adding(c), others(c))], [], rng)
+    assert all(len(s) == S for s in sums) and len(set(counts.values())) == 1
+
+
+@pytest.mark.parametrize("S", [2, 3, 5, 8])
+@pytest.mark.parametrize("over,gated", [(False, False), (False, True), (True, True)])
+def test_a_clusters_exchange(S, over, gated):
+    for seed in range(40):
+        exchange(S, over, gated, random.Random(seed * 10 + S))
+
+
+def test_an_exchange_without_its_first_barrier_is_seen():
+    with pytest.raises(AssertionError, match="begun|still read"):
+        for seed in range(40):
+            exchange(4, True, True, random.Random(seed), early=True)
+
+
+def test_all_warps_take_the_clusters_barriers_alike():
+    """In the source: before the roles, by those that add up, and by the others behind them."""
+    body = re.sub(r"//[^\n]*", "", SRC[SRC.index("fp8_stream_kernel(const __grid"):])
+    body = body[:re.search(r"\n}\n", body).start()]
+    calls = re.findall(r"(?:if \([^()]*\) )?\{? ?cluster_(?:arrive_relaxed|arrive|wait)\(\);", body)
+    take = lambda part: ["over: arrive" if "p.over" in c and "arrive()" in c else re.search(r"arrive_relaxed|arrive|wait", c).group() for c in part]
+    assert "CLUSTER && !p.over" in calls[0] and take(calls) == ["arrive_relaxed"] + 2 * ["over: arrive", "wait", "arrive", "wait", "arrive", "wait"]
+    assert body.count("if constexpr (GATED) {\n          // the block's largest") <= 1 and "if (GATED) { cluster_arrive(); cluster_wait(); }" in body
