@@ -18,7 +18,11 @@ class FreshWeights {
     std::lock_guard<std::mutex> lock(m_);
     for (const Key& o : streams_)
       if (o == k) return;
-    streams_.push_back(k);
+    try {
+      streams_.push_back(k);
+    } catch (...) {                              // (callers are C: without room for it, every stream's products are ordinary from now on)
+      all_ = true;
+    }
     some_.store(true, std::memory_order_release);
   }
   // Whether a product on `stream` has to be an ordinary launch; asked once for a launch that then is.  capturing(): whether the stream records a graph, whose
@@ -33,11 +37,11 @@ class FreshWeights {
         if (!capturing()) {
           streams_[i] = streams_.back();
           streams_.pop_back();
-          some_.store(!streams_.empty(), std::memory_order_release);
+          some_.store(all_ || !streams_.empty(), std::memory_order_release);
         }
         return true;
       }
-    return false;
+    return all_;
   }
 
  private:
@@ -52,6 +56,7 @@ class FreshWeights {
   }
   std::mutex m_;
   std::vector<Key> streams_;                     // few: an entry stays until its stream's next product, once for a stream
+  bool all_ = false;
   std::atomic<bool> some_{false};
 };
 }  // namespace kge
