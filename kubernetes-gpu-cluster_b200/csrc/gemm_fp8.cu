@@ -165,7 +165,7 @@ __device__ __forceinline__ void count_tiles(const Fp8Params& p, int tile_rows, G
 // A tile: rows [row, row + rows) of the tokens and column tile n of group e.
 struct Tile { int e, n, row, rows; };
 // A value that all lanes of a converged warp have, so that the compiler knows it: what comes out of shared memory it takes for different in each (gated 8192 x
-// 28672 x 4096 802 us without, 796 with).
+// 28672 x 4096 802 us without, 796 with, both before what gated results cost now).
 __device__ __forceinline__ int same(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ Tile same(const Tile& t) { return Tile{same(t.e), same(t.n), same(t.row), same(t.rows)}; }
 // From a tile's number; the group is looked for from `e` on (numbers come in rising order).  Tiles of a group run over BAND token tiles (0: all), then
@@ -504,8 +504,8 @@ __device__ __forceinline__ float lds1(uint32_t at) {
 // distributed shared memory; they are added in the order of K, so the result's bits are the same each time.
 // Otherwise shares (of grouped rows, whose number of tiles the host does not know) go through the workspace: the last to arrive adds them, in that order too.
 // Bound by the weights' way from memory, and at one or two tiles a CTA by what is before and behind it: about 2 us from the launch to the first bytes and 2
-// to 3 for the last tile's sums, exchange and stores.  64 tokens: eight each of 128 experts, gated 1536 x 2048 (376 MB) 69 us, 5.4 TB/s; gated 28672 x 4096
-// (119 MB) 25.0 us; 4096 x 6144 (26 MB) 10.5 us; one token, 4096 x 14336 (59 MB) 14.7 us.
+// to 3 for the last tile's sums, exchange and stores.  64 tokens: eight each of 128 experts, gated 1536 x 2048 (376 MB) 70.4 us, 5.3 TB/s; gated 28672 x 4096
+// (119 MB) 25.5 us; 6144 x 4096 (26 MB) 10.8 us; one token, 4096 x 14336 (59 MB) 14.4 us.
 template <int NT, bool GATED, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
@@ -922,9 +922,9 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_consta
 // A block of K is 32 KB of codes and 512 cycles of MMAs a CTA; its 128 x 256 sums are 256 cycles of the fp32 pipe.  Both run side by side: tensor memory holds
 // two blocks, and the first and the second 128 columns of each are handed over apart, as soon as their four warps have read them.  Six stages and 2 KB a warp
 // through which rows are stored; four stages and a whole tile stored by copies from shared memory took 410 us where this took 399.
-// Bound by the power limit when it runs over and over, else by the 573 cycles that a block of K takes and by a tile's end (3000 cycles, gated 3400, under which
-// two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 380 us (2.5 PFLOP/s; over and over 430; copies and MMAs alone 334), gated 28672 x
-// 4096 796 us (2.4 PFLOP/s; 880; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 66 us.
+// Bound by the power limit when it runs over and over, else by the 585 cycles that a block of K takes and by a tile's end (3000 cycles, gated 3900, under which
+// two blocks of the next tile are multiplied).  8192 tokens: 4096 x 14336 377 us (2.5 PFLOP/s; over and over 450; copies and MMAs alone 334), gated 28672 x
+// 4096 808 us (2.4 PFLOP/s; 938; 655).  12288 rows of 64 experts, 2048 x 1408 (253 MB): 69 us, gated 2816 x 2048 127 us.
 template <bool GATED, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Fp8Params p) {
